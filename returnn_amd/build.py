@@ -1,5 +1,5 @@
 """
-Ahead-of-time build of ``librtn_native_lstm2.so`` for gfx950 with hipcc.
+Ahead-of-time build of ``librtn_native_lstm2.so`` and ``librtn_sequence_ops.so`` for gfx950 with hipcc.
 
 Takes the place of the reference's run-time compile-and-cache step for native ops
 (returnn/util/native_code_compiler.py:216-354, returnn/torch/util/native_op_code_compiler.py:94-131):
@@ -28,11 +28,18 @@ TABLE_PARTS = 17
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 VGPR_FORM_PARTS = (1, 2, 14)
 SOURCES = [HOST_SOURCE, TABLES_SOURCE]
-HEADERS = ["lstm2_kernels.h", "lstm2_step_kernel.h", "lstm2_wide_kernel.h", "lstm2_solo_kernel.h", "lstm2_dual_kernel.h", "lstm2_sparse_kernel.h", "lstm2_bwd_kernels.h", "lstm2_bwd_local_kernel.h", "lstm2_bwd_wide_kernel.h", "weight_grad_kernel.h", "lstm2_params.h", "lstm2_kernel_tables.h",
+HEADERS = ["gate_functions.h", "lstm2_kernels.h", "lstm2_step_kernel.h", "lstm2_wide_kernel.h", "lstm2_solo_kernel.h", "lstm2_dual_kernel.h", "lstm2_sparse_kernel.h", "lstm2_bwd_kernels.h", "lstm2_bwd_local_kernel.h", "lstm2_bwd_wide_kernel.h", "weight_grad_kernel.h", "lstm2_params.h", "lstm2_kernel_tables.h",
            os.path.join("..", "..", "include", "rtn_native_lstm2.h")]  # fmt: skip
 # the torch side of the calls (host code only)
 BINDING_SOURCE = "rtn_torch_binding.cpp"
 BINDING_PATH = os.path.join(_dir, "_rtn_torch.so")
+# the operators around the recurrent layers: a library of their own, and its torch side
+SEQUENCE_SOURCE = "rtn_sequence_ops.hip"
+SEQUENCE_HEADERS = ["gate_functions.h", "sequence_common.h", "gated_recurrence_kernels.h", "dropout_kernel.h", "token_scores_kernels.h",
+                    os.path.join("..", "..", "include", "rtn_sequence_ops.h"), os.path.join("..", "..", "include", "rtn_native_lstm2.h")]  # fmt: skip
+SEQUENCE_LIB_PATH = os.path.join(CSRC_DIR, "librtn_sequence_ops.so")
+SEQUENCE_BINDING_SOURCE = "rtn_sequence_binding.cpp"
+SEQUENCE_BINDING_PATH = os.path.join(_dir, "_rtn_sequence.so")
 OBJ_DIR = os.path.join(CSRC_DIR, "_obj")
 OFFLOAD_ARCH = "gfx950"
 ROCM_LIB_DIR = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib")  # rocBLAS (weight-gradient GEMM of the backward op)
@@ -84,8 +91,13 @@ def link_command(output: Optional[str] = None, obj_dir: Optional[str] = None) ->
     ]  # fmt: skip
 
 
-def binding_command(output: Optional[str] = None) -> List[str]:
-    """The g++ line of the torch binding: against the torch and HIP headers, no device code.  The HIP runtime is the one
+def sequence_command(output: Optional[str] = None) -> List[str]:
+    """The hipcc line that makes the library of the sequence operators."""
+    return [hipcc_path()] + _flags() + ["-shared", os.path.join(CSRC_DIR, SEQUENCE_SOURCE), "-o", output or SEQUENCE_LIB_PATH]
+
+
+def binding_command(output: Optional[str] = None, source: str = BINDING_SOURCE) -> List[str]:
+    """The g++ line of a torch binding: against the torch and HIP headers, no device code.  The HIP runtime is the one
     torch has loaded by then."""
     import sysconfig
 
@@ -94,17 +106,18 @@ def binding_command(output: Optional[str] = None) -> List[str]:
 
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas", "-Wno-attributes"]
-    cmd += ["-D_GLIBCXX_USE_CXX11_ABI=%i" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_rtn_torch"]
+    cmd += ["-D_GLIBCXX_USE_CXX11_ABI=%i" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=" + {BINDING_SOURCE: "_rtn_torch", SEQUENCE_BINDING_SOURCE: "_rtn_sequence"}[source]]
     cmd += ["-isystem" + d for d in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]] if os.path.isdir(d)]
-    cmd += [os.path.join(CSRC_DIR, BINDING_SOURCE), "-o", output or BINDING_PATH, "-L" + torch_lib, "-L" + ROCM_LIB_DIR]
+    cmd += [os.path.join(CSRC_DIR, source), "-o", output or {BINDING_SOURCE: BINDING_PATH, SEQUENCE_BINDING_SOURCE: SEQUENCE_BINDING_PATH}[source], "-L" + torch_lib, "-L" + ROCM_LIB_DIR]
     return cmd + ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python", "-lamdhip64"]
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH) or not os.path.exists(BINDING_PATH):
+    built = (LIB_PATH, BINDING_PATH, SEQUENCE_LIB_PATH, SEQUENCE_BINDING_PATH)
+    if not all(os.path.exists(path) for path in built):
         return True
-    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(BINDING_PATH))
-    deps = [os.path.join(CSRC_DIR, f) for f in SOURCES + HEADERS + [BINDING_SOURCE]] + [os.path.abspath(__file__)]
+    t = min(os.path.getmtime(path) for path in built)
+    deps = [os.path.join(CSRC_DIR, f) for f in SOURCES + HEADERS + [BINDING_SOURCE, SEQUENCE_SOURCE, SEQUENCE_BINDING_SOURCE] + SEQUENCE_HEADERS] + [os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
@@ -118,7 +131,7 @@ def _jobs() -> int:
 
 def build_library(force: bool = True, verbose: bool = False) -> str:
     """
-    Compile the HIP library in-tree: the objects side by side (as many at once as the machine has cores, or MAX_JOBS),
+    Compile the HIP libraries in-tree: the objects side by side (as many at once as the machine has cores, or MAX_JOBS),
     then one link.
 
     :param force: rebuild even if the library is newer than its sources
@@ -132,6 +145,7 @@ def build_library(force: bool = True, verbose: bool = False) -> str:
     os.makedirs(obj_dir, exist_ok=True)
     tmp = LIB_PATH + ".tmp.%i" % os.getpid()
     tmp_binding = BINDING_PATH + ".tmp.%i" % os.getpid()
+    tmp_sequence, tmp_sequence_binding = SEQUENCE_LIB_PATH + ".tmp.%i" % os.getpid(), SEQUENCE_BINDING_PATH + ".tmp.%i" % os.getpid()
 
     def run(cmd):
         if verbose:
@@ -141,7 +155,8 @@ def build_library(force: bool = True, verbose: bool = False) -> str:
 
     try:
         with ThreadPoolExecutor(max_workers=_jobs()) as pool:
-            results = list(pool.map(run, [binding_command(tmp_binding)] + compile_commands(obj_dir)))
+            results = list(pool.map(run, [binding_command(tmp_binding), binding_command(tmp_sequence_binding, SEQUENCE_BINDING_SOURCE), sequence_command(tmp_sequence)]
+                                    + compile_commands(obj_dir)))  # fmt: skip
         results.append(run(link_command(tmp, obj_dir)) if all(rc == 0 for _, rc, _ in results) else (["(link skipped)"], 0, ""))
         for cmd, rc, out in results:
             if rc != 0:
@@ -150,9 +165,11 @@ def build_library(force: bool = True, verbose: bool = False) -> str:
                 print(out, file=sys.stderr)
         os.replace(tmp, LIB_PATH)
         os.replace(tmp_binding, BINDING_PATH)
+        os.replace(tmp_sequence, SEQUENCE_LIB_PATH)
+        os.replace(tmp_sequence_binding, SEQUENCE_BINDING_PATH)
     finally:
         shutil.rmtree(obj_dir, ignore_errors=True)
-        for left in (tmp, tmp_binding):
+        for left in (tmp, tmp_binding, tmp_sequence, tmp_sequence_binding):
             if os.path.exists(left):
                 os.remove(left)
     return LIB_PATH

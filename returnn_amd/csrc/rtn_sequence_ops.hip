@@ -1,0 +1,185 @@
+// Host side of librtn_sequence_ops.so: argument checks and launches (include/rtn_sequence_ops.h).
+#include "../../include/rtn_sequence_ops.h"
+
+#include <hip/hip_runtime.h>
+
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <string>
+
+#include "dropout_kernel.h"
+#include "gated_recurrence_kernels.h"
+#include "token_scores_kernels.h"
+
+namespace rtn {
+namespace {
+
+thread_local std::string g_last_error;
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? RTN_OK : fail(RTN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+bool known(int dtype) { return dtype == RTN_DTYPE_F32 || dtype == RTN_DTYPE_BF16; }
+int size_of(int dtype) { return dtype == RTN_DTYPE_BF16 ? 2 : 4; }
+bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
+constexpr int64_t kMaxBlocks = 0x7FFFFFFF;
+
+// Calls f with a value of the element type.
+template <typename F>
+void with_type(int dtype, F f) {
+  if (dtype == RTN_DTYPE_BF16)
+    f((__bf16)0.f);
+  else
+    f(0.f);
+}
+
+// ---- gated recurrence ---------------------------------------------------------------------------------------------
+int64_t recurrence_chunks(int64_t T) { return (T + kRecurrenceFrames - 1) / kRecurrenceFrames; }
+
+// The checks that both directions share; `ld` is set where it was left out.
+int recurrence_check(const char* what, const void* X, int64_t* ldX, const float* c0, const int64_t* lens, int64_t T, int32_t B, int32_t n, int32_t dtype, int32_t direction) {
+  if (T < 0 || B < 0 || n < 0) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d n=%d", what, (long long)T, B, n);
+  if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+  if (direction != 1 && direction != -1) return fail(RTN_ERR_RANGE, "%s: direction must be 1 or -1, got %d", what, direction);
+  if (!*ldX) *ldX = 4 * (int64_t)n;
+  if (*ldX < 4 * (int64_t)n) return fail(RTN_ERR_SHAPE, "%s: rows of X are %lld elements apart, but have %lld", what, (long long)*ldX, 4ll * n);
+  if (T && B && n && !X) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(X, size_of(dtype)) || !aligned(c0, 4) || !aligned(lens, 8)) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  return RTN_OK;
+}
+
+}  // namespace
+}  // namespace rtn
+
+using namespace rtn;
+
+extern "C" {
+
+int rtn_sequence_ops_abi_version(void) { return 1; }
+const char* rtn_sequence_last_error(void) { return g_last_error.c_str(); }
+
+size_t rtn_gated_recurrence_saved_bytes(int64_t T, int32_t B, int32_t n, int32_t) {
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : (size_t)recurrence_chunks(T) * (size_t)B * (size_t)n * 4;
+}
+size_t rtn_gated_recurrence_fwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
+size_t rtn_gated_recurrence_bwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
+
+int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, void* Y, float* cN, void* saved, int64_t T, int32_t B, int32_t n,
+                             int32_t dtype, int32_t direction, void*, size_t, void* hip_stream) {
+  g_last_error.clear();
+  const int rc = recurrence_check("gated recurrence", X, &ldX, c0, lens, T, B, n, dtype, direction);
+  if (rc != RTN_OK) return rc;
+  if (B == 0 || n == 0) return RTN_OK;
+  if ((T && !Y) || !cN) return fail(RTN_ERR_ARG, "gated recurrence: null pointer");
+  if (!aligned(Y, size_of(dtype)) || !aligned(cN, 4) || !aligned(saved, 16)) return fail(RTN_ERR_ARG, "gated recurrence: misaligned pointer");
+  const int64_t blocks = ((int64_t)B * n + 255) / 256;
+  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
+  const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0};
+  with_type(dtype, [&](auto type) {
+    hipLaunchKernelGGL((k_recurrence_fwd<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
+  });
+  return launched("gated recurrence");
+}
+
+int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, const void* saved, const void* DY, int64_t ldDY, const float* DcN, void* DX,
+                             float* Dc0, int64_t T, int32_t B, int32_t n, int32_t dtype, int32_t direction, void*, size_t, void* hip_stream) {
+  g_last_error.clear();
+  const int rc = recurrence_check("gated recurrence gradient", X, &ldX, c0, lens, T, B, n, dtype, direction);
+  if (rc != RTN_OK) return rc;
+  if (B == 0 || n == 0) return RTN_OK;
+  if (!ldDY) ldDY = n;
+  if (ldDY < n) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: rows of DY are %lld elements apart, but have %d", (long long)ldDY, n);
+  if ((T && (!DX || !DY || !saved)) || !Dc0) return fail(RTN_ERR_ARG, "gated recurrence gradient: null pointer");
+  if (!aligned(DY, size_of(dtype)) || !aligned(DX, size_of(dtype)) || !aligned(Dc0, 4) || !aligned(DcN, 4) || !aligned(saved, 16))
+    return fail(RTN_ERR_ARG, "gated recurrence gradient: misaligned pointer");
+  const int64_t blocks = ((int64_t)B * n + 255) / 256;
+  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
+  const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0};
+  with_type(dtype, [&](auto type) {
+    hipLaunchKernelGGL((k_recurrence_bwd<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
+  });
+  return launched("gated recurrence gradient");
+}
+
+int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t times, int64_t rows, int64_t width, int32_t dtype, int32_t threshold,
+                uint64_t seed, uint64_t offset, const int64_t* offset_ptr, int32_t same_over_time, void* hip_stream) {
+  g_last_error.clear();
+  if (times < 0 || rows < 0 || width < 0) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld]", (long long)times, (long long)rows, (long long)width);
+  if (!known(dtype)) return fail(RTN_ERR_ARG, "dropout: unknown dtype %d", dtype);
+  if (threshold < 0 || threshold > 65536) return fail(RTN_ERR_RANGE, "dropout: threshold %d is not in 0..65536", threshold);
+  if (!ldx) ldx = width;
+  if (!ldr) ldr = width;
+  if (ldx < width || ldr < width) return fail(RTN_ERR_SHAPE, "dropout: rows are %lld and %lld elements apart, but have %lld", (long long)ldx, (long long)ldr, (long long)width);
+  if (!times || !rows || !width) return RTN_OK;
+  if (!x || !y) return fail(RTN_ERR_ARG, "dropout: null pointer");
+  const int e = size_of(dtype);
+  if (!aligned(x, e) || !aligned(y, e) || !aligned(residual, e) || !aligned(offset_ptr, 8)) return fail(RTN_ERR_ARG, "dropout: misaligned pointer");
+  const float scale = threshold == 65536 ? 0.f : 65536.f / (float)(65536 - threshold);
+  const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr, same_over_time};
+  const int64_t count = (same_over_time ? 1 : times) * rows * width, blocks = ((count + 7) / 8 + 255) / 256;
+  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
+  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_dropout<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  return launched("dropout");
+}
+
+// ---- scores of tokens ---------------------------------------------------------------------------------------------
+static int scores_check(const char* what, const void* logits, int64_t* ld, const int64_t* targets, int64_t rows, int64_t V, int32_t dtype) {
+  if (rows < 0 || V < 0 || V > 0x7FFFFFFF) return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld logits", what, (long long)rows, (long long)V);
+  if (rows > kMaxBlocks) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
+  if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+  if (!*ld) *ld = V;
+  if (*ld < V) return fail(RTN_ERR_SHAPE, "%s: rows are %lld elements apart, but have %lld", what, (long long)*ld, (long long)V);
+  if (rows && V == 0) return fail(RTN_ERR_SHAPE, "%s: rows without a logit", what);
+  if (rows && !logits) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(logits, size_of(dtype)) || !aligned(targets, 8)) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  return RTN_OK;
+}
+
+size_t rtn_token_log_probs_workspace_bytes(int64_t, int64_t, int32_t, int32_t) { return 0; }
+
+int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t V, int32_t dtype, int32_t top_k, float* log_prob, float* norm,
+                            float* entropy, float* top_log_prob, int64_t* top_ids, void*, size_t, void* hip_stream) {
+  g_last_error.clear();
+  const int rc = scores_check("token log probabilities", logits, &ld, targets, rows, V, dtype);
+  if (rc != RTN_OK) return rc;
+  if (top_k < 0 || top_k > kMaxAlternatives || (rows && top_k > V))
+    return fail(RTN_ERR_RANGE, "token log probabilities: %d alternatives of %lld tokens (at most %d)", top_k, (long long)V, kMaxAlternatives);
+  if (rows == 0) return RTN_OK;
+  if (log_prob && !targets) return fail(RTN_ERR_ARG, "token log probabilities: no targets");
+  if (top_k && (!top_log_prob || !top_ids)) return fail(RTN_ERR_ARG, "token log probabilities: null pointer");
+  if (!aligned(log_prob, 4) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(top_log_prob, 4) || !aligned(top_ids, 8))
+    return fail(RTN_ERR_ARG, "token log probabilities: misaligned pointer");
+  const ScoresArgs a{logits, ld, targets, rows, V, top_k, log_prob, norm, entropy, top_log_prob, top_ids, nullptr, nullptr, nullptr};
+  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_token_scores<decltype(type)>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  return launched("token log probabilities");
+}
+
+int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm, const float* entropy, const float* d_log_prob, const float* d_entropy,
+                            void* D, int64_t rows, int64_t V, int32_t dtype, void* hip_stream) {
+  g_last_error.clear();
+  const int rc = scores_check("token log probabilities gradient", logits, &ld, targets, rows, V, dtype);
+  if (rc != RTN_OK) return rc;
+  if (rows == 0) return RTN_OK;
+  if (!D || !norm || (d_entropy && !entropy) || (d_log_prob && !targets)) return fail(RTN_ERR_ARG, "token log probabilities gradient: null pointer");
+  if (!aligned(D, size_of(dtype)) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(d_log_prob, 4) || !aligned(d_entropy, 4))
+    return fail(RTN_ERR_ARG, "token log probabilities gradient: misaligned pointer");
+  const ScoresArgs a{logits, ld, targets, rows, V, 0, nullptr, (float*)norm, (float*)entropy, nullptr, nullptr, d_log_prob, d_entropy, D};
+  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_token_scores_bwd<decltype(type)>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  return launched("token log probabilities gradient");
+}
+
+}  // extern "C"

@@ -1,0 +1,240 @@
+"""
+CPU-side checks of the sequence operators: the library loads and exports what its header declares, refusals come before
+any launch, the definitions that the GPU tests compare with hold (published vectors, differences, closed forms).
+"""
+
+from __future__ import annotations
+
+import os
+import re
+import subprocess
+
+import numpy
+import pytest
+import torch
+
+import _sequence_ref as ref
+import test_generated_code as generated
+from returnn_amd import build, lib, sequence_lib
+from returnn_amd.dropout import Dropout, dropout
+from returnn_amd.recurrence import GatedRecurrence, gated_recurrence
+from returnn_amd.scoring import token_log_probs
+
+_root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+F32, BF16 = lib.DTYPE_F32, lib.DTYPE_BF16
+
+
+@pytest.fixture(scope="module")
+def cabi():
+    if not os.path.exists(build.SEQUENCE_LIB_PATH):
+        build.build_library()
+    return sequence_lib.load()
+
+
+def test_header_symbols_are_exported(cabi):
+    header = open(os.path.join(_root, "include", "rtn_sequence_ops.h")).read()
+    declared = set(re.findall(r"^(?:int|size_t|const char\*) (rtn_[a-z0-9_]+)\(", header, re.M))
+    assert declared == set(sequence_lib.SYMBOLS)
+    for name in declared:
+        assert getattr(cabi, name) is not None
+    assert re.findall(r"ABI version of this header: (\d+)\.", header) == [str(sequence_lib.EXPECTED_ABI)]
+    assert cabi.rtn_sequence_ops_abi_version() == sequence_lib.EXPECTED_ABI
+
+
+def test_loader_refuses_another_abi_version(monkeypatch):
+    monkeypatch.setattr(sequence_lib, "_lib", None)
+    monkeypatch.setattr(sequence_lib, "EXPECTED_ABI", sequence_lib.EXPECTED_ABI + 1)
+    with pytest.raises(lib.NativeLibraryMismatch):
+        sequence_lib.load()
+
+
+def test_the_library_is_never_built_silently(monkeypatch, tmp_path):
+    monkeypatch.setattr(sequence_lib, "_lib", None)
+    monkeypatch.setattr(build, "SEQUENCE_LIB_PATH", str(tmp_path / "none.so"))
+    with pytest.raises(lib.NativeLibraryMissing):
+        sequence_lib.load()
+
+
+P = 1 << 20  # an address that is never looked at: every call below is refused by the host, or has nothing to do
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
+        (dict(T=-1), lib.RTN_ERR_SHAPE), (dict(B=-1), lib.RTN_ERR_SHAPE), (dict(n=-2), lib.RTN_ERR_SHAPE), (dict(ldX=31), lib.RTN_ERR_SHAPE),
+        (dict(dtype=2), lib.RTN_ERR_ARG), (dict(direction=0), lib.RTN_ERR_RANGE), (dict(direction=2), lib.RTN_ERR_RANGE),
+        (dict(X=None), lib.RTN_ERR_ARG), (dict(Y=None), lib.RTN_ERR_ARG), (dict(cN=None), lib.RTN_ERR_ARG),
+        (dict(X=P + 1), lib.RTN_ERR_ARG), (dict(X=P + 2, dtype=F32), lib.RTN_ERR_ARG), (dict(c0=P + 2), lib.RTN_ERR_ARG), (dict(lens=P + 4), lib.RTN_ERR_ARG),
+        (dict(Y=P + 1), lib.RTN_ERR_ARG), (dict(cN=P + 1), lib.RTN_ERR_ARG), (dict(saved=P + 4), lib.RTN_ERR_ARG),
+        (dict(B=0), lib.RTN_OK), (dict(n=0), lib.RTN_OK),
+    ],
+)  # fmt: skip
+def test_recurrence_refusals(cabi, change, code):
+    a = dict(X=P, ldX=0, c0=P, lens=P, Y=P, cN=P, saved=P, T=5, B=3, n=8, dtype=BF16, direction=1)
+    a.update(change)
+    assert cabi.rtn_gated_recurrence_fwd(*a.values(), None, 0, None) == code
+    assert bool(sequence_lib.last_error()) == (code != lib.RTN_OK)
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
+        (dict(T=-1), lib.RTN_ERR_SHAPE), (dict(ldX=31), lib.RTN_ERR_SHAPE), (dict(ldDY=7), lib.RTN_ERR_SHAPE), (dict(dtype=5), lib.RTN_ERR_ARG),
+        (dict(direction=0), lib.RTN_ERR_RANGE), (dict(saved=None), lib.RTN_ERR_ARG), (dict(DY=None), lib.RTN_ERR_ARG), (dict(DX=None), lib.RTN_ERR_ARG),
+        (dict(Dc0=None), lib.RTN_ERR_ARG), (dict(DY=P + 1), lib.RTN_ERR_ARG), (dict(DX=P + 1), lib.RTN_ERR_ARG), (dict(DcN=P + 2), lib.RTN_ERR_ARG),
+        (dict(B=0), lib.RTN_OK),
+    ],
+)  # fmt: skip
+def test_recurrence_gradient_refusals(cabi, change, code):
+    a = dict(X=P, ldX=0, c0=P, lens=P, saved=P, DY=P, ldDY=0, DcN=P, DX=P, Dc0=P, T=5, B=3, n=8, dtype=BF16, direction=1)
+    a.update(change)
+    assert cabi.rtn_gated_recurrence_bwd(*a.values(), None, 0, None) == code
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
+        (dict(times=-1), lib.RTN_ERR_SHAPE), (dict(rows=-1), lib.RTN_ERR_SHAPE), (dict(width=-1), lib.RTN_ERR_SHAPE), (dict(ldx=7), lib.RTN_ERR_SHAPE),
+        (dict(ldr=7), lib.RTN_ERR_SHAPE), (dict(dtype=-1), lib.RTN_ERR_ARG), (dict(threshold=-1), lib.RTN_ERR_RANGE), (dict(threshold=65537), lib.RTN_ERR_RANGE),
+        (dict(x=None), lib.RTN_ERR_ARG), (dict(y=None), lib.RTN_ERR_ARG), (dict(x=P + 1), lib.RTN_ERR_ARG), (dict(residual=P + 1), lib.RTN_ERR_ARG),
+        (dict(offset_ptr=P + 4), lib.RTN_ERR_ARG), (dict(rows=0), lib.RTN_OK), (dict(width=0), lib.RTN_OK), (dict(times=0), lib.RTN_OK),
+    ],
+)  # fmt: skip
+def test_dropout_refusals(cabi, change, code):
+    a = dict(x=P, ldx=0, residual=P, ldr=0, y=P, times=3, rows=4, width=8, dtype=BF16, threshold=100, seed=1, offset=2, offset_ptr=None, same=0)
+    a.update(change)
+    assert cabi.rtn_dropout(*a.values(), None) == code
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
+        (dict(rows=-1), lib.RTN_ERR_SHAPE), (dict(V=-1), lib.RTN_ERR_SHAPE), (dict(V=0, top_k=0), lib.RTN_ERR_SHAPE), (dict(V=1 << 31), lib.RTN_ERR_SHAPE),
+        (dict(rows=1 << 31), lib.RTN_ERR_SHAPE), (dict(ld=99), lib.RTN_ERR_SHAPE), (dict(dtype=3), lib.RTN_ERR_ARG), (dict(top_k=-1), lib.RTN_ERR_RANGE),
+        (dict(top_k=65), lib.RTN_ERR_RANGE), (dict(top_k=5, V=4), lib.RTN_ERR_RANGE), (dict(logits=None), lib.RTN_ERR_ARG), (dict(targets=None), lib.RTN_ERR_ARG),
+        (dict(top_ids=None), lib.RTN_ERR_ARG), (dict(top=None), lib.RTN_ERR_ARG), (dict(logits=P + 1), lib.RTN_ERR_ARG), (dict(targets=P + 4), lib.RTN_ERR_ARG),
+        (dict(log_prob=P + 2), lib.RTN_ERR_ARG), (dict(norm=P + 4), lib.RTN_ERR_ARG), (dict(top_ids=P + 4), lib.RTN_ERR_ARG), (dict(rows=0), lib.RTN_OK),
+    ],
+)  # fmt: skip
+def test_scores_refusals(cabi, change, code):
+    a = dict(logits=P, ld=0, targets=P, rows=6, V=100, dtype=BF16, top_k=4, log_prob=P, norm=P, entropy=P, top=P, top_ids=P)
+    a.update(change)
+    assert cabi.rtn_token_log_probs_fwd(*a.values(), None, 0, None) == code
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
+        (dict(rows=-1), lib.RTN_ERR_SHAPE), (dict(ld=99), lib.RTN_ERR_SHAPE), (dict(norm=None), lib.RTN_ERR_ARG), (dict(D=None), lib.RTN_ERR_ARG),
+        (dict(entropy=None), lib.RTN_ERR_ARG), (dict(targets=None), lib.RTN_ERR_ARG), (dict(D=P + 1), lib.RTN_ERR_ARG), (dict(rows=0), lib.RTN_OK),
+    ],
+)  # fmt: skip
+def test_scores_gradient_refusals(cabi, change, code):
+    a = dict(logits=P, ld=0, targets=P, norm=P, entropy=P, d_log_prob=P, d_entropy=P, D=P, rows=6, V=100, dtype=BF16)
+    a.update(change)
+    assert cabi.rtn_token_log_probs_bwd(*a.values(), None) == code
+
+
+def test_cpu_tensors_and_bad_arguments_are_refused(cabi):
+    x = torch.zeros((2, 3, 8))
+    with pytest.raises(RuntimeError, match="HIP"):
+        gated_recurrence(x)
+    with pytest.raises(RuntimeError, match="HIP"):
+        GatedRecurrence(5, 2)(torch.zeros((2, 3, 5)))
+    with pytest.raises(RuntimeError, match="HIP"):
+        dropout(x, 0.5, seed=1)
+    with pytest.raises(RuntimeError, match="HIP"):
+        token_log_probs(x)
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError):
+            dropout(x, p, seed=1)
+        with pytest.raises(ValueError):
+            Dropout(p)
+    with pytest.raises(ValueError):
+        GatedRecurrence(5, 2)(torch.zeros((2, 3, 4)))
+
+
+def test_dropout_module_in_evaluation_is_the_identity():
+    x, r = torch.randn((3, 4)), torch.randn((3, 4))
+    m = Dropout(0.5).eval()
+    assert m(x) is x and torch.equal(m(x, residual=r), x + r) and m.offset == 0
+
+
+# ---- the definitions that the GPU tests compare with ----
+@pytest.mark.parametrize(
+    "counter,key,want",
+    [  # the published vectors of the generator
+        ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+        ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+        ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0), (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+    ],
+)
+def test_philox_vectors(counter, key, want):
+    assert tuple(ref.philox(counter, key)) == want
+
+
+def test_draws_are_even():
+    """Of 64 Ki draws the share below a threshold is that of the threshold, within five standard deviations."""
+    d = ref.draws(0, 1 << 16, 12345, 7)
+    for p in (0.1, 0.5, 0.9):
+        assert abs((d < p * 65536).mean() - p) < 5 * numpy.sqrt(p * (1 - p) / len(d))
+
+
+@pytest.mark.parametrize("direction", [1, -1])
+def test_recurrence_gradient_against_differences(direction):
+    rng = numpy.random.default_rng(3)
+    T, B, n = 7, 3, 2
+    x, c0, lens = rng.normal(size=(T, B, 4 * n)), rng.normal(size=(B, n)), [7, 0, 4]
+    dy, dc = rng.normal(size=(T, B, n)), rng.normal(size=(B, n))
+    dx, dc0, _, _ = ref.recurrence_grad(x, dy, dc, c0, lens, direction)
+
+    def value(x, c0):
+        y, c, _ = ref.recurrence(x, c0, lens, direction)
+        return (y * dy).sum() + (c * dc).sum()
+
+    h = 1e-5  # (errors of h^2 and 1e-16 / h)
+    for a, d in ((x, dx), (c0, dc0)):
+        for at in numpy.ndindex(a.shape):
+            old = a[at]
+            a[at] = old + h
+            up = value(x, c0)
+            a[at] = old - h
+            down = value(x, c0)
+            a[at] = old
+            assert abs((up - down) / (2 * h) - d[at]) < 1e-8
+
+
+def test_scores_gradient_against_differences():
+    rng = numpy.random.default_rng(4)
+    R, V = 4, 9
+    x, targets = rng.normal(size=(R, V)), numpy.array([3, -1, 8, 0])
+    g, ge = rng.normal(size=R), rng.normal(size=R)
+    d = ref.scores_grad(x, targets, g, ge)
+
+    def value():
+        lp, h, _, _, _ = ref.scores(x, targets)
+        return (lp * g).sum() + (h * ge).sum()
+
+    h = 1e-5
+    for at in numpy.ndindex(x.shape):
+        old = x[at]
+        x[at] = old + h
+        up = value()
+        x[at] = old - h
+        down = value()
+        x[at] = old
+        assert abs((up - down) / (2 * h) - d[at]) < 1e-8
+
+
+def test_no_kernel_loses_a_copy(tmp_path):
+    """As for the LSTM kernels: no value is copied between the end of a masked block and the switch back to all lanes."""
+    if not os.path.exists(build.SEQUENCE_LIB_PATH) or not os.path.exists(generated.OBJDUMP):
+        pytest.skip("no library or no llvm-objdump")
+    with open(build.SEQUENCE_LIB_PATH, "rb") as f:
+        objects = list(generated._code_objects(f.read()))
+    assert len(objects) == 1
+    path = tmp_path / "code.elf"
+    path.write_bytes(objects[0])
+    lines = subprocess.run([generated.OBJDUMP, "-d", str(path)], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines(keepends=True)
+    assert sum("k_recurrence" in line for line in lines if line.endswith(">:\n")) > 0
+    assert not generated.lost_copies(lines)

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "dropout_kernel.h"
 #include "gated_recurrence_kernels.h"
@@ -45,6 +46,15 @@ void with_type(int dtype, F f) {
     f((__bf16)0.f);
   else
     f(0.f);
+}
+
+// Calls f with std::true_type or std::false_type.
+template <typename F>
+void with_bool(bool v, F f) {
+  if (v)
+    f(std::true_type());
+  else
+    f(std::false_type());
 }
 
 // ---- gated recurrence ---------------------------------------------------------------------------------------------
@@ -129,10 +139,30 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
   const int e = size_of(dtype);
   if (!aligned(x, e) || !aligned(y, e) || !aligned(residual, e) || !aligned(offset_ptr, 8)) return fail(RTN_ERR_ARG, "dropout: misaligned pointer");
   const float scale = threshold == 65536 ? 0.f : 65536.f / (float)(65536 - threshold);
-  const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr, same_over_time};
-  const int64_t count = (same_over_time ? 1 : times) * rows * width, blocks = ((count + 7) / 8 + 255) / 256;
+  if (!same_over_time) {
+    if (rows > INT64_MAX / times) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
+    rows *= times, times = 1;
+  }
+  const int64_t count = rows * width, groups = (count + 7) / 8;
+  const bool flat = rows == 1 || (ldx == width && (!residual || ldr == width)), shared = times > 1;
+  // Frames per thread that share their draws: no more than leave every SIMD 8 wavefronts.
+  const int64_t frames = std::max<int64_t>({1, std::min<int64_t>(16, times * groups / (256 * 2048)), (times + 65534) / 65535});
+  const int64_t per_block = flat && !shared ? 512 : 256, blocks = (groups + per_block - 1) / per_block;
   if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
-  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_dropout<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, count, frames, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr};
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    with_bool(residual != nullptr, [&](auto add) {
+      constexpr bool ADD = decltype(add)::value;
+      const hipStream_t stream = (hipStream_t)hip_stream;
+      if (!flat)
+        hipLaunchKernelGGL((k_dropout_rows<AT, ADD>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+      else if (shared)
+        hipLaunchKernelGGL((k_dropout<AT, ADD, true>), dim3((unsigned)blocks, (unsigned)((times + frames - 1) / frames)), dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_dropout<AT, ADD, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    });
+  });
   return launched("dropout");
 }
 

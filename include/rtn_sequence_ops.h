@@ -76,7 +76,7 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
 /*
  * Log probabilities under softmax over the last axis.
  *
- * logits  [rows,V], row r at element r*ld (0: V)
+ * logits  [rows,V], row r at element r*ld (0: V); V up to 2^26
  * targets [rows] token per row, or NULL (no log_prob; every row counts).  A negative target marks a row without a token:
  *         it is not read, log_prob and entropy are 0, the alternatives -inf with index -1, its gradient 0.
  *         A target of V or more gives a log_prob of NaN and a row of NaN as gradient.

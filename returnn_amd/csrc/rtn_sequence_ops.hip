@@ -168,7 +168,7 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
 
 // ---- scores of tokens ---------------------------------------------------------------------------------------------
 static int scores_check(const char* what, const void* logits, int64_t* ld, const int64_t* targets, int64_t rows, int64_t V, int32_t dtype) {
-  if (rows < 0 || V < 0 || V > 0x7FFFFFFF) return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld logits", what, (long long)rows, (long long)V);
+  if (rows < 0 || V < 0 || V > kMaxTokens) return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld logits (at most %lld)", what, (long long)rows, (long long)V, (long long)kMaxTokens);
   if (rows > kMaxBlocks) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
   if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
   if (!*ld) *ld = V;
@@ -179,10 +179,17 @@ static int scores_check(const char* what, const void* logits, int64_t* ld, const
   return RTN_OK;
 }
 
-size_t rtn_token_log_probs_workspace_bytes(int64_t, int64_t, int32_t, int32_t) { return 0; }
+// Pieces of a row: it is one while 16 wavefronts hold it in registers.
+static int64_t scores_splits(int64_t V) { return (V + kMaxSegment - 1) / kMaxSegment; }
+
+size_t rtn_token_log_probs_workspace_bytes(int64_t rows, int64_t V, int32_t, int32_t top_k) {
+  if (rows <= 0 || V <= 0 || top_k < 0) return 0;
+  const int64_t splits = scores_splits(V);
+  return splits == 1 ? 0 : (size_t)rows * (size_t)splits * (16 + 8 * (size_t)top_k);
+}
 
 int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t V, int32_t dtype, int32_t top_k, float* log_prob, float* norm,
-                            float* entropy, float* top_log_prob, int64_t* top_ids, void*, size_t, void* hip_stream) {
+                            float* entropy, float* top_log_prob, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* hip_stream) {
   g_last_error.clear();
   const int rc = scores_check("token log probabilities", logits, &ld, targets, rows, V, dtype);
   if (rc != RTN_OK) return rc;
@@ -193,8 +200,35 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   if (top_k && (!top_log_prob || !top_ids)) return fail(RTN_ERR_ARG, "token log probabilities: null pointer");
   if (!aligned(log_prob, 4) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(top_log_prob, 4) || !aligned(top_ids, 8))
     return fail(RTN_ERR_ARG, "token log probabilities: misaligned pointer");
-  const ScoresArgs a{logits, ld, targets, rows, V, top_k, log_prob, norm, entropy, top_log_prob, top_ids, nullptr, nullptr, nullptr};
-  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_token_scores<decltype(type)>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  const int64_t splits = scores_splits(V), segment = splits == 1 ? V : ((V + splits - 1) / splits + 7) / 8 * 8;
+  const size_t need = rtn_token_log_probs_workspace_bytes(rows, V, dtype, top_k);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "token log probabilities: workspace of %zu bytes needed", need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "token log probabilities: workspace must be 16-byte aligned");
+  if (rows > kMaxBlocks / splits) return fail(RTN_ERR_SHAPE, "token log probabilities: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
+  const ScoresArgs a{logits, ld,      targets, rows,    V,           top_k,           log_prob,
+                     norm,   entropy, top_log_prob, top_ids, nullptr, nullptr, nullptr,
+                     (int)splits, segment, (float*)workspace, (unsigned long long*)((char*)workspace + (size_t)rows * (size_t)splits * 16)};
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    with_bool(top_k > 0, [&](auto top) {
+      constexpr bool TOP = decltype(top)::value;
+      const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4));
+      if (segment <= 512)
+        hipLaunchKernelGGL((k_token_scores<AT, 1, 8, TOP>), four, dim3(256), 0, stream, a);
+      else if (segment <= 2048)
+        hipLaunchKernelGGL((k_token_scores<AT, 4, 8, TOP>), one, dim3(256), 0, stream, a);
+      else if (segment <= 4096)
+        hipLaunchKernelGGL((k_token_scores<AT, 4, 16, TOP>), one, dim3(256), 0, stream, a);
+      else if (segment <= 8192)
+        hipLaunchKernelGGL((k_token_scores<AT, 4, 32, TOP>), one, dim3(256), 0, stream, a);
+      else if (segment <= 16384)
+        hipLaunchKernelGGL((k_token_scores<AT, 8, 32, TOP>), one, dim3(512), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_token_scores<AT, 16, 32, TOP>), one, dim3(1024), 0, stream, a);
+    });
+    if (splits > 1) hipLaunchKernelGGL((k_token_scores_join<AT>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+  });
   return launched("token log probabilities");
 }
 
@@ -207,8 +241,17 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
   if (!D || !norm || (d_entropy && !entropy) || (d_log_prob && !targets)) return fail(RTN_ERR_ARG, "token log probabilities gradient: null pointer");
   if (!aligned(D, size_of(dtype)) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(d_log_prob, 4) || !aligned(d_entropy, 4))
     return fail(RTN_ERR_ARG, "token log probabilities gradient: misaligned pointer");
-  const ScoresArgs a{logits, ld, targets, rows, V, 0, nullptr, (float*)norm, (float*)entropy, nullptr, nullptr, d_log_prob, d_entropy, D};
-  with_type(dtype, [&](auto type) { hipLaunchKernelGGL((k_token_scores_bwd<decltype(type)>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  const int64_t pieces = (V + kBwdPiece - 1) / kBwdPiece;
+  if (rows > kMaxBlocks / pieces) return fail(RTN_ERR_SHAPE, "token log probabilities gradient: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
+  const ScoresArgs a{logits,  ld,      targets, rows,       V,         0, nullptr,     (float*)norm, (float*)entropy,
+                     nullptr, nullptr, d_log_prob, d_entropy, D, (int)pieces, 0, nullptr, nullptr};
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    if (V <= 2048)
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)hip_stream, a);
+    else
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, false>), dim3((unsigned)(rows * pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
+  });
   return launched("token log probabilities gradient");
 }
 

@@ -179,12 +179,13 @@ static int scores_check(const char* what, const void* logits, int64_t* ld, const
   return RTN_OK;
 }
 
-// Pieces of a row: it is one while 16 wavefronts hold it in registers.
-static int64_t scores_splits(int64_t V) { return (V + kMaxSegment - 1) / kMaxSegment; }
+// Pieces of a row: where alternatives are wanted, as many as it takes for 16 wavefronts to hold a piece in registers; else one, but as many where few
+// rows would leave most of the device idle.
+static int64_t scores_splits(int64_t rows, int64_t V, int32_t top_k) { return top_k > 0 || rows < 256 ? (V + kMaxSegment - 1) / kMaxSegment : 1; }
 
 size_t rtn_token_log_probs_workspace_bytes(int64_t rows, int64_t V, int32_t, int32_t top_k) {
   if (rows <= 0 || V <= 0 || top_k < 0) return 0;
-  const int64_t splits = scores_splits(V);
+  const int64_t splits = scores_splits(rows, V, top_k);
   return splits == 1 ? 0 : (size_t)rows * (size_t)splits * (16 + 8 * (size_t)top_k);
 }
 
@@ -200,7 +201,7 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   if (top_k && (!top_log_prob || !top_ids)) return fail(RTN_ERR_ARG, "token log probabilities: null pointer");
   if (!aligned(log_prob, 4) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(top_log_prob, 4) || !aligned(top_ids, 8))
     return fail(RTN_ERR_ARG, "token log probabilities: misaligned pointer");
-  const int64_t splits = scores_splits(V), segment = splits == 1 ? V : ((V + splits - 1) / splits + 7) / 8 * 8;
+  const int64_t splits = scores_splits(rows, V, top_k), segment = splits == 1 ? V : ((V + splits - 1) / splits + 7) / 8 * 8;
   const size_t need = rtn_token_log_probs_workspace_bytes(rows, V, dtype, top_k);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "token log probabilities: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "token log probabilities: workspace must be 16-byte aligned");
@@ -211,22 +212,31 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   const hipStream_t stream = (hipStream_t)hip_stream;
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
-    with_bool(top_k > 0, [&](auto top) {
-      constexpr bool TOP = decltype(top)::value;
-      const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4));
+    const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4));
+    if (top_k > 0) {
       if (segment <= 512)
-        hipLaunchKernelGGL((k_token_scores<AT, 1, 8, TOP>), four, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 8>), four, dim3(256), 0, stream, a);
       else if (segment <= 2048)
-        hipLaunchKernelGGL((k_token_scores<AT, 4, 8, TOP>), one, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 8>), one, dim3(256), 0, stream, a);
       else if (segment <= 4096)
-        hipLaunchKernelGGL((k_token_scores<AT, 4, 16, TOP>), one, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 16>), one, dim3(256), 0, stream, a);
       else if (segment <= 8192)
-        hipLaunchKernelGGL((k_token_scores<AT, 4, 32, TOP>), one, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 32>), one, dim3(256), 0, stream, a);
       else if (segment <= 16384)
-        hipLaunchKernelGGL((k_token_scores<AT, 8, 32, TOP>), one, dim3(512), 0, stream, a);
+        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 32>), one, dim3(512), 0, stream, a);
       else
-        hipLaunchKernelGGL((k_token_scores<AT, 16, 32, TOP>), one, dim3(1024), 0, stream, a);
-    });
+        hipLaunchKernelGGL((k_token_scores_top<AT, 16, 32>), one, dim3(1024), 0, stream, a);
+    } else {
+      with_bool(entropy != nullptr, [&](auto with_entropy) {
+        constexpr bool ENTROPY = decltype(with_entropy)::value;
+        if (segment <= 1024)
+          hipLaunchKernelGGL((k_token_scores<AT, 1, ENTROPY>), four, dim3(256), 0, stream, a);
+        else if (rows >= 256 || segment <= 8192)
+          hipLaunchKernelGGL((k_token_scores<AT, 4, ENTROPY>), one, dim3(256), 0, stream, a);
+        else
+          hipLaunchKernelGGL((k_token_scores<AT, 16, ENTROPY>), one, dim3(1024), 0, stream, a);
+      });
+    }
     if (splits > 1) hipLaunchKernelGGL((k_token_scores_join<AT>), dim3((unsigned)rows), dim3(256), 0, stream, a);
   });
   return launched("token log probabilities");

@@ -58,14 +58,6 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ float wave_sum(float v) {
   return over_wave(v, [](float p, float q) { return p + q; });
 }
-// The largest over groups of G lanes, in all of them.
-template <int G>
-__device__ __forceinline__ float group_max(float v) {
-  if (G >= 2) v = __builtin_fmaxf(v, dpp<0xB1>(v));
-  if (G >= 4) v = __builtin_fmaxf(v, dpp<0x4E>(v));
-  if (G >= 8) v = __builtin_fmaxf(v, dpp<0x141>(v));
-  return v;
-}
 __device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
 #pragma unroll
   for (int step = 32; step; step /= 2) {
@@ -78,6 +70,7 @@ __device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
 constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;  // where maxima start: minus infinity less this is minus infinity, no NaN
 
+constexpr float kNothing = -1e30f;         // 2^(it less a logit) is 0, and so is its product with it
 constexpr float kNoPower = -1e4f;          // 2 to it is 0, and so is its product with it; that of minus infinity would be NaN (maximum keeps a NaN)
 
 // Maximum and sums of part of a row: s = sum 2^t, w = sum t 2^t, t = (x - m) log2 e.
@@ -126,18 +119,16 @@ __device__ __forceinline__ void put_alternative(const ScoresArgs& a, long long r
   }
 }
 
-// W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
-constexpr int kCandidates = 256;
+// Sums and alternatives: W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
+constexpr int kCandidates = 512;
 constexpr int kMaxSegment = 16 * 64 * 32;
 constexpr long long kMaxTokens = 1 << 26;  // (pieces are a multiple of 8 long: with many more of them nothing would be left for the last)
-template <typename AT, int W, int E, bool TOP>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
-  constexpr int R = W == 1 ? 4 : 1;                  // rows per workgroup
-  constexpr int GROUPS = W == 1 ? 64 : 128;          // of lanes, whose maxima bound the alternatives from below
-  constexpr int GROUP = 64 * W / GROUPS;
+template <typename AT, int W, int E>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(ScoresArgs a) {
+  constexpr int R = W == 1 ? 4 : 1;  // rows per workgroup
   __shared__ float sums_of[R][W][4];
-  __shared__ float group_of[TOP ? R : 1][TOP ? GROUPS : 1];
-  __shared__ unsigned long long list_of[TOP ? R : 1][TOP ? kCandidates : 1];
+  __shared__ float most_of[W][64];
+  __shared__ unsigned long long list_of[R][W == 1 ? 512 : kCandidates];
   __shared__ int listed_of[R];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, sub = W == 1 ? threadIdx.x >> 6 : 0, thread = wave * 64 + lane;
   const long long item = blockIdx.x * (long long)R + sub;
@@ -153,11 +144,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
   const long long v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
   const float inf = __builtin_inff();
   float x[E];
-  int index[W == 1 ? 1 : E / 8];  // of a lane's eight, from v0 on
   if constexpr (W == 1) {
 #pragma unroll
     for (int k = 0; k < E; ++k) x[k] = k * 64 + lane < v1 ? load_f32(row + k * 64 + lane) : -inf;
-    index[0] = lane;
   } else {
     // Eight neighbours are one load; those that reach past the end of the row are its last eight (there are more than eight), of which the
     // ones that an earlier lane has are left out.
@@ -165,25 +154,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
     Eight<AT> q[E / 8];
 #pragma unroll
     for (int j = 0; j < E / 8; ++j) {
-      index[j] = (j * 64 * W + thread) * 8;
-      const long long at = v0 + index[j];
+      const long long at = v0 + (j * 64 * W + thread) * 8;
       q[j].load(row + (at < a.V - 8 ? at : a.V - 8));
     }
 #pragma unroll
     for (int j = 0; j < E / 8; ++j) {
       float v[8];
       q[j].get(v);
-      if (__any(index[j] + 8 > count)) {
-        const int from = index[j], begin = v0 + from < a.V - 8 ? from : (int)(a.V - 8 - v0);
+      const int from = (j * 64 * W + thread) * 8;
+      if (__any(from + 8 > count)) {
+        const int begin = v0 + from < a.V - 8 ? from : (int)(a.V - 8 - v0);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = begin + k >= from && begin + k < count ? v[k] : -inf;
-        index[j] = begin;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[8 * j + k] = v[k];
     }
   }
-  auto index_of = [&](int k) { return (unsigned)(v0 + (W == 1 ? k * 64 + index[0] : index[k / 8] + k % 8)); };
 
   float most = kLowest;
 #pragma unroll
@@ -197,17 +184,87 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
     w = __builtin_fmaf(t, e, w);
   }
   RowSums sums{m, wave_sum(s), wave_sum(w)};
-  if constexpr (W > 1) {
+  bool finite = sums.s < inf;  // (neither a NaN nor an infinity in the row)
+  float group = most, top = m;
+  if constexpr (W == 1) {
+    if (lane == 0) listed_of[sub] = 0;
+  } else {
+    most_of[wave][lane] = most;
     if (lane == 0) sums_of[0][wave][0] = sums.m, sums_of[0][wave][1] = sums.s, sums_of[0][wave][2] = sums.w;
-    if (TOP) {
-      const float g = group_max<GROUP>(most);
-      if (lane % GROUP == 0) group_of[0][thread / GROUP] = g;
-      if (thread == 0) listed_of[0] = 0;
-    }
+    if (thread == 0) listed_of[0] = 0;
     __syncthreads();
     sums = lane < W ? RowSums{sums_of[0][lane % W][0], sums_of[0][lane % W][1], sums_of[0][lane % W][2]} : RowSums{kLowest, 0.f, 0.f};
-    sums = join_sums(sums);
+    finite = !__any(!(sums.s < inf));
+#pragma unroll
+    for (int o = 0; o < W; ++o) group = __builtin_fmaxf(group, most_of[o][lane]);
+    top = wave_max(group);
   }
+  auto meet = [&]() {
+    if constexpr (W > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  // (where logit k of this lane lies, from v0 on)
+  auto index_of = [&](int k) {
+    if constexpr (W == 1) return (unsigned)(v0 + k * 64 + lane);
+    const long long at = v0 + ((k >> 3) * 64 * W + thread) * 8;
+    return (unsigned)((at < a.V - 8 ? at : a.V - 8) + (k & 7));
+  };
+  unsigned long long* list = list_of[sub];
+  int* listed = &listed_of[sub];
+  int n = 0;
+  float bound = kLowest;
+  // Lists what reaches the bound, in any order.
+  auto make_list = [&]() {
+    unsigned hits = 0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) hits |= x[k] >= bound ? 1u << k : 0u;
+    if (hits) {
+      int at = atomicAdd(listed, __popc(hits));
+      for (; hits && at < kCandidates; hits &= hits - 1, ++at) {
+        const unsigned index = index_of(__ffs(hits) - 1);
+        list[at] = alternative(load_f32(row + index), index);
+      }
+    }
+    meet();
+    n = *(volatile int*)listed;
+  };
+  if (finite) {
+    // A bound from below: the logits are dealt to 16, 32 or 64 groups, no fewer than alternatives are wanted, and every group's maximum reaches the
+    // least of them.  What reaches it is listed (of N groups about N log N), and finds its rank in the list.  (The top_k-th largest of 128 maxima,
+    // found bit by bit, is closer, but takes longer than all the rest: 12 rows of 32768 float32 with 12 alternatives 9.6 us, with this @TOP@.)
+    if (a.top_k <= 32) group = __builtin_fmaxf(group, dpp<0xB1>(group));
+    if (a.top_k <= 16) group = __builtin_fmaxf(group, dpp<0x4E>(group));
+    bound = -wave_max(-group);
+    make_list();
+    if (W > 1 && n > kCandidates) {
+      // Too many: the largest bound that top_k lanes still reach, to within a 4096th of what is in question.
+      float high = top;
+#pragma unroll 1
+      for (int step = 0; step < 12; ++step) {
+        const float mid = 0.5f * bound + 0.5f * high;
+        meet();  // (everyone has read what is written here)
+        if (thread == 0) *listed = 0;
+        meet();
+        const int reach = __popcll(__ballot(most >= mid));
+        if (lane == 0) atomicAdd(listed, reach);
+        meet();
+        if (*(volatile int*)listed >= a.top_k)
+          bound = mid;
+        else
+          high = mid;
+      }
+      meet();
+      if (thread == 0) *listed = 0;
+      meet();
+      make_list();
+    }
+  }
+  // (fewer than wanted, but all that are not minus infinity, are also good)
+  const bool found = finite && n <= kCandidates && (n >= a.top_k || bound == kLowest);
+  if (W > 1 && wave > 0 && found && wave * 64 >= n) return;
+  if constexpr (W > 1) sums = join_sums(sums);
   if (thread == 0) {
     if (a.splits > 1) {
       float* part = a.part + (r * a.splits + split) * 4;
@@ -216,81 +273,139 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
       row_results<AT>(a, r, target, sums);
     }
   }
-  if constexpr (TOP) {
-    const RowNorm norm(sums);
-    unsigned long long* list = list_of[sub];
-    int* listed = &listed_of[sub];
-    bool found = false;
-    if (sums.s > 0.f && sums.s < inf) {
-      // A bound from below: the top_k-th largest of the groups' maxima, found bit by bit from the top (bfloat16 has 16).
-      unsigned low0, low1 = 0;
-      if constexpr (W == 1) {
-        low0 = order_of(most);
-        if (lane == 0) *listed = 0;
-      } else {
-        low0 = order_of(group_of[0][lane]);
-        low1 = order_of(group_of[0][64 + lane]);
+  const RowNorm norm(sums);
+  if (found) {
+    for (int j = thread; j < n; j += 64 * W) {
+      const unsigned long long mine = list[j];
+      int rank = 0;
+#pragma unroll 8
+      for (int o = 0; o < n; ++o) rank += list[o] > mine;
+      if (rank < a.top_k) put_alternative(a, r, split, rank, mine, norm);
+    }
+    // The first ones that are minus infinity: among the first top_k of the row, then, there are as many as are wanted.
+    if (wave == 0)
+      for (long long v = v0; n < a.top_k && v < v1; v += 64) {
+        const bool is = v + lane < v1 && load_f32(row + v + lane) == -inf;
+        const unsigned long long all = __ballot(is);
+        const int rank = n + __popcll(all & ((1ull << lane) - 1));
+        if (is && rank < a.top_k) put_alternative(a, r, split, rank, alternative(-inf, (unsigned)(v + lane)), norm);
+        n += __popcll(all);
       }
-      unsigned bound = 0;
+    return;
+  }
+  // More equal logits than the list holds, or a NaN: the best one of all, and again.  Every lane knows its best one; whose turn it was looks for
+  // its next.  (What a lane holds of another lane's it skips.)
+  meet();  // (the list is read no more)
+  unsigned long long last = ~0ull, mine = 0;
 #pragma unroll 1
-      for (unsigned bit = 0x80000000u; bit > (sizeof(AT) == 2 ? 0x8000u : 0u); bit >>= 1) {
-        const unsigned next = bound | bit;
-        const int over = __popcll(__ballot(low0 >= next)) + (W == 1 ? 0 : __popcll(__ballot(low1 >= next)));
-        if (over >= a.top_k) bound = next;
-      }
-      const float at_least = logit_of((unsigned long long)bound << 32);
-      // What reaches it is listed, in any order, and every listed one finds its rank among them.
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (x[k] >= at_least) {
-          const int at = atomicAdd(listed, 1);
-          if (at < kCandidates) list[at] = alternative(x[k], index_of(k));
-        }
-      if constexpr (W > 1)
+  for (int k = -1; k < a.top_k; ++k) {
+    unsigned long long best = last;
+    if (k >= 0) {
+      best = wave_max(mine);
+      if constexpr (W > 1) {
+        if (lane == 0) list[(k & 1) * W + wave] = best;
         __syncthreads();
-      else
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const int n = *(volatile int*)listed;
-      found = n >= a.top_k && n <= kCandidates;
-      if (found)
-        for (int j = thread; j < n; j += 64 * W) {
-          const unsigned long long mine = list[j];
-          int rank = 0;
-          for (int o = 0; o < n; ++o) rank += list[o] > mine;
-          if (rank < a.top_k) put_alternative(a, r, split, rank, mine, norm);
-        }
+        best = wave_max(list[(k & 1) * W + lane % W]);
+      }
+      if (thread == 0) put_alternative(a, r, split, k, best, norm);
     }
-    if (!found) {
-      // More equal logits than the list holds, fewer finite ones than wanted, a NaN: the best one of all, and again.  Every lane knows its best
-      // one; whose turn it was looks for its next.  (What a lane holds past the end, or of another lane's, is minus infinity at the last indices
-      // of the row: it comes after more real ones than are ever wanted.)
-      if constexpr (W > 1) __syncthreads();  // (the list is read no more)
-      unsigned long long last = ~0ull, mine = 0;
-      auto look = [&]() {
-        mine = 0;
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-          const unsigned long long q = alternative(x[k], index_of(k));
-          const bool real = W == 1 ? k * 64 + lane < v1 : true;
-          if (q < last && q > mine && real) mine = q;
-        }
-      };
-      look();
-#pragma unroll 1
-      for (int k = 0; k < a.top_k; ++k) {
-        unsigned long long best = wave_max(mine);
-        if constexpr (W > 1) {
-          if (lane == 0) list[(k & 1) * W + wave] = best;
-          __syncthreads();
-          best = wave_max(list[(k & 1) * W + lane % W]);
-        }
-        if (thread == 0) put_alternative(a, r, split, k, best, norm);
-        if (mine == best) {
-          last = best;
-          look();
+    if (k < 0 || mine == best) {
+      last = best;
+      mine = 0;
+#pragma unroll 8
+      for (int j = 0; j < E; ++j) {
+        const long long at = W == 1 ? v0 + j * 64 + lane : v0 + ((j >> 3) * 64 * W + thread) * 8 + (j & 7);
+        if (at < v1) {
+          const unsigned long long q = alternative(load_f32(row + at), (unsigned)at);
+          if (q < last && q > mine) mine = q;
         }
       }
     }
+  }
+}
+
+// Sums without alternatives, read as they come: W wavefronts per row or piece of one (W = 1: four rows per workgroup), U times eight logits per
+// lane in flight.  The wavefront's reference, which stands for the maximum, is that of its first 512 logits: sums relative to it are as good as long as they
+// stay finite.  Where they do not, or a product of minus infinity with 0 is NaN, or all that the reference is made of may be less than kNothing, which
+// stands for what is not there, the wavefront takes its sums again, with the true maximum and t cut.
+template <typename AT, int W, bool ENTROPY>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
+  constexpr int R = W == 1 ? 4 : 1, U = 4;
+  __shared__ float sums_of[W][4];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, thread = wave * 64 + lane;
+  const long long item = blockIdx.x * (long long)R + (W == 1 ? threadIdx.x >> 6 : 0);
+  if (W == 1 && item >= a.rows) return;
+  const long long r = a.splits > 1 ? (unsigned)item / (unsigned)a.splits : item;
+  const int split = a.splits > 1 ? (int)(item - r * a.splits) : 0;
+  const long long target = a.targets ? a.targets[r] : 0;
+  if (target < 0) {
+    if (a.splits == 1) no_row(a, r, thread, 64 * W);
+    return;
+  }
+  const AT* row = (const AT*)a.logits + r * a.ld;
+  const long long v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
+  RowSums sums{kLowest, 0.f, 0.f};
+  const bool vector = a.V >= 8;
+#pragma unroll 1
+  for (long long from = v0; vector && from + wave * 512 < v1; from += 512ll * W * U) {
+    Eight<AT> q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const long long at = from + (j * 64 * W + thread) * 8;
+      q[j].load(row + (at < a.V - 8 ? at : a.V - 8));
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const long long at = from + (j * 64 * W + wave * 64) * 8;  // (the wavefront's first)
+      if (at >= v1) break;
+      float v[8];
+      q[j].get(v);
+      if (at + 512 > v1) {  // see above: the last eight of the row, those of an earlier lane left out
+        const long long mine = at + lane * 8, begin = mine < a.V - 8 ? mine : a.V - 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = begin + k >= mine && begin + k < v1 ? v[k] : kNothing;
+      }
+      if (j == 0 && from == v0) {
+        float most = kLowest;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = __builtin_fmaxf(most, v[k]);
+        sums.m = wave_max(most);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float t = (v[k] - sums.m) * kLog2E, e = __builtin_amdgcn_exp2f(t);
+        sums.s += e;
+        if (ENTROPY) sums.w = __builtin_fmaf(t, e, sums.w);
+      }
+    }
+  }
+  if (__any(!(sums.s + sums.w < __builtin_inff()) || sums.m <= kNothing)) {
+    float most = kLowest;
+    for (long long v = v0 + thread * 8; v < v1; v += 512 * W)
+      for (int k = 0; k < 8 && v + k < v1; ++k) most = __builtin_fmaxf(most, load_f32(row + v + k));
+    sums = {wave_max(most), 0.f, 0.f};
+    for (long long v = v0 + thread * 8; v < v1; v += 512 * W)
+      for (int k = 0; k < 8 && v + k < v1; ++k) {
+        const float t = __builtin_elementwise_maximum((load_f32(row + v + k) - sums.m) * kLog2E, kNoPower), e = __builtin_amdgcn_exp2f(t);
+        sums.s += e;
+        sums.w = __builtin_fmaf(t, e, sums.w);
+      }
+  }
+  sums.s = wave_sum(sums.s);
+  if (ENTROPY) sums.w = wave_sum(sums.w);
+  if constexpr (W > 1) {
+    if (lane == 0) sums_of[wave][0] = sums.m, sums_of[wave][1] = sums.s, sums_of[wave][2] = sums.w;
+    __syncthreads();
+    if (wave > 0) return;
+    sums = lane < W ? RowSums{sums_of[lane % W][0], sums_of[lane % W][1], sums_of[lane % W][2]} : RowSums{kLowest, 0.f, 0.f};
+    sums = join_sums(sums);
+  }
+  if (thread > 0) return;
+  if (a.splits > 1) {
+    float* part = a.part + (r * a.splits + split) * 4;
+    part[0] = sums.m, part[1] = sums.s, part[2] = sums.w;
+  } else {
+    row_results<AT>(a, r, target, sums);
   }
 }
 

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
 #pragma unroll
     for (int j = 0; j < G; ++j) {
       drop<AT, ADD>(x[j], r[j], philox((unsigned long long)(g0 + 256 * j), offset, a.key0, a.key1), a.threshold, a.scale);
-      x[j].store((AT*)a.y + (g0 + 256 * j) * 8);
+      x[j].store_streamed((AT*)a.y + (g0 + 256 * j) * 8);
     }
     return;
   }

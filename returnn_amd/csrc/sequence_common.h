@@ -32,6 +32,10 @@ struct Eight {
 #pragma unroll
     for (int j = 0; j < kWords; ++j) ((seq_u32x4_any*)p)[j] = w[j];
   }
+  __device__ __forceinline__ void store_streamed(AT* p) const {  // of what is not read again before much else is
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) __builtin_nontemporal_store(w[j], (seq_u32x4_any*)p + j);
+  }
   __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
     for (int k = 0; k < 8; ++k)

@@ -469,7 +469,8 @@ template <typename AT, bool ROW>
 __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {
   constexpr int THREADS = ROW ? 64 : 256, N = ROW ? 1 : kBwdPiece / (256 * 8);
   const int thread = ROW ? threadIdx.x & 63 : threadIdx.x;
-  const long long item = ROW ? blockIdx.x * 4ll + (threadIdx.x >> 6) : blockIdx.x;
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const long long item = ROW ? block * 4ll + (threadIdx.x >> 6) : block;
   if (ROW && item >= a.rows) return;
   const long long r = ROW ? item : (unsigned)item / (unsigned)a.splits, v0 = ROW ? 0 : (item - r * a.splits) * kBwdPiece;
   const long long v1 = ROW ? a.V : (v0 + kBwdPiece < a.V ? v0 + kBwdPiece : a.V);
@@ -510,7 +511,7 @@ __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {
           }
         }
         q[j].set(v);
-        q[j].store(D + at);
+        q[j].store_streamed(D + at);
       }
     } else {
 #pragma unroll 1

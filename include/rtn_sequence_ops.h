@@ -39,7 +39,7 @@ const char* rtn_sequence_last_error(void);
  *       state stays.  direction -1: from each sequence's last frame to its first.
  * Y     [T,B,n] in X's type; cN [B,n] float32, the state after the last frame visited
  * saved what the gradient wants to know (rtn_gated_recurrence_saved_bytes), or NULL
- * The state is float32 throughout, whatever the type.
+ * The state is float32 throughout, whatever the type.  T up to 2^30, n up to 2^26.
  */
 size_t rtn_gated_recurrence_saved_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype);
 size_t rtn_gated_recurrence_fwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype);

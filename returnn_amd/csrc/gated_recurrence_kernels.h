@@ -4,14 +4,24 @@
 //
 // Gradient, with g_t the error of c_t:  g_t = dy_t o_t + f_{t+1} g_{t+1},  dz = g i (1 - z^2),  di = g z i (1 - i),
 // df = g c_{t-1} f (1 - f),  do = dy c o (1 - o)  (of the activated gates), dc0 = f_0 g_0.
+//
+// Any run of frames turns the state before it, c, into A c + S: A is the product of its forget gates, S what it would leave of a state of 0.  Runs
+// after one another are joined by (A2 A1, A2 S1 + S2).  So a wavefront takes F frames of 64 lanes' channels, whose gates it holds in registers
+// after reading them once; the W wavefronts of a workgroup take runs of F frames that follow each other and hand (A, S) over through LDS; and the
+// workgroup goes on to the next W F frames, whose gates were asked for before the hand-over.  The gradient runs from the last frame to the first with
+// (A, Q) for the errors, and the states inside a run are computed again from those that the forward pass leaves every kSavedFrames frames.
+// Where sequences and channels are too few to fill the device, the frames are cut into segments: a first kernel leaves (A, S) or (A, Q) of every
+// segment, and the second starts each from those before it, joined in order.  All sums are in a fixed order.
 #pragma once
+
+#include <type_traits>
 
 #include "gate_functions.h"
 #include "sequence_common.h"
 
 namespace rtn {
 
-constexpr int kRecurrenceFrames = 16;  // frames from one saved state to the next
+constexpr int kSavedFrames = 16;  // frames from one saved state to the next
 
 struct RecurrenceArgs {
   const void* X;
@@ -20,7 +30,7 @@ struct RecurrenceArgs {
   const int64_t* lens;
   void* Y;
   float* cN;
-  float* saved;  // [chunks][B][n] the state before every kRecurrenceFrames-th frame visited
+  float* saved;  // [ceil(T/kSavedFrames)][B][n] the state before every kSavedFrames-th frame visited
   const void* DY;
   long long ldDY;
   const float* DcN;
@@ -28,75 +38,445 @@ struct RecurrenceArgs {
   float* Dc0;
   long long T;
   int B, n, back;
+  int strips;         // of 64 lanes' channels, in n
+  unsigned chains;    // strips times sequences
+  long long segment;  // frames of a segment
+  int segments;
+  float* runs;        // [segments][chains][64 lanes][VEC][2] A and S, or A and Q, of the segments
 };
 
-// One thread per sequence and channel, frame by frame.
-template <typename AT>
-__global__ void k_recurrence_fwd(RecurrenceArgs a) {
-  const long long id = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-  if (id >= (long long)a.B * a.n) return;
-  const int b = (int)(id / a.n), k = (int)(id % a.n);
-  const long long frames = frames_of(a.lens, b, a.T);
-  float c = a.c0 ? a.c0[id] : 0.f;
-  for (long long s = 0; s < a.T; ++s) {
-    const long long t = a.back ? a.T - 1 - s : s;
-    if (a.saved && s % kRecurrenceFrames == 0) a.saved[s / kRecurrenceFrames * a.B * a.n + id] = c;
-    float y = 0.f;
-    if (t < frames) {
-      const AT* x = (const AT*)a.X + (t * a.B + b) * a.ldX + k;
-      const float z = Act<AT>::tanh(load_f32(x)), i = Act<AT>::sigmoid(load_f32(x + a.n)), f = Act<AT>::sigmoid(load_f32(x + 2 * (long long)a.n)),
-                  o = Act<AT>::sigmoid(load_f32(x + 3 * (long long)a.n));
-      c = __builtin_fmaf(f, c, i * z);
-      y = o * c;
-    }
-    store_f32((AT*)a.Y + (t * a.B + b) * a.n + k, y);
+// VEC neighbouring channels of a lane: one load, at any element's address.
+template <typename AT, int VEC>
+struct Channels;
+template <>
+struct Channels<float, 1> {
+  typedef unsigned Raw;
+  static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, r); }
+  static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned, v[0]); }
+};
+template <>
+struct Channels<__bf16, 1> {
+  typedef unsigned short Raw;
+  static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b16(row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b16(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, (unsigned)r << 16); }
+  static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned short, (__bf16)v[0]); }
+};
+template <>
+struct Channels<__bf16, 2> {
+  typedef unsigned Raw;
+  static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void get(Raw r, float (&v)[2]) {
+    v[0] = __builtin_bit_cast(float, r << 16);
+    v[1] = __builtin_bit_cast(float, r & 0xFFFF0000u);
   }
-  a.cN[id] = c;
+  static __device__ __forceinline__ Raw set(const float (&v)[2]) {
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+    const bf16x2 pair = {(__bf16)v[0], (__bf16)v[1]};
+    return __builtin_bit_cast(unsigned, pair);
+  }
+};
+
+// Rows of one sequence in an array of frames: frame t begins `frame` bytes after frame t - 1, a row has `bytes`.
+struct Rows {
+  char* base;
+  long long frame;
+  int bytes;
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int t) const { return __builtin_amdgcn_make_buffer_rsrc(base + t * frame, 0, bytes, 0x00020000); }
+};
+
+// What a workgroup works on: one sequence, 64 lanes' channels, a segment of the frames.  Frames are counted in the order of the recurrence: step s is
+// frame s, or T - 1 - s.
+template <typename AT, int VEC>
+struct Chain {
+  typedef Channels<AT, VEC> C;
+  typedef typename C::Raw Raw;
+  int b, lane;
+  unsigned k;        // the lane's first channel; lanes past the last repeat the last ones
+  unsigned at[4];    // where it is in a row of gates, in bytes
+  bool active;       // has channels of its own
+  int low, high;     // steps inside the sequence
+  int first, stride;  // frame of step 0, of the next one
+  __device__ __forceinline__ Chain(const RecurrenceArgs& a, unsigned chain) {
+    lane = threadIdx.x & 63;
+    b = chain / a.strips;
+    const unsigned own = (chain - b * a.strips) * 64 * VEC + lane * VEC;
+    active = own < (unsigned)a.n;
+    k = own + VEC <= (unsigned)a.n ? own : a.n - VEC;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) at[g] = (k + g * (unsigned)a.n) * (unsigned)sizeof(AT);
+    const int T = (int)a.T, frames = (int)frames_of(a.lens, b, a.T);
+    low = a.back ? T - frames : 0;
+    high = a.back ? T : frames;
+    first = a.back ? T - 1 : 0;
+    stride = a.back ? -1 : 1;
+  }
+  __device__ __forceinline__ bool inside(int s) const { return s >= low && s < high; }
+  __device__ __forceinline__ int frame(int s) const { return first + stride * s; }
+  // the frame of a step that is read in its place: itself, or one inside (there is one where any step near it is inside)
+  __device__ __forceinline__ int frame_inside(int s) const {
+    s = s < low ? low : s;
+    return frame(s < high ? s : high - 1);
+  }
+  __device__ __forceinline__ bool any_inside(int s, int count) const { return s < high && s + count > low && low < high; }
+  __device__ __forceinline__ bool all_inside(int s, int count) const { return s >= low && s + count <= high; }
+  static __device__ __forceinline__ Rows rows(const RecurrenceArgs& a, const void* p, int b, long long ld, int width) {
+    return {(char*)p + b * ld * (long long)sizeof(AT), a.B * ld * (long long)sizeof(AT), width * (int)sizeof(AT)};
+  }
+};
+
+// (A, S) of a lane's channels.
+template <int VEC>
+struct Run {
+  float a[VEC], s[VEC];
+  static __device__ __forceinline__ Run none() {
+    Run r;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) r.a[v] = 1.f, r.s[v] = 0.f;
+    return r;
+  }
+  __device__ __forceinline__ void then(const Run& next) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s[v] = __builtin_fmaf(next.a[v], s[v], next.s[v]), a[v] *= next.a[v];
+  }
+  __device__ __forceinline__ void apply(float (&c)[VEC]) const {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) c[v] = __builtin_fmaf(a[v], c[v], s[v]);
+  }
+};
+
+// The state (or error) with which segment `segment` starts, from that of the first and the segments' runs; FORWARD: those before it, else those after it.
+// All wavefronts of the workgroup call this: each joins a share of the runs.
+template <int VEC, int W, bool FORWARD>
+__device__ __forceinline__ void start_of_segment(const RecurrenceArgs& a, unsigned chain, int segment, int wave, int lane, Run<VEC> (*shared)[64], float (&c)[VEC]) {
+  const int count = FORWARD ? segment : a.segments - 1 - segment;
+  if (W == 1 || count == 0) return;
+  const int share = (count + W - 1) / W;
+  Run<VEC> mine = Run<VEC>::none();
+#pragma unroll 4
+  for (int j = wave * share; j < (wave + 1) * share && j < count; ++j) {
+    const int at = FORWARD ? j : a.segments - 1 - j;
+    mine.then(((const Run<VEC>*)a.runs)[((size_t)at * a.chains + chain) * 64 + lane]);
+  }
+  shared[wave][lane] = mine;
+  __syncthreads();
+#pragma unroll 4
+  for (int j = 0; j < W; ++j) shared[j][lane].apply(c);
+  __syncthreads();
 }
 
-template <typename AT>
-__global__ void k_recurrence_bwd(RecurrenceArgs a) {
-  const long long id = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-  if (id >= (long long)a.B * a.n) return;
-  const int b = (int)(id / a.n), k = (int)(id % a.n);
-  const long long frames = frames_of(a.lens, b, a.T), n = a.n;
-  float g = a.DcN ? a.DcN[id] : 0.f;
-  for (long long s0 = ((a.T + kRecurrenceFrames - 1) / kRecurrenceFrames - 1) * kRecurrenceFrames; s0 >= 0; s0 -= kRecurrenceFrames) {
-    float before[kRecurrenceFrames], c = a.saved[s0 / kRecurrenceFrames * a.B * n + id];
+// ---- forward ----
+// W wavefronts, F frames each.  handed: the runs of the wavefronts, and in [W] the state that the next turn starts from, which the last wavefront
+// leaves there; both twice, so that one barrier a turn is enough.
+template <typename AT, int VEC, int F, int W>
+__global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
+  typedef Chain<AT, VEC> C;
+  __shared__ Run<VEC> handed[2][W + 1][64];
+  const unsigned chain = blockIdx.x % a.chains;
+  const int segment = blockIdx.x / a.chains, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const C q(a, chain);
+  const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
+  const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), Y = C::rows(a, a.Y, q.b, a.n, a.n);
+  const size_t own = (size_t)q.b * a.n + q.k;
+
+  typename C::Raw raw[F][4];
+  auto ask = [&](int j, int s) {
+    const __amdgpu_buffer_rsrc_t row = X.at(q.frame_inside(s));
 #pragma unroll
-    for (int j = 0; j < kRecurrenceFrames; ++j) {
-      const long long s = s0 + j, t = a.back ? a.T - 1 - s : s;
-      before[j] = c;
-      if (s < a.T && t < frames) {
-        const AT* x = (const AT*)a.X + (t * a.B + b) * a.ldX + k;
-        c = __builtin_fmaf(Act<AT>::sigmoid(load_f32(x + 2 * n)), c, Act<AT>::sigmoid(load_f32(x + n)) * Act<AT>::tanh(load_f32(x)));
+    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(row, q.at[g]);
+  };
+  if (q.any_inside(begin + wave * F, F)) {
+#pragma unroll
+    for (int j = 0; j < F; ++j) ask(j, begin + wave * F + j);
+  }
+  float c[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) c[v] = a.c0 ? a.c0[own + v] : 0.f;
+  start_of_segment<VEC, W, true>(a, chain, segment, wave, q.lane, handed[0], c);
+
+  int turn = 0;
+#pragma unroll 1
+  for (int from = begin; from < end; from += F * W, turn ^= 1) {
+    const int s0 = from + wave * F, next = s0 + F * W;
+    const bool all = q.all_inside(s0, F), more = from + F * W < end && q.any_inside(next, F);
+    float A[F][VEC], S[F][VEC], o[F][VEC];  // of the run up to frame j
+    auto activate = [&](auto all) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        float z[VEC], i[VEC], f[VEC];
+        C::C::get(raw[j][0], z);
+        C::C::get(raw[j][1], i);
+        C::C::get(raw[j][2], f);
+        C::C::get(raw[j][3], o[j]);
+        const bool in = all || q.inside(s0 + j);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float fv = in ? Act<AT>::sigmoid(f[v]) : 1.f, iz = in ? Act<AT>::sigmoid(i[v]) * Act<AT>::tanh(z[v]) : 0.f;
+          o[j][v] = Act<AT>::sigmoid(o[j][v]);
+          A[j][v] = j ? A[j - 1][v] * fv : fv;
+          S[j][v] = j ? __builtin_fmaf(fv, S[j - 1][v], iz) : iz;
+        }
+        if (more) ask(j, next + j);  // (as soon as the registers are free: the loads go on while the gates are worked on)
+      }
+    };
+    if (all)
+      activate(std::true_type());
+    else
+      activate(std::false_type());
+    Run<VEC> run;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) run.a[v] = A[F - 1][v], run.s[v] = S[F - 1][v];
+    if constexpr (W > 1) {
+      handed[turn][wave][q.lane] = run;
+      __syncthreads();
+      if (from > begin) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) c[v] = handed[turn][W][q.lane].s[v];
+      }
+#pragma unroll 4
+      for (int j = 0; j < wave; ++j) handed[turn][j][q.lane].apply(c);
+    }
+    if (a.saved && q.active && s0 % kSavedFrames == 0 && s0 < (int)a.T) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) a.saved[(size_t)(s0 / kSavedFrames) * a.B * a.n + own + v] = c[v];
+    }
+    if (q.active) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        if (s0 + j >= end) break;
+        float y[VEC];
+        const bool in = all || q.inside(s0 + j);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) y[v] = in ? o[j][v] * __builtin_fmaf(A[j][v], c[v], S[j][v]) : 0.f;
+        C::C::store(Y.at(q.frame(s0 + j)), q.at[0], C::C::set(y));
       }
     }
+    if (W == 1 || wave == W - 1) {
+      run.apply(c);
+      if constexpr (W > 1) {
 #pragma unroll
-    for (int j = kRecurrenceFrames - 1; j >= 0; --j) {
-      const long long s = s0 + j, t = a.back ? a.T - 1 - s : s;
-      if (s >= a.T) continue;
-      float dz = 0.f, di = 0.f, df = 0.f, d_o = 0.f;
-      if (t < frames) {
-        const AT* x = (const AT*)a.X + (t * a.B + b) * a.ldX + k;
-        const float z = Act<AT>::tanh(load_f32(x)), i = Act<AT>::sigmoid(load_f32(x + n)), f = Act<AT>::sigmoid(load_f32(x + 2 * n)), o = Act<AT>::sigmoid(load_f32(x + 3 * n));
-        const float dy = load_f32((const AT*)a.DY + (t * a.B + b) * a.ldDY + k);
-        const float after = __builtin_fmaf(f, before[j], i * z);
-        g = __builtin_fmaf(dy, o, g);
-        dz = g * i * (1.f - z * z);
-        di = g * z * i * (1.f - i);
-        df = g * before[j] * f * (1.f - f);
-        d_o = dy * after * o * (1.f - o);
-        g *= f;
+        for (int v = 0; v < VEC; ++v) run.s[v] = c[v];
+        handed[turn ^ 1][W][q.lane] = run;
       }
-      AT* d = (AT*)a.DX + (t * a.B + b) * 4 * n + k;
-      store_f32(d, dz);
-      store_f32(d + n, di);
-      store_f32(d + 2 * n, df);
-      store_f32(d + 3 * n, d_o);
     }
   }
-  a.Dc0[id] = g;
+  if (q.active && wave == W - 1 && segment == a.segments - 1) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a.cN[own + v] = c[v];
+  }
+}
+
+// ---- gradient ----
+template <typename AT, int VEC, int F, int W>
+__global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
+  typedef Chain<AT, VEC> C;
+  constexpr int GROUP = kSavedFrames / F;  // wavefronts from one saved state to the next
+  static_assert(W == 1 || W % GROUP == 0, "saved states lie where wavefronts begin");
+  __shared__ Run<VEC> handed[2][W + 1][64];
+  __shared__ Run<VEC> states[2][W][64];
+  const unsigned chain = blockIdx.x % a.chains;
+  const int segment = a.segments - 1 - (int)(blockIdx.x / a.chains), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const C q(a, chain);
+  const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
+  const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), DY = C::rows(a, a.DY, q.b, a.ldDY, a.n), DX = C::rows(a, a.DX, q.b, 4 * (long long)a.n, 4 * a.n);
+  const size_t own = (size_t)q.b * a.n + q.k;
+
+  typename C::Raw raw[F][5];
+  float before[VEC];  // the saved state of the wavefront's group
+  auto ask = [&](int j, int s) {
+    const int t = q.frame_inside(s);
+    const __amdgpu_buffer_rsrc_t row = X.at(t);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(row, q.at[g]);
+    raw[j][4] = C::C::load(DY.at(t), q.at[0]);
+  };
+  auto ask_state = [&](int s0) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) before[v] = s0 < (int)a.T ? a.saved[(size_t)(s0 / kSavedFrames) * a.B * a.n + own + v] : 0.f;
+  };
+  const int last = begin + ((end - begin + F * W - 1) / (F * W) - 1) * (F * W);
+  if (last >= begin) {
+    if (q.any_inside(last + wave * F, F)) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) ask(j, last + wave * F + j);
+    }
+    ask_state(last + wave * F);
+  }
+  float g[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) g[v] = a.DcN ? a.DcN[own + v] : 0.f;
+  start_of_segment<VEC, W, false>(a, chain, segment, wave, q.lane, handed[0], g);
+
+  int turn = 0;
+#pragma unroll 1
+  for (int from = last; from >= begin; from -= F * W, turn ^= 1) {
+    const int s0 = from + wave * F, next = s0 - F * W;
+    const bool all = q.all_inside(s0, F), more = from > begin && q.any_inside(next, F);
+    float z[F][VEC], i[F][VEC], f[F][VEC], o[F][VEC], e[F][VEC], c[VEC];
+    auto activate = [&](auto all) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        C::C::get(raw[j][0], z[j]);
+        C::C::get(raw[j][1], i[j]);
+        C::C::get(raw[j][2], f[j]);
+        C::C::get(raw[j][3], o[j]);
+        C::C::get(raw[j][4], e[j]);
+        const bool in = all || q.inside(s0 + j);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          z[j][v] = in ? Act<AT>::tanh(z[j][v]) : 0.f;
+          i[j][v] = in ? Act<AT>::sigmoid(i[j][v]) : 0.f;
+          f[j][v] = in ? Act<AT>::sigmoid(f[j][v]) : 1.f;
+          o[j][v] = in ? Act<AT>::sigmoid(o[j][v]) : 0.f;
+          e[j][v] = in ? e[j][v] : 0.f;
+        }
+        if (more) ask(j, next + j);
+      }
+    };
+    if (all)
+      activate(std::true_type());
+    else
+      activate(std::false_type());
+    Run<VEC> forth = Run<VEC>::none(), back = forth;
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        forth.a[v] *= f[j][v];
+        forth.s[v] = __builtin_fmaf(f[j][v], forth.s[v], i[j][v] * z[j][v]);
+        const int l = F - 1 - j;
+        back.s[v] = f[l][v] * __builtin_fmaf(e[l][v], o[l][v], back.s[v]);
+      }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) back.a[v] = forth.a[v], c[v] = before[v];
+    if (from > begin) ask_state(next);
+    if constexpr (W > 1) {
+      handed[turn][wave][q.lane] = back;
+      states[turn][wave][q.lane] = forth;
+      __syncthreads();
+      if (from < last) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) g[v] = handed[turn][W][q.lane].s[v];
+      }
+#pragma unroll 1
+      for (int j = wave / GROUP * GROUP; j < wave; ++j) states[turn][j][q.lane].apply(c);
+#pragma unroll 4
+      for (int j = W - 1; j > wave; --j) handed[turn][j][q.lane].apply(g);
+    }
+    if (wave == 0) {  // the error that the turn before this one starts from
+      Run<VEC> left;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) left.a[v] = 0.f, left.s[v] = g[v];
+      left.then(back);
+      if constexpr (W > 1) {
+        handed[turn ^ 1][W][q.lane] = left;
+      }
+      if (q.active && from == begin && segment == 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) a.Dc0[own + v] = left.s[v];
+      }
+    }
+    if (q.active) {
+      float states_before[F + 1][VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        states_before[0][v] = c[v];
+#pragma unroll
+        for (int j = 0; j < F; ++j) states_before[j + 1][v] = __builtin_fmaf(f[j][v], states_before[j][v], i[j][v] * z[j][v]);
+      }
+      auto write = [&](auto all) {
+#pragma unroll
+        for (int j = F - 1; j >= 0; --j) {
+          const bool in = all || q.inside(s0 + j);
+          float dz[VEC], di[VEC], df[VEC], d_o[VEC];
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float zv = z[j][v], iv = i[j][v], fv = f[j][v], ov = o[j][v], eo = e[j][v] * ov;
+            const float total = g[v] + eo, gi = total * iv, gf = total * fv;
+            dz[v] = in ? gi * __builtin_fmaf(-zv, zv, 1.f) : 0.f;
+            di[v] = in ? gi * zv * (1.f - iv) : 0.f;
+            df[v] = in ? gf * states_before[j][v] * (1.f - fv) : 0.f;
+            d_o[v] = in ? eo * states_before[j + 1][v] * (1.f - ov) : 0.f;
+            g[v] = in ? gf : g[v];
+          }
+          if (!all && s0 + j >= end) continue;
+          const __amdgpu_buffer_rsrc_t row = DX.at(q.frame(s0 + j));
+          C::C::store(row, q.at[0], C::C::set(dz));
+          C::C::store(row, q.at[1], C::C::set(di));
+          C::C::store(row, q.at[2], C::C::set(df));
+          C::C::store(row, q.at[3], C::C::set(d_o));
+        }
+      };
+      if (all)
+        write(std::true_type());
+      else
+        write(std::false_type());
+    }
+  }
+  if (last < begin && q.active && wave == 0) {  // no frames at all
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a.Dc0[own + v] = g[v];
+  }
+}
+
+// ---- the runs of segments: (A, S), or (A, Q) of the errors ----
+// A wavefront takes a share of the segment's frames that follow each other, F at a time.
+template <typename AT, int VEC, int F, int W, bool FORWARD>
+__global__ __launch_bounds__(64 * W) void k_recurrence_runs(RecurrenceArgs a) {
+  typedef Chain<AT, VEC> C;
+  __shared__ Run<VEC> handed[W][64];
+  const unsigned chain = blockIdx.x % a.chains;
+  const int segment = (int)(blockIdx.x / a.chains) + (FORWARD ? 0 : 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (the last one's, or the first one's, nobody needs)
+  const C q(a, chain);
+  const int share = (int)a.segment / W, begin = segment * (int)a.segment + wave * share;
+  const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), DY = C::rows(a, a.DY, q.b, a.ldDY, a.n);
+  Run<VEC> run = Run<VEC>::none();
+#pragma unroll 1
+  for (int k = 0; k < share; k += F) {
+    const int s0 = FORWARD ? begin + k : begin + share - F - k;
+    if (!q.any_inside(s0, F)) continue;  // (frames outside the sequence change nothing)
+    typename C::Raw raw[F][3];
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      const int t = q.frame_inside(s0 + j);
+      const __amdgpu_buffer_rsrc_t row = X.at(t);
+      raw[j][0] = C::C::load(row, FORWARD ? q.at[0] : q.at[3]);
+      raw[j][1] = FORWARD ? C::C::load(row, q.at[1]) : C::C::load(DY.at(t), q.at[0]);
+      raw[j][2] = C::C::load(row, q.at[2]);
+    }
+    auto add = [&](auto all) {
+#pragma unroll
+      for (int l = 0; l < F; ++l) {
+        const int j = FORWARD ? l : F - 1 - l;
+        float p[VEC], r[VEC], f[VEC];
+        C::C::get(raw[j][0], p);
+        C::C::get(raw[j][1], r);
+        C::C::get(raw[j][2], f);
+        const bool in = all || q.inside(s0 + j);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float fv = in ? Act<AT>::sigmoid(f[v]) : 1.f;
+          const float add = FORWARD ? Act<AT>::sigmoid(r[v]) * Act<AT>::tanh(p[v]) : r[v] * Act<AT>::sigmoid(p[v]);
+          run.a[v] *= fv;
+          run.s[v] = FORWARD ? __builtin_fmaf(fv, run.s[v], in ? add : 0.f) : fv * (run.s[v] + (in ? add : 0.f));
+        }
+      }
+    };
+    if (q.all_inside(s0, F))
+      add(std::true_type());
+    else
+      add(std::false_type());
+  }
+  handed[wave][q.lane] = run;
+  __syncthreads();
+  if (wave > 0) return;
+  Run<VEC> all = Run<VEC>::none();
+#pragma unroll
+  for (int j = 0; j < W; ++j) all.then(handed[FORWARD ? j : W - 1 - j][q.lane]);
+  ((Run<VEC>*)a.runs)[((size_t)segment * a.chains + chain) * 64 + q.lane] = all;
 }
 
 }  // namespace rtn

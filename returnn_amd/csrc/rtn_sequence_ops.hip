@@ -58,11 +58,60 @@ void with_bool(bool v, F f) {
 }
 
 // ---- gated recurrence ---------------------------------------------------------------------------------------------
-int64_t recurrence_chunks(int64_t T) { return (T + kRecurrenceFrames - 1) / kRecurrenceFrames; }
+// Frames that a wavefront holds at once, forward and in the gradient: as many as leave 16 wavefronts their registers.
+template <typename AT>
+constexpr int kForwardFrames = sizeof(AT) == 2 ? 8 : 4;
+constexpr int kGradientFrames = 4;
+int forward_frames(int dtype) { return dtype == RTN_DTYPE_BF16 ? kForwardFrames<__bf16> : kForwardFrames<float>; }
+
+constexpr int64_t kMaxFrames = 1 << 30, kMaxChannels = 1 << 26;  // (steps are 32-bit numbers, and so is a place in a row, in bytes)
+
+struct RecurrencePlan {
+  int vec, waves, strips, segments;
+  int64_t chains, segment;
+};
+// Wavefronts: one where it takes all frames by itself, four where they take all frames or the chains fill the device, else 16.  Segments: where fewer
+// than 128 chains leave most of the device idle, as many as make 512 workgroups of at least one turn, from six turns on.
+RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, int frames) {
+  RecurrencePlan p;
+  p.vec = dtype == RTN_DTYPE_BF16 && n > 1 ? 2 : 1;
+  p.strips = (n + 64 * p.vec - 1) / (64 * p.vec);
+  p.chains = (int64_t)p.strips * B;
+  p.waves = T <= frames ? 1 : (T <= 4 * frames || p.chains >= 2048 ? 4 : 16);
+  const int64_t turn = (int64_t)p.waves * frames, turns = std::max<int64_t>(1, (T + turn - 1) / turn);
+  int64_t segments = 1;
+  if (p.waves == 16 && p.chains < 128 && turns >= 6) segments = std::min<int64_t>(turns, (512 + p.chains - 1) / p.chains);
+  const int64_t each = (turns + segments - 1) / segments;
+  p.segment = each * turn;
+  p.segments = (int)((turns + each - 1) / each);
+  return p;
+}
+size_t recurrence_runs_bytes(const RecurrencePlan& p) { return p.segments > 1 ? (size_t)p.segments * (size_t)p.chains * 64 * p.vec * 8 : 0; }
+
+// Calls f with a value of the element type and the number of channels per lane and of wavefronts as types.
+template <int N>
+using Count = std::integral_constant<int, N>;
+template <typename F>
+void with_recurrence(int dtype, const RecurrencePlan& p, F f) {
+  auto waves = [&](auto type, auto vec) {
+    if (p.waves == 1)
+      f(type, vec, Count<1>());
+    else if (p.waves == 4)
+      f(type, vec, Count<4>());
+    else
+      f(type, vec, Count<16>());
+  };
+  if (dtype == RTN_DTYPE_F32)
+    waves(0.f, Count<1>());
+  else if (p.vec == 2)
+    waves((__bf16)0.f, Count<2>());
+  else
+    waves((__bf16)0.f, Count<1>());
+}
 
 // The checks that both directions share; `ld` is set where it was left out.
 int recurrence_check(const char* what, const void* X, int64_t* ldX, const float* c0, const int64_t* lens, int64_t T, int32_t B, int32_t n, int32_t dtype, int32_t direction) {
-  if (T < 0 || B < 0 || n < 0) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d n=%d", what, (long long)T, B, n);
+  if (T < 0 || B < 0 || n < 0 || T > kMaxFrames || n > kMaxChannels) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d n=%d", what, (long long)T, B, n);
   if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
   if (direction != 1 && direction != -1) return fail(RTN_ERR_RANGE, "%s: direction must be 1 or -1, got %d", what, direction);
   if (!*ldX) *ldX = 4 * (int64_t)n;
@@ -83,30 +132,44 @@ int rtn_sequence_ops_abi_version(void) { return 1; }
 const char* rtn_sequence_last_error(void) { return g_last_error.c_str(); }
 
 size_t rtn_gated_recurrence_saved_bytes(int64_t T, int32_t B, int32_t n, int32_t) {
-  return T <= 0 || B <= 0 || n <= 0 ? 0 : (size_t)recurrence_chunks(T) * (size_t)B * (size_t)n * 4;
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : (size_t)((T + kSavedFrames - 1) / kSavedFrames) * (size_t)B * (size_t)n * 4;
 }
-size_t rtn_gated_recurrence_fwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
-size_t rtn_gated_recurrence_bwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
+size_t rtn_gated_recurrence_fwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype) {
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, forward_frames(dtype)));
+}
+size_t rtn_gated_recurrence_bwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype) {
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, kGradientFrames));
+}
 
 int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, void* Y, float* cN, void* saved, int64_t T, int32_t B, int32_t n,
-                             int32_t dtype, int32_t direction, void*, size_t, void* hip_stream) {
+                             int32_t dtype, int32_t direction, void* workspace, size_t workspace_bytes, void* hip_stream) {
   g_last_error.clear();
   const int rc = recurrence_check("gated recurrence", X, &ldX, c0, lens, T, B, n, dtype, direction);
   if (rc != RTN_OK) return rc;
   if (B == 0 || n == 0) return RTN_OK;
   if ((T && !Y) || !cN) return fail(RTN_ERR_ARG, "gated recurrence: null pointer");
   if (!aligned(Y, size_of(dtype)) || !aligned(cN, 4) || !aligned(saved, 16)) return fail(RTN_ERR_ARG, "gated recurrence: misaligned pointer");
-  const int64_t blocks = ((int64_t)B * n + 255) / 256;
-  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
-  const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0};
-  with_type(dtype, [&](auto type) {
-    hipLaunchKernelGGL((k_recurrence_fwd<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
+  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, forward_frames(dtype));
+  const size_t need = recurrence_runs_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes needed", need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence: workspace must be 16-byte aligned");
+  if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
+  const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, (float*)workspace};
+  with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
+    typedef decltype(type) AT;
+    constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;
+    const hipStream_t stream = (hipStream_t)hip_stream;
+    if constexpr (W == 16)
+      if (p.segments > 1)
+        hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kForwardFrames<AT>, W, true>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((k_recurrence_fwd<AT, VEC, kForwardFrames<AT>, W>), dim3((unsigned)(p.chains * p.segments)), dim3(64 * W), 0, stream, a);
   });
   return launched("gated recurrence");
 }
 
 int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, const void* saved, const void* DY, int64_t ldDY, const float* DcN, void* DX,
-                             float* Dc0, int64_t T, int32_t B, int32_t n, int32_t dtype, int32_t direction, void*, size_t, void* hip_stream) {
+                             float* Dc0, int64_t T, int32_t B, int32_t n, int32_t dtype, int32_t direction, void* workspace, size_t workspace_bytes,
+                             void* hip_stream) {
   g_last_error.clear();
   const int rc = recurrence_check("gated recurrence gradient", X, &ldX, c0, lens, T, B, n, dtype, direction);
   if (rc != RTN_OK) return rc;
@@ -116,11 +179,20 @@ int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const 
   if ((T && (!DX || !DY || !saved)) || !Dc0) return fail(RTN_ERR_ARG, "gated recurrence gradient: null pointer");
   if (!aligned(DY, size_of(dtype)) || !aligned(DX, size_of(dtype)) || !aligned(Dc0, 4) || !aligned(DcN, 4) || !aligned(saved, 16))
     return fail(RTN_ERR_ARG, "gated recurrence gradient: misaligned pointer");
-  const int64_t blocks = ((int64_t)B * n + 255) / 256;
-  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
-  const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0};
-  with_type(dtype, [&](auto type) {
-    hipLaunchKernelGGL((k_recurrence_bwd<decltype(type)>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
+  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, kGradientFrames);
+  const size_t need = recurrence_runs_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence gradient: workspace of %zu bytes needed", need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence gradient: workspace must be 16-byte aligned");
+  if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
+  const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, (float*)workspace};
+  with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
+    typedef decltype(type) AT;
+    constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;
+    const hipStream_t stream = (hipStream_t)hip_stream;
+    if constexpr (W == 16)
+      if (p.segments > 1)
+        hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kGradientFrames, W, false>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((k_recurrence_bwd<AT, VEC, kGradientFrames, W>), dim3((unsigned)(p.chains * p.segments)), dim3(64 * W), 0, stream, a);
   });
   return launched("gated recurrence gradient");
 }

@@ -22,6 +22,7 @@
 namespace rtn {
 
 constexpr int kSavedFrames = 16;  // frames from one saved state to the next
+constexpr int kStreamed = 2;      // cache policy of stores: not kept
 
 struct RecurrenceArgs {
   const void* X;
@@ -52,7 +53,7 @@ template <>
 struct Channels<float, 1> {
   typedef unsigned Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, kStreamed); }
   static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, r); }
   static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned, v[0]); }
 };
@@ -60,7 +61,7 @@ template <>
 struct Channels<__bf16, 1> {
   typedef unsigned short Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b16(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b16(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b16(v, row, at, 0, kStreamed); }
   static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, (unsigned)r << 16); }
   static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned short, (__bf16)v[0]); }
 };
@@ -68,15 +69,13 @@ template <>
 struct Channels<__bf16, 2> {
   typedef unsigned Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, 0); }
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, kStreamed); }
   static __device__ __forceinline__ void get(Raw r, float (&v)[2]) {
     v[0] = __builtin_bit_cast(float, r << 16);
     v[1] = __builtin_bit_cast(float, r & 0xFFFF0000u);
   }
   static __device__ __forceinline__ Raw set(const float (&v)[2]) {
-    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-    const bf16x2 pair = {(__bf16)v[0], (__bf16)v[1]};
-    return __builtin_bit_cast(unsigned, pair);
+    return pack_bf16(v[0], v[1]);
   }
 };
 
@@ -85,7 +84,8 @@ struct Rows {
   char* base;
   long long frame;
   int bytes;
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int t) const { return __builtin_amdgcn_make_buffer_rsrc(base + t * frame, 0, bytes, 0x00020000); }
+  __device__ __forceinline__ char* of(int t) const { return base + t * frame; }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(char* row) const { return __builtin_amdgcn_make_buffer_rsrc(row, 0, bytes, 0x00020000); }
 };
 
 // What a workgroup works on: one sequence, 64 lanes' channels, a segment of the frames.  Frames are counted in the order of the recurrence: step s is
@@ -168,6 +168,30 @@ __device__ __forceinline__ void start_of_segment(const RecurrenceArgs& a, unsign
   __syncthreads();
 }
 
+// Calls f with all and more as types.
+template <typename F>
+__device__ __forceinline__ void by_kind(bool all, bool more, F f) {
+  if (all && more)
+    f(std::true_type(), std::true_type());
+  else if (all)
+    f(std::true_type(), std::false_type());
+  else if (more)
+    f(std::false_type(), std::true_type());
+  else
+    f(std::false_type(), std::false_type());
+}
+
+// The turns of a workgroup, of `frames` steps each, that have steps of the sequence: first, first + frames, ... below stop.
+struct Turns {
+  int first, stop;
+  template <typename C>
+  __device__ __forceinline__ Turns(const C& q, int begin, int end, int frames) {
+    const int low = q.low > begin ? q.low : begin, high = q.high < end ? q.high : end;
+    first = low < high ? begin + (low - begin) / frames * frames : end;
+    stop = low < high ? begin + (high - begin + frames - 1) / frames * frames : end;
+  }
+};
+
 // ---- forward ----
 // W wavefronts, F frames each.  handed: the runs of the wavefronts, and in [W] the state that the next turn starts from, which the last wavefront
 // leaves there; both twice, so that one barrier a turn is enough.
@@ -179,18 +203,18 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
   const int segment = blockIdx.x / a.chains, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const C q(a, chain);
   const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
+  const Turns turns(q, begin, end, F * W);
   const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), Y = C::rows(a, a.Y, q.b, a.n, a.n);
   const size_t own = (size_t)q.b * a.n + q.k;
 
   typename C::Raw raw[F][4];
-  auto ask = [&](int j, int s) {
-    const __amdgpu_buffer_rsrc_t row = X.at(q.frame_inside(s));
+  auto ask = [&](int j, char* row) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(row, q.at[g]);
+    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(X.at(row), q.at[g]);
   };
-  if (q.any_inside(begin + wave * F, F)) {
+  if (turns.first < turns.stop && q.any_inside(turns.first + wave * F, F)) {
 #pragma unroll
-    for (int j = 0; j < F; ++j) ask(j, begin + wave * F + j);
+    for (int j = 0; j < F; ++j) ask(j, X.of(q.frame_inside(turns.first + wave * F + j)));
   }
   float c[VEC];
 #pragma unroll
@@ -199,11 +223,12 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
 
   int turn = 0;
 #pragma unroll 1
-  for (int from = begin; from < end; from += F * W, turn ^= 1) {
+  for (int from = turns.first; from < turns.stop; from += F * W, turn ^= 1) {
     const int s0 = from + wave * F, next = s0 + F * W;
-    const bool all = q.all_inside(s0, F), more = from + F * W < end && q.any_inside(next, F);
+    const bool all = q.all_inside(s0, F), more = next < turns.stop && q.all_inside(next, F);
     float A[F][VEC], S[F][VEC], o[F][VEC];  // of the run up to frame j
-    auto activate = [&](auto all) {
+    by_kind(all, more, [&](auto all, auto more) {
+      char* row = X.of(q.frame(next));
 #pragma unroll
       for (int j = 0; j < F; ++j) {
         float z[VEC], i[VEC], f[VEC];
@@ -219,20 +244,21 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
           A[j][v] = j ? A[j - 1][v] * fv : fv;
           S[j][v] = j ? __builtin_fmaf(fv, S[j - 1][v], iz) : iz;
         }
-        if (more) ask(j, next + j);  // (as soon as the registers are free: the loads go on while the gates are worked on)
+        __builtin_amdgcn_sched_barrier(0);  // (the registers of frame j take the next turn's: the loads go on while the gates are worked on)
+        if (more) ask(j, row), row += q.stride * X.frame;
       }
-    };
-    if (all)
-      activate(std::true_type());
-    else
-      activate(std::false_type());
+    });
+    if (!more && next < turns.stop && q.any_inside(next, F)) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) ask(j, X.of(q.frame_inside(next + j)));
+    }
     Run<VEC> run;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) run.a[v] = A[F - 1][v], run.s[v] = S[F - 1][v];
     if constexpr (W > 1) {
       handed[turn][wave][q.lane] = run;
       __syncthreads();
-      if (from > begin) {
+      if (from > turns.first) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) c[v] = handed[turn][W][q.lane].s[v];
       }
@@ -244,15 +270,22 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
       for (int v = 0; v < VEC; ++v) a.saved[(size_t)(s0 / kSavedFrames) * a.B * a.n + own + v] = c[v];
     }
     if (q.active) {
+      auto write = [&](auto all) {
+        char* row = Y.of(q.frame(s0));
 #pragma unroll
-      for (int j = 0; j < F; ++j) {
-        if (s0 + j >= end) break;
-        float y[VEC];
-        const bool in = all || q.inside(s0 + j);
+        for (int j = 0; j < F; ++j, row += q.stride * Y.frame) {
+          if (!all && s0 + j >= end) break;
+          float y[VEC];
+          const bool in = all || q.inside(s0 + j);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) y[v] = in ? o[j][v] * __builtin_fmaf(A[j][v], c[v], S[j][v]) : 0.f;
-        C::C::store(Y.at(q.frame(s0 + j)), q.at[0], C::C::set(y));
-      }
+          for (int v = 0; v < VEC; ++v) y[v] = in ? o[j][v] * __builtin_fmaf(A[j][v], c[v], S[j][v]) : 0.f;
+          C::C::store(Y.at(row), q.at[0], C::C::set(y));
+        }
+      };
+      if (all)
+        write(std::true_type());
+      else
+        write(std::false_type());
     }
     if (W == 1 || wave == W - 1) {
       run.apply(c);
@@ -263,10 +296,16 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
       }
     }
   }
-  if (q.active && wave == W - 1 && segment == a.segments - 1) {
+  if (!q.active) return;
+  if (wave == W - 1 && segment == a.segments - 1) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) a.cN[own + v] = c[v];
   }
+  // what is past the end of the sequence
+  const float zero[VEC] = {};
+#pragma unroll 1
+  for (int s = begin + wave; s < end; s += W)
+    if (s < turns.first || s >= turns.stop) C::C::store(Y.at(Y.of(q.frame(s))), q.at[0], C::C::set(zero));
 }
 
 // ---- gradient ----
@@ -281,42 +320,48 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
   const int segment = a.segments - 1 - (int)(blockIdx.x / a.chains), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const C q(a, chain);
   const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
+  const Turns turns(q, begin, end, F * W);
   const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), DY = C::rows(a, a.DY, q.b, a.ldDY, a.n), DX = C::rows(a, a.DX, q.b, 4 * (long long)a.n, 4 * a.n);
   const size_t own = (size_t)q.b * a.n + q.k;
 
   typename C::Raw raw[F][5];
   float before[VEC];  // the saved state of the wavefront's group
-  auto ask = [&](int j, int s) {
-    const int t = q.frame_inside(s);
-    const __amdgpu_buffer_rsrc_t row = X.at(t);
+  auto ask = [&](int j, char* row, char* row_dy) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(row, q.at[g]);
-    raw[j][4] = C::C::load(DY.at(t), q.at[0]);
+    for (int g = 0; g < 4; ++g) raw[j][g] = C::C::load(X.at(row), q.at[g]);
+    raw[j][4] = C::C::load(DY.at(row_dy), q.at[0]);
+  };
+  auto ask_near = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      const int t = q.frame_inside(s0 + j);
+      ask(j, X.of(t), DY.of(t));
+    }
   };
   auto ask_state = [&](int s0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) before[v] = s0 < (int)a.T ? a.saved[(size_t)(s0 / kSavedFrames) * a.B * a.n + own + v] : 0.f;
   };
-  const int last = begin + ((end - begin + F * W - 1) / (F * W) - 1) * (F * W);
-  if (last >= begin) {
-    if (q.any_inside(last + wave * F, F)) {
-#pragma unroll
-      for (int j = 0; j < F; ++j) ask(j, last + wave * F + j);
-    }
+  const int last = turns.stop - F * W;
+  if (turns.first < turns.stop) {
+    if (q.any_inside(last + wave * F, F)) ask_near(last + wave * F);
     ask_state(last + wave * F);
   }
-  float g[VEC];
+  float g[VEC], left[VEC];  // the error of the wavefront's last state; what the first wavefront leaves
 #pragma unroll
   for (int v = 0; v < VEC; ++v) g[v] = a.DcN ? a.DcN[own + v] : 0.f;
   start_of_segment<VEC, W, false>(a, chain, segment, wave, q.lane, handed[0], g);
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) left[v] = g[v];
 
   int turn = 0;
 #pragma unroll 1
-  for (int from = last; from >= begin; from -= F * W, turn ^= 1) {
+  for (int from = last; from >= turns.first && turns.first < turns.stop; from -= F * W, turn ^= 1) {
     const int s0 = from + wave * F, next = s0 - F * W;
-    const bool all = q.all_inside(s0, F), more = from > begin && q.any_inside(next, F);
+    const bool all = q.all_inside(s0, F), more = from > turns.first && q.all_inside(next, F);
     float z[F][VEC], i[F][VEC], f[F][VEC], o[F][VEC], e[F][VEC], c[VEC];
-    auto activate = [&](auto all) {
+    by_kind(all, more, [&](auto all, auto more) {
+      char *row = X.of(q.frame(next)), *row_dy = DY.of(q.frame(next));
 #pragma unroll
       for (int j = 0; j < F; ++j) {
         C::C::get(raw[j][0], z[j]);
@@ -333,13 +378,11 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
           o[j][v] = in ? Act<AT>::sigmoid(o[j][v]) : 0.f;
           e[j][v] = in ? e[j][v] : 0.f;
         }
-        if (more) ask(j, next + j);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) ask(j, row, row_dy), row += q.stride * X.frame, row_dy += q.stride * DY.frame;
       }
-    };
-    if (all)
-      activate(std::true_type());
-    else
-      activate(std::false_type());
+    });
+    if (!more && from > turns.first && q.any_inside(next, F)) ask_near(next);
     Run<VEC> forth = Run<VEC>::none(), back = forth;
 #pragma unroll
     for (int j = 0; j < F; ++j)
@@ -352,7 +395,7 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
       }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) back.a[v] = forth.a[v], c[v] = before[v];
-    if (from > begin) ask_state(next);
+    if (from > turns.first) ask_state(next);
     if constexpr (W > 1) {
       handed[turn][wave][q.lane] = back;
       states[turn][wave][q.lane] = forth;
@@ -367,17 +410,9 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
       for (int j = W - 1; j > wave; --j) handed[turn][j][q.lane].apply(g);
     }
     if (wave == 0) {  // the error that the turn before this one starts from
-      Run<VEC> left;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) left.a[v] = 0.f, left.s[v] = g[v];
-      left.then(back);
-      if constexpr (W > 1) {
-        handed[turn ^ 1][W][q.lane] = left;
-      }
-      if (q.active && from == begin && segment == 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) a.Dc0[own + v] = left.s[v];
-      }
+      for (int v = 0; v < VEC; ++v) left[v] = back.s[v] = __builtin_fmaf(back.a[v], g[v], back.s[v]);
+      if (W > 1) handed[turn ^ 1][W][q.lane] = back;
     }
     if (q.active) {
       float states_before[F + 1][VEC];
@@ -388,8 +423,9 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
         for (int j = 0; j < F; ++j) states_before[j + 1][v] = __builtin_fmaf(f[j][v], states_before[j][v], i[j][v] * z[j][v]);
       }
       auto write = [&](auto all) {
+        char* row = DX.of(q.frame(s0 + F - 1));
 #pragma unroll
-        for (int j = F - 1; j >= 0; --j) {
+        for (int j = F - 1; j >= 0; --j, row -= q.stride * DX.frame) {
           const bool in = all || q.inside(s0 + j);
           float dz[VEC], di[VEC], df[VEC], d_o[VEC];
 #pragma unroll
@@ -403,11 +439,10 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
             g[v] = in ? gf : g[v];
           }
           if (!all && s0 + j >= end) continue;
-          const __amdgpu_buffer_rsrc_t row = DX.at(q.frame(s0 + j));
-          C::C::store(row, q.at[0], C::C::set(dz));
-          C::C::store(row, q.at[1], C::C::set(di));
-          C::C::store(row, q.at[2], C::C::set(df));
-          C::C::store(row, q.at[3], C::C::set(d_o));
+          C::C::store(DX.at(row), q.at[0], C::C::set(dz));
+          C::C::store(DX.at(row), q.at[1], C::C::set(di));
+          C::C::store(DX.at(row), q.at[2], C::C::set(df));
+          C::C::store(DX.at(row), q.at[3], C::C::set(d_o));
         }
       };
       if (all)
@@ -416,10 +451,19 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
         write(std::false_type());
     }
   }
-  if (last < begin && q.active && wave == 0) {  // no frames at all
+  if (!q.active) return;
+  if (wave == 0 && segment == 0) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) a.Dc0[own + v] = g[v];
+    for (int v = 0; v < VEC; ++v) a.Dc0[own + v] = left[v];
   }
+  // what is past the end of the sequence
+  const float zero[VEC] = {};
+#pragma unroll 1
+  for (int s = begin + wave; s < end; s += W)
+    if (s < turns.first || s >= turns.stop) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) C::C::store(DX.at(DX.of(q.frame(s))), q.at[k], C::C::set(zero));
+    }
 }
 
 // ---- the runs of segments: (A, S), or (A, Q) of the errors ----
@@ -442,9 +486,9 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_runs(RecurrenceArgs a) {
 #pragma unroll
     for (int j = 0; j < F; ++j) {
       const int t = q.frame_inside(s0 + j);
-      const __amdgpu_buffer_rsrc_t row = X.at(t);
+      const __amdgpu_buffer_rsrc_t row = X.at(X.of(t));
       raw[j][0] = C::C::load(row, FORWARD ? q.at[0] : q.at[3]);
-      raw[j][1] = FORWARD ? C::C::load(row, q.at[1]) : C::C::load(DY.at(t), q.at[0]);
+      raw[j][1] = FORWARD ? C::C::load(row, q.at[1]) : C::C::load(DY.at(DY.of(t)), q.at[0]);
       raw[j][2] = C::C::load(row, q.at[2]);
     }
     auto add = [&](auto all) {

@@ -16,6 +16,13 @@ __device__ __forceinline__ void store_f32(AT* p, float v) {  // rounds to neares
   *p = (AT)v;
 }
 
+// Two numbers rounded to bfloat16, the first in the lower half.
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+  typedef __attribute__((__vector_size__(2 * sizeof(float)))) float pair_f32;
+  typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 pair_bf16;
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((pair_f32){a, b}, pair_bf16));
+}
+
 // Eight neighbouring elements as they lie in memory, at any element's address: one load of 16 bytes in bfloat16, two in float32 (the
 // hardware takes them at any address).
 typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned seq_u32x4;
@@ -50,11 +57,7 @@ struct Eight {
       if constexpr (sizeof(AT) == 4) w[k >> 2][k & 3] = __builtin_bit_cast(unsigned, v[k]);
     if constexpr (sizeof(AT) == 2) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-        const bf16x2 pair = {(__bf16)v[2 * k], (__bf16)v[2 * k + 1]};
-        w[0][k] = __builtin_bit_cast(unsigned, pair);
-      }
+      for (int k = 0; k < 4; ++k) w[0][k] = pack_bf16(v[2 * k], v[2 * k + 1]);
     }
   }
 };

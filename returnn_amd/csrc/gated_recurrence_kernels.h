@@ -22,7 +22,7 @@
 namespace rtn {
 
 constexpr int kSavedFrames = 16;  // frames from one saved state to the next
-constexpr int kStreamed = 2;      // cache policy of stores: not kept
+constexpr int kStreamed = 2;      // cache policy of stores: not kept in the caches
 
 struct RecurrenceArgs {
   const void* X;
@@ -43,6 +43,7 @@ struct RecurrenceArgs {
   unsigned chains;    // strips times sequences
   long long segment;  // frames of a segment
   int segments;
+  int apart;          // strips share no cache line
   float* runs;        // [segments][chains][64 lanes][VEC][2] A and S, or A and Q, of the segments
 };
 
@@ -53,7 +54,10 @@ template <>
 struct Channels<float, 1> {
   typedef unsigned Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, kStreamed); }
+  template <bool STREAMED>
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
+    __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, STREAMED ? kStreamed : 0);
+  }
   static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, r); }
   static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned, v[0]); }
 };
@@ -61,7 +65,10 @@ template <>
 struct Channels<__bf16, 1> {
   typedef unsigned short Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b16(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b16(v, row, at, 0, kStreamed); }
+  template <bool STREAMED>
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
+    __builtin_amdgcn_raw_buffer_store_b16(v, row, at, 0, STREAMED ? kStreamed : 0);
+  }
   static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, (unsigned)r << 16); }
   static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned short, (__bf16)v[0]); }
 };
@@ -69,7 +76,10 @@ template <>
 struct Channels<__bf16, 2> {
   typedef unsigned Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) { __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, kStreamed); }
+  template <bool STREAMED>
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
+    __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, STREAMED ? kStreamed : 0);
+  }
   static __device__ __forceinline__ void get(Raw r, float (&v)[2]) {
     v[0] = __builtin_bit_cast(float, r << 16);
     v[1] = __builtin_bit_cast(float, r & 0xFFFF0000u);
@@ -87,6 +97,14 @@ struct Rows {
   __device__ __forceinline__ char* of(int t) const { return base + t * frame; }
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(char* row) const { return __builtin_amdgcn_make_buffer_rsrc(row, 0, bytes, 0x00020000); }
 };
+
+// The number of the workgroup among its kernel's.  Workgroup i runs on XCD i mod 8, which has an L2 of its own.  Where neighbouring strips share cache
+// lines, each XCD takes numbers that follow each other, and lines are read once and written whole (n = 1001 float32, T = 333, 11 rows: forward 27.2 / 23.8 us,
+// gradient 38.9 / 33.0; n = 1000 bf16, T = 1000, 32 rows: gradient 186 / 146); where they do not, neighbours on different XCDs are a little faster (n = 1024 bf16, T = 1000, 32 rows: 69 and 118 us instead of 72 and 121).
+__device__ __forceinline__ unsigned workgroup_number(const RecurrenceArgs& a) {
+  const unsigned x = blockIdx.x % 8, i = blockIdx.x / 8, each = gridDim.x / 8, more = gridDim.x % 8;
+  return a.apart ? blockIdx.x : x * each + (x < more ? x : more) + i;
+}
 
 // What a workgroup works on: one sequence, 64 lanes' channels, a segment of the frames.  Frames are counted in the order of the recurrence: step s is
 // frame s, or T - 1 - s.
@@ -168,7 +186,7 @@ __device__ __forceinline__ void start_of_segment(const RecurrenceArgs& a, unsign
   __syncthreads();
 }
 
-// Calls f with all and more as types.
+// Calls f with two truths as types.
 template <typename F>
 __device__ __forceinline__ void by_kind(bool all, bool more, F f) {
   if (all && more)
@@ -199,8 +217,8 @@ template <typename AT, int VEC, int F, int W>
 __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
   typedef Chain<AT, VEC> C;
   __shared__ Run<VEC> handed[2][W + 1][64];
-  const unsigned chain = blockIdx.x % a.chains;
-  const int segment = blockIdx.x / a.chains, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned number = workgroup_number(a), chain = number % a.chains;
+  const int segment = number / a.chains, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const C q(a, chain);
   const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
   const Turns turns(q, begin, end, F * W);
@@ -226,7 +244,8 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
   for (int from = turns.first; from < turns.stop; from += F * W, turn ^= 1) {
     const int s0 = from + wave * F, next = s0 + F * W;
     const bool all = q.all_inside(s0, F), more = next < turns.stop && q.all_inside(next, F);
-    float A[F][VEC], S[F][VEC], o[F][VEC];  // of the run up to frame j
+    float A[F][VEC], S[F][VEC];  // of the run up to frame j
+    typename C::Raw out[F];      // the output gates as they came
     by_kind(all, more, [&](auto all, auto more) {
       char* row = X.of(q.frame(next));
 #pragma unroll
@@ -235,12 +254,11 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
         C::C::get(raw[j][0], z);
         C::C::get(raw[j][1], i);
         C::C::get(raw[j][2], f);
-        C::C::get(raw[j][3], o[j]);
+        out[j] = raw[j][3];
         const bool in = all || q.inside(s0 + j);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           const float fv = in ? Act<AT>::sigmoid(f[v]) : 1.f, iz = in ? Act<AT>::sigmoid(i[v]) * Act<AT>::tanh(z[v]) : 0.f;
-          o[j][v] = Act<AT>::sigmoid(o[j][v]);
           A[j][v] = j ? A[j - 1][v] * fv : fv;
           S[j][v] = j ? __builtin_fmaf(fv, S[j - 1][v], iz) : iz;
         }
@@ -270,22 +288,19 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
       for (int v = 0; v < VEC; ++v) a.saved[(size_t)(s0 / kSavedFrames) * a.B * a.n + own + v] = c[v];
     }
     if (q.active) {
-      auto write = [&](auto all) {
+      by_kind(all, a.apart, [&](auto all, auto apart) {
         char* row = Y.of(q.frame(s0));
 #pragma unroll
         for (int j = 0; j < F; ++j, row += q.stride * Y.frame) {
           if (!all && s0 + j >= end) break;
-          float y[VEC];
+          float o[VEC], y[VEC];
+          C::C::get(out[j], o);
           const bool in = all || q.inside(s0 + j);
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) y[v] = in ? o[j][v] * __builtin_fmaf(A[j][v], c[v], S[j][v]) : 0.f;
-          C::C::store(Y.at(row), q.at[0], C::C::set(y));
+          for (int v = 0; v < VEC; ++v) y[v] = in ? Act<AT>::sigmoid(o[v]) * __builtin_fmaf(A[j][v], c[v], S[j][v]) : 0.f;
+          C::C::template store<decltype(apart)::value>(Y.at(row), q.at[0], C::C::set(y));
         }
-      };
-      if (all)
-        write(std::true_type());
-      else
-        write(std::false_type());
+      });
     }
     if (W == 1 || wave == W - 1) {
       run.apply(c);
@@ -305,7 +320,7 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
   const float zero[VEC] = {};
 #pragma unroll 1
   for (int s = begin + wave; s < end; s += W)
-    if (s < turns.first || s >= turns.stop) C::C::store(Y.at(Y.of(q.frame(s))), q.at[0], C::C::set(zero));
+    if (s < turns.first || s >= turns.stop) C::C::template store<false>(Y.at(Y.of(q.frame(s))), q.at[0], C::C::set(zero));
 }
 
 // ---- gradient ----
@@ -316,8 +331,8 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
   static_assert(W == 1 || W % GROUP == 0, "saved states lie where wavefronts begin");
   __shared__ Run<VEC> handed[2][W + 1][64];
   __shared__ Run<VEC> states[2][W][64];
-  const unsigned chain = blockIdx.x % a.chains;
-  const int segment = a.segments - 1 - (int)(blockIdx.x / a.chains), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned number = workgroup_number(a), chain = number % a.chains;
+  const int segment = a.segments - 1 - (int)(number / a.chains), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const C q(a, chain);
   const int begin = segment * (int)a.segment, end = begin + (int)a.segment < (int)a.T ? begin + (int)a.segment : (int)a.T;
   const Turns turns(q, begin, end, F * W);
@@ -359,7 +374,8 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
   for (int from = last; from >= turns.first && turns.first < turns.stop; from -= F * W, turn ^= 1) {
     const int s0 = from + wave * F, next = s0 - F * W;
     const bool all = q.all_inside(s0, F), more = from > turns.first && q.all_inside(next, F);
-    float z[F][VEC], i[F][VEC], f[F][VEC], o[F][VEC], e[F][VEC], c[VEC];
+    float z[F][VEC], i[F][VEC], f[F][VEC], o[F][VEC], c[VEC];
+    typename C::Raw error[F];  // of the outputs, as they came
     by_kind(all, more, [&](auto all, auto more) {
       char *row = X.of(q.frame(next)), *row_dy = DY.of(q.frame(next));
 #pragma unroll
@@ -368,7 +384,7 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
         C::C::get(raw[j][1], i[j]);
         C::C::get(raw[j][2], f[j]);
         C::C::get(raw[j][3], o[j]);
-        C::C::get(raw[j][4], e[j]);
+        error[j] = raw[j][4];
         const bool in = all || q.inside(s0 + j);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -376,7 +392,6 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
           i[j][v] = in ? Act<AT>::sigmoid(i[j][v]) : 0.f;
           f[j][v] = in ? Act<AT>::sigmoid(f[j][v]) : 1.f;
           o[j][v] = in ? Act<AT>::sigmoid(o[j][v]) : 0.f;
-          e[j][v] = in ? e[j][v] : 0.f;
         }
         __builtin_amdgcn_sched_barrier(0);
         if (more) ask(j, row, row_dy), row += q.stride * X.frame, row_dy += q.stride * DY.frame;
@@ -385,14 +400,18 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
     if (!more && from > turns.first && q.any_inside(next, F)) ask_near(next);
     Run<VEC> forth = Run<VEC>::none(), back = forth;
 #pragma unroll
-    for (int j = 0; j < F; ++j)
+    for (int j = 0; j < F; ++j) {
+      const int l = F - 1 - j;
+      float e[VEC];
+      C::C::get(error[l], e);
+      const bool in = q.inside(s0 + l);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         forth.a[v] *= f[j][v];
         forth.s[v] = __builtin_fmaf(f[j][v], forth.s[v], i[j][v] * z[j][v]);
-        const int l = F - 1 - j;
-        back.s[v] = f[l][v] * __builtin_fmaf(e[l][v], o[l][v], back.s[v]);
+        back.s[v] = f[l][v] * __builtin_fmaf(in ? e[v] : 0.f, o[l][v], back.s[v]);
       }
+    }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) back.a[v] = forth.a[v], c[v] = before[v];
     if (from > turns.first) ask_state(next);
@@ -422,15 +441,17 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
 #pragma unroll
         for (int j = 0; j < F; ++j) states_before[j + 1][v] = __builtin_fmaf(f[j][v], states_before[j][v], i[j][v] * z[j][v]);
       }
-      auto write = [&](auto all) {
+      by_kind(all, a.apart, [&](auto all, auto apart) {
+        constexpr bool STREAMED = decltype(apart)::value;  // (past the caches, but not parts of lines)
         char* row = DX.of(q.frame(s0 + F - 1));
 #pragma unroll
         for (int j = F - 1; j >= 0; --j, row -= q.stride * DX.frame) {
           const bool in = all || q.inside(s0 + j);
-          float dz[VEC], di[VEC], df[VEC], d_o[VEC];
+          float e[VEC], dz[VEC], di[VEC], df[VEC], d_o[VEC];
+          C::C::get(error[j], e);
 #pragma unroll
           for (int v = 0; v < VEC; ++v) {
-            const float zv = z[j][v], iv = i[j][v], fv = f[j][v], ov = o[j][v], eo = e[j][v] * ov;
+            const float zv = z[j][v], iv = i[j][v], fv = f[j][v], ov = o[j][v], eo = e[v] * ov;
             const float total = g[v] + eo, gi = total * iv, gf = total * fv;
             dz[v] = in ? gi * __builtin_fmaf(-zv, zv, 1.f) : 0.f;
             di[v] = in ? gi * zv * (1.f - iv) : 0.f;
@@ -439,16 +460,12 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
             g[v] = in ? gf : g[v];
           }
           if (!all && s0 + j >= end) continue;
-          C::C::store(DX.at(row), q.at[0], C::C::set(dz));
-          C::C::store(DX.at(row), q.at[1], C::C::set(di));
-          C::C::store(DX.at(row), q.at[2], C::C::set(df));
-          C::C::store(DX.at(row), q.at[3], C::C::set(d_o));
+          C::C::template store<STREAMED>(DX.at(row), q.at[0], C::C::set(dz));
+          C::C::template store<STREAMED>(DX.at(row), q.at[1], C::C::set(di));
+          C::C::template store<STREAMED>(DX.at(row), q.at[2], C::C::set(df));
+          C::C::template store<STREAMED>(DX.at(row), q.at[3], C::C::set(d_o));
         }
-      };
-      if (all)
-        write(std::true_type());
-      else
-        write(std::false_type());
+      });
     }
   }
   if (!q.active) return;
@@ -462,7 +479,7 @@ __global__ __launch_bounds__(64 * W) void k_recurrence_bwd(RecurrenceArgs a) {
   for (int s = begin + wave; s < end; s += W)
     if (s < turns.first || s >= turns.stop) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) C::C::store(DX.at(DX.of(q.frame(s))), q.at[k], C::C::set(zero));
+      for (int k = 0; k < 4; ++k) C::C::template store<false>(DX.at(DX.of(q.frame(s))), q.at[k], C::C::set(zero));
     }
 }
 
@@ -472,8 +489,8 @@ template <typename AT, int VEC, int F, int W, bool FORWARD>
 __global__ __launch_bounds__(64 * W) void k_recurrence_runs(RecurrenceArgs a) {
   typedef Chain<AT, VEC> C;
   __shared__ Run<VEC> handed[W][64];
-  const unsigned chain = blockIdx.x % a.chains;
-  const int segment = (int)(blockIdx.x / a.chains) + (FORWARD ? 0 : 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (the last one's, or the first one's, nobody needs)
+  const unsigned number = workgroup_number(a), chain = number % a.chains;
+  const int segment = (int)(number / a.chains) + (FORWARD ? 0 : 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (the last one's, or the first one's, nobody needs)
   const C q(a, chain);
   const int share = (int)a.segment / W, begin = segment * (int)a.segment + wave * share;
   const Rows X = C::rows(a, a.X, q.b, a.ldX, 4 * a.n), DY = C::rows(a, a.DY, q.b, a.ldDY, a.n);

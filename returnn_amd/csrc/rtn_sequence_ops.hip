@@ -7,6 +7,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -59,10 +60,7 @@ void with_bool(bool v, F f) {
 
 // ---- gated recurrence ---------------------------------------------------------------------------------------------
 // Frames that a wavefront holds at once, forward and in the gradient: as many as leave 16 wavefronts their registers.
-template <typename AT>
-constexpr int kForwardFrames = sizeof(AT) == 2 ? 8 : 4;
-constexpr int kGradientFrames = 4;
-int forward_frames(int dtype) { return dtype == RTN_DTYPE_BF16 ? kForwardFrames<__bf16> : kForwardFrames<float>; }
+constexpr int kForwardFrames = 8, kGradientFrames = 4;
 
 constexpr int64_t kMaxFrames = 1 << 30, kMaxChannels = 1 << 26;  // (steps are 32-bit numbers, and so is a place in a row, in bytes)
 
@@ -70,23 +68,46 @@ struct RecurrencePlan {
   int vec, waves, strips, segments;
   int64_t chains, segment;
 };
-// Wavefronts: one where it takes all frames by itself, four where they take all frames or the chains fill the device, else 16.  Segments: where fewer
-// than 128 chains leave most of the device idle, as many as make 512 workgroups of at least one turn, from six turns on.
-RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, int frames) {
+// Wavefronts: as few as take all frames at once, but no more than give every compute unit the 16 that it has registers for: 16 below 512 chains, 8 below
+// 2048, else 4.  (us, 16 / 8: T=500 64 rows of n=512 float32 78 / 73; T=64 64 rows of n=2048 bf16 forward 23.5 / 18.5, gradient 33.4 / 28.6.)
+// Segments: as many as the time estimate is least for, in turns of W F frames: a workgroup takes its turns one after the other and half of one to start, 256 run
+// at once; more than one segment costs the pre-pass, whose bytes are 0.6 (gradient 0.33) of the others, and a launch of 1.5.  Measured (us, one segment / these):
+// T=4000 1 row of n=1024 bf16 forward 164 / 19, gradient 251 / 24; T=333 11 rows of n=1001 bf16 gradient 31.5 / 27.9; T=1000 32 rows of n=512 bf16 gradient 91 / 76.
+RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, bool gradient) {
+  const int frames = gradient ? kGradientFrames : kForwardFrames;
   RecurrencePlan p;
   p.vec = dtype == RTN_DTYPE_BF16 && n > 1 ? 2 : 1;
   p.strips = (n + 64 * p.vec - 1) / (64 * p.vec);
   p.chains = (int64_t)p.strips * B;
-  p.waves = T <= frames ? 1 : (T <= 4 * frames || p.chains >= 2048 ? 4 : 16);
+  const int most = p.chains >= 2048 ? 4 : (p.chains >= 512 ? 8 : 16);
+  p.waves = 1;
+  for (int w : {4, 8, 16})
+    if (p.waves * frames < T && w <= most) p.waves = w;
   const int64_t turn = (int64_t)p.waves * frames, turns = std::max<int64_t>(1, (T + turn - 1) / turn);
   int64_t segments = 1;
-  if (p.waves == 16 && p.chains < 128 && turns >= 6) segments = std::min<int64_t>(turns, (512 + p.chains - 1) / p.chains);
+  if (p.waves == 16 && p.chains <= 256) {
+    auto estimate = [&](int64_t k) { return (double)((p.chains * k + 255) / 256) * ((turns + k - 1) / k + 0.5); };
+    double least = estimate(1);
+    for (int64_t k = 2; k <= std::min<int64_t>(turns, 512 / p.chains); ++k) {
+      const double t = estimate(k) * (gradient ? 1.33 : 1.6) + 1.5;
+      if (t < least) least = t, segments = k;
+    }
+  }
   const int64_t each = (turns + segments - 1) / segments;
   p.segment = each * turn;
   p.segments = (int)((turns + each - 1) / each);
   return p;
 }
 size_t recurrence_runs_bytes(const RecurrencePlan& p) { return p.segments > 1 ? (size_t)p.segments * (size_t)p.chains * 64 * p.vec * 8 : 0; }
+
+// Whether no two strips of a row share a cache line of 128 bytes, in any of the arrays.
+bool strips_apart(const RecurrencePlan& p, int B, int n, int dtype, std::initializer_list<const void*> arrays, std::initializer_list<int64_t> pitches) {
+  const int64_t e = size_of(dtype);
+  bool apart = n * e % 128 == 0;
+  for (const void* q : arrays) apart = apart && aligned(q, 128);
+  for (int64_t ld : pitches) apart = apart && ld * e % 128 == 0;
+  return apart || p.chains == B;  // (or there is one strip to a row)
+}
 
 // Calls f with a value of the element type and the number of channels per lane and of wavefronts as types.
 template <int N>
@@ -98,6 +119,8 @@ void with_recurrence(int dtype, const RecurrencePlan& p, F f) {
       f(type, vec, Count<1>());
     else if (p.waves == 4)
       f(type, vec, Count<4>());
+    else if (p.waves == 8)
+      f(type, vec, Count<8>());
     else
       f(type, vec, Count<16>());
   };
@@ -135,10 +158,10 @@ size_t rtn_gated_recurrence_saved_bytes(int64_t T, int32_t B, int32_t n, int32_t
   return T <= 0 || B <= 0 || n <= 0 ? 0 : (size_t)((T + kSavedFrames - 1) / kSavedFrames) * (size_t)B * (size_t)n * 4;
 }
 size_t rtn_gated_recurrence_fwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype) {
-  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, forward_frames(dtype)));
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, false));
 }
 size_t rtn_gated_recurrence_bwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype) {
-  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, kGradientFrames));
+  return T <= 0 || B <= 0 || n <= 0 ? 0 : recurrence_runs_bytes(recurrence_plan(T, B, n, dtype, true));
 }
 
 int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, void* Y, float* cN, void* saved, int64_t T, int32_t B, int32_t n,
@@ -149,20 +172,21 @@ int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const 
   if (B == 0 || n == 0) return RTN_OK;
   if ((T && !Y) || !cN) return fail(RTN_ERR_ARG, "gated recurrence: null pointer");
   if (!aligned(Y, size_of(dtype)) || !aligned(cN, 4) || !aligned(saved, 16)) return fail(RTN_ERR_ARG, "gated recurrence: misaligned pointer");
-  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, forward_frames(dtype));
+  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, false);
   const size_t need = recurrence_runs_bytes(p);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence: workspace must be 16-byte aligned");
   if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
-  const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, (float*)workspace};
+  const int apart = strips_apart(p, B, n, dtype, {X, Y}, {ldX, n});
+  const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, apart, (float*)workspace};
   with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
     typedef decltype(type) AT;
     constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;
     const hipStream_t stream = (hipStream_t)hip_stream;
     if constexpr (W == 16)
       if (p.segments > 1)
-        hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kForwardFrames<AT>, W, true>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
-    hipLaunchKernelGGL((k_recurrence_fwd<AT, VEC, kForwardFrames<AT>, W>), dim3((unsigned)(p.chains * p.segments)), dim3(64 * W), 0, stream, a);
+        hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kForwardFrames, W, true>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((k_recurrence_fwd<AT, VEC, kForwardFrames, W>), dim3((unsigned)(p.chains * p.segments)), dim3(64 * W), 0, stream, a);
   });
   return launched("gated recurrence");
 }
@@ -179,12 +203,13 @@ int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const 
   if ((T && (!DX || !DY || !saved)) || !Dc0) return fail(RTN_ERR_ARG, "gated recurrence gradient: null pointer");
   if (!aligned(DY, size_of(dtype)) || !aligned(DX, size_of(dtype)) || !aligned(Dc0, 4) || !aligned(DcN, 4) || !aligned(saved, 16))
     return fail(RTN_ERR_ARG, "gated recurrence gradient: misaligned pointer");
-  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, kGradientFrames);
+  const RecurrencePlan p = recurrence_plan(T, B, n, dtype, true);
   const size_t need = recurrence_runs_bytes(p);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence gradient: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence gradient: workspace must be 16-byte aligned");
   if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
-  const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, (float*)workspace};
+  const int apart = strips_apart(p, B, n, dtype, {X, DY, DX}, {ldX, ldDY, 4 * (int64_t)n});
+  const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, apart, (float*)workspace};
   with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
     typedef decltype(type) AT;
     constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;

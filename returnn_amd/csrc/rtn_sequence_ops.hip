@@ -303,9 +303,9 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "token log probabilities: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "token log probabilities: workspace must be 16-byte aligned");
   if (rows > kMaxBlocks / splits) return fail(RTN_ERR_SHAPE, "token log probabilities: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
-  const ScoresArgs a{logits, ld,      targets, rows,    V,           top_k,           log_prob,
+  const ScoresArgs a{logits, ld,      targets, rows,    (int)V,      top_k,           log_prob,
                      norm,   entropy, top_log_prob, top_ids, nullptr, nullptr, nullptr,
-                     (int)splits, segment, (float*)workspace, (unsigned long long*)((char*)workspace + (size_t)rows * (size_t)splits * 16)};
+                     (int)splits, (int)segment, (float*)workspace, (unsigned long long*)((char*)workspace + (size_t)rows * (size_t)splits * 16)};
   const hipStream_t stream = (hipStream_t)hip_stream;
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
@@ -350,7 +350,7 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
     return fail(RTN_ERR_ARG, "token log probabilities gradient: misaligned pointer");
   const int64_t pieces = (V + kBwdPiece - 1) / kBwdPiece;
   if (rows > kMaxBlocks / pieces) return fail(RTN_ERR_SHAPE, "token log probabilities gradient: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
-  const ScoresArgs a{logits,  ld,      targets, rows,       V,         0, nullptr,     (float*)norm, (float*)entropy,
+  const ScoresArgs a{logits,  ld,      targets, rows,       (int)V,    0, nullptr,     (float*)norm, (float*)entropy,
                      nullptr, nullptr, d_log_prob, d_entropy, D, (int)pieces, 0, nullptr, nullptr};
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;

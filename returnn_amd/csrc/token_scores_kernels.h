@@ -14,14 +14,15 @@ struct ScoresArgs {
   const void* logits;
   long long ld;
   const int64_t* targets;
-  long long rows, V;
+  long long rows;
+  int V;
   int top_k;
   float *log_prob, *norm, *entropy, *top_log_prob;
   int64_t* top_ids;
   const float *d_log_prob, *d_entropy;
   void* D;
   int splits;          // pieces of a row
-  long long segment;   // logits of a piece
+  int segment;         // logits of a piece
   float* part;         // [rows][splits][4] of the pieces: maximum, sums
   unsigned long long* part_top;  // [rows][splits][top_k]
 };
@@ -84,18 +85,46 @@ __device__ __forceinline__ RowSums join_sums(RowSums p) {
   return {m, wave_sum(c * p.s), wave_sum(c * __builtin_fmaf(t, p.s, p.w))};
 }
 
+// ... of the 16 lanes of a quarter, in all of them.
+template <typename F>
+__device__ __forceinline__ float over_quarter(float v, F join) {
+  v = join(v, dpp<0xB1>(v));
+  v = join(v, dpp<0x4E>(v));
+  v = join(v, dpp<0x141>(v));
+  return join(v, dpp<0x140>(v));
+}
+// The k-th largest of what the 16 lanes of a quarter have, k = 1 to 16, in all of them.
+template <int R>
+__device__ __forceinline__ int larger_in_quarter(float v) {
+  if constexpr (R == 0)
+    return 0;
+  else
+    return larger_in_quarter<R - 1>(v) + (dpp<0x120 + R>(v) > v);  // (the lane R further, around)
+}
+__device__ __forceinline__ float kth_of_quarter(float v, int k) {
+  return over_quarter(larger_in_quarter<15>(v) < k ? v : __builtin_inff(), [](float x, float y) { return __builtin_fminf(x, y); });
+}
+__device__ __forceinline__ RowSums join_quarter(RowSums p) {
+  auto add = [](float x, float y) { return x + y; };
+  const float m = over_quarter(p.m, [](float x, float y) { return __builtin_fmaxf(x, y); }), t = __builtin_fmaxf((p.m - m) * kLog2E, kNoPower);
+  const float c = __builtin_amdgcn_exp2f(t);
+  return {m, over_quarter(c * p.s, add), over_quarter(c * __builtin_fmaf(t, p.s, p.w), add)};
+}
+
 // Results of a row from its sums (one lane), and what a log probability is made of.
 struct RowNorm {
   float base, log_s;
+  RowNorm() = default;
   __device__ __forceinline__ RowNorm(RowSums r) : base(r.m), log_s(logf(r.s)) {}
   __device__ __forceinline__ float log_prob(float x) const { return x == -__builtin_inff() ? x : (x - base) - log_s; }
 };
 template <typename AT>
-__device__ __forceinline__ void row_results(const ScoresArgs& a, long long r, long long target, RowSums sums) {
+__device__ __forceinline__ RowNorm row_results(const ScoresArgs& a, long long r, long long target, RowSums sums) {
   const RowNorm norm(sums);
   if (a.norm) a.norm[2 * r] = norm.base, a.norm[2 * r + 1] = norm.log_s;
   if (a.log_prob) a.log_prob[r] = target < a.V ? norm.log_prob(load_f32((const AT*)a.logits + r * a.ld + target)) : __builtin_nanf("");
   if (a.entropy) a.entropy[r] = sums.s == 0.f ? 0.f : norm.log_s - kLn2 * (sums.w / sums.s);
+  return norm;
 }
 // ... of a row without a token, by `threads` threads
 __device__ __forceinline__ void no_row(const ScoresArgs& a, long long r, int thread, int threads) {
@@ -119,6 +148,18 @@ __device__ __forceinline__ void put_alternative(const ScoresArgs& a, long long r
   }
 }
 
+// How many of the n of a list are larger than `mine`, of which 16 neighbouring lanes look at every 16th: the same in all of them.  (One lane by itself goes through
+// a chain of look-ups and 64-bit comparisons: of 44, which is usual for 12 alternatives, 3000 clocks, a fifth of the kernel.)
+__device__ __forceinline__ int rank_in(const unsigned long long* list, int n, unsigned long long mine, int lane) {
+  int rank = 0;
+#pragma unroll 4
+  for (int o = lane & 15; o < n; o += 16) rank += list[o] > mine;
+  rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);
+  rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);
+  rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true);
+  return rank + __builtin_amdgcn_update_dpp(0, rank, 0x140, 0xF, 0xF, true);
+}
+
 // Sums and alternatives: W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
 constexpr int kCandidates = 512;
 constexpr int kMaxSegment = 16 * 64 * 32;
@@ -128,8 +169,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
   constexpr int R = W == 1 ? 4 : 1;  // rows per workgroup
   __shared__ float sums_of[R][W][4];
   __shared__ float most_of[W][64];
-  __shared__ unsigned long long list_of[R][W == 1 ? 512 : kCandidates];
+  __shared__ unsigned long long list_of[R][kCandidates];
   __shared__ int listed_of[R];
+  __shared__ float norm_of[R][2];
+  __shared__ int larger_of[64];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, sub = W == 1 ? threadIdx.x >> 6 : 0, thread = wave * 64 + lane;
   const long long item = blockIdx.x * (long long)R + sub;
   if (W == 1 && item >= a.rows) return;
@@ -141,31 +184,28 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
     return;
   }
   const AT* row = (const AT*)a.logits + r * a.ld;
-  const long long v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
+  const int v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
   const float inf = __builtin_inff();
   float x[E];
+  // (where the eight number j of this lane begins, and where its logits are read: the last ones of the row are its last eight -- there are more than
+  // eight --, of which the ones that an earlier lane has are left out)
+  auto own = [&](int j) { return v0 + (j * 64 * W + thread) * 8; };
+  auto read = [&](int j) { return own(j) < a.V - 8 ? own(j) : a.V - 8; };
   if constexpr (W == 1) {
 #pragma unroll
     for (int k = 0; k < E; ++k) x[k] = k * 64 + lane < v1 ? load_f32(row + k * 64 + lane) : -inf;
   } else {
-    // Eight neighbours are one load; those that reach past the end of the row are its last eight (there are more than eight), of which the
-    // ones that an earlier lane has are left out.
-    const int count = (int)(v1 - v0);
     Eight<AT> q[E / 8];
 #pragma unroll
-    for (int j = 0; j < E / 8; ++j) {
-      const long long at = v0 + (j * 64 * W + thread) * 8;
-      q[j].load(row + (at < a.V - 8 ? at : a.V - 8));
-    }
+    for (int j = 0; j < E / 8; ++j) q[j].load(row + read(j));
 #pragma unroll
     for (int j = 0; j < E / 8; ++j) {
       float v[8];
       q[j].get(v);
-      const int from = (j * 64 * W + thread) * 8;
-      if (__any(from + 8 > count)) {
-        const int begin = v0 + from < a.V - 8 ? from : (int)(a.V - 8 - v0);
+      if (__any(own(j) + 8 > v1)) {
+        const int from = own(j) - read(j), to = v1 - read(j);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = begin + k >= from && begin + k < count ? v[k] : -inf;
+        for (int k = 0; k < 8; ++k) v[k] = k >= from && k < to ? v[k] : -inf;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[8 * j + k] = v[k];
@@ -185,19 +225,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
   }
   RowSums sums{m, wave_sum(s), wave_sum(w)};
   bool finite = sums.s < inf;  // (neither a NaN nor an infinity in the row)
-  float group = most, top = m;
+  float group = most;
   if constexpr (W == 1) {
     if (lane == 0) listed_of[sub] = 0;
   } else {
     most_of[wave][lane] = most;
     if (lane == 0) sums_of[0][wave][0] = sums.m, sums_of[0][wave][1] = sums.s, sums_of[0][wave][2] = sums.w;
     if (thread == 0) listed_of[0] = 0;
+    if (wave == 0) larger_of[lane] = 0;
     __syncthreads();
     sums = lane < W ? RowSums{sums_of[0][lane % W][0], sums_of[0][lane % W][1], sums_of[0][lane % W][2]} : RowSums{kLowest, 0.f, 0.f};
     finite = !__any(!(sums.s < inf));
-#pragma unroll
-    for (int o = 0; o < W; ++o) group = __builtin_fmaxf(group, most_of[o][lane]);
-    top = wave_max(group);
   }
   auto meet = [&]() {
     if constexpr (W > 1)
@@ -205,42 +243,80 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
     else
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  // (where logit k of this lane lies, from v0 on)
-  auto index_of = [&](int k) {
-    if constexpr (W == 1) return (unsigned)(v0 + k * 64 + lane);
-    const long long at = v0 + ((k >> 3) * 64 * W + thread) * 8;
-    return (unsigned)((at < a.V - 8 ? at : a.V - 8) + (k & 7));
-  };
   unsigned long long* list = list_of[sub];
   int* listed = &listed_of[sub];
   int n = 0;
   float bound = kLowest;
   // Lists what reaches the bound, in any order.
   auto make_list = [&]() {
-    unsigned hits = 0;
 #pragma unroll
-    for (int k = 0; k < E; ++k) hits |= x[k] >= bound ? 1u << k : 0u;
-    if (hits) {
-      int at = atomicAdd(listed, __popc(hits));
-      for (; hits && at < kCandidates; hits &= hits - 1, ++at) {
-        const unsigned index = index_of(__ffs(hits) - 1);
-        list[at] = alternative(load_f32(row + index), index);
+    for (int j = 0; j < E / 8; ++j) {
+      unsigned hits = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) hits |= x[8 * j + k] >= bound ? 1u << k : 0u;
+      if (hits) {
+        int at = atomicAdd(listed, __popc(hits));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (hits >> k & 1u) {
+            if (at < kCandidates) list[at] = alternative(x[8 * j + k], (unsigned)(W == 1 ? k * 64 + lane : read(j) + k));
+            ++at;
+          }
       }
     }
     meet();
     n = *(volatile int*)listed;
   };
   if (finite) {
-    // A bound from below: the logits are dealt to 16, 32 or 64 groups, no fewer than alternatives are wanted, and every group's maximum reaches the
-    // least of them.  What reaches it is listed (of N groups about N log N), and finds its rank in the list.  (The top_k-th largest of 128 maxima,
-    // found bit by bit, is closer, but takes longer than all the rest: 12 rows of 32768 float32 with 12 alternatives 9.6 us, with this @TOP@.)
-    if (a.top_k <= 32) group = __builtin_fmaxf(group, dpp<0xB1>(group));
-    if (a.top_k <= 16) group = __builtin_fmaxf(group, dpp<0x4E>(group));
-    bound = -wave_max(-group);
+    // A bound from below: the logits are dealt to 16 groups, or to 64 for more than 16 alternatives, and the top_k-th largest of the groups' maxima is
+    // reached by top_k logits at least.  What reaches it is listed (for 1, 12, 20, 64 alternatives about 1, 21, 24, 300) and finds its rank in the list.  (The
+    // top_k-th largest of 128 maxima, found bit by bit, took longer than all the rest: one row of 32768 float32 with 12 alternatives 9.6 us, with this 6.3.)
+    // The groups are the wavefronts, or what neighbouring lanes of all wavefronts have.
+    if constexpr (W > 1) {
+      if (W < 16 || a.top_k > 16) {
+#pragma unroll
+        for (int o = 0; o < W; ++o) group = __builtin_fmaxf(group, most_of[o][lane]);
+      }
+    }
+    if (a.top_k <= 16) {
+      if (W == 16) {
+        group = sums.m;
+      } else {
+        group = __builtin_fmaxf(group, dpp<0xB1>(group));
+        group = __builtin_fmaxf(group, dpp<0x4E>(group));
+        group = __shfl(group, lane * 4 & 63);
+      }
+      bound = lane_of(kth_of_quarter(group, a.top_k), 0);
+    } else {
+      int larger = 0;  // (every wavefront looks at some of the others)
+#pragma unroll 4
+      for (int o = 0; o < 64 / W; ++o) larger += __shfl(group, lane + wave * (64 / W) + o & 63) > group;
+      if constexpr (W > 1) {
+        atomicAdd(&larger_of[lane], larger);
+        __syncthreads();
+        larger = larger_of[lane];
+      }
+      bound = -wave_max(larger < a.top_k ? -group : -inf);
+    }
+  }
+  RowNorm norm;
+  if (wave == 0) {  // (the others are at their lists)
+    if constexpr (W > 1) sums = join_quarter(sums);
+    if (lane == 0) {
+      if (a.splits > 1) {
+        float* part = a.part + (r * a.splits + split) * 4;
+        part[0] = sums.m, part[1] = sums.s, part[2] = sums.w;
+      } else {
+        norm = row_results<AT>(a, r, target, sums);
+      }
+      norm_of[sub][0] = norm.base, norm_of[sub][1] = norm.log_s;
+    }
+  }
+  if (finite) {
     make_list();
     if (W > 1 && n > kCandidates) {
       // Too many: the largest bound that top_k lanes still reach, to within a 4096th of what is in question.
-      float high = top;
+      float high = wave_max(lane < W ? sums_of[0][lane % W][0] : kLowest);
 #pragma unroll 1
       for (int step = 0; step < 12; ++step) {
         const float mid = 0.5f * bound + 0.5f * high;
@@ -260,31 +336,31 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
       meet();
       make_list();
     }
+  } else {
+    meet();
   }
+  norm.base = norm_of[sub][0], norm.log_s = norm_of[sub][1];
   // (fewer than wanted, but all that are not minus infinity, are also good)
-  const bool found = finite && n <= kCandidates && (n >= a.top_k || bound == kLowest);
-  if (W > 1 && wave > 0 && found && wave * 64 >= n) return;
-  if constexpr (W > 1) sums = join_sums(sums);
-  if (thread == 0) {
-    if (a.splits > 1) {
-      float* part = a.part + (r * a.splits + split) * 4;
-      part[0] = sums.m, part[1] = sums.s, part[2] = sums.w;
+  if (finite && n <= kCandidates && (n >= a.top_k || bound == kLowest)) {
+    // (by 16 lanes each where there are many, see rank_in; but that is more work, which counts where rows are short and many)
+    if constexpr (W >= 8) {
+      for (int j = thread >> 4; j < n; j += 4 * W) {
+        const unsigned long long mine = list[j];
+        const int rank = rank_in(list, n, mine, lane);
+        if ((lane & 15) == 0 && rank < a.top_k) put_alternative(a, r, split, rank, mine, norm);
+      }
     } else {
-      row_results<AT>(a, r, target, sums);
-    }
-  }
-  const RowNorm norm(sums);
-  if (found) {
-    for (int j = thread; j < n; j += 64 * W) {
-      const unsigned long long mine = list[j];
-      int rank = 0;
+      for (int j = thread; j < n; j += 64 * W) {
+        const unsigned long long mine = list[j];
+        int rank = 0;
 #pragma unroll 8
-      for (int o = 0; o < n; ++o) rank += list[o] > mine;
-      if (rank < a.top_k) put_alternative(a, r, split, rank, mine, norm);
+        for (int o = 0; o < n; ++o) rank += list[o] > mine;
+        if (rank < a.top_k) put_alternative(a, r, split, rank, mine, norm);
+      }
     }
     // The first ones that are minus infinity: among the first top_k of the row, then, there are as many as are wanted.
     if (wave == 0)
-      for (long long v = v0; n < a.top_k && v < v1; v += 64) {
+      for (int v = v0; n < a.top_k && v < v1; v += 64) {
         const bool is = v + lane < v1 && load_f32(row + v + lane) == -inf;
         const unsigned long long all = __ballot(is);
         const int rank = n + __popcll(all & ((1ull << lane) - 1));
@@ -314,7 +390,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
       mine = 0;
 #pragma unroll 8
       for (int j = 0; j < E; ++j) {
-        const long long at = W == 1 ? v0 + j * 64 + lane : v0 + ((j >> 3) * 64 * W + thread) * 8 + (j & 7);
+        const int at = W == 1 ? v0 + j * 64 + lane : own(j >> 3) + (j & 7);
         if (at < v1) {
           const unsigned long long q = alternative(load_f32(row + at), (unsigned)at);
           if (q < last && q > mine) mine = q;
@@ -343,25 +419,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
     return;
   }
   const AT* row = (const AT*)a.logits + r * a.ld;
-  const long long v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
+  const int v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
   RowSums sums{kLowest, 0.f, 0.f};
   const bool vector = a.V >= 8;
 #pragma unroll 1
-  for (long long from = v0; vector && from + wave * 512 < v1; from += 512ll * W * U) {
+  for (int from = v0; vector && from + wave * 512 < v1; from += 512 * W * U) {
     Eight<AT> q[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const long long at = from + (j * 64 * W + thread) * 8;
+      const int at = from + (j * 64 * W + thread) * 8;
       q[j].load(row + (at < a.V - 8 ? at : a.V - 8));
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const long long at = from + (j * 64 * W + wave * 64) * 8;  // (the wavefront's first)
+      const int at = from + (j * 64 * W + wave * 64) * 8;  // (the wavefront's first)
       if (at >= v1) break;
       float v[8];
       q[j].get(v);
       if (at + 512 > v1) {  // see above: the last eight of the row, those of an earlier lane left out
-        const long long mine = at + lane * 8, begin = mine < a.V - 8 ? mine : a.V - 8;
+        const int mine = at + lane * 8, begin = mine < a.V - 8 ? mine : a.V - 8;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = begin + k >= mine && begin + k < v1 ? v[k] : kNothing;
       }
@@ -381,10 +457,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
   }
   if (__any(!(sums.s + sums.w < __builtin_inff()) || sums.m <= kNothing)) {
     float most = kLowest;
-    for (long long v = v0 + thread * 8; v < v1; v += 512 * W)
+    for (int v = v0 + thread * 8; v < v1; v += 512 * W)
       for (int k = 0; k < 8 && v + k < v1; ++k) most = __builtin_fmaxf(most, load_f32(row + v + k));
     sums = {wave_max(most), 0.f, 0.f};
-    for (long long v = v0 + thread * 8; v < v1; v += 512 * W)
+    for (int v = v0 + thread * 8; v < v1; v += 512 * W)
       for (int k = 0; k < 8 && v + k < v1; ++k) {
         const float t = __builtin_elementwise_maximum((load_f32(row + v + k) - sums.m) * kLog2E, kNoPower), e = __builtin_amdgcn_exp2f(t);
         sums.s += e;
@@ -409,8 +485,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
   }
 }
 
-// The pieces of a row joined.  One workgroup per row; the alternatives of the pieces are sorted lists, and every one finds its rank in all of them.
-constexpr int kJoinInLds = 4096;
+// The pieces of a row joined.  One workgroup per row; the alternatives of the pieces are sorted lists, and every one finds its rank among all of them: where
+// they are many by halving in every list.
+constexpr int kJoinInLds = 4096, kJoinByLook = 512;
 template <typename AT>
 __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
   __shared__ unsigned long long held[kJoinInLds];
@@ -440,6 +517,17 @@ __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
     for (int j = threadIdx.x; j < n; j += 256) held[j] = all[j];
     __syncthreads();
   }
+  if (n <= kJoinByLook) {
+    for (int j = threadIdx.x >> 4; j < n; j += 16) {
+      const unsigned long long mine = held[j];
+      const int rank = rank_in(held, (int)n, mine, lane);
+      if ((lane & 15) == 0 && rank < a.top_k) {
+        a.top_log_prob[r * a.top_k + rank] = norm.log_prob(logit_of(mine));
+        a.top_ids[r * a.top_k + rank] = (int64_t)(unsigned)~(unsigned)mine;
+      }
+    }
+    return;
+  }
   for (long long j = threadIdx.x; j < n; j += 256) {
     const unsigned long long mine = n <= kJoinInLds ? held[j] : all[j];
     long long rank = 0;
@@ -455,7 +543,7 @@ __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
       }
       rank += low;
     }
-    if (rank < a.top_k && mine) {
+    if (rank < a.top_k) {
       a.top_log_prob[r * a.top_k + rank] = norm.log_prob(logit_of(mine));
       a.top_ids[r * a.top_k + rank] = (int64_t)(unsigned)~(unsigned)mine;
     }

@@ -83,23 +83,31 @@ class RecurrentLanguageModel(torch.nn.Module):
         :return: :func:`token_log_probs` of the logits, new state
         """
         logits, state = self.logits(tokens, state=state, seq_lens=seq_lens)
-        if targets is not None and seq_lens is not None:
-            inside = torch.arange(tokens.shape[0], device=tokens.device)[:, None] < seq_lens.to(tokens.device)[None, :]
-            targets = torch.where(inside, targets, -1)
+        if targets is not None:
+            targets = self._inside(targets, seq_lens)
         return token_log_probs(logits, targets, entropy=entropy, top_k=top_k), state
+
+    @staticmethod
+    def _inside(targets: torch.Tensor, seq_lens: Optional[torch.Tensor]) -> torch.Tensor:
+        """The targets, [T,B] or [B], with none past the sequences' lengths."""
+        if seq_lens is None:
+            return targets
+        frame = torch.arange(targets.shape[0], device=targets.device)[:, None] if targets.dim() == 2 else 0
+        return torch.where(seq_lens.to(targets.device) > frame, targets, -1)
 
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, *, seq_lens: Optional[torch.Tensor] = None, entropy_scale: float = 0.0) -> torch.Tensor:
         """
-        Cross entropy per token, less ``entropy_scale`` times the entropy.
+        Cross entropy per token that there is, less ``entropy_scale`` times the entropy.
 
-        :param tokens, targets: [T,B]
+        :param tokens, targets: [T,B]; a negative target is none
         """
-        s, _ = self.scores(tokens, targets, seq_lens=seq_lens, entropy=entropy_scale != 0.0)
-        count = tokens.numel() if seq_lens is None else seq_lens.to(tokens.device).clamp(0, tokens.shape[0]).sum().clamp(min=1)
+        targets = self._inside(targets, seq_lens)
+        logits, _ = self.logits(tokens, seq_lens=seq_lens)
+        s = token_log_probs(logits, targets, entropy=entropy_scale != 0.0)
         total = -s.log_probs.sum()
         if entropy_scale:
             total = total - entropy_scale * s.entropy.sum()
-        return total / count
+        return total / (targets >= 0).sum().clamp(min=1)
 
     @torch.no_grad()
     def search(self, start: torch.Tensor, *, beam: int, length: int) -> Hypotheses:

@@ -68,6 +68,22 @@ def test_steps_are_the_sequence(layer, dtype):
             assert (one.log_probs - whole.log_probs[t]).abs().max() < bound and (one.entropy - whole.entropy[t]).abs().max() < bound
 
 
+def test_frames_without_a_target():
+    """They are not among the tokens that the loss is a mean over; and a step of sequences that have ended has none."""
+    announce("language model frames without a target")
+    T, B, V = 6, 3, 30
+    m = model(V=V).eval()
+    tokens, targets, lens = torch.randint(0, V, (T, B), device=DEV), torch.randint(0, V, (T, B), device=DEV), torch.tensor([6, 3, 5])
+    targets[1, 0] = targets[0, 1] = -1
+    with torch.no_grad():
+        whole, _ = m.scores(tokens, targets, seq_lens=lens)
+        # (two orders of 12 float32 terms)
+        assert abs(float(m.loss(tokens, targets, seq_lens=lens)) + float(whole.log_probs.sum()) / 12) < 1e-5
+        one, _ = m.scores(tokens[0], targets[0], seq_lens=torch.tensor([1, 1, 0]))
+        assert float(one.log_probs[0]) < 0 and one.log_probs[1:].tolist() == [0.0, 0.0]
+        assert float(m.loss(tokens, torch.full_like(targets, -1))) == 0.0
+
+
 def test_dropout_repeats_with_its_offsets():
     announce("language model dropout")
     m = model(V=40, dim=24, drop_prob=0.3)

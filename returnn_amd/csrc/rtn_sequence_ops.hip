@@ -241,21 +241,19 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
     rows *= times, times = 1;
   }
   const int64_t count = rows * width, groups = (count + 7) / 8;
-  const bool flat = rows == 1 || (ldx == width && (!residual || ldr == width)), shared = times > 1;
-  // Frames per thread that share their draws: no more than leave every SIMD 8 wavefronts.
-  const int64_t frames = std::max<int64_t>({1, std::min<int64_t>(16, times * groups / (256 * 2048)), (times + 65534) / 65535});
-  const int64_t per_block = flat && !shared ? 512 : 256, blocks = (groups + per_block - 1) / per_block;
+  const bool flat = (rows == 1 && times == 1) || (ldx == width && (!residual || ldr == width));
+  const int64_t blocks = flat ? (groups * times + 511) / 512 : (groups + 255) / 256;
   if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
-  const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, count, frames, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr};
+  const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, count, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr};
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
     with_bool(residual != nullptr, [&](auto add) {
       constexpr bool ADD = decltype(add)::value;
       const hipStream_t stream = (hipStream_t)hip_stream;
       if (!flat)
-        hipLaunchKernelGGL((k_dropout_rows<AT, ADD>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-      else if (shared)
-        hipLaunchKernelGGL((k_dropout<AT, ADD, true>), dim3((unsigned)blocks, (unsigned)((times + frames - 1) / frames)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_dropout_rows<AT, ADD>), dim3((unsigned)blocks, (unsigned)std::min<int64_t>(times, 65535)), dim3(256), 0, stream, a);
+      else if (times > 1)
+        hipLaunchKernelGGL((k_dropout<AT, ADD, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
       else
         hipLaunchKernelGGL((k_dropout<AT, ADD, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     });
@@ -311,12 +309,17 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
     typedef decltype(type) AT;
     const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4));
     if (top_k > 0) {
-      if (segment <= 512)
+      // As few wavefronts as hold a piece, but where rows are few, more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
+      // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).
+      const bool few = rows <= 512;
+      if (segment <= 64 || (segment <= 512 && !few))
         hipLaunchKernelGGL((k_token_scores_top<AT, 1, 8>), four, dim3(256), 0, stream, a);
       else if (segment <= 2048)
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 8>), one, dim3(256), 0, stream, a);
       else if (segment <= 4096)
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 16>), one, dim3(256), 0, stream, a);
+      else if (segment <= 8192 && few)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 16>), one, dim3(512), 0, stream, a);
       else if (segment <= 8192)
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 32>), one, dim3(256), 0, stream, a);
       else if (segment <= 16384)
@@ -326,7 +329,8 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
     } else {
       with_bool(entropy != nullptr, [&](auto with_entropy) {
         constexpr bool ENTROPY = decltype(with_entropy)::value;
-        if (segment <= 1024)
+        // (us of bf16 rows, one wavefront / four: 9000 of 1500 9.4 / 11.5, 9000 of 6000 25.0 / 21.5; four / sixteen: 100 of 32000 7.1 / 5.8, 4096 of 16000 30.2 / 35.5)
+        if (segment <= 1536)
           hipLaunchKernelGGL((k_token_scores<AT, 1, ENTROPY>), four, dim3(256), 0, stream, a);
         else if (rows >= 256 || segment <= 8192)
           hipLaunchKernelGGL((k_token_scores<AT, 4, ENTROPY>), one, dim3(256), 0, stream, a);
@@ -354,6 +358,7 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
                      nullptr, nullptr, d_log_prob, d_entropy, D, (int)pieces, 0, nullptr, nullptr};
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
+    // (us of 9000 bf16 rows, a wavefront per row / a workgroup per piece: of 500 8.6 / 13.5, of 2000 18.4 / 19.7, of 5000 46.6 / 37.7)
     if (V <= 2048)
       hipLaunchKernelGGL((k_token_scores_bwd<AT, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)hip_stream, a);
     else

@@ -119,6 +119,23 @@ def test_the_mask_is_that_of_the_index():
     check(leaf.grad, torch.ones_like(x), ref.keep_factors((T, B, n), p, seed, 0))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,n", [(1, 3), (2, 9)])
+def test_many_frames_share_a_mask(B, n, dtype):
+    """More of them than a grid has rows, in one piece and with a pitch."""
+    announce("dropout many frames", B, n, dtype)
+    T, p, seed = 70001, 0.4, 21
+    wide = torch.randn((T, B, n + 2), device=DEV).to(_DTYPES[dtype])
+    factors = torch.from_numpy(ref.keep_factors((1, B, n), p, seed, 0, True).copy()).to(DEV)
+    for x in (wide[..., :n], wide[..., :n].contiguous()):
+        for r in (None, wide[..., 1 : n + 1]):
+            y = dropout(x, p, seed=seed, residual=r, same_over_time=True)
+            want = x.double() * factors + (0.0 if r is None else r.double())
+            size = (x.double() * factors).abs() + (0.0 if r is None else r.double().abs())
+            half = 2.0**-8 if dtype == "bf16" else U
+            assert torch.all((y.double() - want).abs() <= 4 * U * size + half * want.abs())
+
+
 def test_empty_and_refusals():
     announce("dropout refusals")
     for shape in ((0,), (0, 3), (3, 0), (2, 0, 4)):

@@ -98,7 +98,8 @@ def run(logits, targets, top_k, entropy=True, seed=1):
 
 
 SHAPES = [((1,), 1), ((3,), 2), ((2, 2), 7), ((5,), 63), ((4,), 64), ((130,), 65), ((2, 3), 127), ((9,), 500), ((2,), 1023), ((3,), 1025), ((1,), 4096), ((2, 7), 2047), ((17,), 5003),
-          ((1,), 10007), ((3,), 32000), ((1,), 131072), ((2,), 65537), ((600,), 33)]  # fmt: skip
+          ((1,), 10007), ((3,), 32000), ((1,), 131072), ((2,), 65537), ((600,), 33),
+          ((700,), 200), ((3,), 8000), ((600,), 6001)]  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

@@ -96,7 +96,8 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
   }
 }
 
-// Rows with a pitch: one thread per group of the mask, for every gridDim.y-th of the frames that share it.
+// Rows with a pitch: one thread per group of the mask, for every gridDim.y-th of the frames that share it.  [1000,32,500] bf16 in rows of 512: 21 us (64 MB, 3.0 TB/s;
+// one group in 63 takes the way of single elements, and nearly every wavefront has one).
 template <typename AT, bool ADD>
 __global__ __launch_bounds__(256) void k_dropout_rows(DropoutArgs a) {
   const long long g = blockIdx.x * 256ll + threadIdx.x, e = g * 8;

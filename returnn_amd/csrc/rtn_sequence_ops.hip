@@ -68,8 +68,9 @@ struct RecurrencePlan {
   int vec, waves, strips, segments;
   int64_t chains, segment;
 };
-// Wavefronts: as few as take all frames at once, but no more than give every compute unit the 16 that it has registers for: 16 below 512 chains, 8 below
-// 2048, else 4.  (us, 16 / 8: T=500 64 rows of n=512 float32 78 / 73; T=64 64 rows of n=2048 bf16 forward 23.5 / 18.5, gradient 33.4 / 28.6.)
+// Wavefronts: as few as take all frames at once, but no more than give every compute unit the 16 that it has registers for: 16 below 512 chains, else 8.
+// (us, 16 / 8: T=500 64 rows of n=512 float32 78 / 73; T=64 64 rows of n=2048 bf16 forward 23.5 / 18.5, gradient 33.4 / 28.6.  8 / 4 with 2048 chains
+// and more: T=500 256 rows of n=1024 bf16 270 / 282 and 473 / 482, T=200 500 rows of n=512 float32 221 / 210 and 381 / 384.)
 // Segments: as many as the time estimate is least for, in turns of W F frames: a workgroup takes its turns one after the other and half of one to start, 256 run
 // at once; more than one segment costs the pre-pass, whose bytes are 0.6 (gradient 0.33) of the others, and a launch of 1.5.  Measured (us, one segment / these):
 // T=4000 1 row of n=1024 bf16 forward 164 / 19, gradient 251 / 24; T=333 11 rows of n=1001 bf16 gradient 31.5 / 27.9; T=1000 32 rows of n=512 bf16 gradient 91 / 76.
@@ -79,7 +80,7 @@ RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, b
   p.vec = dtype == RTN_DTYPE_BF16 && n > 1 ? 2 : 1;
   p.strips = (n + 64 * p.vec - 1) / (64 * p.vec);
   p.chains = (int64_t)p.strips * B;
-  const int most = p.chains >= 2048 ? 4 : (p.chains >= 512 ? 8 : 16);
+  const int most = p.chains >= 512 ? 8 : 16;
   p.waves = 1;
   for (int w : {4, 8, 16})
     if (p.waves * frames < T && w <= most) p.waves = w;

@@ -161,6 +161,8 @@ __device__ __forceinline__ int rank_in(const unsigned long long* list, int n, un
 }
 
 // Sums and alternatives: W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
+// For few rows bound by latency: 12 rows of 32000 bf16 with 12 alternatives 6.8 us, with 1 6.0, the sums alone 4.4; for many by memory and the lists' barriers:
+// 3000 such rows 53 us (192 MB, 3.6 TB/s), the sums alone 40.
 constexpr int kCandidates = 512;
 constexpr int kMaxSegment = 16 * 64 * 32;
 constexpr long long kMaxTokens = 1 << 26;  // (pieces are a multiple of 8 long: with many more of them nothing would be left for the last)
@@ -404,6 +406,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
 // lane in flight.  The wavefront's reference, which stands for the maximum, is that of its first 512 logits: sums relative to it are as good as long as they
 // stay finite.  Where they do not, or a product of minus infinity with 0 is NaN, or all that the reference is made of may be less than kNothing, which
 // stands for what is not there, the wavefront takes its sums again, with the true maximum and t cut.
+// Bound by memory: 4096 rows of 32000 bf16 51 us (262 MB, 5.1 TB/s).
 template <typename AT, int W, bool ENTROPY>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
   constexpr int R = W == 1 ? 4 : 1, U = 4;
@@ -486,7 +489,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
 }
 
 // The pieces of a row joined.  One workgroup per row; the alternatives of the pieces are sorted lists, and every one finds its rank among all of them: where
-// they are many by halving in every list.
+// they are many by halving in every list.  One row of 131072 with 20 alternatives: 4 us.
 constexpr int kJoinInLds = 4096, kJoinByLook = 512;
 template <typename AT>
 __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
@@ -551,7 +554,8 @@ __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
 }
 
 // D = p (A + B t), plus d_log_prob at the target; t = log2 p.  ROW: a wavefront per row, four rows per workgroup; else a workgroup per piece of
-// kBwdPiece logits of a row.
+// kBwdPiece logits of a row.  The last rows go first: their logits, which the forward pass read last, may still lie in the Infinity Cache (4096 rows of 32000
+// bf16, with the forward pass 141 us from the first row on, 137 from the last, 121.5 with results stored past the caches as well).  Bound by memory: 70 us of those, 524 MB.
 constexpr int kBwdPiece = 8192;
 template <typename AT, bool ROW>
 __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {

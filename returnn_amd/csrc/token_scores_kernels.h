@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
 
 // D = p (A + B t), plus d_log_prob at the target; t = log2 p.  ROW: a wavefront per row, four rows per workgroup; else a workgroup per piece of
 // kBwdPiece logits of a row.  The last rows go first: their logits, which the forward pass read last, may still lie in the Infinity Cache (4096 rows of 32000
-// bf16, with the forward pass 141 us from the first row on, 137 from the last, 121.5 with results stored past the caches as well).  Bound by memory: 70 us of those, 524 MB.
+// bf16, a quarter of them without a token, with the forward pass: 141 us from the first row on, 137 from the last, 122 with results stored past the caches
+// as well).  Bound by memory: 70 us of those, 459 MB.
 constexpr int kBwdPiece = 8192;
 template <typename AT, bool ROW>
 __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {

@@ -275,9 +275,15 @@ static int scores_check(const char* what, const void* logits, int64_t* ld, const
   return RTN_OK;
 }
 
-// Pieces of a row: where alternatives are wanted, as many as it takes for 16 wavefronts to hold a piece in registers; else one, but as many where few
-// rows would leave most of the device idle.
-static int64_t scores_splits(int64_t rows, int64_t V, int32_t top_k) { return top_k > 0 || rows < 256 ? (V + kMaxSegment - 1) / kMaxSegment : 1; }
+// Pieces of a row: where alternatives are wanted, as many as it takes for 16 wavefronts to hold a piece in registers, or, where that are several and few rows leave
+// most of the device idle, for 8 wavefronts with half as many logits each (us, the former / the latter, 20 alternatives of float32: one row of 131072 10.4 / 8.6, 12 rows of
+// 131072 11.5 / 10.3, 40 rows of 131072 13.8 / 14.8, one row of 10^6 11.8 / 24.3).  Else one, but where rows are few as many as in the first case.
+constexpr int kSmallSegment = 8 * 64 * 16;
+static int64_t scores_splits(int64_t rows, int64_t V, int32_t top_k) {
+  const int64_t pieces = (V + kMaxSegment - 1) / kMaxSegment, small = (V + kSmallSegment - 1) / kSmallSegment;
+  if (top_k > 0 && pieces > 1 && small <= 64 && rows * small <= 256) return small;
+  return top_k > 0 || rows < 256 ? pieces : 1;
+}
 
 size_t rtn_token_log_probs_workspace_bytes(int64_t rows, int64_t V, int32_t, int32_t top_k) {
   if (rows <= 0 || V <= 0 || top_k < 0) return 0;
@@ -339,7 +345,11 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
           hipLaunchKernelGGL((k_token_scores<AT, 16, ENTROPY>), one, dim3(1024), 0, stream, a);
       });
     }
-    if (splits > 1) hipLaunchKernelGGL((k_token_scores_join<AT>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+    if (splits > 1) {
+      // (16 lanes per alternative, but no more wavefronts than are there at once)
+      const unsigned threads = rows > 512 ? 256 : (unsigned)std::clamp<int64_t>((16 * splits * top_k + 63) / 64 * 64, 256, 1024);
+      hipLaunchKernelGGL((k_token_scores_join<AT>), dim3((unsigned)rows), dim3(threads), 0, stream, a);
+    }
   });
   return launched("token log probabilities");
 }

@@ -4,6 +4,8 @@
 //   D_v = d_log_prob (1[v = target] - p_v) - d_entropy p_v (log p_v + entropy)
 #pragma once
 
+#include <type_traits>
+
 #include "sequence_common.h"
 
 namespace rtn {
@@ -66,6 +68,17 @@ __device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
     v = o > v ? o : v;
   }
   return v;
+}
+
+__device__ __forceinline__ unsigned wave_min(unsigned v) {
+  auto other = [&](auto ctrl) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true); };
+  auto least = [](unsigned p, unsigned q) { return p < q ? p : q; };
+  v = least(v, other(std::integral_constant<int, 0xB1>()));  // (as in over_wave)
+  v = least(v, other(std::integral_constant<int, 0x4E>()));
+  v = least(v, other(std::integral_constant<int, 0x141>()));
+  v = least(v, other(std::integral_constant<int, 0x140>()));
+  auto at = [&](int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); };
+  return least(least(at(0), at(16)), least(at(32), at(48)));
 }
 
 constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
@@ -148,33 +161,40 @@ __device__ __forceinline__ void put_alternative(const ScoresArgs& a, long long r
   }
 }
 
+// The sum over 16 neighbouring lanes, in all of them.
+__device__ __forceinline__ int quarter_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);
+}
 // How many of the n of a list are larger than `mine`, of which 16 neighbouring lanes look at every 16th: the same in all of them.  (One lane by itself goes through
 // a chain of look-ups and 64-bit comparisons: of 44, which is usual for 12 alternatives, 3000 clocks, a fifth of the kernel.)
 __device__ __forceinline__ int rank_in(const unsigned long long* list, int n, unsigned long long mine, int lane) {
   int rank = 0;
 #pragma unroll 4
   for (int o = lane & 15; o < n; o += 16) rank += list[o] > mine;
-  rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);
-  rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);
-  rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true);
-  return rank + __builtin_amdgcn_update_dpp(0, rank, 0x140, 0xF, 0xF, true);
+  return quarter_sum(rank);
 }
 
 // Sums and alternatives: W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
 // For few rows bound by latency: 12 rows of 32000 bf16 with 12 alternatives 6.8 us, with 1 6.0, the sums alone 4.4; for many by memory and the lists' barriers:
 // 3000 such rows 53 us (192 MB, 3.6 TB/s), the sums alone 40.
 constexpr int kCandidates = 512;
+constexpr int kCoarse = 48;  // alternatives up to which 64 groups are enough
 constexpr int kMaxSegment = 16 * 64 * 32;
 constexpr long long kMaxTokens = 1 << 26;  // (pieces are a multiple of 8 long: with many more of them nothing would be left for the last)
 template <typename AT, int W, int E>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(ScoresArgs a) {
-  constexpr int R = W == 1 ? 4 : 1;  // rows per workgroup
+  constexpr int R = W == 1 ? 4 : 1;            // rows per workgroup
+  constexpr int LANES = W == 1 ? 1 : W / 4;  // that have one of 256 groups
   __shared__ float sums_of[R][W][4];
-  __shared__ float most_of[W][64];
+  __shared__ alignas(16) float most_of[W][64];
   __shared__ unsigned long long list_of[R][kCandidates];
   __shared__ int listed_of[R];
   __shared__ float norm_of[R][2];
   __shared__ int larger_of[64];
+  __shared__ float bound_of[W];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, sub = W == 1 ? threadIdx.x >> 6 : 0, thread = wave * 64 + lane;
   const long long item = blockIdx.x * (long long)R + sub;
   if (W == 1 && item >= a.rows) return;
@@ -231,7 +251,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
   if constexpr (W == 1) {
     if (lane == 0) listed_of[sub] = 0;
   } else {
-    most_of[wave][lane] = most;
+    if (a.top_k > kCoarse) {
+      if (W >= 8) group = __builtin_fmaxf(group, dpp<0xB1>(group));
+      if (W == 16) group = __builtin_fmaxf(group, dpp<0x4E>(group));
+      if (lane % LANES == 0) (&most_of[0][0])[thread / LANES] = group;
+    } else {
+      most_of[wave][lane] = most;
+    }
     if (lane == 0) sums_of[0][wave][0] = sums.m, sums_of[0][wave][1] = sums.s, sums_of[0][wave][2] = sums.w;
     if (thread == 0) listed_of[0] = 0;
     if (wave == 0) larger_of[lane] = 0;
@@ -270,12 +296,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
     n = *(volatile int*)listed;
   };
   if (finite) {
-    // A bound from below: the logits are dealt to 16 groups, or to 64 for more than 16 alternatives, and the top_k-th largest of the groups' maxima is
-    // reached by top_k logits at least.  What reaches it is listed (for 1, 12, 20, 64 alternatives about 1, 21, 24, 300) and finds its rank in the list.  (The
-    // top_k-th largest of 128 maxima, found bit by bit, took longer than all the rest: one row of 32768 float32 with 12 alternatives 9.6 us, with this 6.3.)
-    // The groups are the wavefronts, or what neighbouring lanes of all wavefronts have.
+    // A bound from below: the logits are dealt to 16 groups, to 64 for more than 16 alternatives or (unless the row has one wavefront) to 256 for more than
+    // kCoarse, and the top_k-th largest of the groups' maxima is reached by top_k logits at least.  What reaches it is listed (for 1, 12, 20, 64 alternatives
+    // about 1, 21, 24, 74) and finds its rank in the list.  (The top_k-th largest of 128 maxima, found bit by bit, took longer than all the rest: one row of
+    // 32768 float32 with 12 alternatives 9.6 us, with this 6.3.  64 groups for 64 alternatives: 12 rows of 32000 bf16 16.5 us, with 256 9.1; 16 groups
+    // and 64 for 5: 9000 rows of 500 12.5 and 17.1.)  The groups are the wavefronts, or what neighbouring lanes have, of all wavefronts or of one.
     if constexpr (W > 1) {
-      if (W < 16 || a.top_k > 16) {
+      if ((W < 16 || a.top_k > 16) && a.top_k <= kCoarse) {
 #pragma unroll
         for (int o = 0; o < W; ++o) group = __builtin_fmaxf(group, most_of[o][lane]);
       }
@@ -289,6 +316,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
         group = __shfl(group, lane * 4 & 63);
       }
       bound = lane_of(kth_of_quarter(group, a.top_k), 0);
+    } else if (W > 1 && a.top_k > kCoarse) {
+      const float* maxima = &most_of[0][0];
+      const int part = thread % LANES;
+      group = maxima[thread / LANES];
+      int larger = 0;  // (a group's lanes look at a part of the others each, from different banks on)
+#pragma unroll 4
+      for (int o = 0; o < 256 / LANES; o += 4) {
+        const float* four = maxima + part * (256 / LANES) + (o + 4 * part) % (256 / LANES);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) larger += four[k] > group;
+      }
+      if (LANES > 1) larger += __builtin_amdgcn_update_dpp(0, larger, 0xB1, 0xF, 0xF, true);
+      if (LANES > 2) larger += __builtin_amdgcn_update_dpp(0, larger, 0x4E, 0xF, 0xF, true);
+      bound = wave_max(larger < a.top_k ? -group : -inf);
+      if (lane == 0) bound_of[wave] = bound;
+      __syncthreads();
+      bound = -wave_max(lane < W ? bound_of[lane % W] : -inf);
     } else {
       int larger = 0;  // (every wavefront looks at some of the others)
 #pragma unroll 4
@@ -488,16 +532,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
   }
 }
 
-// The pieces of a row joined.  One workgroup per row; the alternatives of the pieces are sorted lists, and every one finds its rank among all of them: where
-// they are many by halving in every list.  One row of 131072 with 20 alternatives: 4 us.
-constexpr int kJoinInLds = 4096, kJoinByLook = 512;
+// The pieces of a row joined.  One workgroup per row.  The alternatives of the pieces are sorted lists: with P of them, the least of their ceil(top_k / P)-th
+// ones is reached by top_k at least; what reaches it finds its rank among what does.  One row of 131072 with 20 alternatives, 16 pieces:
+// 2 us of 8.6; with a rank among all of them, 44 instead of about 30 look-ups, 4.5.
+constexpr int kJoinInLds = 4096;
 template <typename AT>
-__global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
-  __shared__ unsigned long long held[kJoinInLds];
+__global__ __launch_bounds__(1024) void k_token_scores_join(ScoresArgs a) {
+  __shared__ unsigned long long list[kJoinInLds];
+  __shared__ int listed;
+  const int threads = blockDim.x;
   const long long r = blockIdx.x;
   const long long target = a.targets ? a.targets[r] : 0;
   if (target < 0) {
-    no_row(a, r, threadIdx.x, 256);
+    no_row(a, r, threadIdx.x, threads);
     return;
   }
   const int lane = threadIdx.x & 63;
@@ -516,40 +563,53 @@ __global__ __launch_bounds__(256) void k_token_scores_join(ScoresArgs a) {
   const RowNorm norm(sums);
   const long long n = (long long)a.splits * a.top_k;
   const unsigned long long* all = a.part_top + r * n;
-  if (n <= kJoinInLds) {
-    for (int j = threadIdx.x; j < n; j += 256) held[j] = all[j];
-    __syncthreads();
+  unsigned bound = 0xFFFFFFFFu;
+  for (int p = lane; p < a.splits; p += 64) {
+    const unsigned reach = (unsigned)(all[(long long)p * a.top_k + (a.top_k - 1) / a.splits] >> 32);
+    bound = reach < bound ? reach : bound;
   }
-  if (n <= kJoinByLook) {
-    for (int j = threadIdx.x >> 4; j < n; j += 16) {
-      const unsigned long long mine = held[j];
-      const int rank = rank_in(held, (int)n, mine, lane);
-      if ((lane & 15) == 0 && rank < a.top_k) {
-        a.top_log_prob[r * a.top_k + rank] = norm.log_prob(logit_of(mine));
-        a.top_ids[r * a.top_k + rank] = (int64_t)(unsigned)~(unsigned)mine;
-      }
+  bound = wave_min(bound);
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  for (long long j = threadIdx.x; j < n; j += threads) {
+    const unsigned long long q = all[j];
+    if ((unsigned)(q >> 32) >= bound) {
+      const int at = atomicAdd(&listed, 1);
+      if (at < kJoinInLds) list[at] = q;
+    }
+  }
+  __syncthreads();
+  auto put = [&](int rank, unsigned long long q) {
+    if ((lane & 15) == 0 && rank < a.top_k) {
+      a.top_log_prob[r * a.top_k + rank] = norm.log_prob(logit_of(q));
+      a.top_ids[r * a.top_k + rank] = (int64_t)(unsigned)~(unsigned)q;
+    }
+  };
+  if (listed <= kJoinInLds) {
+    const int count = listed;
+    for (int j = threadIdx.x >> 4; j < count; j += threads >> 4) {
+      const unsigned long long q = list[j];
+      put(rank_in(list, count, q, lane), q);
     }
     return;
   }
-  for (long long j = threadIdx.x; j < n; j += 256) {
-    const unsigned long long mine = n <= kJoinInLds ? held[j] : all[j];
-    long long rank = 0;
-    for (int p = 0; p < a.splits && rank < a.top_k; ++p) {
-      int low = 0, high = a.top_k;  // how many of piece p are larger
+  // Too many (there are more than 64 pieces, of logits most of which are equal): 16 lanes look at 16 of the pieces' lists at once, by halving.
+  for (long long j = threadIdx.x >> 4; j < n; j += threads >> 4) {
+    const unsigned long long q = all[j];
+    int rank = 0;
+    for (int p0 = 0; p0 < a.splits && rank < a.top_k; p0 += 16) {
+      const int p = p0 + (lane & 15);
+      int low = 0, high = p < a.splits ? a.top_k : 0;  // how many of piece p are larger
       while (low < high) {
         const int mid = (low + high) / 2;
-        const unsigned long long q = n <= kJoinInLds ? held[p * a.top_k + mid] : all[(long long)p * a.top_k + mid];
-        if (q > mine)
+        if (all[(long long)p * a.top_k + mid] > q)
           low = mid + 1;
         else
           high = mid;
       }
-      rank += low;
+      rank += quarter_sum(low);
     }
-    if (rank < a.top_k) {
-      a.top_log_prob[r * a.top_k + rank] = norm.log_prob(logit_of(mine));
-      a.top_ids[r * a.top_k + rank] = (int64_t)(unsigned)~(unsigned)mine;
-    }
+    put(rank, q);
   }
 }
 

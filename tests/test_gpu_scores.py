@@ -205,6 +205,24 @@ def test_ties(V):
             assert numpy.array_equal(s.top_ids.cpu().numpy(), ids), (dtype, k)
 
 
+@pytest.mark.parametrize("V,k", [(40000, 64), (65540, 33), (131072, 64), (500001, 7), (3000000, 64)])
+def test_alternatives_of_rows_in_pieces(V, k):
+    """Equal logits everywhere, or in one of the pieces, and best ones that all lie in one piece: ties go to the lower index."""
+    announce("scores pieces", V, k)
+    flat = torch.zeros((1, V), device=DEV)
+    late = flat.clone()
+    late[0, V - 100 : V - 100 + 2 * k : 2] = 1.0
+    spread = flat.clone()
+    spread[0, :: V // 50] = 2.0
+    for logits in (flat, late, spread):
+        s = token_log_probs(logits, top_k=k)
+        want = torch.sort(logits[0].cpu(), descending=True, stable=True).indices[:k]
+        assert torch.equal(s.top_ids[0].cpu(), want)
+        # (a float32 result: the logarithm of a sum of 64-bit terms, and the sum's roundings, some units of 2^-24 each of up to 16)
+        exact = torch.log_softmax(logits[0].double(), dim=-1)[s.top_ids[0]]
+        assert (s.top_log_probs[0].double() - exact).abs().max() < 64 * 2.0**-24 * 16
+
+
 def test_large_logits():
     """What a sum of one number for lse would round away: logits around 1e4, differences of a few."""
     announce("scores large")

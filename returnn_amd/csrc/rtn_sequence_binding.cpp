@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -54,7 +55,10 @@ void same_device(const Tensor& t, const Tensor& as, const char* what, const char
 Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
 Tensor packed(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 void* pointer(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
-Tensor scratch(size_t bytes, const Tensor& like) { return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor(); }
+// (not through the dispatcher: host time of the alternatives of 12 rows 5.6 us with it, 5.0 without)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return fresh(sizes, like.scalar_type(), like); }
+Tensor scratch(size_t bytes, const Tensor& like) { return bytes ? fresh({(int64_t)bytes}, at::kByte, like) : Tensor(); }
 
 // Elements from one row to the next where a row is what the last axis holds and the rows, in order, are equally far apart; 0 where they are not.
 int64_t row_pitch(const Tensor& t) {
@@ -94,8 +98,8 @@ Recurrence recurrence_forward(const Tensor& x_in, const Tensor& c0, const Tensor
   const int dtype = dtype_of(x);
   c10::DeviceGuard guard(x.device());
   Recurrence r;
-  r.y = at::empty({T, B, n}, x.options());
-  r.c = at::empty({B, n}, x.options().dtype(at::kFloat));
+  r.y = fresh({T, B, n}, x);
+  r.c = fresh({B, n}, at::kFloat, x);
   if (keep) r.saved = scratch(abi.recurrence_saved_bytes(T, (int)B, (int)n, dtype), x);
   const size_t bytes = abi.recurrence_fwd_workspace_bytes(T, (int)B, (int)n, dtype);
   const Tensor ws = scratch(bytes, x);
@@ -124,7 +128,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
     c10::DeviceGuard guard(x.device());
     const Tensor dy = rows_of(grads[0].defined() ? grads[0] : at::zeros({T, B, n}, x.options()), &ldd);
     const Tensor dc = grads[1].defined() ? packed(grads[1]) : Tensor();
-    const Tensor dx = at::empty({T, B, 4 * n}, x.options()), dc0 = at::empty({B, n}, x.options().dtype(at::kFloat));
+    const Tensor dx = fresh({T, B, 4 * n}, x), dc0 = fresh({B, n}, at::kFloat, x);
     const size_t bytes = abi.recurrence_bwd_workspace_bytes(T, (int)B, (int)n, dtype);
     const Tensor ws = scratch(bytes, x);
     check_rc(abi.recurrence_bwd(pointer(x), ld, nullptr, (const int64_t*)pointer(lens), pointer(saved[2]), pointer(dy), ldd, (const float*)pointer(dc), pointer(dx),
@@ -186,7 +190,7 @@ Tensor dropout_call(const Tensor& x_in, const Tensor& residual_in, const Tensor&
     if (residual.defined()) residual = rows_of(residual, &ldr);
   }
   c10::DeviceGuard guard(x.device());
-  const Tensor y = at::empty(x.sizes(), x.options());
+  const Tensor y = fresh(x.sizes(), x);
   if (y.numel())
     check_rc(abi.dropout(pointer(x), ldx, pointer(residual), ldr, pointer(y), times, rows, width, dtype_of(x), (int)key.threshold, key.seed, key.offset,
                          (const int64_t*)pointer(offset), key.same_over_time, current_stream(x.device())));
@@ -245,15 +249,14 @@ Scores scores_forward(const Tensor& logits_in, const Tensor& targets, bool entro
   const int64_t V = logits.size(-1), rows = c10::multiply_integers(lead);
   const int dtype = dtype_of(logits);
   c10::DeviceGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
   Scores s;
-  if (targets.defined()) s.log_prob = at::empty(lead, f32);
-  if (entropy) s.entropy = at::empty(lead, f32);
+  if (targets.defined()) s.log_prob = fresh(lead, at::kFloat, logits);
+  if (entropy) s.entropy = fresh(lead, at::kFloat, logits);
   std::vector<int64_t> alternatives(lead.begin(), lead.end());
   alternatives.push_back(top_k);
-  s.top_log_prob = at::empty(alternatives, f32);
-  s.top_ids = at::empty(alternatives, f32.dtype(at::kLong));
-  if (keep) s.norm = at::empty({rows, 2}, f32);
+  s.top_log_prob = fresh(alternatives, at::kFloat, logits);
+  s.top_ids = fresh(alternatives, at::kLong, logits);
+  if (keep) s.norm = fresh({rows, 2}, at::kFloat, logits);
   const size_t bytes = abi.scores_workspace_bytes(rows, V, dtype, (int)top_k);
   const Tensor ws = scratch(bytes, logits);
   check_rc(abi.scores_fwd(pointer(logits), ld, (const int64_t*)pointer(targets), rows, V, dtype, (int)top_k, (float*)pointer(s.log_prob), (float*)pointer(s.norm),
@@ -285,7 +288,7 @@ struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
     const Tensor g = targets.defined() ? grads[at_grad++] : Tensor(), ge = entropy.defined() ? grads[at_grad++] : Tensor();
     c10::DeviceGuard guard(logits.device());
     const Tensor g1 = g.defined() ? packed(g) : Tensor(), g2 = ge.defined() ? packed(ge) : Tensor();
-    const Tensor D = at::empty(logits.sizes(), logits.options());
+    const Tensor D = fresh(logits.sizes(), logits);
     const int64_t V = logits.size(-1), rows = norm.size(0);
     check_rc(abi.scores_bwd(pointer(logits), ld, (const int64_t*)pointer(targets), (const float*)pointer(norm), (const float*)pointer(entropy), (const float*)pointer(g1),
                             (const float*)pointer(g2), pointer(D), rows, V, dtype_of(logits), current_stream(logits.device())));

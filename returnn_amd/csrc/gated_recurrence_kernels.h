@@ -51,17 +51,6 @@ struct RecurrenceArgs {
 template <typename AT, int VEC>
 struct Channels;
 template <>
-struct Channels<float, 1> {
-  typedef unsigned Raw;
-  static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
-  template <bool STREAMED>
-  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
-    __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, STREAMED ? kStreamed : 0);
-  }
-  static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, r); }
-  static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned, v[0]); }
-};
-template <>
 struct Channels<__bf16, 1> {
   typedef unsigned short Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b16(row, at, 0, 0); }
@@ -72,21 +61,52 @@ struct Channels<__bf16, 1> {
   static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, (unsigned)r << 16); }
   static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned short, (__bf16)v[0]); }
 };
-template <>
-struct Channels<__bf16, 2> {
+struct OneWord {
   typedef unsigned Raw;
   static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b32(row, at, 0, 0); }
   template <bool STREAMED>
   static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
     __builtin_amdgcn_raw_buffer_store_b32(v, row, at, 0, STREAMED ? kStreamed : 0);
   }
+};
+struct TwoWords {
+  typedef unsigned Raw __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ Raw load(__amdgpu_buffer_rsrc_t row, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b64(row, at, 0, 0); }
+  template <bool STREAMED>
+  static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t row, unsigned at, Raw v) {
+    __builtin_amdgcn_raw_buffer_store_b64(v, row, at, 0, STREAMED ? kStreamed : 0);
+  }
+};
+template <>
+struct Channels<float, 1> : OneWord {
+  static __device__ __forceinline__ void get(Raw r, float (&v)[1]) { v[0] = __builtin_bit_cast(float, r); }
+  static __device__ __forceinline__ Raw set(const float (&v)[1]) { return __builtin_bit_cast(unsigned, v[0]); }
+};
+template <>
+struct Channels<float, 2> : TwoWords {
+  static __device__ __forceinline__ void get(Raw r, float (&v)[2]) {
+    v[0] = __builtin_bit_cast(float, (unsigned)r.x);
+    v[1] = __builtin_bit_cast(float, (unsigned)r.y);
+  }
+  static __device__ __forceinline__ Raw set(const float (&v)[2]) { return Raw{__builtin_bit_cast(unsigned, v[0]), __builtin_bit_cast(unsigned, v[1])}; }
+};
+template <>
+struct Channels<__bf16, 2> : OneWord {
   static __device__ __forceinline__ void get(Raw r, float (&v)[2]) {
     v[0] = __builtin_bit_cast(float, r << 16);
     v[1] = __builtin_bit_cast(float, r & 0xFFFF0000u);
   }
-  static __device__ __forceinline__ Raw set(const float (&v)[2]) {
-    return pack_bf16(v[0], v[1]);
+  static __device__ __forceinline__ Raw set(const float (&v)[2]) { return pack_bf16(v[0], v[1]); }
+};
+template <>
+struct Channels<__bf16, 4> : TwoWords {
+  static __device__ __forceinline__ void get(Raw r, float (&v)[4]) {
+    v[0] = __builtin_bit_cast(float, (unsigned)r.x << 16);
+    v[1] = __builtin_bit_cast(float, (unsigned)r.x & 0xFFFF0000u);
+    v[2] = __builtin_bit_cast(float, (unsigned)r.y << 16);
+    v[3] = __builtin_bit_cast(float, (unsigned)r.y & 0xFFFF0000u);
   }
+  static __device__ __forceinline__ Raw set(const float (&v)[4]) { return Raw{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}; }
 };
 
 // Rows of one sequence in an array of frames: frame t begins `frame` bytes after frame t - 1, a row has `bytes`.
@@ -214,7 +234,8 @@ struct Turns {
 // W wavefronts, F frames each.  handed: the runs of the wavefronts, and in [W] the state that the next turn starts from, which the last wavefront
 // leaves there; both twice, so that one barrier a turn is enough.
 // Bound by memory where there are 256 chains or more: T=1000, 32 rows of n=1024 bf16 69 us (328 MB, 4.75 TB/s; a copy of this size reaches 5.4; with gates that
-// cost nothing 67), T=500, 64 rows of n=512 float32 73.5 us (4.5; 71.5).  Ragged lengths save bytes but not the longest sequence's turns: 67 us each of 3/4 of the gates.
+// cost nothing 67), T=500, 64 rows of n=512 float32, two channels a lane, 66.5 us (4.9).  Ragged lengths save bytes but not the longest sequence's turns: 67 and 61.5 us
+// with 3/4 of the gates.
 template <typename AT, int VEC, int F, int W>
 __global__ __launch_bounds__(64 * W) void k_recurrence_fwd(RecurrenceArgs a) {
   typedef Chain<AT, VEC> C;

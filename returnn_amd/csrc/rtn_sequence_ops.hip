@@ -59,34 +59,41 @@ void with_bool(bool v, F f) {
 }
 
 // ---- gated recurrence ---------------------------------------------------------------------------------------------
-// Frames that a wavefront holds at once, forward and in the gradient: as many as leave 16 wavefronts their registers.
-constexpr int kForwardFrames = 8, kGradientFrames = 4;
+// Frames that a wavefront holds at once, forward, with twice as many channels, and in the gradient: as many as leave 16 wavefronts their registers.
+constexpr int kForwardFrames = 8, kWideFrames = 4, kGradientFrames = 4;
 
 constexpr int64_t kMaxFrames = 1 << 30, kMaxChannels = 1 << 26;  // (steps are 32-bit numbers, and so is a place in a row, in bytes)
 
 struct RecurrencePlan {
   int vec, waves, strips, segments;
+  bool wide;
   int64_t chains, segment;
 };
-// Wavefronts: as few as take all frames at once, but no more than give every compute unit the 16 that it has registers for: 16 below 512 chains, else 8.
-// (us, 16 / 8: T=500 64 rows of n=512 float32 78 / 73; T=64 64 rows of n=2048 bf16 forward 23.5 / 18.5, gradient 33.4 / 28.6.  8 / 4 with 2048 chains
+// Channels of a lane: what a word of 32 bits holds, pieces of 256 bytes for a wavefront.  Forward, twice as many where that makes half as many workgroups that still fill the
+// device (they read faster, 4.9 instead of 4.5 TB/s, but rounds that are not full cost more).  us, narrow / wide: T=500 n=1024 bf16 36 rows 56.9 / 52.4, 64 rows 72.7 / 67.7,
+// 80 rows 94 / 105, 112 rows 128 / 121, 160 rows 170 / 179, 192 rows 208 / 194; T=300 n=512 float32 64 rows 47.3 / 42.6; T=64 64 rows of n=2048 bf16 18.2 / 19.1.
+// (The gradient: 64 rows 130 / 128, with ragged lengths 117 / 129; 128 rows 243 / 227, 230 / 237.  It stays narrow.)
+// Wavefronts: as few as take all frames at once, but no more than give every compute unit the 16 that it has registers for: 16 where all chains run at once so, else
+// 8.  (us, 16 / 8: T=300 40 rows of n=512 float32 41.9 / 34.2; T=64 64 rows of n=2048 bf16 forward 23.5 / 18.5, gradient 33.4 / 28.6.  8 / 4 with 2048 chains
 // and more: T=500 256 rows of n=1024 bf16 270 / 282 and 473 / 482, T=200 500 rows of n=512 float32 221 / 210 and 381 / 384.)
 // Segments: as many as the time estimate is least for, in turns of W F frames: a workgroup takes its turns one after the other and half of one to start, 256 run
 // at once; more than one segment costs the pre-pass, whose bytes are 0.6 (gradient 0.33) of the others, and a launch of 1.5.  Measured (us, one segment / these):
 // T=4000 1 row of n=1024 bf16 forward 164 / 19, gradient 251 / 24; T=333 11 rows of n=1001 bf16 gradient 31.5 / 27.9; T=1000 32 rows of n=512 bf16 gradient 91 / 76.
 RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, bool gradient) {
-  const int frames = gradient ? kGradientFrames : kForwardFrames;
   RecurrencePlan p;
   p.vec = dtype == RTN_DTYPE_BF16 && n > 1 ? 2 : 1;
   p.strips = (n + 64 * p.vec - 1) / (64 * p.vec);
+  const int64_t half = (int64_t)p.strips / 2 * B, full_rounds = (half + 255) / 256 * 256;
+  p.wide = !gradient && p.strips % 2 == 0 && T > 64 && half > 128 && (half <= 256 || 8 * half >= 7 * full_rounds);
+  if (p.wide) p.vec *= 2, p.strips /= 2;
   p.chains = (int64_t)p.strips * B;
-  const int most = p.chains >= 512 ? 8 : 16;
+  const int frames = gradient ? kGradientFrames : (p.wide ? kWideFrames : kForwardFrames), most = p.chains > 256 ? 8 : 16;
   p.waves = 1;
   for (int w : {4, 8, 16})
     if (p.waves * frames < T && w <= most) p.waves = w;
   const int64_t turn = (int64_t)p.waves * frames, turns = std::max<int64_t>(1, (T + turn - 1) / turn);
   int64_t segments = 1;
-  if (p.waves == 16 && p.chains <= 256) {
+  if (p.waves == 16 && !p.wide && p.chains <= 256) {
     auto estimate = [&](int64_t k) { return (double)((p.chains * k + 255) / 256) * ((turns + k - 1) / k + 0.5); };
     double least = estimate(1);
     for (int64_t k = 2; k <= std::min<int64_t>(turns, 512 / p.chains); ++k) {
@@ -131,6 +138,20 @@ void with_recurrence(int dtype, const RecurrencePlan& p, F f) {
     waves((__bf16)0.f, Count<2>());
   else
     waves((__bf16)0.f, Count<1>());
+}
+// ... of a wide plan (more frames than one turn, so 8 or 16 wavefronts).
+template <typename F>
+void with_wide_recurrence(int dtype, const RecurrencePlan& p, F f) {
+  auto waves = [&](auto type, auto vec) {
+    if (p.waves == 8)
+      f(type, vec, Count<8>());
+    else
+      f(type, vec, Count<16>());
+  };
+  if (dtype == RTN_DTYPE_F32)
+    waves(0.f, Count<2>());
+  else
+    waves((__bf16)0.f, Count<4>());
 }
 
 // The checks that both directions share; `ld` is set where it was left out.
@@ -180,15 +201,22 @@ int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const 
   if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
   const int apart = strips_apart(p, B, n, dtype, {X, Y}, {ldX, n});
   const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, apart, (float*)workspace};
-  with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
-    typedef decltype(type) AT;
-    constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;
-    const hipStream_t stream = (hipStream_t)hip_stream;
-    if constexpr (W == 16)
-      if (p.segments > 1)
-        hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kForwardFrames, W, true>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
-    hipLaunchKernelGGL((k_recurrence_fwd<AT, VEC, kForwardFrames, W>), dim3((unsigned)(p.chains * p.segments)), dim3(64 * W), 0, stream, a);
-  });
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  const dim3 grid((unsigned)(p.chains * p.segments));
+  if (p.wide)
+    with_wide_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
+      constexpr int W = decltype(waves)::value;
+      hipLaunchKernelGGL((k_recurrence_fwd<decltype(type), decltype(vec)::value, kWideFrames, W>), grid, dim3(64 * W), 0, stream, a);
+    });
+  else
+    with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
+      typedef decltype(type) AT;
+      constexpr int VEC = decltype(vec)::value, W = decltype(waves)::value;
+      if constexpr (W == 16)
+        if (p.segments > 1)
+          hipLaunchKernelGGL((k_recurrence_runs<AT, VEC, kForwardFrames, W, true>), dim3((unsigned)(p.chains * (p.segments - 1))), dim3(64 * W), 0, stream, a);
+      hipLaunchKernelGGL((k_recurrence_fwd<AT, VEC, kForwardFrames, W>), grid, dim3(64 * W), 0, stream, a);
+    });
   return launched("gated recurrence");
 }
 

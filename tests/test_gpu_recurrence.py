@@ -94,6 +94,21 @@ def test_against_the_definition(T, B, n, dtype):
         check_gradient(dx, dc0, x, dy, dc, c0, lens, direction)
 
 
+@pytest.mark.parametrize("T,B,n,dtype", [(131, 70, 201, "f32"), (70, 230, 201, "f32"), (131, 140, 201, "bf16"), (67, 460, 130, "bf16"), (90, 48, 640, "f32"), (80, 64, 512, "bf16")])
+def test_many_rows(T, B, n, dtype):
+    """Enough of them for lanes that have more channels, in one round and in several; and rows with a pitch."""
+    announce("recurrence many rows", T, B, n, dtype)
+    for direction in (1, -1):
+        x, c0, dy, dc, lens = problem(T, B, n, dtype, "ragged", seed=T + B)
+        y, c, dx, dc0 = run(x, c0, dy, dc, lens, direction, True)
+        check_forward(y, c, x, c0, lens, direction)
+        check_gradient(dx, dc0, x, dy, dc, c0, lens, direction)
+        wide = torch.full((T, B, 4 * n + 3), float("nan"), dtype=x.dtype, device=DEV)
+        wide[..., 1 : 4 * n + 1] = x.to(DEV)
+        y2, c2 = gated_recurrence(wide[..., 1 : 4 * n + 1], state=c0.to(DEV), seq_lens=torch.as_tensor(lens), direction=direction)
+        assert torch.equal(y, y2) and torch.equal(c, c2)
+
+
 @pytest.mark.parametrize("keep", [-30.0, 0.0, 8.0, 100.0])
 def test_gates_that_forget_or_keep_everything(keep):
     """Products of many forget gates that underflow, and states that add up over all frames."""

@@ -129,7 +129,8 @@ struct RowNorm {
   float base, log_s;
   RowNorm() = default;
   __device__ __forceinline__ RowNorm(RowSums r) : base(r.m), log_s(logf(r.s)) {}
-  __device__ __forceinline__ float log_prob(float x) const { return x == -__builtin_inff() ? x : (x - base) - log_s; }
+  // (minus infinity of a token that is not allowed, but not beside a NaN)
+  __device__ __forceinline__ float log_prob(float x) const { return x == -__builtin_inff() && log_s == log_s ? x : (x - base) - log_s; }
 };
 template <typename AT>
 __device__ __forceinline__ RowNorm row_results(const ScoresArgs& a, long long r, long long target, RowSums sums) {
@@ -447,10 +448,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
 }
 
 // Sums without alternatives, read as they come: W wavefronts per row or piece of one (W = 1: four rows per workgroup), U times eight logits per
-// lane in flight.  The wavefront's reference, which stands for the maximum, is that of its first 512 logits: sums relative to it are as good as long as they
-// stay finite.  Where they do not, or a product of minus infinity with 0 is NaN, or all that the reference is made of may be less than kNothing, which
-// stands for what is not there, the wavefront takes its sums again, with the true maximum and t cut.
-// Bound by memory: 4096 rows of 32000 bf16 51 us (262 MB, 5.1 TB/s).
+// lane in flight.  The wavefront's reference, which stands for the maximum, is that of the first 512 logits among which one is above kNothing (of tokens that are
+// not allowed, minus infinity or the type's lowest value, nothing is left beside it): sums relative to it are as good as long as they stay finite.  Where they
+// do not, or there is no such reference, the wavefront takes its sums again, with the true maximum.
+// Bound by memory: 4096 rows of 32000 bf16 54 us (262 MB, 4.9 TB/s).  (Products of minus infinity left to be NaN and found afterwards: 52, but 262 where
+// tokens are masked.)
 template <typename AT, int W, bool ENTROPY>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
   constexpr int R = W == 1 ? 4 : 1, U = 4;
@@ -469,6 +471,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
   const int v0 = split * a.segment, v1 = v0 + a.segment < a.V ? v0 + a.segment : a.V;
   RowSums sums{kLowest, 0.f, 0.f};
   const bool vector = a.V >= 8;
+  bool referred = false;
 #pragma unroll 1
   for (int from = v0; vector && from + wave * 512 < v1; from += 512 * W * U) {
     Eight<AT> q[U];
@@ -488,31 +491,50 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = begin + k >= mine && begin + k < v1 ? v[k] : kNothing;
       }
-      if (j == 0 && from == v0) {
+      if (!referred) {
         float most = kLowest;
 #pragma unroll
         for (int k = 0; k < 8; ++k) most = __builtin_fmaxf(most, v[k]);
-        sums.m = wave_max(most);
+        sums = {wave_max(most), 0.f, 0.f};
+        referred = sums.m > kNothing;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float t = (v[k] - sums.m) * kLog2E, e = __builtin_amdgcn_exp2f(t);
+        float t = (v[k] - sums.m) * kLog2E;
+        if (ENTROPY) t = __builtin_elementwise_maximum(t, kNoPower);  // (a product of minus infinity with 0 would be NaN)
+        const float e = __builtin_amdgcn_exp2f(t);
         sums.s += e;
         if (ENTROPY) sums.w = __builtin_fmaf(t, e, sums.w);
       }
     }
   }
-  if (__any(!(sums.s + sums.w < __builtin_inff()) || sums.m <= kNothing)) {
-    float most = kLowest;
-    for (int v = v0 + thread * 8; v < v1; v += 512 * W)
-      for (int k = 0; k < 8 && v + k < v1; ++k) most = __builtin_fmaxf(most, load_f32(row + v + k));
-    sums = {wave_max(most), 0.f, 0.f};
-    for (int v = v0 + thread * 8; v < v1; v += 512 * W)
-      for (int k = 0; k < 8 && v + k < v1; ++k) {
-        const float t = __builtin_elementwise_maximum((load_f32(row + v + k) - sums.m) * kLog2E, kNoPower), e = __builtin_amdgcn_exp2f(t);
-        sums.s += e;
-        sums.w = __builtin_fmaf(t, e, sums.w);
+  if (__any(!(sums.s + sums.w < __builtin_inff())) || !referred) {
+    auto each = [&](auto f) {
+#pragma unroll 2
+      for (int at = v0 + thread * 8; at < v1; at += 512 * W) {
+        const int begin = !vector || at < a.V - 8 ? at : a.V - 8;
+        float v[8];
+        if (vector) {
+          Eight<AT> q;
+          q.load(row + begin);
+          q.get(v);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = at + k < v1 ? load_f32(row + at + k) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (begin + k >= at && begin + k < v1) f(v[k]);
       }
+    };
+    float most = kLowest;
+    each([&](float v) { most = __builtin_fmaxf(most, v); });
+    sums = {wave_max(most), 0.f, 0.f};
+    each([&](float v) {
+      const float t = __builtin_elementwise_maximum((v - sums.m) * kLog2E, kNoPower), e = __builtin_amdgcn_exp2f(t);
+      sums.s += e;
+      sums.w = __builtin_fmaf(t, e, sums.w);
+    });
   }
   sums.s = wave_sum(sums.s);
   if (ENTROPY) sums.w = wave_sum(sums.w);

@@ -151,6 +151,34 @@ def test_masked_logits(V, dtype):
     assert not grads[2][2].any() and not grads[2][7].any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(9, 1), (9, 50), (300, 1000), (9, 5000), (300, 9001), (9, 20000), (9, 70001)])
+def test_masked_logits_without_alternatives(rows, V, dtype):
+    """The same, and masks of whole ranges of tokens, from the first one on; and values that are not finite."""
+    announce("scores masked sums", rows, V, dtype)
+    lowest = torch.finfo(_DTYPES[dtype]).min
+    logits, targets = problem((rows,), V, dtype, seed=6)
+    blocked = torch.rand((rows, V), generator=torch.Generator().manual_seed(5)) < 0.5
+    logits[0][blocked[0]] = -INF
+    logits[1][blocked[1]] = lowest
+    logits[2] = -INF
+    logits[3] = lowest
+    logits[4, : V // 2] = -INF
+    logits[5, : V - V // 3] = lowest
+    logits[6, V // 4 :] = -INF
+    logits[7] = -INF
+    logits[7, V - 1] = -2.0
+    logits[8, : V // 2] = lowest
+    logits[8, V // 2 :] = -1e9
+    s, grads = run(logits, targets, 0)
+    check(logits, targets, 0, s, grads)
+    for k, bad in enumerate((float("nan"), INF)):
+        logits[k, V - 1 - k * (V // 3)] = bad
+        logits[k + 2, (k + 1) * V // 4] = bad
+    s, _ = run(logits, targets, 0)
+    assert torch.isnan(s.log_probs[:4]).all() and torch.isnan(s.entropy[:4]).all() and not torch.isnan(s.entropy[4:]).any()
+
+
 @pytest.mark.parametrize("V", [3, 90, 3000, 40000])
 def test_not_finite_logits(V):
     """A NaN or an infinity makes its row NaN and no other; it comes first among the alternatives."""

@@ -69,7 +69,10 @@ struct RecurrencePlan {
   bool wide;
   int64_t chains, segment;
 };
-// Channels of a lane: what a word of 32 bits holds, pieces of 256 bytes for a wavefront.  Forward, twice as many where that makes half as many workgroups that still fill the
+// Channels of a lane: what a word of 32 bits holds, pieces of 256 bytes for a wavefront.  In bf16 one, where two would leave half the lanes without any, or where that makes
+// the most workgroups that run at once: each then has half the gates to compute (us, two / one: T=642 89 rows of n=64 forward 31.4 / 23.2, gradient 39.0 / 30.2; T=1000 n=512 32 rows
+// 50.5 / 40.8 and 71.4 / 71.1, 16 rows 29.4 / 35.9 and 42.5 / 50.4; T=300 n=1024 10 rows 17.2 / 13.8 and 19.1 / 18.2, 20 rows 19.5 / 20.5 and 29.4 / 36.8).
+// Forward, twice as many where that makes half as many workgroups that still fill the
 // device (they read faster, 4.9 instead of 4.5 TB/s, but rounds that are not full cost more).  us, narrow / wide: T=500 n=1024 bf16 36 rows 56.9 / 52.4, 64 rows 72.7 / 67.7,
 // 80 rows 94 / 105, 112 rows 128 / 121, 160 rows 170 / 179, 192 rows 208 / 194; T=300 n=512 float32 64 rows 47.3 / 42.6; T=64 64 rows of n=2048 bf16 18.2 / 19.1.
 // (The gradient: 64 rows 130 / 128, with ragged lengths 117 / 129; 128 rows 243 / 227, 230 / 237.  It stays narrow.)
@@ -81,7 +84,8 @@ struct RecurrencePlan {
 // T=4000 1 row of n=1024 bf16 forward 164 / 19, gradient 251 / 24; T=333 11 rows of n=1001 bf16 gradient 31.5 / 27.9; T=1000 32 rows of n=512 bf16 gradient 91 / 76.
 RecurrencePlan recurrence_plan(int64_t T, int32_t B, int32_t n, int32_t dtype, bool gradient) {
   RecurrencePlan p;
-  p.vec = dtype == RTN_DTYPE_BF16 && n > 1 ? 2 : 1;
+  const int64_t of_one = (int64_t)((n + 63) / 64) * B;
+  p.vec = dtype == RTN_DTYPE_BF16 && n > 64 && (of_one <= 128 || of_one > 256) ? 2 : 1;
   p.strips = (n + 64 * p.vec - 1) / (64 * p.vec);
   const int64_t half = (int64_t)p.strips / 2 * B, full_rounds = (half + 255) / 256 * 256;
   p.wide = !gradient && p.strips % 2 == 0 && T > 64 && half > 128 && (half <= 256 || 8 * half >= 7 * full_rounds);

@@ -350,9 +350,14 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
     if (top_k > 0) {
       // As few wavefronts as hold a piece, but where rows are few, more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
       // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).
-      const bool few = rows <= 512;
+      // Many of up to 2048 logits take one wavefront, without barriers (29000 rows of 1000 bf16 four 61, one 27, of 2000 64 and 38; 700 rows of 2000 5.2 and 5.7).
+      const bool few = rows <= 512, many = rows > 1024;
       if (segment <= 64 || (segment <= 512 && !few))
         hipLaunchKernelGGL((k_token_scores_top<AT, 1, 8>), four, dim3(256), 0, stream, a);
+      else if (segment <= 1024 && many)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 16>), four, dim3(256), 0, stream, a);
+      else if (segment <= 2048 && many)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 32>), four, dim3(256), 0, stream, a);
       else if (segment <= 2048)
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 8>), one, dim3(256), 0, stream, a);
       else if (segment <= 4096)

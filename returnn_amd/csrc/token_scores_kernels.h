@@ -189,6 +189,7 @@ template <typename AT, int W, int E>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(ScoresArgs a) {
   constexpr int R = W == 1 ? 4 : 1;            // rows per workgroup
   constexpr int LANES = W == 1 ? 1 : W / 4;  // that have one of 256 groups
+  constexpr bool SINGLE = E == 8 && W == 1;  // logits one by one, not by eights, of which there have to be some
   __shared__ float sums_of[R][W][4];
   __shared__ alignas(16) float most_of[W][64];
   __shared__ unsigned long long list_of[R][kCandidates];
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
   // eight --, of which the ones that an earlier lane has are left out)
   auto own = [&](int j) { return v0 + (j * 64 * W + thread) * 8; };
   auto read = [&](int j) { return own(j) < a.V - 8 ? own(j) : a.V - 8; };
-  if constexpr (W == 1) {
+  if constexpr (SINGLE) {
 #pragma unroll
     for (int k = 0; k < E; ++k) x[k] = k * 64 + lane < v1 ? load_f32(row + k * 64 + lane) : -inf;
   } else {
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (hits >> k & 1u) {
-            if (at < kCandidates) list[at] = alternative(x[8 * j + k], (unsigned)(W == 1 ? k * 64 + lane : read(j) + k));
+            if (at < kCandidates) list[at] = alternative(x[8 * j + k], (unsigned)(SINGLE ? k * 64 + lane : read(j) + k));
             ++at;
           }
       }
@@ -361,9 +362,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
   }
   if (finite) {
     make_list();
-    if (W > 1 && n > kCandidates) {
+    if (!SINGLE && n > kCandidates) {
       // Too many: the largest bound that top_k lanes still reach, to within a 4096th of what is in question.
-      float high = wave_max(lane < W ? sums_of[0][lane % W][0] : kLowest);
+      float high = W > 1 ? wave_max(lane < W ? sums_of[0][lane % W][0] : kLowest) : sums.m;
 #pragma unroll 1
       for (int step = 0; step < 12; ++step) {
         const float mid = 0.5f * bound + 0.5f * high;
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
       mine = 0;
 #pragma unroll 8
       for (int j = 0; j < E; ++j) {
-        const int at = W == 1 ? v0 + j * 64 + lane : own(j >> 3) + (j & 7);
+        const int at = SINGLE ? v0 + j * 64 + lane : own(j >> 3) + (j & 7);
         if (at < v1) {
           const unsigned long long q = alternative(load_f32(row + at), (unsigned)at);
           if (q < last && q > mine) mine = q;
@@ -655,10 +656,11 @@ __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {
   const float base = a.norm[2 * r], log_s = a.norm[2 * r + 1];
   const float g = a.d_log_prob ? a.d_log_prob[r] : 0.f, ge = a.d_entropy ? a.d_entropy[r] : 0.f, h = a.d_entropy ? a.entropy[r] : 0.f;
   const bool none = target < 0 || log_s == -__builtin_inff();
-  const float A = a.targets && target >= a.V ? __builtin_nanf("") : -__builtin_fmaf(ge, h, g), B = -ge * kLn2, c = -log_s * kLog2E;
+  // (256 p is what is multiplied: p may be below the normal numbers where p log p is not)
+  const float A = a.targets && target >= a.V ? __builtin_nanf("") : __builtin_fmaf(ge, h, g) * -0x1p-8f, B = -ge * kLn2 * 0x1p-8f, c = -log_s * kLog2E;
   auto one = [&](float v) {
     const float t = __builtin_elementwise_maximum(__builtin_fmaf(v - base, kLog2E, c), kNoPower);
-    return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(B, t, A);
+    return __builtin_amdgcn_exp2f(t + 8.f) * __builtin_fmaf(B, t, A);
   };
   const bool known = a.targets != nullptr && !none;
   for (long long from = v0; from < v1; from += (long long)THREADS * 8 * N) {

@@ -99,7 +99,7 @@ def run(logits, targets, top_k, entropy=True, seed=1):
 
 SHAPES = [((1,), 1), ((3,), 2), ((2, 2), 7), ((5,), 63), ((4,), 64), ((130,), 65), ((2, 3), 127), ((9,), 500), ((2,), 1023), ((3,), 1025), ((1,), 4096), ((2, 7), 2047), ((17,), 5003),
           ((1,), 10007), ((3,), 32000), ((1,), 131072), ((2,), 65537), ((600,), 33),
-          ((700,), 200), ((3,), 8000), ((600,), 6001)]  # fmt: skip
+          ((700,), 200), ((3,), 8000), ((600,), 6001), ((1100,), 513), ((1100,), 1025)]  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -231,6 +231,30 @@ def test_ties(V):
             s = token_log_probs(logits.to(DEV), top_k=k)
             _, _, _, ids, _ = ref.scores(array(logits), None, k)
             assert numpy.array_equal(s.top_ids.cpu().numpy(), ids), (dtype, k)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [64, 500, 513, 1000, 1025, 2048])
+def test_many_short_rows(V, dtype):
+    """Masks, ties and rows of nothing else, in more rows than have a workgroup each."""
+    announce("scores many short rows", V, dtype)
+    rows, lowest = 1201, torch.finfo(_DTYPES[dtype]).min
+    logits, targets = problem((rows,), V, dtype, seed=8)
+    blocked = torch.rand((rows, V), generator=torch.Generator().manual_seed(9)) < 0.5
+    kind = torch.arange(rows) % 12
+    logits[(kind == 0)[:, None] & blocked] = -INF
+    logits[(kind == 1)[:, None] & blocked] = lowest
+    logits[kind == 2] = -INF
+    logits[kind == 3] = lowest
+    logits[kind == 4] = 0.5
+    logits[kind == 5] = torch.arange(V).div(7, rounding_mode="floor").to(logits.dtype)
+    logits[kind == 6] = -torch.arange(V).to(logits.dtype)
+    logits[kind == 7, V // 3 :] = 9.0
+    logits[kind == 8, : V - 1] = -INF
+    targets[kind == 9] = -1
+    for k in (1, 16, 64):
+        s, grads = run(logits, targets, k)
+        check(logits, targets, k, s, grads)
 
 
 @pytest.mark.parametrize("V,k", [(40000, 64), (65540, 33), (131072, 64), (500001, 7), (3000000, 64)])

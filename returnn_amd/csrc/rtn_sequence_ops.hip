@@ -346,7 +346,16 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   const hipStream_t stream = (hipStream_t)hip_stream;
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
-    const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4));
+    const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4)), sixteen((unsigned)((rows + 15) / 16));
+    // Short rows 16 at a time, but not for many alternatives, of which 16 lanes' maxima tell too little (us, 2000 rows of 96 bf16, one wavefront per row / this: sums 3.5 / 2.7, 5 alternatives 4.6 / 4.1,
+    // 16 alternatives 7.1 / 15.0; 70000 rows 25 / 6.7, 41 / 13.5, 56 / 86).
+    if (V >= 8 && V <= 256 && top_k <= 8) {
+      if (V <= 128)
+        hipLaunchKernelGGL((k_token_scores_short<AT, 8>), sixteen, dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_token_scores_short<AT, 16>), sixteen, dim3(256), 0, stream, a);
+      return;
+    }
     if (top_k > 0) {
       // As few wavefronts as hold a piece, but where rows are few, more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
       // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).

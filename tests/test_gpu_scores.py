@@ -234,7 +234,7 @@ def test_ties(V):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("V", [64, 500, 513, 1000, 1025, 2048])
+@pytest.mark.parametrize("V", [8, 9, 64, 100, 129, 256, 500, 513, 1000, 1025, 2048])
 def test_many_short_rows(V, dtype):
     """Masks, ties and rows of nothing else, in more rows than have a workgroup each."""
     announce("scores many short rows", V, dtype)
@@ -252,9 +252,9 @@ def test_many_short_rows(V, dtype):
     logits[kind == 7, V // 3 :] = 9.0
     logits[kind == 8, : V - 1] = -INF
     targets[kind == 9] = -1
-    for k in (1, 16, 64):
-        s, grads = run(logits, targets, k)
-        check(logits, targets, k, s, grads)
+    for k in (0, 1, 8, 16, 64):
+        s, grads = run(logits, targets, min(k, V))
+        check(logits, targets, min(k, V), s, grads)
 
 
 @pytest.mark.parametrize("V,k", [(40000, 64), (65540, 33), (131072, 64), (500001, 7), (3000000, 64)])

@@ -415,11 +415,14 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
                      nullptr, nullptr, d_log_prob, d_entropy, D, (int)pieces, 0, nullptr, nullptr};
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
-    // (us of 9000 bf16 rows, a wavefront per row / a workgroup per piece: of 500 8.6 / 13.5, of 2000 18.4 / 19.7, of 5000 46.6 / 37.7)
-    if (V <= 2048)
-      hipLaunchKernelGGL((k_token_scores_bwd<AT, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)hip_stream, a);
+    // (us of bf16 rows, a wavefront per row / 16 lanes: 70000 of 96 21.4 / 9.0, 10000 of 256 6.2 / 5.3, 37 of 256 3.4 / 3.6; a wavefront / a workgroup per piece: 9000 of 500
+    // 8.6 / 13.5, of 2000 18.4 / 19.7, of 5000 46.6 / 37.7)
+    if (V <= 256)
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, (hipStream_t)hip_stream, a);
+    else if (V <= 2048)
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)hip_stream, a);
     else
-      hipLaunchKernelGGL((k_token_scores_bwd<AT, false>), dim3((unsigned)(rows * pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 256>), dim3((unsigned)(rows * pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
   });
   return launched("token log probabilities gradient");
 }

@@ -714,17 +714,18 @@ __global__ __launch_bounds__(1024) void k_token_scores_join(ScoresArgs a) {
   }
 }
 
-// D = p (A + B t), plus d_log_prob at the target; t = log2 p.  ROW: a wavefront per row, four rows per workgroup; else a workgroup per piece of
+// D = p (A + B t), plus d_log_prob at the target; t = log2 p.  THREADS: 16 or 64 lanes per row, or 256 for a piece of
 // kBwdPiece logits of a row.  The last rows go first: their logits, which the forward pass read last, may still lie in the Infinity Cache (4096 rows of 32000
 // bf16, a quarter of them without a token, with the forward pass: 141 us from the first row on, 137 from the last, 122 with results stored past the caches
 // as well).  Bound by memory: 70 us of those, 459 MB.
 constexpr int kBwdPiece = 8192;
-template <typename AT, bool ROW>
+template <typename AT, int THREADS>
 __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {
-  constexpr int THREADS = ROW ? 64 : 256, N = ROW ? 1 : kBwdPiece / (256 * 8);
-  const int thread = ROW ? threadIdx.x & 63 : threadIdx.x;
+  constexpr bool ROW = THREADS < 256;
+  constexpr int N = ROW ? 1 : kBwdPiece / (256 * 8);
+  const int thread = threadIdx.x % THREADS;
   const unsigned block = gridDim.x - 1 - blockIdx.x;
-  const long long item = ROW ? block * 4ll + (threadIdx.x >> 6) : block;
+  const long long item = ROW ? block * (256ll / THREADS) + threadIdx.x / THREADS : block;
   if (ROW && item >= a.rows) return;
   const long long r = ROW ? item : (unsigned)item / (unsigned)a.splits, v0 = ROW ? 0 : (item - r * a.splits) * kBwdPiece;
   const long long v1 = ROW ? a.V : (v0 + kBwdPiece < a.V ? v0 + kBwdPiece : a.V);

@@ -358,7 +358,8 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
     }
     if (top_k > 0) {
       // As few wavefronts as hold a piece, but where rows are few, more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
-      // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).
+      // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).  Lanes hold no
+      // more than it takes (3000 rows of 20000 bf16 32 logits 46.7, 24 41.5; 5000 of 10007 42.5 / 38.2).
       // Many of up to 2048 logits take one wavefront, without barriers (29000 rows of 1000 bf16 four 61, one 27, of 2000 64 and 38; 700 rows of 2000 5.2 and 5.7).
       const bool few = rows <= 512, many = rows > 1024;
       if (segment <= 64 || (segment <= 512 && !few))
@@ -373,10 +374,16 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 16>), one, dim3(256), 0, stream, a);
       else if (segment <= 8192 && few)
         hipLaunchKernelGGL((k_token_scores_top<AT, 8, 16>), one, dim3(512), 0, stream, a);
+      else if (segment <= 6144)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 24>), one, dim3(256), 0, stream, a);
       else if (segment <= 8192)
         hipLaunchKernelGGL((k_token_scores_top<AT, 4, 32>), one, dim3(256), 0, stream, a);
+      else if (segment <= 12288)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 24>), one, dim3(512), 0, stream, a);
       else if (segment <= 16384)
         hipLaunchKernelGGL((k_token_scores_top<AT, 8, 32>), one, dim3(512), 0, stream, a);
+      else if (segment <= 24576)
+        hipLaunchKernelGGL((k_token_scores_top<AT, 16, 24>), one, dim3(1024), 0, stream, a);
       else
         hipLaunchKernelGGL((k_token_scores_top<AT, 16, 32>), one, dim3(1024), 0, stream, a);
     } else {

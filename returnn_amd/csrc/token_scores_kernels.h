@@ -179,8 +179,8 @@ __device__ __forceinline__ int rank_in(const unsigned long long* list, int n, un
 }
 
 // Sums and alternatives: W wavefronts per row or piece of one (W = 1: four rows per workgroup), E logits per lane, all in registers.
-// For few rows bound by latency: 12 rows of 32000 bf16 with 12 alternatives 6.8 us, with 1 6.0, the sums alone 4.4; for many by memory and the lists' barriers:
-// 3000 such rows 53 us (192 MB, 3.6 TB/s), the sums alone 40.
+// For few rows bound by latency: 12 rows of 32000 bf16 with 12 alternatives 6.8 us, with 1 6.0, the sums alone 4.8; for many by memory and the lists' barriers:
+// 3000 such rows 52 us (192 MB, 3.7 TB/s), the sums alone 42.
 constexpr int kCandidates = 512;
 constexpr int kCoarse = 48;  // alternatives up to which 64 groups are enough
 constexpr int kMaxSegment = 16 * 64 * 32;
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
 
 // The pieces of a row joined.  One workgroup per row.  The alternatives of the pieces are sorted lists: with P of them, the least of their ceil(top_k / P)-th
 // ones is reached by top_k at least; what reaches it finds its rank among what does.  One row of 131072 with 20 alternatives, 16 pieces:
-// 2 us of 8.6; with a rank among all of them, 44 instead of about 30 look-ups, 4.5.
+// 3.4 us of 8.6 (by itself; with a rank among all 320 of them 5.8).
 constexpr int kJoinInLds = 4096;
 template <typename AT>
 __global__ __launch_bounds__(1024) void k_token_scores_join(ScoresArgs a) {

@@ -714,7 +714,7 @@ __global__ __launch_bounds__(1024) void k_token_scores_join(ScoresArgs a) {
   }
 }
 
-// D = p (A + B t), plus d_log_prob at the target; t = log2 p.  THREADS: 16 or 64 lanes per row, or 256 for a piece of
+// D = p (A + B t), plus d_log_prob at the target; t = log2 p / 2.  THREADS: 16 or 64 lanes per row, or 256 for a piece of
 // kBwdPiece logits of a row.  The last rows go first: their logits, which the forward pass read last, may still lie in the Infinity Cache (4096 rows of 32000
 // bf16, a quarter of them without a token, with the forward pass: 141 us from the first row on, 137 from the last, 122 with results stored past the caches
 // as well).  Bound by memory: 70 us of those, 459 MB.
@@ -735,11 +735,11 @@ __global__ __launch_bounds__(256) void k_token_scores_bwd(ScoresArgs a) {
   const float base = a.norm[2 * r], log_s = a.norm[2 * r + 1];
   const float g = a.d_log_prob ? a.d_log_prob[r] : 0.f, ge = a.d_entropy ? a.d_entropy[r] : 0.f, h = a.d_entropy ? a.entropy[r] : 0.f;
   const bool none = target < 0 || log_s == -__builtin_inff();
-  // (256 p is what is multiplied: p may be below the normal numbers where p log p is not)
-  const float A = a.targets && target >= a.V ? __builtin_nanf("") : __builtin_fmaf(ge, h, g) * -0x1p-8f, B = -ge * kLn2 * 0x1p-8f, c = -log_s * kLog2E;
+  // (The square root of p, twice: p may be below the normal numbers where its products are not.  t is half of log2 p.)
+  const float A = a.targets && target >= a.V ? __builtin_nanf("") : -__builtin_fmaf(ge, h, g), B = -2.f * kLn2 * ge, c = -0.5f * kLog2E * log_s;
   auto one = [&](float v) {
-    const float t = __builtin_elementwise_maximum(__builtin_fmaf(v - base, kLog2E, c), kNoPower);
-    return __builtin_amdgcn_exp2f(t + 8.f) * __builtin_fmaf(B, t, A);
+    const float t = __builtin_elementwise_maximum(__builtin_fmaf(v - base, 0.5f * kLog2E, c), kNoPower), root = __builtin_amdgcn_exp2f(t);
+    return root * (root * __builtin_fmaf(B, t, A));
   };
   const bool known = a.targets != nullptr && !none;
   for (long long from = v0; from < v1; from += (long long)THREADS * 8 * N) {

@@ -434,3 +434,27 @@ def test_entry_points_fill_every_byte_and_no_other(R, V, k, dtype):
     check(logits, targets, k, s, (g, None, inside("D", x.dtype).view(R, V)))
     for name, b in buf.items():
         assert bool((b[:256] == 0xFF).all()) and bool((b[256 + sizes[name] :] == 0xFF).all()), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [200, 1000, 5000])
+def test_gradient_of_probabilities_that_are_no_normal_numbers(V, dtype):
+    """
+    A large error of the entropy makes normal numbers of them: p is below 2^-126, its products are not.
+
+    (Bound: as above, and the entropy's own, 4 (1 + log V) S, times p and the entropy's error: the entropy is some 1e-32 here, and so is
+    what the token with nearly all of the probability is made of.)
+    """
+    announce("scores small probabilities", V, dtype)
+    logits = torch.linspace(-80.0, -103.0, V)[None].repeat(3, 1)
+    logits[:, V // 3] = torch.tensor([0.0, 0.125, -0.25])
+    logits = logits.to(_DTYPES[dtype])
+    leaf, ge = logits.to(DEV).requires_grad_(), torch.tensor([1000.0, -300.0, 3.0], device=DEV)
+    s = token_log_probs(leaf, None, entropy=True)
+    (D,) = torch.autograd.grad(s.entropy, leaf, ge)
+    check(logits, None, 0, s)
+    _, entropy, _, _, log_p = ref.scores(array(logits))
+    want = ref.scores_grad(array(logits), None, numpy.zeros(3), array(ge))
+    S, h, made_of = (V / 64 + 2 * math.log(V) + 96) * U, entropy[:, None], numpy.exp(log_p) * numpy.abs(array(ge))[:, None]
+    half = 2.0**-8 if dtype == "bf16" else U
+    near(array(D), want, 4 * S * made_of * ((2 + numpy.abs(log_p) + h) * (numpy.abs(log_p) + h) + 1 + math.log(V)) + half * numpy.abs(want) + 2.0**-126)

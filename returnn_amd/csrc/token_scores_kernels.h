@@ -528,10 +528,13 @@ __global__ __launch_bounds__(256) void k_token_scores_short(ScoresArgs a) {
 
 // Sums without alternatives, read as they come: W wavefronts per row or piece of one (W = 1: four rows per workgroup), U times eight logits per
 // lane in flight.  The wavefront's reference, which stands for the maximum, is that of the first 512 logits among which one is above kNothing (of tokens that are
-// not allowed, minus infinity or the type's lowest value, nothing is left beside it): sums relative to it are as good as long as they stay finite.  Where they
-// do not, or there is no such reference, the wavefront takes its sums again, with the true maximum.
+// not allowed, minus infinity or the type's lowest value, nothing is left beside it).  Where a lane's sum passes kRise, the logits that are held are added
+// once more, relative to the largest so far: so no logit is more than 14 above its reference, and sums of all lanes, wavefronts and pieces are far from what
+// float32 ends at.  (A maximum of every logit beforehand would be one instruction more for each; this is one for 32 of them.)  Where the sums are not finite all the same, or
+// there is no such reference, the wavefront takes them again, with the true maximum.
 // Bound by memory: 4096 rows of 32000 bf16 54 us (262 MB, 4.9 TB/s).  (Products of minus infinity left to be NaN and found afterwards: 52, but 262 where
 // tokens are masked.)
+constexpr float kRise = 0x1p20f;  // (a lane's sum of equal logits of the longest row is a quarter of it)
 template <typename AT, int W, bool ENTROPY>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
   constexpr int R = W == 1 ? 4 : 1, U = 4;
@@ -559,24 +562,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
       const int at = from + (j * 64 * W + thread) * 8;
       q[j].load(row + (at < a.V - 8 ? at : a.V - 8));
     }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int at = from + (j * 64 * W + wave * 64) * 8;  // (the wavefront's first)
-      if (at >= v1) break;
-      float v[8];
+    const RowSums before = sums;
+    auto first = [&](int j) { return from + (j * 64 * W + wave * 64) * 8; };  // of the wavefront's logits
+    auto get = [&](int j, float (&v)[8]) {
       q[j].get(v);
-      if (at + 512 > v1) {  // see above: the last eight of the row, those of an earlier lane left out
-        const int mine = at + lane * 8, begin = mine < a.V - 8 ? mine : a.V - 8;
+      if (first(j) + 512 > v1) {  // see above: the last eight of the row, those of an earlier lane left out
+        const int mine = first(j) + lane * 8, begin = mine < a.V - 8 ? mine : a.V - 8;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = begin + k >= mine && begin + k < v1 ? v[k] : kNothing;
       }
-      if (!referred) {
-        float most = kLowest;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) most = __builtin_fmaxf(most, v[k]);
-        sums = {wave_max(most), 0.f, 0.f};
-        referred = sums.m > kNothing;
-      }
+    };
+    auto add = [&](const float (&v)[8]) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         float t = (v[k] - sums.m) * kLog2E;
@@ -584,6 +580,42 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresAr
         const float e = __builtin_amdgcn_exp2f(t);
         sums.s += e;
         if (ENTROPY) sums.w = __builtin_fmaf(t, e, sums.w);
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (first(j) >= v1) break;
+      float v[8];
+      get(j, v);
+      if (!referred) {
+        float most = kLowest;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = __builtin_fmaxf(most, v[k]);
+        sums = {wave_max(most), 0.f, 0.f};
+        referred = sums.m > kNothing;
+      }
+      add(v);
+    }
+    if (__any(sums.s > kRise)) {
+      float most = before.m;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (first(j) >= v1) break;
+        float v[8];
+        get(j, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = __builtin_fmaxf(most, v[k]);
+      }
+      most = wave_max(most);
+      referred = most > kNothing;
+      const float t = __builtin_fmaxf((before.m - most) * kLog2E, kNoPower), c = __builtin_amdgcn_exp2f(t);
+      sums = {most, c * before.s, ENTROPY ? c * __builtin_fmaf(t, before.s, before.w) : 0.f};
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (first(j) >= v1) break;
+        float v[8];
+        get(j, v);
+        add(v);
       }
     }
   }

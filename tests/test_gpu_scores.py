@@ -458,3 +458,34 @@ def test_gradient_of_probabilities_that_are_no_normal_numbers(V, dtype):
     S, h, made_of = (V / 64 + 2 * math.log(V) + 96) * U, entropy[:, None], numpy.exp(log_p) * numpy.abs(array(ge))[:, None]
     half = 2.0**-8 if dtype == "bf16" else U
     near(array(D), want, 4 * S * made_of * ((2 + numpy.abs(log_p) + h) * (numpy.abs(log_p) + h) + 1 + math.log(V)) + half * numpy.abs(want) + 2.0**-126)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(24, 1000), (300, 1000), (24, 1500), (24, 6000), (300, 6000), (24, 32000), (300, 32000), (24, 70001), (300, 70001)])
+def test_first_logits_that_are_low(rows, V, dtype):
+    """
+    The largest logits far above those at the beginning of their row, by what a float32 sum of exponentials can just hold and by more; all of the
+    later ones, or one in eight.  In rows of one wavefront, of several, and in pieces.
+
+    (Sums relative to a logit up to 14 below the largest: an exponential of them is good to (14 + log V + 8 + 8) u, and what it takes to join
+    the lanes', wavefronts' and pieces' sums is 23 additions, so that S as above has room for those and for the roundings of the difference
+    to the reference and of the logarithm, which are below 14 + log V each.)
+    """
+    announce("scores low first logits", rows, V, dtype)
+    logits, targets = problem((rows,), V, dtype, seed=V + rows, spread=1.0)
+    where = torch.arange(V)
+    for r in range(rows):
+        low = (20.0, 60.0, 70.0, 76.0, 78.0, 80.0, 83.0, 85.0, 87.0, 88.0, 90.0, 130.0)[r % 12]
+        lead = (512, 2048, 8192)[r // 12 % 3]
+        high = where >= min(lead, V - 8)
+        if r // 36 % 2:
+            high &= where % 8 == 0
+        logits[r][~high] -= low
+        if r % 4 == 3:  # (all the high ones alike: the sums are as large as they get)
+            logits[r][high] = 0.5
+        if r % 3:
+            targets[r] = V - 1 - int(high.flip(0).int().argmax())
+    s, grads = run(logits, targets, 0)
+    check(logits, targets, 0, s, grads)
+    s, grads = run(logits, targets, 0, entropy=False)
+    check(logits, targets, 0, s, grads)

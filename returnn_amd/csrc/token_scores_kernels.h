@@ -441,7 +441,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores_top(Scor
         const int at = SINGLE ? v0 + j * 64 + lane : own(j >> 3) + (j & 7);
         if (at < v1) {
           const unsigned long long q = alternative(load_f32(row + at), (unsigned)at);
-          if (q < last && q > mine) mine = q;
+          if ((k < 0 || q < last) && q > mine) mine = q;  // (nothing is larger than a NaN at index 0)
         }
       }
     }

@@ -489,3 +489,29 @@ def test_first_logits_that_are_low(rows, V, dtype):
     check(logits, targets, 0, s, grads)
     s, grads = run(logits, targets, 0, entropy=False)
     check(logits, targets, 0, s, grads)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(5, 1), (5, 3), (5, 7), (5, 8), (5, 9), (5, 12), (700, 12), (5, 64), (700, 64), (5, 90), (700, 200), (1100, 700), (1100, 2000), (5, 3000), (5, 40000)])
+def test_alternatives_with_a_nan_anywhere(rows, V, dtype):
+    """A NaN comes before everything, at the first index and the last as well, and NaN among themselves by index: every token is listed once."""
+    announce("scores nan anywhere", rows, V, dtype)
+    logits, _ = problem((rows,), V, dtype, seed=12)
+    for r in range(rows):
+        kind = r % 5
+        if kind == 0:
+            logits[r, 0] = float("nan")
+        elif kind == 1:
+            logits[r] = float("nan")
+        elif kind == 2:
+            logits[r, V - 1] = float("nan")
+        elif kind == 3:
+            logits[r, 0] = logits[r, V // 2] = float("nan")
+            logits[r, V // 3] = -INF
+        else:
+            logits[r, V // 2] = INF
+    for k in sorted({1, min(V, 8), min(V, 9), min(V, 64)}):
+        s = token_log_probs(logits.to(DEV), top_k=k)
+        with numpy.errstate(invalid="ignore"):
+            _, _, _, ids, _ = ref.scores(array(logits), None, k)
+        assert numpy.array_equal(s.top_ids.cpu().numpy(), ids), k

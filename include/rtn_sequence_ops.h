@@ -7,7 +7,7 @@
  * work on that stream: no device synchronisation, no allocation (scratch comes in through `workspace`, 16-byte aligned,
  * whose contents are neither expected nor kept), inputs are never written, outputs are caller-allocated and fully
  * overwritten.  All entries can be recorded into a HIP graph.  Nothing is enqueued where a status other than RTN_OK is
- * returned for a reason that the host can see.
+ * returned for a reason that the host can see; sizes whose launch would have 2^32 threads or more are such a reason (RTN_ERR_SHAPE).
  */
 #ifndef RTN_SEQUENCE_OPS_H
 #define RTN_SEQUENCE_OPS_H

@@ -38,7 +38,9 @@ int launched(const char* what) {
 bool known(int dtype) { return dtype == RTN_DTYPE_F32 || dtype == RTN_DTYPE_BF16; }
 int size_of(int dtype) { return dtype == RTN_DTYPE_BF16 ? 2 : 4; }
 bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
-constexpr int64_t kMaxBlocks = 0x7FFFFFFF;
+// Workgroups of a launch: its threads are counted in 32 bits.
+constexpr int64_t max_blocks(int64_t threads) { return 0xFFFFFFFFll / threads; }
+constexpr int64_t kMaxRows = 0x7FFFFFFF;
 
 // Calls f with a value of the element type.
 template <typename F>
@@ -202,7 +204,7 @@ int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const 
   const size_t need = recurrence_runs_bytes(p);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence: workspace must be 16-byte aligned");
-  if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
+  if (p.chains * p.segments > max_blocks(64 * p.waves)) return fail(RTN_ERR_SHAPE, "gated recurrence: B=%d n=%d are too many channels for one call", B, n);
   const int apart = strips_apart(p, B, n, dtype, {X, Y}, {ldX, n});
   const RecurrenceArgs a{X, ldX, c0, lens, Y, cN, (float*)saved, nullptr, 0, nullptr, nullptr, nullptr, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, apart, (float*)workspace};
   const hipStream_t stream = (hipStream_t)hip_stream;
@@ -240,7 +242,7 @@ int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const 
   const size_t need = recurrence_runs_bytes(p);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "gated recurrence gradient: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "gated recurrence gradient: workspace must be 16-byte aligned");
-  if (p.chains * p.segments > kMaxBlocks) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
+  if (p.chains * p.segments > max_blocks(64 * p.waves)) return fail(RTN_ERR_SHAPE, "gated recurrence gradient: B=%d n=%d are too many channels for one call", B, n);
   const int apart = strips_apart(p, B, n, dtype, {X, DY, DX}, {ldX, ldDY, 4 * (int64_t)n});
   const RecurrenceArgs a{X, ldX, c0, lens, nullptr, nullptr, (float*)saved, DY, ldDY, DcN, DX, Dc0, T, B, n, direction < 0, p.strips, (unsigned)p.chains, p.segment, p.segments, apart, (float*)workspace};
   with_recurrence(dtype, p, [&](auto type, auto vec, auto waves) {
@@ -276,7 +278,7 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
   const int64_t count = rows * width, groups = (count + 7) / 8;
   const bool flat = (rows == 1 && times == 1) || (ldx == width && (!residual || ldr == width));
   const int64_t blocks = flat ? (groups * times + 511) / 512 : (groups + 255) / 256;
-  if (blocks > kMaxBlocks) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
+  if (blocks > max_blocks(256)) return fail(RTN_ERR_SHAPE, "dropout: [%lld,%lld,%lld] is too large for one call", (long long)times, (long long)rows, (long long)width);
   const DropoutArgs a{x, residual, y, ldx, ldr, times, rows, width, count, (unsigned)threshold, scale, (unsigned)seed, (unsigned)(seed >> 32), offset, offset_ptr};
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
@@ -297,7 +299,7 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
 // ---- scores of tokens ---------------------------------------------------------------------------------------------
 static int scores_check(const char* what, const void* logits, int64_t* ld, const int64_t* targets, int64_t rows, int64_t V, int32_t dtype) {
   if (rows < 0 || V < 0 || V > kMaxTokens) return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld logits (at most %lld)", what, (long long)rows, (long long)V, (long long)kMaxTokens);
-  if (rows > kMaxBlocks) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
+  if (rows > kMaxRows) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
   if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
   if (!*ld) *ld = V;
   if (*ld < V) return fail(RTN_ERR_SHAPE, "%s: rows are %lld elements apart, but have %lld", what, (long long)*ld, (long long)V);
@@ -339,21 +341,26 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
   const size_t need = rtn_token_log_probs_workspace_bytes(rows, V, dtype, top_k);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "token log probabilities: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "token log probabilities: workspace must be 16-byte aligned");
-  if (rows > kMaxBlocks / splits) return fail(RTN_ERR_SHAPE, "token log probabilities: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
   const ScoresArgs a{logits, ld,      targets, rows,    (int)V,      top_k,           log_prob,
                      norm,   entropy, top_log_prob, top_ids, nullptr, nullptr, nullptr,
                      (int)splits, (int)segment, (float*)workspace, (unsigned long long*)((char*)workspace + (size_t)rows * (size_t)splits * 16)};
-  const hipStream_t stream = (hipStream_t)hip_stream;
+  const int64_t one = rows * splits, four = (rows + 3) / 4, sixteen = (rows + 15) / 16;
+  bool fits = true;
+  auto launch = [&](void (*kernel)(ScoresArgs), int64_t blocks, int threads) {
+    if (blocks > max_blocks(threads))
+      fits = false;
+    else
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, (hipStream_t)hip_stream, a);
+  };
   with_type(dtype, [&](auto type) {
     typedef decltype(type) AT;
-    const dim3 one((unsigned)(rows * splits)), four((unsigned)((rows + 3) / 4)), sixteen((unsigned)((rows + 15) / 16));
     // Short rows 16 at a time, but not for many alternatives, of which 16 lanes' maxima tell too little (us, 2000 rows of 96 bf16, one wavefront per row / this: sums 3.5 / 2.7, 5 alternatives 4.6 / 4.1,
     // 16 alternatives 7.1 / 15.0; 70000 rows 25 / 6.7, 41 / 13.5, 56 / 86).
     if (V >= 8 && V <= 256 && top_k <= 8) {
       if (V <= 128)
-        hipLaunchKernelGGL((k_token_scores_short<AT, 8>), sixteen, dim3(256), 0, stream, a);
+        launch(k_token_scores_short<AT, 8>, sixteen, 256);
       else
-        hipLaunchKernelGGL((k_token_scores_short<AT, 16>), sixteen, dim3(256), 0, stream, a);
+        launch(k_token_scores_short<AT, 16>, sixteen, 256);
       return;
     }
     if (top_k > 0) {
@@ -363,47 +370,48 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
       // Many of up to 2048 logits take one wavefront, without barriers (29000 rows of 1000 bf16 four 61, one 27, of 2000 64 and 38; 700 rows of 2000 5.2 and 5.7).
       const bool few = rows <= 512, many = rows > 1024;
       if (segment <= 64 || (segment <= 512 && !few))
-        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 8>), four, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 1, 8>, four, 256);
       else if (segment <= 1024 && many)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 16>), four, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 1, 16>, four, 256);
       else if (segment <= 2048 && many)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 1, 32>), four, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 1, 32>, four, 256);
       else if (segment <= 2048)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 8>), one, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 4, 8>, one, 256);
       else if (segment <= 4096)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 16>), one, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 4, 16>, one, 256);
       else if (segment <= 8192 && few)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 16>), one, dim3(512), 0, stream, a);
+        launch(k_token_scores_top<AT, 8, 16>, one, 512);
       else if (segment <= 6144)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 24>), one, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 4, 24>, one, 256);
       else if (segment <= 8192)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 4, 32>), one, dim3(256), 0, stream, a);
+        launch(k_token_scores_top<AT, 4, 32>, one, 256);
       else if (segment <= 12288)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 24>), one, dim3(512), 0, stream, a);
+        launch(k_token_scores_top<AT, 8, 24>, one, 512);
       else if (segment <= 16384)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 8, 32>), one, dim3(512), 0, stream, a);
+        launch(k_token_scores_top<AT, 8, 32>, one, 512);
       else if (segment <= 24576)
-        hipLaunchKernelGGL((k_token_scores_top<AT, 16, 24>), one, dim3(1024), 0, stream, a);
+        launch(k_token_scores_top<AT, 16, 24>, one, 1024);
       else
-        hipLaunchKernelGGL((k_token_scores_top<AT, 16, 32>), one, dim3(1024), 0, stream, a);
+        launch(k_token_scores_top<AT, 16, 32>, one, 1024);
     } else {
       with_bool(entropy != nullptr, [&](auto with_entropy) {
         constexpr bool ENTROPY = decltype(with_entropy)::value;
         // (us of bf16 rows, one wavefront / four: 9000 of 1500 9.4 / 11.5, 9000 of 6000 25.0 / 21.5; four / sixteen: 100 of 32000 7.1 / 5.8, 4096 of 16000 30.2 / 35.5)
         if (segment <= 1536)
-          hipLaunchKernelGGL((k_token_scores<AT, 1, ENTROPY>), four, dim3(256), 0, stream, a);
+          launch(k_token_scores<AT, 1, ENTROPY>, four, 256);
         else if (rows >= 256 || segment <= 8192)
-          hipLaunchKernelGGL((k_token_scores<AT, 4, ENTROPY>), one, dim3(256), 0, stream, a);
+          launch(k_token_scores<AT, 4, ENTROPY>, one, 256);
         else
-          hipLaunchKernelGGL((k_token_scores<AT, 16, ENTROPY>), one, dim3(1024), 0, stream, a);
+          launch(k_token_scores<AT, 16, ENTROPY>, one, 1024);
       });
     }
-    if (splits > 1) {
+    if (splits > 1 && fits) {
       // (16 lanes per alternative, but no more wavefronts than are there at once)
-      const unsigned threads = rows > 512 ? 256 : (unsigned)std::clamp<int64_t>((16 * splits * top_k + 63) / 64 * 64, 256, 1024);
-      hipLaunchKernelGGL((k_token_scores_join<AT>), dim3((unsigned)rows), dim3(threads), 0, stream, a);
+      const int threads = rows > 512 ? 256 : (int)std::clamp<int64_t>((16 * splits * top_k + 63) / 64 * 64, 256, 1024);
+      launch(k_token_scores_join<AT>, rows, threads);
     }
   });
+  if (!fits) return fail(RTN_ERR_SHAPE, "token log probabilities: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
   return launched("token log probabilities");
 }
 
@@ -417,7 +425,8 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
   if (!aligned(D, size_of(dtype)) || !aligned(norm, 8) || !aligned(entropy, 4) || !aligned(d_log_prob, 4) || !aligned(d_entropy, 4))
     return fail(RTN_ERR_ARG, "token log probabilities gradient: misaligned pointer");
   const int64_t pieces = (V + kBwdPiece - 1) / kBwdPiece;
-  if (rows > kMaxBlocks / pieces) return fail(RTN_ERR_SHAPE, "token log probabilities gradient: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
+  const int64_t blocks = V <= 256 ? (rows + 15) / 16 : (V <= 2048 ? (rows + 3) / 4 : rows * pieces);
+  if (blocks > max_blocks(256)) return fail(RTN_ERR_SHAPE, "token log probabilities gradient: %lld rows of %lld are too many for one call", (long long)rows, (long long)V);
   const ScoresArgs a{logits,  ld,      targets, rows,       (int)V,    0, nullptr,     (float*)norm, (float*)entropy,
                      nullptr, nullptr, d_log_prob, d_entropy, D, (int)pieces, 0, nullptr, nullptr};
   with_type(dtype, [&](auto type) {
@@ -425,11 +434,11 @@ int rtn_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targe
     // (us of bf16 rows, a wavefront per row / 16 lanes: 70000 of 96 21.4 / 9.0, 10000 of 256 6.2 / 5.3, 37 of 256 3.4 / 3.6; a wavefront / a workgroup per piece: 9000 of 500
     // 8.6 / 13.5, of 2000 18.4 / 19.7, of 5000 46.6 / 37.7)
     if (V <= 256)
-      hipLaunchKernelGGL((k_token_scores_bwd<AT, 16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, (hipStream_t)hip_stream, a);
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 16>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
     else if (V <= 2048)
-      hipLaunchKernelGGL((k_token_scores_bwd<AT, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)hip_stream, a);
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 64>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
     else
-      hipLaunchKernelGGL((k_token_scores_bwd<AT, 256>), dim3((unsigned)(rows * pieces)), dim3(256), 0, (hipStream_t)hip_stream, a);
+      hipLaunchKernelGGL((k_token_scores_bwd<AT, 256>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a);
   });
   return launched("token log probabilities gradient");
 }

@@ -238,3 +238,17 @@ def test_no_kernel_loses_a_copy(tmp_path):
     lines = subprocess.run([generated.OBJDUMP, "-d", str(path)], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines(keepends=True)
     assert sum("k_recurrence" in line for line in lines if line.endswith(">:\n")) > 0
     assert not generated.lost_copies(lines)
+
+
+def test_launches_of_more_threads_than_32_bits_count_are_refused(cabi):
+    """Sizes that the types of the arguments can hold, but a launch cannot: refused as a shape, before anything is enqueued."""
+    for T, B, n, dtype in ((5, (1 << 31) - 1, 8, BF16), (100, 1 << 24, 64, F32)):
+        assert cabi.rtn_gated_recurrence_fwd(P, 0, P, P, P, P, P, T, B, n, dtype, 1, None, 0, None) == lib.RTN_ERR_SHAPE
+        assert cabi.rtn_gated_recurrence_bwd(P, 0, P, P, P, P, 0, P, P, P, T, B, n, dtype, 1, None, 0, None) == lib.RTN_ERR_SHAPE
+    for width, ldx in ((8, 0), (8, 16)):
+        assert cabi.rtn_dropout(P, ldx, None, 0, P, 1, 1 << 37, width, BF16, 100, 1, 2, None, 0, None) == lib.RTN_ERR_SHAPE
+    for rows, V, top_k in ((1 << 30, 8, 1), (1 << 27, 300, 9), (1 << 23, 20000, 1), (1 << 28, 1000, 0), (1 << 25, 6000, 0)):
+        assert cabi.rtn_token_log_probs_fwd(P, 0, P, rows, V, BF16, top_k, P, P, P, P, P, None, 0, None) == lib.RTN_ERR_SHAPE
+    assert cabi.rtn_token_log_probs_fwd(P, 0, P, 1 << 22, 100000, F32, 3, P, P, P, P, P, P, 1 << 40, None) == lib.RTN_ERR_SHAPE  # (in pieces)
+    for rows, V in ((1 << 29, 200), (1 << 27, 2000), (1 << 25, 3000)):
+        assert cabi.rtn_token_log_probs_bwd(P, 0, P, P, P, P, P, P, rows, V, BF16, None) == lib.RTN_ERR_SHAPE

@@ -42,11 +42,17 @@ void check_rc(int rc) {
 
 hipStream_t current_stream(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
+// The ops have a gradient, but none in forward mode: a tangent would be lost.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": derivatives in forward mode are not implemented for this op");
+}
+
 // What every op wants of its main input.
 void check_input(const Tensor& t, const char* what) {
   TORCH_CHECK(ready, what, ": the library is not loaded");
   TORCH_CHECK(t.is_cuda(), what, ": this build implements the op for HIP (MI355X) tensors only; got a CPU tensor");
   TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, what, ": float32 or bfloat16 needed, got ", t.scalar_type());
+  no_tangent(t, what);
 }
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? RTN_DTYPE_BF16 : RTN_DTYPE_F32; }
 void same_device(const Tensor& t, const Tensor& as, const char* what, const char* name) {
@@ -150,6 +156,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_in, const std::optio
   if (state.has_value()) {
     TORCH_CHECK(state->sizes() == at::IntArrayRef({B, n}), what, ": state ", state->sizes(), ", expected ", at::IntArrayRef({B, n}));
     same_device(*state, x_in, what, "the state");
+    no_tangent(*state, what);
     TORCH_CHECK(at::isFloatingType(state->scalar_type()), what, ": state of type ", state->scalar_type());
     c0 = packed(as_type(*state, at::kFloat));
   }
@@ -228,6 +235,7 @@ Tensor dropout(const Tensor& x, int64_t threshold, uint64_t seed, uint64_t base,
     TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(), what, ": residual ", residual->sizes(), " of ", residual->scalar_type(),
                 ", expected ", x.sizes(), " of ", x.scalar_type());
     same_device(*residual, x, what, "the residual");
+    no_tangent(*residual, what);
   }
   if (offset.has_value()) {
     TORCH_CHECK(offset->scalar_type() == at::kLong && offset->numel() == 1, what, ": an offset on the device is one int64, got ", offset->sizes(), " of ", offset->scalar_type());

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -65,6 +66,12 @@ void* pointer(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() 
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return fresh(sizes, like.scalar_type(), like); }
 Tensor scratch(size_t bytes, const Tensor& like) { return bytes ? fresh({(int64_t)bytes}, at::kByte, like) : Tensor(); }
+
+// What a matrix product of an autocast region gives, as these ops take it: as for the LSTM layers bfloat16 where that is the region's type, else float32.  (The cast
+// is one that autograd sees.)  Outside a region float16 is refused.
+Tensor in_region(const Tensor& t) {
+  return t.scalar_type() == at::kHalf && t.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA) ? t.to(at::kFloat) : t;
+}
 
 // Elements from one row to the next where a row is what the last axis holds and the rows, in order, are equally far apart; 0 where they are not.
 int64_t row_pitch(const Tensor& t) {
@@ -143,8 +150,9 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
   }
 };
 
-std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_in, const std::optional<Tensor>& state, const std::optional<Tensor>& lens_in, int64_t direction) {
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& source, const std::optional<Tensor>& state, const std::optional<Tensor>& lens_in, int64_t direction) {
   const char* what = "gated_recurrence";
+  const Tensor x_in = in_region(source);
   check_input(x_in, what);
   TORCH_CHECK(x_in.dim() == 2 || x_in.dim() == 3, what, ": the input must be [T,B,4n] or [B,4n], got ", x_in.sizes());
   TORCH_CHECK(x_in.size(-1) % 4 == 0, what, ": the last axis of the input holds four gates of one width, got ", x_in.sizes());
@@ -227,8 +235,12 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
   }
 };
 
-Tensor dropout(const Tensor& x, int64_t threshold, uint64_t seed, uint64_t base, const std::optional<Tensor>& offset, const std::optional<Tensor>& residual, bool same_over_time) {
+Tensor dropout(const Tensor& source, int64_t threshold, uint64_t seed, uint64_t base, const std::optional<Tensor>& offset, const std::optional<Tensor>& residual_in,
+               bool same_over_time) {
   const char* what = "dropout";
+  const Tensor x = in_region(source);
+  std::optional<Tensor> residual;
+  if (residual_in.has_value()) residual = in_region(*residual_in);
   check_input(x, what);
   TORCH_CHECK(x.dim() >= 1, what, ": the input has no axis");
   if (residual.has_value()) {
@@ -305,8 +317,9 @@ struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
 };
 
 // (log_probs or None, entropy or None, top_log_probs, top_ids)
-py::tuple token_log_probs(const Tensor& logits, const std::optional<Tensor>& targets_in, bool entropy, int64_t top_k) {
+py::tuple token_log_probs(const Tensor& logits_in, const std::optional<Tensor>& targets_in, bool entropy, int64_t top_k) {
   const char* what = "token_log_probs";
+  const Tensor logits = in_region(logits_in);
   check_input(logits, what);
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0, what, ": logits ", logits.sizes(), " have no tokens");
   TORCH_CHECK(top_k >= 0 && top_k <= 64 && top_k <= logits.size(-1), what, ": top_k must be in 0..", std::min<int64_t>(64, logits.size(-1)), ", got ", top_k);

@@ -29,7 +29,8 @@ def dropout(
     same_over_time: bool = False,
 ) -> torch.Tensor:
     """
-    :param source: any shape, float32 or bfloat16, on the GPU; time-major where ``same_over_time``
+    :param source: any shape, float32 or bfloat16, on the GPU; time-major where ``same_over_time``.  (In a region of ``torch.autocast``
+        float16 is taken as float32.)
     :param drop_prob: in [0,1], used as the nearest multiple of 1/65536, but neither 0 nor 1 where it is not; what is kept is scaled by
         ``1 / (1 - drop_prob)`` of that multiple
     :param seed: 64 bits
@@ -66,6 +67,9 @@ class Dropout(torch.nn.Module):
     def forward(self, source: torch.Tensor, *, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.drop_prob == 0.0:
             return source if residual is None else source + residual
+        if residual is not None and residual.dtype != source.dtype:  # (as the addition in evaluation; a layer in an autocast region on a float32 input)
+            both = torch.promote_types(source.dtype, residual.dtype)
+            source, residual = source.to(both), residual.to(both)
         offset = self.offset
         self.offset += 1
         return dropout(source, self.drop_prob, seed=self.seed, offset=offset, residual=residual, same_over_time=self.same_over_time)

@@ -28,7 +28,8 @@ def gated_recurrence(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """
     :param source: [T,B,4*out] gates before their activation, time-major, or [B,4*out] for a single step; along the last axis
-        cell-in, input, forget, output; float32 or bfloat16, on the GPU; rows may have a pitch (e.g. a slice of a wider projection)
+        cell-in, input, forget, output; float32 or bfloat16, on the GPU; rows may have a pitch (e.g. a slice of a wider projection).  (In a
+        region of ``torch.autocast`` float16, which a projection gives there, is taken as float32.)
     :param state: [B,out] before the first frame, default zeros
     :param seq_lens: [B] integer lengths (any device), None = all sequences have T frames.  Frames past them are not read, their
         output is 0 and they leave the state as it is.
@@ -69,7 +70,8 @@ class GatedRecurrence(torch.nn.Module):
         :param source: [T,B,in], or [B,in] for a single step
         :param state: [B,out] or None (zeros)
         :param seq_lens: [B] or None
-        :return: output [T,B,out] (or [B,out]), new state [B,out]
+        :return: output [T,B,out] (or [B,out]), new state [B,out].  As for the LSTM layer the projection runs in an autocast region's type, and
+            the output is bfloat16 where that is, else float32.
         """
         if source.shape[-1] != self.in_dim:
             raise ValueError("%s: input %s does not have in_dim %i" % (self, tuple(source.shape), self.in_dim))

@@ -26,7 +26,7 @@ class TokenScores(NamedTuple):
 def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, *, entropy: bool = False, top_k: int = 0) -> TokenScores:
     """
     :param logits: [...,V] float32 or bfloat16, on the GPU; rows may have a pitch (e.g. those of a vocabulary padded in the projection).
-        A logit of minus infinity is a token that is not allowed: probability 0.
+        A logit of minus infinity is a token that is not allowed: probability 0.  (In a region of ``torch.autocast`` float16 is taken as float32.)
     :param targets: [...] integer tokens, or None.  A negative one marks a row without a token (padding): it is not read, its
         log probability, entropy and gradient are 0, its alternatives have log probability minus infinity and index -1.
         One of V or more makes its log probability and the gradient of its row NaN.

@@ -54,7 +54,9 @@ def dropout(
 class Dropout(torch.nn.Module):
     """
     :func:`dropout` in training, nothing (but the residual's addition) in evaluation.  Every call in training takes the next
-    offset; ``seed`` and ``offset`` are all the state there is, and setting them repeats the masks.
+    offset; ``seed`` and ``offset`` are all the state there is, and setting them repeats the masks.  ``offset`` is in the
+    ``state_dict``, so that a training that is taken up again goes on with the next masks.  (``seed`` is not: it belongs to the configuration, and
+    ranks that train side by side on one saved state have seeds of their own.)
     """
 
     def __init__(self, drop_prob: float, *, seed: int = 0, same_over_time: bool = False):
@@ -73,6 +75,18 @@ class Dropout(torch.nn.Module):
         offset = self.offset
         self.offset += 1
         return dropout(source, self.drop_prob, seed=self.seed, offset=offset, residual=residual, same_over_time=self.same_over_time)
+
+    def get_extra_state(self) -> torch.Tensor:
+        """The offset, its 64 bits as an int64 (a tensor, as all else in a ``state_dict``)."""
+        offset = int(self.offset) & ((1 << 64) - 1)
+        return torch.tensor(offset - (1 << 64) if offset >> 63 else offset, dtype=torch.int64)
+
+    def set_extra_state(self, state: torch.Tensor):
+        self.offset = int(state) & ((1 << 64) - 1)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        missing_keys[:] = [k for k in missing_keys if k != prefix + "_extra_state"]  # (saved before there was one: the offset stays)
 
     def extra_repr(self) -> str:
         return "drop_prob=%g, seed=%i, same_over_time=%s" % (self.drop_prob, self.seed, self.same_over_time)

@@ -17,6 +17,7 @@ import _sequence_ref as ref
 import test_generated_code as generated
 from returnn_amd import build, lib, sequence_lib
 from returnn_amd.dropout import Dropout, dropout
+from returnn_amd.language_model import RecurrentLanguageModel
 from returnn_amd.recurrence import GatedRecurrence, gated_recurrence
 from returnn_amd.scoring import token_log_probs
 
@@ -252,3 +253,26 @@ def test_launches_of_more_threads_than_32_bits_count_are_refused(cabi):
     assert cabi.rtn_token_log_probs_fwd(P, 0, P, 1 << 22, 100000, F32, 3, P, P, P, P, P, P, 1 << 40, None) == lib.RTN_ERR_SHAPE  # (in pieces)
     for rows, V in ((1 << 29, 200), (1 << 27, 2000), (1 << 25, 3000)):
         assert cabi.rtn_token_log_probs_bwd(P, 0, P, P, P, P, P, P, rows, V, BF16, None) == lib.RTN_ERR_SHAPE
+
+
+def test_dropout_counters_are_saved(tmp_path):
+    """A training that is taken up again goes on with the masks that come next, of a model's every dropout; what was saved without them still loads."""
+    m = RecurrentLanguageModel(7, 4, 2, drop_prob=0.5)
+    for k, d in enumerate(m.dropouts):
+        d.offset = 11 + k
+    m.dropouts[2].offset = (1 << 64) - 3
+    torch.save(m.state_dict(), tmp_path / "model.pt")
+    state = torch.load(tmp_path / "model.pt", weights_only=True)
+    other = RecurrentLanguageModel(7, 4, 2, drop_prob=0.5, seed=5)
+    seeds = [d.seed for d in other.dropouts]
+    other.load_state_dict(state)
+    assert [d.offset for d in other.dropouts] == [11, 12, (1 << 64) - 3] and [d.seed for d in other.dropouts] == seeds
+    old = {k: v for k, v in state.items() if not k.startswith("dropouts")}
+    missing, unexpected = other.load_state_dict(old)
+    assert not missing and not unexpected and other.dropouts[0].offset == 11
+    single = Dropout(0.5)
+    single.load_state_dict({})
+    single.load_state_dict(Dropout(0.1).state_dict())
+    assert single.offset == 0 and single.drop_prob == 0.5
+    with pytest.raises(RuntimeError, match="embedding"):
+        other.load_state_dict({k: v for k, v in state.items() if "embedding" not in k})

@@ -66,14 +66,22 @@ class Dropout(torch.nn.Module):
         self.drop_prob, self.seed, self.same_over_time = float(drop_prob), int(seed), bool(same_over_time)
         self.offset = 0
 
-    def forward(self, source: torch.Tensor, *, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, source: torch.Tensor, *, residual: Optional[torch.Tensor] = None, offset: Optional[Union[int, torch.Tensor]] = None) -> torch.Tensor:
+        """
+        :param residual: added to what comes out
+        :param offset: of this call, as in :func:`dropout`, instead of the module's next one, which is left as it is.  A step that is recorded into a
+            graph needs one on the GPU: the module's would be the same at every replay.
+        """
         if not self.training or self.drop_prob == 0.0:
             return source if residual is None else source + residual
         if residual is not None and residual.dtype != source.dtype:  # (as the addition in evaluation; a layer in an autocast region on a float32 input)
             both = torch.promote_types(source.dtype, residual.dtype)
             source, residual = source.to(both), residual.to(both)
-        offset = self.offset
-        self.offset += 1
+        if offset is None:
+            if source.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("%s: a recorded call would use one mask at every replay: give an offset on the GPU" % self)
+            offset = self.offset
+            self.offset += 1
         return dropout(source, self.drop_prob, seed=self.seed, offset=offset, residual=residual, same_over_time=self.same_over_time)
 
     def get_extra_state(self) -> torch.Tensor:

@@ -11,7 +11,7 @@ dropout between them, added to what went in, and a projection to the vocabulary,
 from __future__ import annotations
 
 import sys
-from typing import List, NamedTuple, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -58,31 +58,35 @@ class RecurrentLanguageModel(torch.nn.Module):
         """One state per layer: zeros."""
         return [m.default_initial_state(batch_dims=batch_dims, device=device) for m in self.layers]
 
-    def logits(self, tokens: torch.Tensor, *, state: Optional[list] = None, seq_lens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, list]:
+    def logits(
+        self, tokens: torch.Tensor, *, state: Optional[list] = None, seq_lens: Optional[torch.Tensor] = None, offset: Optional[Union[int, torch.Tensor]] = None
+    ) -> Tuple[torch.Tensor, list]:
         """
         :param tokens: [T,B], or [B] for a single step
+        :param offset: of the dropout masks (:class:`Dropout`; one for all of the model's, whose seeds differ), instead of each one's next.  On the GPU for a
+            training step that is recorded into a graph.
         :return: logits of the next token [T,B,num_tokens] (or [B,num_tokens]), new state
         """
         if state is None:
             state = self.default_initial_state(batch_dims=(tokens.shape[-1],), device=tokens.device)
-        x = self.dropouts[0](self.embedding(tokens))
+        x = self.dropouts[0](self.embedding(tokens), offset=offset)
         new_state = []
         for m, drop, s in zip(self.layers, self.dropouts[1:], state):
             y, s = m(x, state=s, seq_lens=seq_lens)
             new_state.append(s)
-            x = drop(y, residual=x)
+            x = drop(y, residual=x, offset=offset)
         return self.output(x), new_state
 
     def scores(
         self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None, *, state: Optional[list] = None, seq_lens: Optional[torch.Tensor] = None,
-        entropy: bool = False, top_k: int = 0,
+        entropy: bool = False, top_k: int = 0, offset: Optional[Union[int, torch.Tensor]] = None,
     ) -> Tuple[TokenScores, list]:  # fmt: skip
         """
         :param tokens: [T,B] or [B]
         :param targets: the tokens that followed, in the same shape; negative where there is none.  Frames past ``seq_lens`` have none.
         :return: :func:`token_log_probs` of the logits, new state
         """
-        logits, state = self.logits(tokens, state=state, seq_lens=seq_lens)
+        logits, state = self.logits(tokens, state=state, seq_lens=seq_lens, offset=offset)
         if targets is not None:
             targets = self._inside(targets, seq_lens)
         return token_log_probs(logits, targets, entropy=entropy, top_k=top_k), state
@@ -95,14 +99,18 @@ class RecurrentLanguageModel(torch.nn.Module):
         frame = torch.arange(targets.shape[0], device=targets.device)[:, None] if targets.dim() == 2 else 0
         return torch.where(seq_lens.to(targets.device) > frame, targets, -1)
 
-    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, *, seq_lens: Optional[torch.Tensor] = None, entropy_scale: float = 0.0) -> torch.Tensor:
+    def loss(
+        self, tokens: torch.Tensor, targets: torch.Tensor, *, seq_lens: Optional[torch.Tensor] = None, entropy_scale: float = 0.0,
+        offset: Optional[Union[int, torch.Tensor]] = None,
+    ) -> torch.Tensor:  # fmt: skip
         """
         Cross entropy per token that there is, less ``entropy_scale`` times the entropy.
 
         :param tokens, targets: [T,B]; a negative target is none
+        :param offset: as of :meth:`logits`
         """
         targets = self._inside(targets, seq_lens)
-        logits, _ = self.logits(tokens, seq_lens=seq_lens)
+        logits, _ = self.logits(tokens, seq_lens=seq_lens, offset=offset)
         s = token_log_probs(logits, targets, entropy=entropy_scale != 0.0)
         total = -s.log_probs.sum()
         if entropy_scale:

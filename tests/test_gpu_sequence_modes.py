@@ -106,3 +106,55 @@ def test_types_that_differ_are_added_as_in_evaluation():
         y = m.train()(a, residual=b)
         assert y.dtype == torch.float32 == m.eval()(a, residual=b).dtype
         assert torch.equal(y, dropout(a.float(), 0.5, seed=2, residual=b.float()))
+
+
+def test_a_recorded_step_draws_anew():
+    """A training step of the language model in a graph: every replay takes the offset that lies on the GPU, and gives what an eager step with it gives."""
+    announce("sequence modes recorded step")
+    torch.manual_seed(8)
+    T, B, V = 12, 3, 40
+    m = RecurrentLanguageModel(V, 64, 2, drop_prob=0.3, device=DEV)
+    tokens, targets = torch.randint(0, V, (T, B), device=DEV), torch.randint(0, V, (T, B), device=DEV)
+    lens = torch.tensor([12, 5, 9], device=DEV)
+    offset = torch.zeros((1,), dtype=torch.int64, device=DEV)
+    weights = [p for k, p in m.named_parameters() if k.startswith("layers")]
+
+    def step(offset):
+        loss = m.loss(tokens, targets, seq_lens=lens, offset=offset)
+        return (loss.detach(),) + torch.autograd.grad(loss, weights)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(offset)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(offset)
+    seen = []
+    for k in (3, 0, 1 << 40, 4):
+        want = step(k)
+        torch.cuda.synchronize()
+        offset.fill_(k)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
+        seen.append(float(out[0]))
+    assert len(set(seen)) == 4 and all(d.offset == 0 for d in m.dropouts)
+
+
+def test_the_modules_own_offset_is_not_recorded():
+    announce("sequence modes recorded module")
+    m, x = Dropout(0.5, seed=3), torch.ones((4, 64), device=DEV)
+    offset = torch.full((1,), 7, dtype=torch.int64, device=DEV)
+    want = dropout(x, 0.5, seed=3, offset=7)
+    assert torch.equal(m(x, offset=7), want) and torch.equal(m(x, offset=offset), want) and m.offset == 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="replay"):
+            m(x)
+        y = m(x, residual=x, offset=offset)
+        z = m.eval()(x, residual=x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert m.offset == 0 and torch.equal(y, want + x) and torch.equal(z, x + x)

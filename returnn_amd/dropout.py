@@ -70,7 +70,8 @@ class Dropout(torch.nn.Module):
         """
         :param residual: added to what comes out
         :param offset: of this call, as in :func:`dropout`, instead of the module's next one, which is left as it is.  A step that is recorded into a
-            graph needs one on the GPU: the module's would be the same at every replay.
+            graph needs one on the GPU: the module's would be the same at every replay.  A segment that is recomputed in the backward pass
+            (``torch.utils.checkpoint``) needs one as well: the module's next one is another than that of the first run.
         """
         if not self.training or self.drop_prob == 0.0:
             return source if residual is None else source + residual
@@ -80,6 +81,8 @@ class Dropout(torch.nn.Module):
         if offset is None:
             if source.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("%s: a recorded call would use one mask at every replay: give an offset on the GPU" % self)
+            if torch._C._current_graph_task_id() != -1:  # (as torch.utils.checkpoint itself finds that it is in a backward pass)
+                raise RuntimeError("%s: a call that is recomputed in a backward pass would take another mask than at first: give both an offset" % self)
             offset = self.offset
             self.offset += 1
         return dropout(source, self.drop_prob, seed=self.seed, offset=offset, residual=residual, same_over_time=self.same_over_time)

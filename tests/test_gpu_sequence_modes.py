@@ -5,11 +5,12 @@ from __future__ import annotations
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.utils.checkpoint import checkpoint
 
 from _gpu_util import announce
 from returnn_amd.dropout import Dropout, dropout
 from returnn_amd.language_model import RecurrentLanguageModel
-from returnn_amd.recurrence import gated_recurrence
+from returnn_amd.recurrence import GatedRecurrence, gated_recurrence
 from returnn_amd.scoring import token_log_probs
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +159,35 @@ def test_the_modules_own_offset_is_not_recorded():
     graph.replay()
     torch.cuda.synchronize()
     assert m.offset == 0 and torch.equal(y, want + x) and torch.equal(z, x + x)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_segments(reentrant):
+    """With an offset of its own a segment's gradients are those without recomputation; the module's next one would be another mask and is refused."""
+    announce("sequence modes recomputed", reentrant)
+    torch.manual_seed(9)
+    m, layer = Dropout(0.5, seed=3), GatedRecurrence(24, 24, device=DEV)
+    x, dy = torch.randn((9, 4, 24), device=DEV, requires_grad=True), torch.randn((9, 4, 24), device=DEV)
+
+    def segment(x, offset):
+        y, _ = layer(m(x, offset=offset))
+        return m(y, residual=x, offset=offset + 1000)
+
+    def gradients(y):
+        for t in (x, *layer.parameters()):
+            t.grad = None
+        y.backward(dy)
+        return tuple(t.grad.clone() for t in (x, *layer.parameters()))
+
+    want = segment(x, 5)
+    plain = gradients(want)
+    y = checkpoint(segment, x, 5, use_reentrant=reentrant)
+    assert torch.equal(y, want)
+    for a, b in zip(gradients(y), plain):
+        assert torch.equal(a, b)
+    y = checkpoint(lambda x: layer(m(x))[0], x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="recomputed"):
+        gradients(y)
+    assert m.offset == 1
+    torch.autograd.grad(m(x), x, dy)  # (nothing of the refusal is left)
+    assert m.offset == 2

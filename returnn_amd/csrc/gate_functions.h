@@ -61,7 +61,7 @@ __device__ __forceinline__ float tanh_f32(float x) { return tanh_of(x, __builtin
 
 // Gate non-linearities.  float32 runs keep to 32 bits (1e-5 relative is the bar there).  bfloat16 runs round every result to 8 bits of
 // mantissa anyway, so they use the hardware exp2 and reciprocal (about 1 ulp of float32 each):
-// sigmoid(x) = 1 / (1 + 2^(-x log2 e)), tanh(x) = 2 sigmoid(2x) - 1.
+// sigmoid(x) = 1 / (1 + 2^(-x log2 e)), tanh(x) = 2 sigmoid(2x) - 1.  The latter's error is 2e-7 absolute: of an |x| below 1e-4 more than the rounding.
 template <typename AT>
 struct Act;
 

@@ -387,3 +387,29 @@ def test_entry_points_fill_every_byte_and_no_other():
         assert torch.equal(got, t.detach()), key
     for key, b in buf.items():
         assert bool((b[:256] == 0xFF).all()) and bool((b[256 + sizes[key] :] == 0xFF).all()), key
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,B,n", [(1, 3, 64), (6, 2, 33), (40, 3, 130), (70, 64, 512), (300, 2, 96)])
+def test_small_cell_inputs(T, B, n, dtype):
+    """
+    Cell inputs down to 1e-30 and no state: everything is as small as they are, and good to as much of itself.
+
+    (All terms have one sign.  The cell input's function is good to 2^-15 of itself in bfloat16, to 4 u in float32; a state whose products of forget gates
+    have up to T factors, and its gradient, to (T + 8) 2^-22 more with the roundings of sums and products in any order; bfloat16 results to 2^-8 more.)
+    """
+    announce("recurrence small cell inputs", T, B, n, dtype)
+    x, _, dy, dc, _ = problem(T, B, n, dtype, seed=16)
+    size = torch.logspace(0, -30, n) * torch.linspace(0.5, 1.0, T * B).view(T, B, 1)
+    x[..., :n] = size.to(x.dtype)
+    dy, dc = dy.abs(), dc.abs()
+    y, c, dx, _ = run(x, torch.zeros((B, n)), dy, dc, None, 1, True)
+    want_y, want_c, _ = ref.recurrence(array(x))
+    want_dx, _, _, _ = ref.recurrence_grad(array(x), array(dy), array(dc))
+    rel = (2.0**-15 if dtype == "bf16" else 0.0) + (T + 8) * 2.0**-22
+    half = 2.0**-8 if dtype == "bf16" else 0.0
+    assert numpy.all(numpy.abs(array(c) - want_c) <= rel * want_c)
+    assert numpy.all(numpy.abs(array(y) - want_y) <= (rel + half) * want_y)
+    # (the input gate's error is proportional to the cell input; of the sigmoid's slope, i (1 - i), 1 - i is good to 4 u of 1, here 1 - i > 0.005)
+    d, want = array(dx)[..., n : 2 * n], want_dx[..., n : 2 * n]
+    assert numpy.all(numpy.abs(d - want) <= (2 * rel + half + 800 * U) * numpy.abs(want) + 2.0**-126)

@@ -49,7 +49,7 @@ int rtn_gated_recurrence_fwd(const void* X, int64_t ldX, const float* c0, const 
 /*
  * Its gradient.  DY [T,B,n] (rows ldDY elements apart, 0: n) in X's type, not read past a sequence's length; DcN [B,n]
  * float32 or NULL (zero).  DX [T,B,4n] contiguous, 0 past a sequence's length; Dc0 [B,n] float32.
- * `saved` is what the forward call with the same X, c0, lens, direction left.
+ * `saved` is what the forward call with the same X, lens, direction left, in which its c0 is held: c0 is not read here and may be NULL.
  */
 size_t rtn_gated_recurrence_bwd_workspace_bytes(int64_t T, int32_t B, int32_t n, int32_t dtype);
 int rtn_gated_recurrence_bwd(const void* X, int64_t ldX, const float* c0, const int64_t* lens, const void* saved, const void* DY, int64_t ldDY, const float* DcN,

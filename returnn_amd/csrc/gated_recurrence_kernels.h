@@ -27,7 +27,7 @@ constexpr int kStreamed = 2;      // cache policy of stores: not kept in the cac
 struct RecurrenceArgs {
   const void* X;
   long long ldX;
-  const float* c0;
+  const float* c0;  // (forward only: for the gradient it is the first of `saved`)
   const int64_t* lens;
   void* Y;
   float* cN;

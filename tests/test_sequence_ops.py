@@ -276,3 +276,51 @@ def test_dropout_counters_are_saved(tmp_path):
     assert single.offset == 0 and single.drop_prob == 0.5
     with pytest.raises(RuntimeError, match="embedding"):
         other.load_state_dict({k: v for k, v in state.items() if "embedding" not in k})
+
+
+# (float64 on both sides: sums of at most a few hundred terms of about 1, each good to 2^-52)
+@pytest.mark.parametrize("direction", [1, -1])
+def test_recurrence_definition_against_autograd(direction):
+    rng = numpy.random.default_rng(5)
+    T, B, n, lens = 11, 4, 3, [11, 0, 6, 1]
+    x, c0 = (torch.from_numpy(rng.normal(size=s)).requires_grad_() for s in ((T, B, 4 * n), (B, n)))
+    dy, dc = rng.normal(size=(T, B, n)), rng.normal(size=(B, n))
+    c, ys = c0, [None] * T
+    for t in range(T) if direction > 0 else reversed(range(T)):
+        z, i, f, o = x[t].chunk(4, dim=-1)
+        inside = (t < torch.tensor(lens))[:, None]
+        c = torch.where(inside, torch.sigmoid(f) * c + torch.sigmoid(i) * torch.tanh(z), c)
+        ys[t] = torch.where(inside, torch.sigmoid(o) * c, 0.0)
+    y = torch.stack(ys)
+    want = (y, c) + torch.autograd.grad((y, c), (x, c0), (torch.from_numpy(dy), torch.from_numpy(dc)))
+    a, b = x.detach().numpy(), c0.detach().numpy()
+    got = ref.recurrence(a, b, lens, direction)[:2] + ref.recurrence_grad(a, dy, dc, b, lens, direction)[:2]
+    for g, w in zip(got, want):
+        assert numpy.abs(g - w.detach().numpy()).max() < 1e-13
+
+
+def test_scores_definition_against_autograd():
+    rng = numpy.random.default_rng(6)
+    R, V, k = 7, 31, 5
+    x = torch.from_numpy(rng.normal(size=(R, V)) * 3).requires_grad_()
+    targets = torch.from_numpy(rng.integers(0, V, size=R))
+    g, ge = rng.normal(size=R), rng.normal(size=R)
+    log_p = torch.log_softmax(x, dim=-1)
+    lp, h = log_p.gather(1, targets[:, None])[:, 0], torch.special.entr(log_p.exp()).sum(-1)
+    (d,) = torch.autograd.grad((lp, h), x, (torch.from_numpy(g), torch.from_numpy(ge)))
+    got = ref.scores(x.detach().numpy(), targets.numpy(), k)
+    top = log_p.detach().topk(k)
+    assert numpy.array_equal(got[3], top.indices.numpy())
+    for a, b in ((got[0], lp), (got[1], h), (got[2], top.values), (ref.scores_grad(x.detach().numpy(), targets.numpy(), g, ge), d)):
+        assert numpy.abs(a - b.detach().numpy()).max() < 1e-13
+
+
+def test_closed_forms():
+    """Gates that stay the same: a geometric series; logits that are all alike: log V; a mask of dropout: what is kept and its scale."""
+    T, f, iz, o = 9, ref.sigmoid(0.7), ref.sigmoid(-0.4) * numpy.tanh(0.9), ref.sigmoid(0.2)
+    y, c, _ = ref.recurrence(numpy.tile(numpy.array([0.9, -0.4, 0.7, 0.2]), (T, 1, 1)), [[2.0]])
+    states = [f**t * 2.0 + iz * (1 - f**t) / (1 - f) for t in range(1, T + 1)]
+    assert numpy.abs(y[:, 0, 0] - o * numpy.array(states)).max() < 1e-14 and abs(c[0, 0] - states[-1]) < 1e-14
+    lp, h, top, ids, _ = ref.scores(numpy.full((1, 50), 3.0), [7], 2)
+    assert max(abs(lp[0] + numpy.log(50)), abs(h[0] - numpy.log(50)), abs(top[0] + numpy.log(50)).max()) < 1e-14 and ids.tolist() == [[0, 1]]
+    assert set(ref.keep_factors((40, 9), 0.25, 3, 4).flatten()) == {0.0, 4 / 3}

@@ -55,7 +55,7 @@ __device__ __forceinline__ void drop(Eight<AT>& x, const Eight<AT>& r, const Dra
 
 // x, y and residual without gaps: one row of `count` elements, or `times` of them with one mask (SHARED), whose groups follow each other from row to row.  A
 // thread takes the groups i and i + 256 of its workgroup's 512.  Bound by memory: [1000,32,1024] bf16 with a residual 36 us (196 MB, 5.4 TB/s), without
-// 21 (6.3; 26.5 with stores that stay in the caches).  The draws of a group are made anew for every frame that shares
+// 21 over several inputs in turn (131 MB, 6.3; 26.5 with stores that stay in the caches), as the gradient behind such a forward pass 22.6 to 24.5.  The draws of a group are made anew for every frame that shares
 // them: with a thread for up to 16 frames of a group 29.1 us instead of 22.7.
 template <typename AT, bool ADD, bool SHARED>
 __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
@@ -96,8 +96,9 @@ __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
   }
 }
 
-// Rows with a pitch: one thread per group of the mask, for every gridDim.y-th of the frames that share it.  [1000,32,500] bf16 in rows of 512: 21 us (64 MB, 3.0 TB/s;
-// one group in 63 takes the way of single elements, and nearly every wavefront has one).
+// Rows with a pitch: one thread per group of the mask, for every gridDim.y-th of the frames that share it.  [1000,32,500] bf16 in rows of 512: 19 us (64 MB, 3.3 TB/s;
+// one group in 63 takes the way of single elements, and nearly every wavefront has one.  Two vectors, of the row's end and of the next one's beginning, would do where
+// rows are not shorter than eight).
 template <typename AT, bool ADD>
 __global__ __launch_bounds__(256) void k_dropout_rows(DropoutArgs a) {
   const long long g = blockIdx.x * 256ll + threadIdx.x, e = g * 8;

@@ -364,10 +364,10 @@ int rtn_token_log_probs_fwd(const void* logits, int64_t ld, const int64_t* targe
       return;
     }
     if (top_k > 0) {
-      // As few wavefronts as hold a piece, but where rows are few, more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
+      // As few wavefronts as hold a piece, but where rows are few (up to 512: two workgroups a compute unit, which leave most of it idle), more of them with less each (us, with 5 alternatives: 64 rows of 500 bf16 a wavefront each 6.5, four
       // 5.1, 1024 rows 5.4 / 6.2; 64 rows of 8000 float32 four 5.8, eight 5.1, 2048 rows 16.9 / 17.3; 3000 rows of 4000 bf16 four 12.3, eight 18.0).  Lanes hold no
       // more than it takes (3000 rows of 20000 bf16 32 logits 46.7, 24 41.5; 5000 of 10007 42.5 / 38.2).
-      // Many of up to 2048 logits take one wavefront, without barriers (29000 rows of 1000 bf16 four 61, one 27, of 2000 64 and 38; 700 rows of 2000 5.2 and 5.7).
+      // Many of up to 2048 logits (above 1024 rows: four wavefronts a compute unit and more, if a row has only one) take one wavefront, without barriers (29000 rows of 1000 bf16 four 61, one 27, of 2000 64 and 38; 700 rows of 2000 5.2 and 5.7).
       const bool few = rows <= 512, many = rows > 1024;
       if (segment <= 64 || (segment <= 512 && !few))
         launch(k_token_scores_top<AT, 1, 8>, four, 256);

@@ -532,8 +532,8 @@ __global__ __launch_bounds__(256) void k_token_scores_short(ScoresArgs a) {
 // once more, relative to the largest so far: so no logit is more than 14 above its reference, and sums of all lanes, wavefronts and pieces are far from what
 // float32 ends at.  (A maximum of every logit beforehand would be one instruction more for each; this is one for 32 of them.)  Where the sums are not finite all the same, or
 // there is no such reference, the wavefront takes them again, with the true maximum.
-// Bound by memory: 4096 rows of 32000 bf16 54 us (262 MB, 4.9 TB/s).  (Products of minus infinity left to be NaN and found afterwards: 52, but 262 where
-// tokens are masked.)
+// Bound by memory: 4096 rows of 32000 bf16 53 us (262 MB, 4.95 TB/s), the same where the first 2048 logits lie 60 lower.  (Products of minus infinity left to be NaN
+// and found afterwards: 1 us less, but 262 where tokens are masked.)
 constexpr float kRise = 0x1p20f;  // (a lane's sum of equal logits of the longest row is a quarter of it)
 template <typename AT, int W, bool ENTROPY>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {

@@ -81,7 +81,7 @@ int rtn_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
  *         it is not read, log_prob and entropy are 0, the alternatives -inf with index -1, its gradient 0.
  *         A target of V or more gives a log_prob of NaN and a row of NaN as gradient.
  * log_prob [rows] = logits[target] - lse, entropy [rows] = -sum p log p
- * norm    [rows,2] the two parts of lse = log sum exp: a reference m, which is the largest logit or at most 14 below it, and log sum exp(logits - m).
+ * norm    [rows,2] the two parts of lse = log sum exp: a reference m, which is the largest logit or at most 22 below it, and log sum exp(logits - m).
  *         (One number would round away what the gradient needs where logits are large.)
  * top_log_prob, top_ids [rows,top_k]: the top_k largest logits of a row in descending order, among equal ones the lower index
  *         first, a NaN before everything; as log probabilities and indices.  0 <= top_k <= min(64, V).

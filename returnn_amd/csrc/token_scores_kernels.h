@@ -529,12 +529,12 @@ __global__ __launch_bounds__(256) void k_token_scores_short(ScoresArgs a) {
 // Sums without alternatives, read as they come: W wavefronts per row or piece of one (W = 1: four rows per workgroup), U times eight logits per
 // lane in flight.  The wavefront's reference, which stands for the maximum, is that of the first 512 logits among which one is above kNothing (of tokens that are
 // not allowed, minus infinity or the type's lowest value, nothing is left beside it).  Where a lane's sum passes kRise, the logits that are held are added
-// once more, relative to the largest so far: so no logit is more than 14 above its reference, and sums of all lanes, wavefronts and pieces are far from what
+// once more, relative to the largest so far: so no logit is more than 22 above its reference, and sums of all lanes, wavefronts and pieces are far from what
 // float32 ends at.  (A maximum of every logit beforehand would be one instruction more for each; this is one for 32 of them.)  Where the sums are not finite all the same, or
 // there is no such reference, the wavefront takes them again, with the true maximum.
 // Bound by memory: 4096 rows of 32000 bf16 53 us (262 MB, 4.95 TB/s), the same where the first 2048 logits lie 60 lower.  (Products of minus infinity left to be NaN
 // and found afterwards: 1 us less, but 262 where tokens are masked.)
-constexpr float kRise = 0x1p20f;  // (a lane's sum of equal logits of the longest row is a quarter of it)
+constexpr float kRise = 0x1p32f;
 template <typename AT, int W, bool ENTROPY>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_token_scores(ScoresArgs a) {
   constexpr int R = W == 1 ? 4 : 1, U = 4;

@@ -467,9 +467,9 @@ def test_first_logits_that_are_low(rows, V, dtype):
     The largest logits far above those at the beginning of their row, by what a float32 sum of exponentials can just hold and by more; all of the
     later ones, or one in eight.  In rows of one wavefront, of several, and in pieces.
 
-    (Sums relative to a logit up to 14 below the largest: an exponential of them is good to (14 + log V + 8 + 8) u, and what it takes to join
-    the lanes', wavefronts' and pieces' sums is 23 additions, so that S as above has room for those and for the roundings of the difference
-    to the reference and of the logarithm, which are below 14 + log V each.)
+    (Sums relative to a logit up to 22 below the largest: an exponential of them is good to (22 + log V + 8 + 8) u, and what it takes to join
+    the lanes', wavefronts' and pieces' sums is 23 additions, so that S as above has room for those and for half a unit each of the difference
+    to the reference and of the logarithm, which are below 22 + log V: together V / 64 + 2 log V + 83.)
     """
     announce("scores low first logits", rows, V, dtype)
     logits, targets = problem((rows,), V, dtype, seed=V + rows, spread=1.0)

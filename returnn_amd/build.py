@@ -1,5 +1,5 @@
 """
-Ahead-of-time build of ``librtn_native_lstm2.so`` and ``librtn_sequence_ops.so`` for gfx950 with hipcc.
+Ahead-of-time build of ``librtn_native_lstm2.so``, ``librtn_sequence_ops.so`` and ``librtn_model_ops.so`` for gfx950 with hipcc.
 
 Takes the place of the reference's run-time compile-and-cache step for native ops
 (returnn/util/native_code_compiler.py:216-354, returnn/torch/util/native_op_code_compiler.py:94-131):
@@ -35,11 +35,20 @@ BINDING_SOURCE = "rtn_torch_binding.cpp"
 BINDING_PATH = os.path.join(_dir, "_rtn_torch.so")
 # the operators around the recurrent layers: a library of their own, and its torch side
 SEQUENCE_SOURCE = "rtn_sequence_ops.hip"
-SEQUENCE_HEADERS = ["gate_functions.h", "sequence_common.h", "gated_recurrence_kernels.h", "dropout_kernel.h", "token_scores_kernels.h",
+SEQUENCE_HEADERS = ["gate_functions.h", "sequence_common.h", "host_common.h", "torch_binding_common.h", "token_order.h", "gated_recurrence_kernels.h", "dropout_kernel.h",
+                    "token_scores_kernels.h",
                     os.path.join("..", "..", "include", "rtn_sequence_ops.h"), os.path.join("..", "..", "include", "rtn_native_lstm2.h")]  # fmt: skip
 SEQUENCE_LIB_PATH = os.path.join(CSRC_DIR, "librtn_sequence_ops.so")
 SEQUENCE_BINDING_SOURCE = "rtn_sequence_binding.cpp"
 SEQUENCE_BINDING_PATH = os.path.join(_dir, "_rtn_sequence.so")
+# the operators of whole language models, likewise
+MODEL_SOURCE = "rtn_model_ops.hip"
+MODEL_HEADERS = ["delta_rule_kernels.h", "embedding_kernels.h", "beam_kernels.h", os.path.join("..", "..", "include", "rtn_model_ops.h")]
+MODEL_LIB_PATH = os.path.join(CSRC_DIR, "librtn_model_ops.so")
+MODEL_BINDING_SOURCE = "rtn_model_binding.cpp"
+MODEL_BINDING_PATH = os.path.join(_dir, "_rtn_model.so")
+# torch module and path of each binding
+BINDINGS = {BINDING_SOURCE: ("_rtn_torch", BINDING_PATH), SEQUENCE_BINDING_SOURCE: ("_rtn_sequence", SEQUENCE_BINDING_PATH), MODEL_BINDING_SOURCE: ("_rtn_model", MODEL_BINDING_PATH)}
 OBJ_DIR = os.path.join(CSRC_DIR, "_obj")
 OFFLOAD_ARCH = "gfx950"
 ROCM_LIB_DIR = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib")  # rocBLAS (weight-gradient GEMM of the backward op)
@@ -96,6 +105,11 @@ def sequence_command(output: Optional[str] = None) -> List[str]:
     return [hipcc_path()] + _flags() + ["-shared", os.path.join(CSRC_DIR, SEQUENCE_SOURCE), "-o", output or SEQUENCE_LIB_PATH]
 
 
+def model_command(output: Optional[str] = None) -> List[str]:
+    """The hipcc line that makes the library of the operators of whole language models."""
+    return [hipcc_path()] + _flags() + ["-shared", os.path.join(CSRC_DIR, MODEL_SOURCE), "-o", output or MODEL_LIB_PATH]
+
+
 def binding_command(output: Optional[str] = None, source: str = BINDING_SOURCE) -> List[str]:
     """The g++ line of a torch binding: against the torch and HIP headers, no device code.  The HIP runtime is the one
     torch has loaded by then."""
@@ -106,18 +120,18 @@ def binding_command(output: Optional[str] = None, source: str = BINDING_SOURCE) 
 
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas", "-Wno-attributes"]
-    cmd += ["-D_GLIBCXX_USE_CXX11_ABI=%i" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=" + {BINDING_SOURCE: "_rtn_torch", SEQUENCE_BINDING_SOURCE: "_rtn_sequence"}[source]]
+    cmd += ["-D_GLIBCXX_USE_CXX11_ABI=%i" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=" + BINDINGS[source][0]]
     cmd += ["-isystem" + d for d in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]] if os.path.isdir(d)]
-    cmd += [os.path.join(CSRC_DIR, source), "-o", output or {BINDING_SOURCE: BINDING_PATH, SEQUENCE_BINDING_SOURCE: SEQUENCE_BINDING_PATH}[source], "-L" + torch_lib, "-L" + ROCM_LIB_DIR]
+    cmd += [os.path.join(CSRC_DIR, source), "-o", output or BINDINGS[source][1], "-L" + torch_lib, "-L" + ROCM_LIB_DIR]
     return cmd + ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python", "-lamdhip64"]
 
 
 def needs_build() -> bool:
-    built = (LIB_PATH, BINDING_PATH, SEQUENCE_LIB_PATH, SEQUENCE_BINDING_PATH)
+    built = (LIB_PATH, SEQUENCE_LIB_PATH, MODEL_LIB_PATH) + tuple(path for _, path in BINDINGS.values())
     if not all(os.path.exists(path) for path in built):
         return True
     t = min(os.path.getmtime(path) for path in built)
-    deps = [os.path.join(CSRC_DIR, f) for f in SOURCES + HEADERS + [BINDING_SOURCE, SEQUENCE_SOURCE, SEQUENCE_BINDING_SOURCE] + SEQUENCE_HEADERS] + [os.path.abspath(__file__)]
+    deps = [os.path.join(CSRC_DIR, f) for f in SOURCES + HEADERS + list(BINDINGS) + [SEQUENCE_SOURCE, MODEL_SOURCE] + SEQUENCE_HEADERS + MODEL_HEADERS] + [os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
@@ -143,9 +157,8 @@ def build_library(force: bool = True, verbose: bool = False) -> str:
 
     obj_dir = OBJ_DIR + ".tmp.%i" % os.getpid()
     os.makedirs(obj_dir, exist_ok=True)
-    tmp = LIB_PATH + ".tmp.%i" % os.getpid()
-    tmp_binding = BINDING_PATH + ".tmp.%i" % os.getpid()
-    tmp_sequence, tmp_sequence_binding = SEQUENCE_LIB_PATH + ".tmp.%i" % os.getpid(), SEQUENCE_BINDING_PATH + ".tmp.%i" % os.getpid()
+    # (everything under a name of its own until all of it is there)
+    tmp = {path: "%s.tmp.%i" % (path, os.getpid()) for path in (LIB_PATH, SEQUENCE_LIB_PATH, MODEL_LIB_PATH) + tuple(path for _, path in BINDINGS.values())}
 
     def run(cmd):
         if verbose:
@@ -155,21 +168,19 @@ def build_library(force: bool = True, verbose: bool = False) -> str:
 
     try:
         with ThreadPoolExecutor(max_workers=_jobs()) as pool:
-            results = list(pool.map(run, [binding_command(tmp_binding), binding_command(tmp_sequence_binding, SEQUENCE_BINDING_SOURCE), sequence_command(tmp_sequence)]
-                                    + compile_commands(obj_dir)))  # fmt: skip
-        results.append(run(link_command(tmp, obj_dir)) if all(rc == 0 for _, rc, _ in results) else (["(link skipped)"], 0, ""))
+            results = list(pool.map(run, [model_command(tmp[MODEL_LIB_PATH]), sequence_command(tmp[SEQUENCE_LIB_PATH])]
+                                    + [binding_command(tmp[path], source) for source, (_, path) in BINDINGS.items()] + compile_commands(obj_dir)))  # fmt: skip
+        results.append(run(link_command(tmp[LIB_PATH], obj_dir)) if all(rc == 0 for _, rc, _ in results) else (["(link skipped)"], 0, ""))
         for cmd, rc, out in results:
             if rc != 0:
                 raise RuntimeError("the compiler failed (%i):\n$ %s\n%s" % (rc, " ".join(cmd), out))
             if verbose and out.strip():
                 print(out, file=sys.stderr)
-        os.replace(tmp, LIB_PATH)
-        os.replace(tmp_binding, BINDING_PATH)
-        os.replace(tmp_sequence, SEQUENCE_LIB_PATH)
-        os.replace(tmp_sequence_binding, SEQUENCE_BINDING_PATH)
+        for path, built in tmp.items():
+            os.replace(built, path)
     finally:
         shutil.rmtree(obj_dir, ignore_errors=True)
-        for left in (tmp, tmp_binding, tmp_sequence, tmp_sequence_binding):
+        for left in tmp.values():
             if os.path.exists(left):
                 os.remove(left)
     return LIB_PATH

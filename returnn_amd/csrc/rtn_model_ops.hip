@@ -1,0 +1,176 @@
+// Host side of librtn_model_ops.so: argument checks and launches (include/rtn_model_ops.h).
+#include "../../include/rtn_model_ops.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "beam_kernels.h"
+#include "delta_rule_kernels.h"
+#include "embedding_kernels.h"
+#include "host_common.h"
+
+namespace rtn {
+namespace {
+
+constexpr int64_t kMaxFrames = 1 << 30;  // (as of the gated recurrence)
+constexpr int kMaxKeyDim = 128, kMaxValueDim = 65536;
+
+// ---- gated delta rule -----------------------------------------------------------------------------------------------
+struct DeltaSizes {
+  int64_t T;
+  int32_t B, key_heads, heads, dk, dv, dtype;
+};
+bool nothing(const DeltaSizes& z) { return z.B == 0 || z.heads == 0; }
+int delta_check(const char* what, const DeltaSizes& z, int32_t direction) {
+  if (z.T < 0 || z.B < 0 || z.key_heads < 0 || z.heads < 0 || z.T > kMaxFrames || z.dk < 1 || z.dk > kMaxKeyDim || z.dv < 1 || z.dv > kMaxValueDim)
+    return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d key_heads=%d heads=%d dk=%d dv=%d (dk 1 to %d, dv 1 to %d)", what, (long long)z.T, z.B, z.key_heads, z.heads, z.dk, z.dv, kMaxKeyDim,
+                kMaxValueDim);
+  if (z.key_heads ? z.heads % z.key_heads : z.heads) return fail(RTN_ERR_SHAPE, "%s: %d heads cannot share %d heads of queries and keys evenly", what, z.heads, z.key_heads);
+  if (!known(z.dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, z.dtype);
+  if (direction != 1 && direction != -1) return fail(RTN_ERR_RANGE, "%s: direction must be 1 or -1, got %d", what, direction);
+  return RTN_OK;
+}
+int pitch_check(const char* what, const char* name, int64_t* ld, int64_t width) {
+  if (!*ld) *ld = width;
+  return *ld < width ? fail(RTN_ERR_SHAPE, "%s: rows of %s are %lld elements apart, but have %lld", what, name, (long long)*ld, (long long)width) : RTN_OK;
+}
+
+}  // namespace
+}  // namespace rtn
+
+using namespace rtn;
+
+extern "C" {
+
+int rtn_model_ops_abi_version(void) { return 1; }
+const char* rtn_model_ops_last_error(void) { return g_last_error.c_str(); }
+
+size_t rtn_delta_rule_fwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+size_t rtn_delta_rule_saved_bytes(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+
+int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* g, const float* beta, const float* s0,
+                       const int64_t* lens, void* y, float* sN, void* saved, int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv,
+                       int32_t dtype, float scale, int32_t direction, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "delta rule";
+  const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
+  int rc = delta_check(what, z, direction);
+  if (rc == RTN_OK) rc = pitch_check(what, "q", &ldq, (int64_t)key_heads * dk);
+  if (rc == RTN_OK) rc = pitch_check(what, "k", &ldk, (int64_t)key_heads * dk);
+  if (rc == RTN_OK) rc = pitch_check(what, "v", &ldv, (int64_t)heads * dv);
+  if (rc != RTN_OK) return rc;
+  if (nothing(z)) return RTN_OK;
+  if ((T && (!q || !k || !v || !g || !beta || !y)) || !sN) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  const int e = size_of(dtype);
+  if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(y, e) || !aligned(g, 4) || !aligned(beta, 4) || !aligned(s0, 4) || !aligned(sN, 4) || !aligned(lens, 8) ||
+      !aligned(saved, 16))
+    return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  const DeltaArgs a{q, k, v, ldq, ldk, ldv, g, beta, s0, lens, y, sN, T, B, key_heads, heads, dk, dv, scale, direction < 0};
+  const int64_t blocks = (int64_t)B * heads * ((dv + 63) / 64);
+  if (blocks > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: B=%d heads=%d dv=%d are too many for one call", what, B, heads, dv);
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    auto launch = [&](void (*kernel)(DeltaArgs)) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a); };
+    if (dk <= 32)
+      launch(k_delta_steps<AT, 2>);
+    else if (dk <= 64)
+      launch(k_delta_steps<AT, 4>);
+    else
+      launch(k_delta_steps<AT, 8>);
+  });
+  return launched(what);
+}
+
+// ---- embedding ------------------------------------------------------------------------------------------------------
+static int embedding_check(const char* what, const int64_t* tokens, const void* in, int64_t* ld, const void* out, int64_t rows, int64_t V, int64_t D, int32_t dtype) {
+  if (rows < 0 || rows > kMaxRows || V < 0 || V > kMaxRows || D < 0) return fail(RTN_ERR_SHAPE, "%s: %lld rows of a table [%lld,%lld]", what, (long long)rows, (long long)V, (long long)D);
+  if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+  if (const int rc = pitch_check(what, "the input", ld, D); rc != RTN_OK) return rc;
+  const int e = size_of(dtype);
+  if (!aligned(tokens, 8) || !aligned(in, e) || !aligned(out, e)) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  return RTN_OK;
+}
+
+int rtn_embedding_fwd(const int64_t* tokens, const void* table, int64_t ld, void* y, int64_t rows, int64_t V, int64_t D, int32_t dtype, float scale, void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "embedding";
+  const int rc = embedding_check(what, tokens, table, &ld, y, rows, V, D, dtype);
+  if (rc != RTN_OK) return rc;
+  if (!rows || !D) return RTN_OK;
+  if (!tokens || !y || (V && !table)) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  const EmbeddingArgs a{tokens, table, ld, y, rows, V, D, scale, nullptr, nullptr};
+  const int64_t groups = (D + 7) / 8;
+  if (groups > max_blocks(256) * 256 / rows) return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld are too many for one call", what, (long long)rows, (long long)D);
+  with_type(dtype, [&](auto type) {
+    hipLaunchKernelGGL(k_embedding<decltype(type)>, dim3((unsigned)((rows * groups + 255) / 256)), dim3(256), 0, (hipStream_t)hip_stream, a);
+  });
+  return launched(what);
+}
+
+size_t rtn_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D, int32_t) { return rows <= 0 || V <= 0 || D <= 0 ? 0 : (size_t)rows * 8; }
+
+int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* Dtable, int64_t rows, int64_t V, int64_t D, int32_t dtype, float scale, void* workspace,
+                      size_t workspace_bytes, void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "embedding gradient";
+  const int rc = embedding_check(what, tokens, dy, &ld, Dtable, rows, V, D, dtype);
+  if (rc != RTN_OK) return rc;
+  if (!V || !D) return RTN_OK;
+  if (!Dtable || (rows && (!tokens || !dy))) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  const size_t need = rtn_embedding_bwd_workspace_bytes(rows, V, D, dtype);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  if (V > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: a table of %lld rows is too large for one call", what, (long long)V);
+  const EmbeddingArgs a{tokens, dy, ld, Dtable, rows, V, D, scale, (unsigned*)workspace, (unsigned*)workspace + rows};
+  if (rows) hipLaunchKernelGGL(k_embedding_order, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, (hipStream_t)hip_stream, a);
+  with_type(dtype, [&](auto type) { hipLaunchKernelGGL(k_embedding_grad<decltype(type)>, dim3((unsigned)V), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  return launched(what);
+}
+
+// ---- beam search ----------------------------------------------------------------------------------------------------
+size_t rtn_beam_select_workspace_bytes(int32_t, int32_t, int64_t, int32_t, int32_t) { return 0; }
+
+int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const uint8_t* ended, int64_t end_token, float* out_totals, int64_t* sources, int64_t* tokens,
+                    int32_t B, int32_t K, int64_t V, int32_t dtype, int32_t beam, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "beam selection";
+  if (B < 0 || K < 1 || V < 1 || V > INT32_MAX / K) return fail(RTN_ERR_SHAPE, "%s: %d searches of %d hypotheses with %lld scores", what, B, K, (long long)V);
+  if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+  if (beam < 1 || beam > kMaxBeam || beam > K * V) return fail(RTN_ERR_RANGE, "%s: beam of %d from %d hypotheses with %lld scores (at most %d)", what, beam, K, (long long)V, kMaxBeam);
+  if (ended && (end_token < 0 || end_token >= V)) return fail(RTN_ERR_RANGE, "%s: end token %lld of %lld", what, (long long)end_token, (long long)V);
+  if (const int rc = pitch_check(what, "the scores", &ld, V); rc != RTN_OK) return rc;
+  if (!B) return RTN_OK;
+  if (!scores || !totals || !out_totals || !sources || !tokens) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(scores, size_of(dtype)) || !aligned(totals, 4) || !aligned(out_totals, 4) || !aligned(sources, 8) || !aligned(tokens, 8))
+    return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  if (B > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: %d searches are too many for one call", what, B);
+  const BeamArgs a{scores, ld, totals, ended, end_token, out_totals, sources, tokens, B, K, beam, V, 1, V, nullptr};
+  with_type(dtype, [&](auto type) { hipLaunchKernelGGL(k_beam_select<decltype(type)>, dim3((unsigned)B), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  return launched(what);
+}
+
+int rtn_reorder_rows(int32_t count, const void* const* in, void* const* out, const int64_t* row_bytes, const int64_t* sources, int32_t B, int32_t K, int32_t beam,
+                     void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "reordering of rows";
+  if (count < 0 || B < 0 || K < 0 || beam < 0) return fail(RTN_ERR_SHAPE, "%s: %d tensors of [%d,%d] to [%d,%d] rows", what, count, B, K, B, beam);
+  if (!count || !B || !beam) return RTN_OK;
+  if (!in || !out || !row_bytes || !sources) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(sources, 8)) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  const int64_t rows = (int64_t)B * beam;
+  if (rows > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
+  for (int n = 0; n < count; ++n) {
+    if (row_bytes[n] < 0) return fail(RTN_ERR_SHAPE, "%s: rows of %lld bytes", what, (long long)row_bytes[n]);
+    if (row_bytes[n] && ((K && !in[n]) || !out[n])) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  }
+  for (int first = 0; first < count; first += kReordered) {
+    ReorderArgs a{{}, {}, {}, sources, B, K, beam, std::min(count - first, kReordered)};
+    for (int n = 0; n < a.count; ++n) a.in[n] = (const char*)in[first + n], a.out[n] = (char*)out[first + n], a.bytes[n] = row_bytes[first + n];
+    hipLaunchKernelGGL(k_reorder_rows, dim3((unsigned)rows, a.count), dim3(256), 0, (hipStream_t)hip_stream, a);
+  }
+  return launched(what);
+}
+
+}  // extern "C"

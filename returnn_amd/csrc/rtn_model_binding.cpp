@@ -11,6 +11,8 @@ struct Abi {
   decltype(&rtn_delta_rule_fwd_workspace_bytes) delta_fwd_workspace_bytes;
   decltype(&rtn_delta_rule_saved_bytes) delta_saved_bytes;
   decltype(&rtn_delta_rule_fwd) delta_fwd;
+  decltype(&rtn_delta_rule_bwd_workspace_bytes) delta_bwd_workspace_bytes;
+  decltype(&rtn_delta_rule_bwd) delta_bwd;
   decltype(&rtn_embedding_fwd) embedding_fwd;
   decltype(&rtn_embedding_bwd_workspace_bytes) embedding_bwd_workspace_bytes;
   decltype(&rtn_embedding_bwd) embedding_bwd;
@@ -58,6 +60,40 @@ Delta delta_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
   return r;
 }
 
+struct DeltaFunction : torch::autograd::Function<DeltaFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const std::optional<Tensor>& s0,
+                               const std::optional<Tensor>& lens, double scale, int64_t direction) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Delta r = delta_forward(q, k, v, g, beta, s0.value_or(Tensor()), lens.value_or(Tensor()), scale, direction, true);
+    ctx->save_for_backward({q, k, v, g, beta, lens.value_or(Tensor()), r.saved});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["direction"] = direction;
+    ctx->saved_data["state"] = s0.has_value();
+    ctx->set_materialize_grads(false);
+    return {r.y, r.s};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("gated_delta_rule");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q_in = saved[0], &k_in = saved[1], &v_in = saved[2], &g = saved[3], &beta = saved[4], &lens = saved[5];
+    const DeltaSizes z = delta_sizes(q_in, v_in);
+    int64_t ldq, ldk, ldv, ldy;
+    c10::DeviceGuard guard(v_in.device());
+    const Tensor q = head_rows(q_in, &ldq), k = head_rows(k_in, &ldk), v = head_rows(v_in, &ldv);
+    const Tensor dy = head_rows(grads[0].defined() ? grads[0] : at::zeros(v_in.sizes(), v_in.options()), &ldy);
+    const Tensor ds = grads[1].defined() ? packed(grads[1]) : Tensor();
+    const Tensor dq = fresh(q_in.sizes(), q), dk = fresh(k_in.sizes(), k), dv = fresh(v_in.sizes(), v), dg = fresh(g.sizes(), g), db = fresh(g.sizes(), g);
+    const Tensor ds0 = fresh({z.B, z.heads, z.dk, z.dv}, g);
+    const size_t bytes = abi.delta_bwd_workspace_bytes(z.T, z.B, z.key_heads, z.heads, z.dk, z.dv, z.dtype);
+    const Tensor ws = scratch(bytes, v);
+    check_rc(abi.delta_bwd(pointer(q), ldq, pointer(k), ldk, pointer(v), ldv, (const float*)pointer(g), (const float*)pointer(beta), (const int64_t*)pointer(lens),
+                           pointer(saved[6]), pointer(dy), ldy, (const float*)pointer(ds), pointer(dq), pointer(dk), pointer(dv), (float*)pointer(dg), (float*)pointer(db),
+                           (float*)pointer(ds0), z.T, z.B, z.key_heads, z.heads, z.dk, z.dv, z.dtype, (float)ctx->saved_data["scale"].toDouble(),
+                           (int)ctx->saved_data["direction"].toInt(), pointer(ws), bytes, current_stream(v.device())));
+    return {dq, dk, dv, dg, db, ctx->saved_data["state"].toBool() ? ds0 : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 std::tuple<Tensor, Tensor> gated_delta_rule(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& decay_in, const Tensor& beta_in,
                                             const std::optional<double>& scale_in, const std::optional<Tensor>& state, const std::optional<Tensor>& lens_in, int64_t direction) {
   const char* what = "gated_delta_rule";
@@ -100,7 +136,14 @@ std::tuple<Tensor, Tensor> gated_delta_rule(const Tensor& query, const Tensor& k
   }
   const double scale = scale_in.value_or(1.0 / std::sqrt((double)dk));
   if (single) q = q.unsqueeze(0), k = k.unsqueeze(0), v = v.unsqueeze(0), g = g.unsqueeze(0), beta = beta.unsqueeze(0);
-  const Delta r = delta_forward(q, k, v, g, beta, s0.value_or(Tensor()), lens.value_or(Tensor()), scale, direction, false);
+  Delta r;
+  const bool wanted = q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || beta.requires_grad() || (s0.has_value() && s0->requires_grad());
+  if (at::GradMode::is_enabled() && wanted) {
+    const variable_list out = DeltaFunction::apply(q, k, v, g, beta, s0, lens, scale, direction);
+    r.y = out[0], r.s = out[1];
+  } else {
+    r = delta_forward(q, k, v, g, beta, s0.value_or(Tensor()), lens.value_or(Tensor()), scale, direction, false);
+  }
   return {single ? r.y.squeeze(0) : r.y, r.s};
 }
 
@@ -232,6 +275,8 @@ void init(const py::dict& symbols) {
   take(abi.delta_fwd_workspace_bytes, symbols, "rtn_delta_rule_fwd_workspace_bytes");
   take(abi.delta_saved_bytes, symbols, "rtn_delta_rule_saved_bytes");
   take(abi.delta_fwd, symbols, "rtn_delta_rule_fwd");
+  take(abi.delta_bwd_workspace_bytes, symbols, "rtn_delta_rule_bwd_workspace_bytes");
+  take(abi.delta_bwd, symbols, "rtn_delta_rule_bwd");
   take(abi.embedding_fwd, symbols, "rtn_embedding_fwd");
   take(abi.embedding_bwd_workspace_bytes, symbols, "rtn_embedding_bwd_workspace_bytes");
   take(abi.embedding_bwd, symbols, "rtn_embedding_bwd");

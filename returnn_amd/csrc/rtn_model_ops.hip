@@ -22,6 +22,39 @@ struct DeltaSizes {
   int32_t B, key_heads, heads, dk, dv, dtype;
 };
 bool nothing(const DeltaSizes& z) { return z.B == 0 || z.heads == 0; }
+bool valid(const DeltaSizes& z) {
+  return z.T >= 0 && z.T <= kMaxFrames && z.B >= 0 && z.key_heads >= 0 && z.heads >= 0 && z.dk >= 1 && z.dk <= kMaxKeyDim && z.dv >= 1 && z.dv <= kMaxValueDim && known(z.dtype);
+}
+constexpr int kStepFrames = 16;
+int delta_frames(const DeltaSizes& z) { return z.dtype == RTN_DTYPE_BF16 ? DeltaChunk<__bf16>::kFrames : DeltaChunk<float>::kFrames; }
+int64_t delta_chunks(const DeltaSizes& z) { return (z.T + delta_frames(z) - 1) / delta_frames(z); }
+size_t delta_all_chunks(const DeltaSizes& z) { return (size_t)z.B * (size_t)z.heads * (size_t)delta_chunks(z); }
+// Numbers of float32 in the sections of what the gradient wants to know, and of its workspace.
+size_t delta_records(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)delta_record(delta_frames(z)); }
+size_t delta_states(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)z.dk * (size_t)z.dv; }
+size_t delta_writes(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)delta_frames(z) * (size_t)z.dv; }
+size_t delta_shared(const DeltaSizes& z) { return z.heads == z.key_heads ? 0 : (size_t)z.T * (size_t)z.B * (size_t)z.heads * (size_t)z.dk; }
+
+// Calls f with a value of the element type and the keys' width in LDS as a type.
+template <int N>
+using Count = std::integral_constant<int, N>;
+template <typename F>
+void with_delta(const DeltaSizes& z, F f) {
+  with_type(z.dtype, [&](auto type) {
+    if (z.dk <= 32)
+      f(type, Count<32>());
+    else if (z.dk <= 64)
+      f(type, Count<64>());
+    else
+      f(type, Count<128>());
+  });
+}
+constexpr int kDeltaWaves = 4;
+int64_t delta_strips(const DeltaSizes& z) { return (z.dv + 16 * kDeltaWaves - 1) / (16 * kDeltaWaves); }
+bool delta_fits(const DeltaSizes& z) {
+  const int64_t most = max_blocks(512) / std::max<int64_t>(1, (int64_t)z.B * z.heads);
+  return delta_chunks(z) <= most && delta_strips(z) <= most && (!delta_shared(z) || delta_shared(z) / 256 < (size_t)max_blocks(256));
+}
 int delta_check(const char* what, const DeltaSizes& z, int32_t direction) {
   if (z.T < 0 || z.B < 0 || z.key_heads < 0 || z.heads < 0 || z.T > kMaxFrames || z.dk < 1 || z.dk > kMaxKeyDim || z.dv < 1 || z.dv > kMaxValueDim)
     return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d key_heads=%d heads=%d dk=%d dv=%d (dk 1 to %d, dv 1 to %d)", what, (long long)z.T, z.B, z.key_heads, z.heads, z.dk, z.dv, kMaxKeyDim,
@@ -46,8 +79,18 @@ extern "C" {
 int rtn_model_ops_abi_version(void) { return 1; }
 const char* rtn_model_ops_last_error(void) { return g_last_error.c_str(); }
 
-size_t rtn_delta_rule_fwd_workspace_bytes(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
-size_t rtn_delta_rule_saved_bytes(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+size_t rtn_delta_rule_fwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype, int32_t keep) {
+  const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
+  return !valid(z) || keep || T <= kStepFrames ? 0 : delta_records(z) * 4;
+}
+size_t rtn_delta_rule_saved_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype) {
+  const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
+  return valid(z) ? (delta_records(z) + delta_states(z) + delta_writes(z)) * 4 : 0;
+}
+size_t rtn_delta_rule_bwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype) {
+  const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
+  return valid(z) ? (delta_states(z) + delta_writes(z) + 2 * delta_shared(z)) * 4 : 0;
+}
 
 int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* g, const float* beta, const float* s0,
                        const int64_t* lens, void* y, float* sN, void* saved, int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv,
@@ -67,17 +110,77 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
       !aligned(saved, 16))
     return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
   const DeltaArgs a{q, k, v, ldq, ldk, ldv, g, beta, s0, lens, y, sN, T, B, key_heads, heads, dk, dv, scale, direction < 0};
-  const int64_t blocks = (int64_t)B * heads * ((dv + 63) / 64);
-  if (blocks > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: B=%d heads=%d dv=%d are too many for one call", what, B, heads, dv);
-  with_type(dtype, [&](auto type) {
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  if (!saved && T <= kStepFrames) {
+    const int64_t blocks = (int64_t)B * heads * ((dv + 63) / 64);
+    if (blocks > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: B=%d heads=%d dv=%d are too many for one call", what, B, heads, dv);
+    with_delta(z, [&](auto type, auto width) {
+      hipLaunchKernelGGL((k_delta_steps<decltype(type), decltype(width)::value / 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    });
+    return launched(what);
+  }
+  if (!delta_fits(z)) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
+  const size_t need = rtn_delta_rule_fwd_workspace_bytes(T, B, key_heads, heads, dk, dv, dtype, saved != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  DeltaChunkArgs c{};
+  c.f = a, c.chunks = (int)delta_chunks(z);
+  c.records = (float*)(saved ? saved : workspace);
+  if (saved) c.states = c.records + delta_records(z), c.writes = c.states + delta_states(z);
+  with_delta(z, [&](auto type, auto width) {
     typedef decltype(type) AT;
-    auto launch = [&](void (*kernel)(DeltaArgs)) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream, a); };
-    if (dk <= 32)
-      launch(k_delta_steps<AT, 2>);
-    else if (dk <= 64)
-      launch(k_delta_steps<AT, 4>);
+    constexpr int DK = decltype(width)::value;
+    const dim3 heads_grid((unsigned)(B * heads * delta_strips(z)));
+    if (T) hipLaunchKernelGGL((k_delta_chunks<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DeltaChunk<AT>::kFrames * 4), 0, stream, c);
+    if (saved)
+      hipLaunchKernelGGL((k_delta_forward<AT, DK, kDeltaWaves, true>), heads_grid, dim3(64 * kDeltaWaves), 0, stream, c);
     else
-      launch(k_delta_steps<AT, 8>);
+      hipLaunchKernelGGL((k_delta_forward<AT, DK, kDeltaWaves, false>), heads_grid, dim3(64 * kDeltaWaves), 0, stream, c);
+  });
+  return launched(what);
+}
+
+int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* g, const float* beta, const int64_t* lens,
+                       const void* saved, const void* dy, int64_t lddy, const float* dsN, void* dq, void* dk_out, void* dv_out, float* dg, float* dbeta, float* ds0, int64_t T,
+                       int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype, float scale, int32_t direction, void* workspace,
+                       size_t workspace_bytes, void* hip_stream) {
+  g_last_error.clear();
+  const char* what = "delta rule gradient";
+  const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
+  int rc = delta_check(what, z, direction);
+  if (rc == RTN_OK) rc = pitch_check(what, "q", &ldq, (int64_t)key_heads * dk);
+  if (rc == RTN_OK) rc = pitch_check(what, "k", &ldk, (int64_t)key_heads * dk);
+  if (rc == RTN_OK) rc = pitch_check(what, "v", &ldv, (int64_t)heads * dv);
+  if (rc == RTN_OK) rc = pitch_check(what, "dy", &lddy, (int64_t)heads * dv);
+  if (rc != RTN_OK) return rc;
+  if (nothing(z)) return RTN_OK;
+  if ((T && (!q || !k || !v || !g || !beta || !dy || !saved || !dq || !dk_out || !dv_out || !dg || !dbeta)) || !ds0) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+  const int e = size_of(dtype);
+  if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(dy, e) || !aligned(dq, e) || !aligned(dk_out, e) || !aligned(dv_out, e) || !aligned(g, 4) || !aligned(beta, 4) ||
+      !aligned(dsN, 4) || !aligned(dg, 4) || !aligned(dbeta, 4) || !aligned(ds0, 4) || !aligned(lens, 8) || !aligned(saved, 16))
+    return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  if (!delta_fits(z)) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
+  const size_t need = rtn_delta_rule_bwd_workspace_bytes(T, B, key_heads, heads, dk, dv, dtype);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+  if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  DeltaChunkArgs c{};
+  c.f = DeltaArgs{q, k, v, ldq, ldk, ldv, g, beta, nullptr, lens, nullptr, nullptr, T, B, key_heads, heads, dk, dv, scale, direction < 0};
+  c.chunks = (int)delta_chunks(z);
+  c.records = (float*)saved, c.states = c.records + delta_records(z), c.writes = c.states + delta_states(z);
+  c.dy = dy, c.lddy = lddy, c.dsN = dsN;
+  c.dstates = (float*)workspace, c.dwrites = c.dstates + delta_states(z);
+  if (delta_shared(z)) c.dq_each = c.dwrites + delta_writes(z), c.dk_each = c.dq_each + delta_shared(z);
+  c.dq = dq, c.dk = dk_out, c.dv = dv_out, c.dg = dg, c.dbeta = dbeta, c.ds0 = ds0;
+  with_delta(z, [&](auto type, auto width) {
+    typedef decltype(type) AT;
+    constexpr int DK = decltype(width)::value;
+    const hipStream_t stream = (hipStream_t)hip_stream;
+    hipLaunchKernelGGL((k_delta_backward<AT, DK, kDeltaWaves>), dim3((unsigned)(B * heads * delta_strips(z))), dim3(64 * kDeltaWaves), 0, stream, c);
+    if (T) hipLaunchKernelGGL((k_delta_gradients<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DK * 4), 0, stream, c);
+    if (delta_shared(z)) {
+      const int64_t items = T * B * key_heads * (int64_t)dk;
+      hipLaunchKernelGGL(k_delta_shared<AT>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, c);
+    }
   });
   return launched(what);
 }

@@ -45,6 +45,7 @@ def gated_delta_rule(
         the state as it is.
     :param direction: +1, or -1 to go from each sequence's last frame to its first
     :return: output like ``value``, state [B,heads,dk,dv] after the last frame visited, float32.
+        Both differentiable (once) with respect to all inputs but the lengths.
     """
     return native().gated_delta_rule(query, key, value, log_decay, beta, scale, state, seq_lens, direction)
 

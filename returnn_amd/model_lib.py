@@ -23,6 +23,8 @@ SYMBOLS = (
     "rtn_delta_rule_fwd_workspace_bytes",
     "rtn_delta_rule_saved_bytes",
     "rtn_delta_rule_fwd",
+    "rtn_delta_rule_bwd_workspace_bytes",
+    "rtn_delta_rule_bwd",
     "rtn_embedding_fwd",
     "rtn_embedding_bwd_workspace_bytes",
     "rtn_embedding_bwd",
@@ -60,6 +62,8 @@ def load() -> ctypes.CDLL:
         lib.rtn_delta_rule_fwd_workspace_bytes.restype, lib.rtn_delta_rule_fwd_workspace_bytes.argtypes = sz, sizes + [i32]
         lib.rtn_delta_rule_saved_bytes.restype, lib.rtn_delta_rule_saved_bytes.argtypes = sz, sizes
         lib.rtn_delta_rule_fwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp] + sizes + [f32, i32, vp, sz, vp]
+        lib.rtn_delta_rule_bwd_workspace_bytes.restype, lib.rtn_delta_rule_bwd_workspace_bytes.argtypes = sz, sizes
+        lib.rtn_delta_rule_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp] + sizes + [f32, i32, vp, sz, vp]
         lib.rtn_embedding_fwd.argtypes = [vp, vp, i64, vp, i64, i64, i64, i32, f32, vp]
         lib.rtn_embedding_bwd_workspace_bytes.restype, lib.rtn_embedding_bwd_workspace_bytes.argtypes = sz, [i64, i64, i64, i32]
         lib.rtn_embedding_bwd.argtypes = [vp, vp, i64, vp, i64, i64, i64, i32, f32, vp, sz, vp]

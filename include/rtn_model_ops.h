@@ -81,10 +81,10 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
  *   joint[b,k,v] = totals[b,k] + scores[b,k,v]   (one addition, rounded to float32)
  *
  * scores [B,K,V], row (b,k) at element (b*K+k)*ld (0: V); totals [B,K] float32
- * ended  [B,K] (0 or not), or NULL: of a hypothesis that has ended, joint is totals[b,k] for v = end_token and -inf for all others; its scores are not
+ * ended  [B,K] (0 or not), or NULL: the scores of a hypothesis that has ended are taken as 0 for v = end_token and -inf for all others, and not
  *        read.  end_token in 0..V-1 where `ended` is not NULL.
  * out_totals, sources, tokens [B,beam]: joint, k and v of the `beam` largest of a search in descending order, among equal ones the lowest k first and
- *        among those the lowest v; a NaN before everything.  1 <= beam <= min(64, K V), K V below 2^31.
+ *        among those the lowest v; a NaN before everything.  1 <= beam <= min(64, K V), V up to 2^26, K V below 2^31.
  */
 size_t rtn_beam_select_workspace_bytes(int32_t B, int32_t K, int64_t V, int32_t dtype, int32_t beam);
 int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const uint8_t* ended, int64_t end_token, float* out_totals, int64_t* sources, int64_t* tokens,

@@ -206,7 +206,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select(const Tensor& scores_in, const Te
   const bool single = scores0.dim() == 2;
   const int64_t K = scores0.size(-2), V = scores0.size(-1), B = single ? 1 : scores0.size(0);
   const auto lead = scores0.sizes().slice(0, scores0.dim() - 1);
-  TORCH_CHECK(K >= 1 && V >= 1 && V <= INT_MAX / K && B <= INT_MAX, what, ": scores ", scores0.sizes(), ", from 1 to 2^31 - 1 continuations of a search needed");
+  TORCH_CHECK(K >= 1 && V >= 1 && V <= 1 << 26 && V <= INT_MAX / K && B <= INT_MAX, what, ": scores ", scores0.sizes(), ", up to 2^26 of a hypothesis and from 1 to 2^31 - 1 of a search needed");
   TORCH_CHECK(beam >= 1 && beam <= 64 && beam <= K * V, what, ": beam must be in 1..", std::min<int64_t>(64, K * V), ", got ", beam);
   TORCH_CHECK(totals_in.sizes() == lead, what, ": totals ", totals_in.sizes(), ", expected ", lead);
   TORCH_CHECK(totals_in.scalar_type() == at::kFloat, what, ": totals of type ", totals_in.scalar_type(), ", float32 needed");

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "beam_kernels.h"
 #include "delta_rule_kernels.h"
@@ -211,7 +212,28 @@ int rtn_embedding_fwd(const int64_t* tokens, const void* table, int64_t ld, void
   return launched(what);
 }
 
-size_t rtn_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D, int32_t) { return rows <= 0 || V <= 0 || D <= 0 ? 0 : (size_t)rows * 8; }
+// Workspace of the gradient: the sorted rows and their tokens, twice and counts of digits where there is more than one pass of sorting; the sums of runs over several pieces.
+struct EmbeddingPlan {
+  int64_t pieces, strips, blocks;
+  int passes;
+  size_t rows, counts, parts;  // of 4 bytes
+  EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
+    pieces = (n + kRun - 1) / kRun, strips = (D + 511) / 512;
+    passes = 0, blocks = 0;
+    if (n > kCountedRows) {
+      blocks = (n + kSortedRows - 1) / kSortedRows;
+      for (int64_t v = V; v; v >>= 8) ++passes;  // (V itself stands for no token)
+    }
+    rows = (size_t)(n + 3) / 4 * 4;
+    counts = (size_t)blocks * kDigits;
+    parts = (size_t)pieces * (size_t)D;
+  }
+  size_t bytes() const { return (rows * (passes > 1 ? 4 : 2) + counts + 2 * parts) * 4; }
+};
+
+size_t rtn_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D, int32_t) {
+  return rows <= 0 || V <= 0 || D <= 0 || rows > kMaxRows || V > kMaxRows ? 0 : EmbeddingPlan(rows, V, D).bytes();
+}
 
 int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* Dtable, int64_t rows, int64_t V, int64_t D, int32_t dtype, float scale, void* workspace,
                       size_t workspace_bytes, void* hip_stream) {
@@ -221,24 +243,69 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
   if (rc != RTN_OK) return rc;
   if (!V || !D) return RTN_OK;
   if (!Dtable || (rows && (!tokens || !dy))) return fail(RTN_ERR_ARG, "%s: null pointer", what);
-  const size_t need = rtn_embedding_bwd_workspace_bytes(rows, V, D, dtype);
+  const EmbeddingPlan p(rows, V, D);
+  const int64_t bare = (V + kBare - 1) / kBare, sums = p.pieces * p.strips;
+  if (p.strips > 4 * max_blocks(256) / (p.pieces + bare + 1) || (rows && D > INT64_MAX / 32 / rows))
+    return fail(RTN_ERR_SHAPE, "%s: %lld rows of a table [%lld,%lld] are too many for one call", what, (long long)rows, (long long)V, (long long)D);
+  const size_t need = rows ? p.bytes() : 0;
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
-  if (V > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: a table of %lld rows is too large for one call", what, (long long)V);
-  const EmbeddingArgs a{tokens, dy, ld, Dtable, rows, V, D, scale, (unsigned*)workspace, (unsigned*)workspace + rows};
-  if (rows) hipLaunchKernelGGL(k_embedding_order, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, (hipStream_t)hip_stream, a);
-  with_type(dtype, [&](auto type) { hipLaunchKernelGGL(k_embedding_grad<decltype(type)>, dim3((unsigned)V), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  unsigned *now = (unsigned*)workspace, *other = now + 2 * p.rows, *counts = now + p.rows * (p.passes > 1 ? 4 : 2);
+  EmbeddingArgs a{tokens, dy, ld, Dtable, rows, V, D, scale, nullptr, nullptr};
+  if (p.passes) {
+    SortArgs s{a, nullptr, nullptr, counts, (int)p.blocks, 0};
+    for (int pass = 0; pass < p.passes; ++pass, s.shift += 8) {
+      s.e.order = now, s.e.token_of = now + p.rows;
+      hipLaunchKernelGGL(k_embedding_digits, dim3((unsigned)p.blocks), dim3(1024), 0, stream, s);
+      hipLaunchKernelGGL(k_embedding_move, dim3((unsigned)p.blocks), dim3(1024), 0, stream, s);
+      s.order = s.e.order, s.token_of = s.e.token_of;
+      std::swap(now, other);
+    }
+    a.order = s.e.order, a.token_of = s.e.token_of;
+  } else {
+    a.order = now, a.token_of = now + p.rows;
+    if (rows) hipLaunchKernelGGL(k_embedding_order, dim3((unsigned)((rows + 63) / 64)), dim3(1024), 0, stream, a);
+  }
+  EmbeddingSumArgs s{a, (float*)(counts + p.counts), (float*)(counts + p.counts) + p.parts, (int)p.pieces, (int)p.strips, sums};
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    hipLaunchKernelGGL(k_embedding_sums<AT>, dim3((unsigned)((sums + bare + 3) / 4)), dim3(256), 0, stream, s);
+    if (rows > kRun) hipLaunchKernelGGL(k_embedding_join<AT>, dim3((unsigned)((sums + 3) / 4)), dim3(256), 0, stream, s);
+  });
   return launched(what);
 }
 
 // ---- beam search ----------------------------------------------------------------------------------------------------
-size_t rtn_beam_select_workspace_bytes(int32_t, int32_t, int64_t, int32_t, int32_t) { return 0; }
+// Pieces: all continuations of a search at once where they are few; else pieces of hypotheses, as long as a workgroup can hold, or shorter where there would be too few
+// of them to fill the device; and as many rounds of joining their choices as it takes.
+struct BeamPlan {
+  int64_t splits, segment, lists;  // lists: of choices, per search, behind the first round
+  BeamPlan(int32_t B, int32_t K, int64_t V, int32_t beam) {
+    if (K * V <= kBeamFew) {
+      splits = 1, segment = V, lists = 0;
+      return;
+    }
+    splits = (V + kBeamLong - 1) / kBeamLong;
+    if (const int64_t small = (V + kBeamShort - 1) / kBeamShort; (int64_t)B * K * small <= 512) splits = small;
+    segment = ((V + splits - 1) / splits + 7) / 8 * 8;
+    lists = K * splits;
+  }
+  size_t bytes(int32_t B, int32_t beam) const {  // two halves: a round reads one and writes the other
+    const size_t first = (size_t)B * (size_t)lists * (size_t)beam * 8;
+    return first + (lists > per(beam) ? (size_t)B * (size_t)((lists + per(beam) - 1) / per(beam)) * (size_t)beam * 8 : 0);
+  }
+  static int64_t per(int32_t beam) { return kBeamJoined / beam; }  // lists that are joined at once
+};
+static bool beam_valid(int32_t B, int32_t K, int64_t V, int32_t beam) { return B >= 0 && K >= 1 && V >= 1 && V <= kMaxScores && V <= INT32_MAX / K && beam >= 1 && beam <= kMaxBeam && beam <= K * V; }
+
+size_t rtn_beam_select_workspace_bytes(int32_t B, int32_t K, int64_t V, int32_t, int32_t beam) { return beam_valid(B, K, V, beam) ? BeamPlan(B, K, V, beam).bytes(B, beam) : 0; }
 
 int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const uint8_t* ended, int64_t end_token, float* out_totals, int64_t* sources, int64_t* tokens,
                     int32_t B, int32_t K, int64_t V, int32_t dtype, int32_t beam, void* workspace, size_t workspace_bytes, void* hip_stream) {
   g_last_error.clear();
   const char* what = "beam selection";
-  if (B < 0 || K < 1 || V < 1 || V > INT32_MAX / K) return fail(RTN_ERR_SHAPE, "%s: %d searches of %d hypotheses with %lld scores", what, B, K, (long long)V);
+  if (B < 0 || K < 1 || V < 1 || V > kMaxScores || V > INT32_MAX / K) return fail(RTN_ERR_SHAPE, "%s: %d searches of %d hypotheses with %lld scores", what, B, K, (long long)V);
   if (!known(dtype)) return fail(RTN_ERR_ARG, "%s: unknown dtype %d", what, dtype);
   if (beam < 1 || beam > kMaxBeam || beam > K * V) return fail(RTN_ERR_RANGE, "%s: beam of %d from %d hypotheses with %lld scores (at most %d)", what, beam, K, (long long)V, kMaxBeam);
   if (ended && (end_token < 0 || end_token >= V)) return fail(RTN_ERR_RANGE, "%s: end token %lld of %lld", what, (long long)end_token, (long long)V);
@@ -247,10 +314,37 @@ int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const u
   if (!scores || !totals || !out_totals || !sources || !tokens) return fail(RTN_ERR_ARG, "%s: null pointer", what);
   if (!aligned(scores, size_of(dtype)) || !aligned(totals, 4) || !aligned(out_totals, 4) || !aligned(sources, 8) || !aligned(tokens, 8))
     return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+  const BeamPlan p(B, K, V, beam);
+  const size_t need = p.bytes(B, beam);
+  if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
-  if (B > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: %d searches are too many for one call", what, B);
-  const BeamArgs a{scores, ld, totals, ended, end_token, out_totals, sources, tokens, B, K, beam, V, 1, V, nullptr};
-  with_type(dtype, [&](auto type) { hipLaunchKernelGGL(k_beam_select<decltype(type)>, dim3((unsigned)B), dim3(256), 0, (hipStream_t)hip_stream, a); });
+  if (std::max<int64_t>(p.lists, 1) > max_blocks(1024) / B) return fail(RTN_ERR_SHAPE, "%s: %d searches of %d hypotheses with %lld scores are too many for one call", what, B, K, (long long)V);
+  BeamArgs a{scores, ld, totals, ended, end_token, out_totals, sources, tokens, B, K, beam, (int)V, (int)p.splits, (int)p.segment, (int)p.lists, 0, nullptr, (unsigned long long*)workspace};
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  with_type(dtype, [&](auto type) {
+    typedef decltype(type) AT;
+    if (!p.lists) {
+      if (K * V <= 2048)
+        hipLaunchKernelGGL((k_beam_all<AT, 4, 8>), dim3((unsigned)B), dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_beam_all<AT, 16, 8>), dim3((unsigned)B), dim3(1024), 0, stream, a);
+      return;
+    }
+    const dim3 grid((unsigned)(B * p.lists));
+    if (p.segment <= kBeamShort)
+      hipLaunchKernelGGL((k_beam_pieces<AT, 4, 32>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_beam_pieces<AT, 16, 32>), grid, dim3(1024), 0, stream, a);
+    for (int64_t lists = p.lists;;) {
+      const int64_t next = (lists + BeamPlan::per(beam) - 1) / BeamPlan::per(beam);
+      a.lists = (int)lists, a.next = (int)next;
+      unsigned long long* const other = (unsigned long long*)workspace + (a.to == workspace ? (size_t)B * (size_t)p.lists * (size_t)beam : 0);
+      a.from = a.to, a.to = other;
+      hipLaunchKernelGGL((k_beam_join<16, kBeamJoined / 1024>), dim3((unsigned)(B * next)), dim3(1024), 0, stream, a);
+      if (next == 1) break;
+      lists = next;
+    }
+  });
   return launched(what);
 }
 
@@ -263,15 +357,24 @@ int rtn_reorder_rows(int32_t count, const void* const* in, void* const* out, con
   if (!in || !out || !row_bytes || !sources) return fail(RTN_ERR_ARG, "%s: null pointer", what);
   if (!aligned(sources, 8)) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
   const int64_t rows = (int64_t)B * beam;
-  if (rows > max_blocks(256)) return fail(RTN_ERR_SHAPE, "%s: %lld rows are too many for one call", what, (long long)rows);
   for (int n = 0; n < count; ++n) {
     if (row_bytes[n] < 0) return fail(RTN_ERR_SHAPE, "%s: rows of %lld bytes", what, (long long)row_bytes[n]);
     if (row_bytes[n] && ((K && !in[n]) || !out[n])) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+    if ((row_bytes[n] + kReorderPiece - 1) / kReorderPiece > max_blocks(256) / rows / kReordered)
+      return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld bytes are too many for one call", what, (long long)rows, (long long)row_bytes[n]);
   }
   for (int first = 0; first < count; first += kReordered) {
-    ReorderArgs a{{}, {}, {}, sources, B, K, beam, std::min(count - first, kReordered)};
-    for (int n = 0; n < a.count; ++n) a.in[n] = (const char*)in[first + n], a.out[n] = (char*)out[first + n], a.bytes[n] = row_bytes[first + n];
-    hipLaunchKernelGGL(k_reorder_rows, dim3((unsigned)rows, a.count), dim3(256), 0, (hipStream_t)hip_stream, a);
+    ReorderArgs a{{}, {}, {}, sources, B, K, beam, 1};
+    const int some = std::min(count - first, kReordered);
+    long long most = 0;
+    for (int n = 0; n < some; ++n) {
+      a.in[n] = (const char*)in[first + n], a.out[n] = (char*)out[first + n], a.bytes[n] = row_bytes[first + n];
+      most = std::max(most, a.bytes[n]);
+    }
+    const int64_t pieces = (most + kReorderPiece - 1) / kReorderPiece;
+    if (!pieces) continue;
+    a.pieces = (int)pieces;
+    hipLaunchKernelGGL(k_reorder_rows, dim3((unsigned)(rows * pieces), some), dim3(256), 0, (hipStream_t)hip_stream, a);
   }
   return launched(what);
 }

@@ -59,4 +59,20 @@ __device__ __forceinline__ unsigned wave_min(unsigned v) {
   return least(least(at(0), at(16)), least(at(32), at(48)));
 }
 
+// The sum over 16 neighbouring lanes, in all of them.
+__device__ __forceinline__ int quarter_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);
+}
+// How many of the n of a list are larger than `mine`, of which 16 neighbouring lanes look at every 16th: the same in all of them.  (One lane by itself goes through
+// a chain of look-ups and 64-bit comparisons: of 44, which is usual for 12 alternatives, 3000 clocks, a fifth of the kernel.)
+__device__ __forceinline__ int rank_in(const unsigned long long* list, int n, unsigned long long mine, int lane) {
+  int rank = 0;
+#pragma unroll 4
+  for (int o = lane & 15; o < n; o += 16) rank += list[o] > mine;
+  return quarter_sum(rank);
+}
+
 }  // namespace rtn

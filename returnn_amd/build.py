@@ -107,7 +107,7 @@ def sequence_command(output: Optional[str] = None) -> List[str]:
 
 def model_command(output: Optional[str] = None) -> List[str]:
     """The hipcc line that makes the library of the operators of whole language models."""
-    return [hipcc_path()] + _flags() + ["-shared", os.path.join(CSRC_DIR, MODEL_SOURCE), "-o", output or MODEL_LIB_PATH]
+    return [hipcc_path()] + _flags() + VGPR_FORM + ["-shared", os.path.join(CSRC_DIR, MODEL_SOURCE), "-o", output or MODEL_LIB_PATH]
 
 
 def binding_command(output: Optional[str] = None, source: str = BINDING_SOURCE) -> List[str]:

@@ -129,6 +129,7 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
 // and, of tile t, rows 4 q + r; the operand wants rows 8 q + 0..7 of it.  So tile t is made of rows 8 q + 4 t + r, which its left operand's lane i = 4 q + r reads.  Left operands lie in LDS
 // with rows in that order (position 16 t + 4 q + r), so that a tile's are neighbours.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 delta_bf16x8;
+typedef delta_bf16x8 __attribute__((aligned(2))) delta_bf16x8_any;
 typedef __attribute__((__vector_size__(8 * sizeof(float)))) float delta_f32x8;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short delta_s16x4;
 
@@ -163,13 +164,21 @@ struct DeltaChunkArgs {
 
 __device__ __forceinline__ int delta_place(int row) { return (row & ~31) | ((row >> 2 & 1) << 4) | ((row >> 3 & 3) << 2) | (row & 3); }
 
-// Eight numbers as N parts.
+// Eight numbers as N parts, by pairs (element by element the compiler rounds each of them twice).
 template <int N>
 __device__ __forceinline__ void delta_parts(delta_f32x8 x, delta_bf16x8 (&p)[N]) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    p[n] = __builtin_convertvector(x, delta_bf16x8);
-    if (n + 1 < N) x -= __builtin_convertvector(p[n], delta_f32x8);
+    seq_u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+      if (n + 1 < N) {
+        x[2 * k] -= __builtin_bit_cast(float, (unsigned)w[k] << 16);
+        x[2 * k + 1] -= __builtin_bit_cast(float, (unsigned)w[k] & 0xFFFF0000u);
+      }
+    }
+    p[n] = __builtin_bit_cast(delta_bf16x8, w);
   }
 }
 template <int N>
@@ -193,7 +202,7 @@ struct DeltaTile {
   alignas(16) char bytes[N][R * PITCH];
   __device__ __forceinline__ void put(int place, int col, const delta_bf16x8 (&p)[N]) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) *(delta_bf16x8*)(bytes[n] + place * PITCH + col * 2) = p[n];
+    for (int n = 0; n < N; ++n) *(delta_bf16x8_any*)(bytes[n] + place * PITCH + col * 2) = p[n];
   }
   // Left operand, 16 rows from `place` on and 32 columns from `col` on.  (Or a right operand, of the transposed matrix.)
   template <int M>
@@ -243,29 +252,33 @@ struct DeltaTile {
 // Pitches that spread 16 rows over all banks: an odd number of 16 bytes; 3 more than a multiple of 128 elements: the transposed reads' four rows and four places too.
 constexpr int delta_pitch(int width) { return width * 2 + (width == 32 ? 16 : 48); }
 
-// Eight neighbours of a row of `width`, 0 past its end.
-__device__ __forceinline__ delta_f32x8 delta_load8(const float* row, int col, int width) {
-  delta_f32x8 x;
-  if (col + 8 <= width) {
-    const delta_f32x4 a = *(const delta_f32x4_any*)(row + col), b = *(const delta_f32x4_any*)(row + col + 4);
+// Eight neighbours of a row, of which it has `left`, and 0 behind them.
+__device__ __forceinline__ int delta_left(int col, int width) { return width - col < 0 ? 0 : (width - col < 8 ? width - col : 8); }
+__device__ __forceinline__ delta_f32x8 delta_load8(const float* at, int left) {
+  if (left == 8) {
+    const delta_f32x4 a = *(const delta_f32x4_any*)at, b = *(const delta_f32x4_any*)(at + 4);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
+  delta_f32x8 x;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = col + j < width ? row[col + j] : 0.f;
+  for (int j = 0; j < 8; ++j) x[j] = j < left ? at[j] : 0.f;
   return x;
 }
-__device__ __forceinline__ delta_bf16x8 delta_load8(const __bf16* row, int col, int width) {
-  if (col + 8 <= width) return __builtin_bit_cast(delta_bf16x8, *(const seq_u32x4_any*)(row + col));
+__device__ __forceinline__ delta_bf16x8 delta_load8(const __bf16* at, int left) {
+  if (left == 8) return __builtin_bit_cast(delta_bf16x8, *(const seq_u32x4_any*)at);
   delta_bf16x8 x;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = col + j < width ? row[col + j] : (__bf16)0.f;
+  for (int j = 0; j < 8; ++j) x[j] = j < left ? at[j] : (__bf16)0.f;
   return x;
 }
 __device__ __forceinline__ void delta_parts(delta_bf16x8 x, delta_bf16x8 (&p)[1]) { p[0] = x; }
 __device__ __forceinline__ delta_f32x8 delta_wide(delta_f32x8 x) { return x; }
 __device__ __forceinline__ delta_f32x8 delta_wide(delta_bf16x8 x) { return __builtin_convertvector(x, delta_f32x8); }
 
-// Which chunk of which head, and where its frames lie.
+// Which chunk of which head, and where its frames lie: the same in all lanes, and said so, so that addresses are made of scalars.
+__device__ __forceinline__ long long delta_same(long long v) {
+  return (long long)(unsigned)__builtin_amdgcn_readfirstlane((int)v) | (long long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
 struct DeltaWhere {
   int b, h, kh, chunk;
   long long n;      // frames of the sequence
@@ -273,7 +286,8 @@ struct DeltaWhere {
   long long first, step;  // row of the chunk's first frame, and from one frame's to the next's
   __device__ __forceinline__ DeltaWhere(const DeltaArgs& a, int bh, int chunk_, int frames) {
     b = bh / a.heads, h = bh - b * a.heads, kh = h / (a.heads / a.key_heads);
-    n = frames_of(a.lens, b, a.T);
+    n = delta_same(frames_of(a.lens, b, a.T));
+    step = a.reverse ? -(long long)a.B : a.B;
     to(a, chunk_, frames);
   }
   __device__ __forceinline__ void to(const DeltaArgs& a, int chunk_, int frames) {
@@ -281,10 +295,20 @@ struct DeltaWhere {
     const long long p = (long long)chunk * frames, left = n - p;
     count = left < 0 ? 0 : (left < frames ? (int)left : frames);
     first = (a.reverse ? n - 1 - p : p) * a.B + b;
-    step = a.reverse ? -(long long)a.B : a.B;
   }
   __device__ __forceinline__ long long row(int i) const { return first + i * step; }
 };
+// The frames of a chunk in a tensor: where the first one's `width` elements of a head are, and how far apart frames are, in elements.
+template <typename T>
+struct DeltaFrames {
+  T* base;
+  long long pitch;
+  __device__ __forceinline__ DeltaFrames(T* tensor, const DeltaWhere& at, long long ld, long long head) : base(tensor + at.first * ld + head), pitch(at.step * ld) {
+    asm("" : "+s"(pitch));  // (its multiples are computed where they are used: kept from chunk to chunk they do not fit into the scalar registers)
+  }
+};
+// Elements i * pitch of a result's lane: rows 8 q + i of 32, and its column.
+__device__ __forceinline__ long long delta_lane(long long pitch, int col) { return (threadIdx.x >> 4 & 3) * 8 * pitch + col; }
 
 // T, P, L and the powers of a chunk, one workgroup of C / 16 wavefronts each, which have 16 rows of L and P each.  The inverse: diagonal blocks of 16 row by row, a column per
 // lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.
@@ -326,9 +350,10 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
   // 16 rows of K and Q against all up to them
   delta_bf16x8 kf[DK / 32][NI], qf[DK / 32][NI];
   auto fetch = [&](const void* base, long long ld, int row, delta_bf16x8(&p)[DK / 32][NI]) {
-    const AT* r = (const AT*)base + at.row(row < at.count ? row : 0) * ld + at.kh * a.f.dk;
+    const DeltaFrames<const AT> frames((const AT*)base, at, ld, at.kh * a.f.dk);
+    const AT* r = frames.base + (row < at.count ? row : 0) * frames.pitch + q4 * 8;
 #pragma unroll
-    for (int b = 0; b < DK / 32; ++b) delta_parts(delta_load8(r, b * 32 + q4 * 8, row < at.count ? a.f.dk : 0), p[b]);
+    for (int b = 0; b < DK / 32; ++b) delta_parts(delta_load8(r + b * 32, row < at.count ? delta_left(b * 32 + q4 * 8, a.f.dk) : 0), p[b]);
   };
   fetch(a.f.k, a.f.ldk, wave * 16 + i16, kf);
   fetch(a.f.q, a.f.ldq, wave * 16 + i16, qf);
@@ -402,66 +427,115 @@ template <typename AT, int DK, int THREADS, int NP>
 struct DeltaStage {
   static constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, BLOCKS = delta_blocks(C);
   static constexpr int kRows = (C * DK / 8 + THREADS - 1) / THREADS, kBlocks = (BLOCKS * 128 + THREADS - 1) / THREADS;
-  typedef decltype(delta_load8((const AT*)nullptr, 0, 0)) Eight8;
+  typedef decltype(delta_load8((const AT*)nullptr, 0)) Eight8;
   struct Tiles {
     DeltaTile<NI, C, delta_pitch(DK)> K, Q;
     DeltaTile<3, BLOCKS * 32, delta_pitch(32)> T;
     DeltaTile<NP, BLOCKS * 32, delta_pitch(32)> P;
     alignas(16) float powers[3][C];  // c, gamma, beta
   };
+  static constexpr int kApart = THREADS * 8 / DK, kPowers = (3 * C + THREADS - 1) / THREADS;  // rows from one of a thread's to the next
+  static_assert(THREADS % (DK / 8) == 0, "a thread's rows have the same columns");
   Eight8 k[kRows], q[kRows];
   delta_f32x8 t[kBlocks], p[kBlocks];
-  static constexpr int kPowers = (3 * C + THREADS - 1) / THREADS;
   float power[kPowers];
-  __device__ __forceinline__ void load(const DeltaChunkArgs& a, const DeltaWhere& at, const float* record) {
+  int count;
+  // Nothing here depends on a condition of a lane, so that nothing waits: rows past the end are read as the last one and put as 0; the last eight columns of a row are read, and put,
+  // where the row has them, some of them twice.  (Heads of up to 32 may have fewer than eight: column by column.)
+  static __device__ __forceinline__ Eight8 eight(const AT* row, int dk) {
+    if constexpr (DK > 32) {
+      return delta_load8(row, 8);
+    } else {
+      const int col = column(dk);
+      Eight8 x;
 #pragma unroll
-    for (int n = 0; n < kRows; ++n) {
-      const int item = n * THREADS + threadIdx.x, row = item / (DK / 8), col = item % (DK / 8) * 8, width = row < at.count ? a.f.dk : 0;
-      const long long r = at.row(row < at.count ? row : 0);
-      k[n] = delta_load8((const AT*)a.f.k + r * a.f.ldk + at.kh * a.f.dk, col, width);
-      q[n] = delta_load8((const AT*)a.f.q + r * a.f.ldq + at.kh * a.f.dk, col, width);
-    }
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      const int item = n * THREADS + threadIdx.x;
-      if (item < BLOCKS * 128) {
-        t[n] = delta_load8(record, item * 8, BLOCKS * 1024);
-        p[n] = delta_load8(record + BLOCKS * 1024, item * 8, BLOCKS * 1024);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < kPowers; ++n) {
-      const int item = n * THREADS + threadIdx.x;
-      power[n] = item < 3 * C ? record[3 * BLOCKS * 1024 + item] : 0.f;
+      for (int j = 0; j < 8; ++j) x[j] = row[col + j < dk ? j : dk - 1 - col];
+      return x;
     }
   }
-  __device__ __forceinline__ void store(Tiles& to) const {
+  static __device__ __forceinline__ int column(int dk) {
+    const int col = threadIdx.x % (DK / 8) * 8;
+    return DK > 32 && col > dk - 8 ? dk - 8 : col;
+  }
+  __device__ __forceinline__ void load(const DeltaChunkArgs& a, const DeltaWhere& at, const float* record) {
+    count = at.count;
+    const DeltaFrames<const AT> kf((const AT*)a.f.k, at, a.f.ldk, at.kh * a.f.dk), qf((const AT*)a.f.q, at, a.f.ldq, at.kh * a.f.dk);
+    const int row = row_of(0), col = column(a.f.dk);
+    if (count == C) {
+      const long long k_lane = row * kf.pitch + col, q_lane = row * qf.pitch + col;
 #pragma unroll
-    for (int n = 0; n < kRows; ++n) {
-      const int item = n * THREADS + threadIdx.x, row = item / (DK / 8), col = item % (DK / 8) * 8;
-      if (C * DK / 8 % THREADS == 0 || row < C) {
-        delta_bf16x8 parts[NI];
-        delta_parts(k[n], parts);
-        to.K.put(delta_place(row), col, parts);
-        delta_parts(q[n], parts);
-        to.Q.put(delta_place(row), col, parts);
+      for (int n = 0; n < kRows; ++n) {
+        k[n] = eight(kf.base + n * kApart % C * kf.pitch + k_lane, a.f.dk);
+        q[n] = eight(qf.base + n * kApart % C * qf.pitch + q_lane, a.f.dk);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kRows; ++n) {
+        const int of = row_of(n) < count ? row_of(n) : count - 1;
+        k[n] = eight(kf.base + (of * kf.pitch + col), a.f.dk);
+        q[n] = eight(qf.base + (of * qf.pitch + col), a.f.dk);
       }
     }
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
-      const int item = n * THREADS + threadIdx.x, row = item >> 2, col = (item & 3) * 8;
-      if (item < BLOCKS * 128) {
-        delta_bf16x8 three[3], some[NP];
-        delta_parts(t[n], three);
-        to.T.put(delta_place(row), col, three);
-        delta_parts(p[n], some);
-        to.P.put(delta_place(row), col, some);
-      }
+      t[n] = delta_load8(record + item_of(n) * 8, 8);
+      p[n] = delta_load8(record + BLOCKS * 1024 + item_of(n) * 8, 8);
     }
 #pragma unroll
-    for (int n = 0; n < kPowers; ++n) {
-      const int item = n * THREADS + threadIdx.x;
-      if (item < 3 * C) to.powers[item / C][item % C] = power[n];
+    for (int n = 0; n < kPowers; ++n) power[n] = record[3 * BLOCKS * 1024 + power_of(n)];
+  }
+  static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x / (DK / 8) + n * kApart) % C; }  // (where threads are more than there is, some do the same)
+  static __device__ __forceinline__ int item_of(int n) {
+    const int item = n * THREADS + threadIdx.x;
+    return BLOCKS * 128 % THREADS == 0 || item < BLOCKS * 128 ? item : BLOCKS * 128 - 1;
+  }
+  static __device__ __forceinline__ int power_of(int n) {
+    const int item = n * THREADS + threadIdx.x;
+    return 3 * C % THREADS == 0 || item < 3 * C ? item : 3 * C - 1;
+  }
+  __device__ __forceinline__ void store(Tiles& to, int dk) const {
+    const int col = column(dk);
+    auto rows = [&](auto whole) {
+#pragma unroll
+      for (int n = 0; n < kRows; ++n) {
+        Eight8 x = k[n], y = q[n];
+        if constexpr (DK == 32 || !decltype(whole)::value) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool in = row_of(n) < count && (DK > 32 || col + j < dk);
+            x[j] = in ? x[j] : 0, y[j] = in ? y[j] : 0;
+          }
+        }
+        delta_bf16x8 parts[NI];
+        delta_parts(x, parts);
+        to.K.put(delta_place(row_of(n)), col, parts);
+        delta_parts(y, parts);
+        to.Q.put(delta_place(row_of(n)), col, parts);
+      }
+    };
+    if (count == C)
+      rows(std::true_type());
+    else
+      rows(std::false_type());
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+      const int row = item_of(n) >> 2, c8 = (item_of(n) & 3) * 8;
+      delta_bf16x8 three[3], some[NP];
+      delta_parts(t[n], three);
+      to.T.put(delta_place(row), c8, three);
+      delta_parts(p[n], some);
+      to.P.put(delta_place(row), c8, some);
+    }
+#pragma unroll
+    for (int n = 0; n < kPowers; ++n) (&to.powers[0][0])[power_of(n)] = power[n];
+  }
+  // Columns that no row has: 0 from the start.
+  static __device__ __forceinline__ void clear(Tiles& to, int dk) {
+    if (DK > 32 && dk < DK) {
+      for (int item = threadIdx.x; item < NI * C * DK; item += THREADS) {
+        const int n = item / (C * DK), row = item / DK % C, col = item % DK;
+        if (col >= dk) *(__bf16*)(to.K.bytes[n] + row * delta_pitch(DK) + col * 2) = *(__bf16*)(to.Q.bytes[n] + row * delta_pitch(DK) + col * 2) = (__bf16)0.f;
+      }
     }
   }
 };
@@ -483,40 +557,61 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
   const float* record = a.records + (long long)bh * a.chunks * delta_record(C);
   const long long matrix = (long long)a.f.dk * a.f.dv;
   delta_f32x4 S[2 * KB];
-  auto row_of = [&](int tile, int r) { return (tile >> 1) * 32 + q4 * 8 + (tile & 1) * 4 + r; };
+  auto first_of = [](int tile) { return (tile >> 1) * 32 + (tile & 1) * 4; };
+  auto row_of = [&](int tile, int r) { return first_of(tile) + q4 * 8 + r; };
 #pragma unroll
   for (int k = 0; k < 2 * KB; ++k)
 #pragma unroll
     for (int r = 0; r < 4; ++r) S[k][r] = a.f.s0 && has && row_of(k, r) < a.f.dk ? a.f.s0[bh * matrix + (long long)row_of(k, r) * a.f.dv + col] : 0.f;
+  const long long lane_state = delta_lane(a.f.dv, col);
+  const bool all_rows = a.f.dk == DK;
+  long long pitch_state = a.f.dv;
   auto put_state = [&](float* to) {
+    if (!has) return;
 #pragma unroll
-    for (int k = 0; k < 2 * KB; ++k)
+    for (int b = 0; b < KB; ++b) {
+      float* row = to + b * 32 * pitch_state;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (has && row_of(k, r) < a.f.dk) to[(long long)row_of(k, r) * a.f.dv + col] = S[k][r];
+      for (int j = 0; j < 8; ++j, row += pitch_state)
+        if (all_rows || b * 32 + q4 * 8 + j < a.f.dk) row[lane_state] = S[2 * b + (j >> 2)][j & 3];
+    }
   };
   Stage stage;
+  Stage::clear(lds, a.f.dk);
   AT v[M][4];
   auto load = [&]() {
     stage.load(a, at, record);
+    const DeltaFrames<const AT> frames((const AT*)a.f.v, at, a.f.ldv, (long long)at.h * a.f.dv);
+    const int of = has ? col : a.f.dv - 1;  // (what is no column is computed as the last one, and what is no row is read as the last one and taken as 0)
+    if (at.count == C) {
+      const long long lane_in = delta_lane(frames.pitch, of);
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+      for (int b = 0; b < NB; ++b) {
+        const AT* from = frames.base + b * 32 * frames.pitch;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = row_of(m, r);
-        v[m][r] = has && i < at.count ? ((const AT*)a.f.v)[at.row(i) * a.f.ldv + at.h * a.f.dv + col] : (AT)0.f;
+        for (int j = 0; j < 8; ++j, from += frames.pitch) v[2 * b + (j >> 2)][j & 3] = from[lane_in];
       }
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[m][r] = frames.base[(row_of(m, r) < at.count ? row_of(m, r) : at.count - 1) * frames.pitch + of];
+    }
   };
   if (chunks) load();
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const DeltaWhere here = at;
+    asm("" : "+s"(pitch_state));
     delta_f32x4 R[M], O[M];
     __syncthreads();
-    stage.store(lds);
+    stage.store(lds, a.f.dk);
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) R[m][r] = load_f32(&v[m][r]);
+      for (int r = 0; r < 4; ++r) {
+        R[m][r] = load_f32(&v[m][r]);
+        if (here.count < C) R[m][r] = row_of(m, r) < here.count ? R[m][r] : 0.f;
+      }
     __syncthreads();
     if (chunk + 1 < chunks) {
       at.to(a.f, chunk + 1, C);
@@ -568,14 +663,21 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         O[m] = delta_mma<OUT>(left, right, O[m]);
       }
     }
+    if (has) {
+      const DeltaFrames<AT> frames((AT*)a.f.y, here, (long long)a.f.heads * a.f.dv, (long long)here.h * a.f.dv);
+      float* writes = a.writes + ((long long)bh * a.chunks + chunk) * C * a.f.dv;
+      const long long lane_out = delta_lane(frames.pitch, col);
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+      for (int b = 0; b < NB; ++b) {
+        AT* to = frames.base + b * 32 * frames.pitch;
+        float* u = writes + b * 32 * pitch_state;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = row_of(m, r);
-        if (has && i < here.count) store_f32((AT*)a.f.y + (here.row(i) * a.f.heads + here.h) * a.f.dv + col, a.f.scale * O[m][r]);
-        if (KEEP && has) a.writes[(((long long)bh * a.chunks + chunk) * C + i) * a.f.dv + col] = U[m][r];
+        for (int j = 0; j < 8; ++j, to += frames.pitch, u += pitch_state) {
+          if (here.count == C || b * 32 + q4 * 8 + j < here.count) store_f32(to + lane_out, a.f.scale * O[2 * b + (j >> 2)][j & 3]);
+          if (KEEP) u[lane_state] = U[2 * b + (j >> 2)][j & 3];
+        }
       }
+    }
     const float end = lds.powers[0][C - 1];
 #pragma unroll
     for (int k = 0; k < 2 * KB; ++k) S[k] *= end;
@@ -619,41 +721,62 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
   const int chunks = (int)((at.n + C - 1) / C);
   const long long matrix = (long long)a.f.dk * a.f.dv;
   delta_f32x4 D[2 * KB];
-  auto row_of = [&](int tile, int r) { return (tile >> 1) * 32 + q4 * 8 + (tile & 1) * 4 + r; };
+  auto first_of = [](int tile) { return (tile >> 1) * 32 + (tile & 1) * 4; };
+  auto row_of = [&](int tile, int r) { return first_of(tile) + q4 * 8 + r; };
 #pragma unroll
   for (int k = 0; k < 2 * KB; ++k)
 #pragma unroll
     for (int r = 0; r < 4; ++r) D[k][r] = a.dsN && has && row_of(k, r) < a.f.dk ? a.dsN[bh * matrix + (long long)row_of(k, r) * a.f.dv + col] : 0.f;
+  const long long lane_state = delta_lane(a.f.dv, col);
+  const bool all_rows = a.f.dk == DK;
+  long long pitch_state = a.f.dv;
   auto put_state = [&](float* to) {
+    if (!has) return;
 #pragma unroll
-    for (int k = 0; k < 2 * KB; ++k)
+    for (int b = 0; b < KB; ++b) {
+      float* row = to + b * 32 * pitch_state;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (has && row_of(k, r) < a.f.dk) to[(long long)row_of(k, r) * a.f.dv + col] = D[k][r];
+      for (int j = 0; j < 8; ++j, row += pitch_state)
+        if (all_rows || b * 32 + q4 * 8 + j < a.f.dk) row[lane_state] = D[2 * b + (j >> 2)][j & 3];
+    }
   };
   Stage stage;
+  Stage::clear(lds, a.f.dk);
   AT y[M][4];
   auto load = [&](int chunk) {
     at.to(a.f, chunk, C);
     stage.load(a, at, a.records + ((long long)bh * a.chunks + chunk) * delta_record(C));
+    const DeltaFrames<const AT> frames((const AT*)a.dy, at, a.lddy, (long long)at.h * a.f.dv);
+    const int of = has ? col : a.f.dv - 1;  // (what is no column is computed as the last one, and what is no row is read as the last one and taken as 0)
+    if (at.count == C) {
+      const long long lane_in = delta_lane(frames.pitch, of);
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+      for (int b = 0; b < NB; ++b) {
+        const AT* from = frames.base + b * 32 * frames.pitch;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = row_of(m, r);
-        y[m][r] = has && i < at.count ? ((const AT*)a.dy)[at.row(i) * a.lddy + at.h * a.f.dv + col] : (AT)0.f;
+        for (int j = 0; j < 8; ++j, from += frames.pitch) y[2 * b + (j >> 2)][j & 3] = from[lane_in];
       }
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[m][r] = frames.base[(row_of(m, r) < at.count ? row_of(m, r) : at.count - 1) * frames.pitch + of];
+    }
   };
   if (chunks) load(chunks - 1);
   for (int chunk = chunks - 1; chunk >= 0; --chunk) {
     const DeltaWhere here = at;
+    asm("" : "+s"(pitch_state));
     delta_f32x4 E[M], R[M], KD[M];
     __syncthreads();
-    stage.store(lds);
+    stage.store(lds, a.f.dk);
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) E[m][r] = load_f32(&y[m][r]);
+      for (int r = 0; r < 4; ++r) {
+        E[m][r] = load_f32(&y[m][r]);
+        if (here.count < C) E[m][r] = row_of(m, r) < here.count ? E[m][r] : 0.f;
+      }
     __syncthreads();
     if (chunk) load(chunk - 1);
     put_state(a.dstates + ((long long)bh * a.chunks + chunk) * matrix);
@@ -696,15 +819,22 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
         R[m] = delta_mma<3>(left, right, R[m]);
       }
     }
+    if (has) {
+      const DeltaFrames<AT> frames((AT*)a.dv, here, (long long)a.f.heads * a.f.dv, (long long)here.h * a.f.dv);
+      float* writes = a.dwrites + ((long long)bh * a.chunks + chunk) * C * a.f.dv;
+      const long long lane_out = delta_lane(frames.pitch, col);
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const delta_f32x4 beta = delta_rows(lds.powers[2], m);
+      for (int b = 0; b < NB; ++b) {
+        AT* to = frames.base + b * 32 * frames.pitch;
+        float* u = writes + b * 32 * pitch_state;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = row_of(m, r);
-        if (has) {
-          a.dwrites[(((long long)bh * a.chunks + chunk) * C + i) * a.f.dv + col] = R[m][r];
-          if (i < here.count) store_f32((AT*)a.dv + (here.row(i) * a.f.heads + here.h) * a.f.dv + col, beta[r] * R[m][r]);
+        for (int t = 0; t < 2; ++t) {
+          const delta_f32x4 dv = delta_rows(lds.powers[2], 2 * b + t) * R[2 * b + t];
+#pragma unroll
+          for (int r = 0; r < 4; ++r, to += frames.pitch, u += pitch_state) {
+            if (here.count == C || b * 32 + q4 * 8 + t * 4 + r < here.count) store_f32(to + lane_out, dv[r]);
+            u[lane_state] = R[2 * b + t][r];
+          }
         }
       }
     }
@@ -789,13 +919,14 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   if (at.count == 0) return;
   const float* record = a.records + ((long long)bh * a.chunks + chunk) * delta_record(C);
   const long long number = (long long)bh * a.chunks + chunk, matrix = (long long)a.f.dk * a.f.dv;
+  const DeltaFrames<const AT> kf((const AT*)a.f.k, at, a.f.ldk, at.kh * a.f.dk), qf((const AT*)a.f.q, at, a.f.ldq, at.kh * a.f.dk);
+  const DeltaFrames<const AT> vf((const AT*)a.f.v, at, a.f.ldv, (long long)at.h * a.f.dv), yf((const AT*)a.dy, at, a.lddy, (long long)at.h * a.f.dv);
   for (int item = threadIdx.x; item < C * DK / 8; item += THREADS) {
-    const int row = item / (DK / 8), c8 = item % (DK / 8) * 8, width = row < at.count ? a.f.dk : 0;
-    const long long r = at.row(row < at.count ? row : 0);
+    const int row = item / (DK / 8), c8 = item % (DK / 8) * 8, left = row < at.count ? delta_left(c8, a.f.dk) : 0;
     delta_bf16x8 parts[NI];
-    delta_parts(delta_load8((const AT*)a.f.k + r * a.f.ldk + at.kh * a.f.dk, c8, width), parts);
+    delta_parts(delta_load8(kf.base + (row * kf.pitch + c8), left), parts);
     K.put(delta_place(row), c8, parts);
-    delta_parts(delta_load8((const AT*)a.f.q + r * a.f.ldq + at.kh * a.f.dk, c8, width), parts);
+    delta_parts(delta_load8(qf.base + (row * qf.pitch + c8), left), parts);
     Q.put(delta_place(row), c8, parts);
   }
   for (int i = threadIdx.x; i < 5 * C; i += THREADS) powers[i / C][i % C] = record[3 * BLOCKS * 1024 + i];
@@ -815,23 +946,22 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     for (int n = 0; n < kOwn; ++n) {
       const int item = n * THREADS + threadIdx.x, row = item >> 2, c8 = (item & 3) * 8;
       if (kItems % THREADS == 0 || item < kItems) {
-        const bool in = row < at.count;
-        const long long r = at.row(in ? row : 0);
-        const delta_f32x8 rr = delta_load8(R + (long long)row * a.f.dv, c0 + c8, a.f.dv);
+        const int left = delta_left(c0 + c8, a.f.dv), in = row < at.count ? left : 0;
+        const delta_f32x8 rr = delta_load8(R + ((long long)row * a.f.dv + c0 + c8), left);
         delta_bf16x8 parts[3], some[NI];
         delta_parts(rr, parts);
         lds.pass.R.put(delta_place(row), c8, parts);
-        delta_parts(delta_load8(U + (long long)row * a.f.dv, c0 + c8, a.f.dv), parts);
+        delta_parts(delta_load8(U + ((long long)row * a.f.dv + c0 + c8), left), parts);
         lds.pass.U.put(delta_place(row), c8, parts);
-        delta_parts(delta_load8((const AT*)a.dy + r * a.lddy + at.h * a.f.dv, c0 + c8, in ? a.f.dv : 0), some);
+        delta_parts(delta_load8(yf.base + (row * yf.pitch + c0 + c8), in), some);
         lds.pass.Y.put(delta_place(row), c8, some);
-        const delta_f32x8 v = delta_wide(delta_load8((const AT*)a.f.v + r * a.f.ldv + at.h * a.f.dv, c0 + c8, in ? a.f.dv : 0));
+        const delta_f32x8 v = delta_wide(delta_load8(vf.base + (row * vf.pitch + c0 + c8), in));
 #pragma unroll
         for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(rr[j], v[j], own_rv[n]);
       }
     }
-    const int width = my_row < a.f.dk ? a.f.dv : 0;
-    const delta_f32x8 s = delta_load8(S + (long long)my_row * a.f.dv, c0 + q4 * 8, width), d = delta_load8(D + (long long)my_row * a.f.dv, c0 + q4 * 8, width);
+    const int left = my_row < a.f.dk ? delta_left(c0 + q4 * 8, a.f.dv) : 0;
+    const delta_f32x8 s = delta_load8(S + ((long long)my_row * a.f.dv + c0 + q4 * 8), left), d = delta_load8(D + ((long long)my_row * a.f.dv + c0 + q4 * 8), left);
     delta_bf16x8 sp[3], dp[3];
 #pragma unroll
     for (int j = 0; j < 8; ++j) ds = __builtin_fmaf(s[j], d[j], ds);

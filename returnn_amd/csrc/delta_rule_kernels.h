@@ -129,7 +129,6 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
 // and, of tile t, rows 4 q + r; the operand wants rows 8 q + 0..7 of it.  So tile t is made of rows 8 q + 4 t + r, which its left operand's lane i = 4 q + r reads.  Left operands lie in LDS
 // with rows in that order (position 16 t + 4 q + r), so that a tile's are neighbours.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 delta_bf16x8;
-typedef delta_bf16x8 __attribute__((aligned(2))) delta_bf16x8_any;
 typedef __attribute__((__vector_size__(8 * sizeof(float)))) float delta_f32x8;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short delta_s16x4;
 
@@ -144,8 +143,10 @@ struct DeltaChunk<float> {
   static constexpr int kFrames = 32, kInput = 3, kOut = 3;  // (K and Q in three parts: 32 frames are what fits into LDS)
 };
 constexpr int delta_blocks(int frames) { return frames == 64 ? 3 : 1; }  // of 32 x 32, of a lower triangular matrix
-// What is kept of a chunk: T, P, L in blocks (0,0), (1,0), (1,1), row-major; then c, gamma, beta, and G in two parts.
-constexpr int delta_record(int frames) { return 3 * delta_blocks(frames) * 1024 + 5 * frames; }
+// What is kept of a chunk, in numbers of float32: T and P in three parts each, as they lie in LDS (DeltaTile, blocks (0,0), (1,0), (1,1)); L, block by block, row-major; c, gamma, beta,
+// and G in two parts.
+constexpr int delta_image(int frames) { return 6 * delta_blocks(frames) * 1024 / 2; }
+constexpr int delta_record(int frames) { return delta_image(frames) + delta_blocks(frames) * 1024 + 5 * frames; }
 
 struct DeltaChunkArgs {
   DeltaArgs f;
@@ -196,30 +197,36 @@ __device__ __forceinline__ delta_f32x4 delta_mma(const delta_bf16x8 (&a)[NA], co
   return c;
 }
 
-// A matrix in LDS as N planes of R rows.
-template <int N, int R, int PITCH>
+// A matrix in LDS as N planes of R rows of COLS columns, without gaps.  Groups of eight columns change places by the row, so that 16 neighbouring rows of a column lie in different banks, and
+// so do four rows of four neighbouring groups.
+template <int N, int R, int COLS>
 struct DeltaTile {
-  alignas(16) char bytes[N][R * PITCH];
+  alignas(16) char bytes[N][R * COLS * 2];
+  static __device__ __forceinline__ int swap_of(int place) {
+    const int low = place & 3, high = place >> 2 & 3;
+    return COLS == 128 ? low << 2 | high : (COLS == 64 ? (low >> 1) << 2 | high : high);
+  }
+  static __device__ __forceinline__ int offset(int place, int col) { return place * (COLS * 2) + (((col >> 3) ^ swap_of(place)) << 4) + (col & 7) * 2; }
   __device__ __forceinline__ void put(int place, int col, const delta_bf16x8 (&p)[N]) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) *(delta_bf16x8_any*)(bytes[n] + place * PITCH + col * 2) = p[n];
+    for (int n = 0; n < N; ++n) *(delta_bf16x8*)(bytes[n] + offset(place, col)) = p[n];
   }
-  // Left operand, 16 rows from `place` on and 32 columns from `col` on.  (Or a right operand, of the transposed matrix.)
-  template <int M>
+  // Left operand, 16 rows from `place` on and 32 columns from `col` on.  (Or a right operand, of the transposed matrix.)  FIRST: its first plane.
+  template <int FIRST = 0, int M>
   __device__ __forceinline__ void left(int place, int col, delta_bf16x8 (&p)[M]) const {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int n = 0; n < M; ++n) p[n] = *(const delta_bf16x8*)(bytes[n] + (place + (lane & 15)) * PITCH + (col + (lane >> 4) * 8) * 2);
+    for (int n = 0; n < M; ++n) p[n] = *(const delta_bf16x8*)(bytes[FIRST + n] + place * (COLS * 2) + offset(lane & 15, col + (lane >> 4) * 8));
   }
   // Left operand of the transposed matrix: rows are the columns 8 q + 4 t + r of the 32 from `col` on, columns the 32 rows from `place` on.
-  template <int M>
+  template <int FIRST = 0, int M>
   __device__ __forceinline__ void transposed(int place, int col, int t, delta_bf16x8 (&p)[M]) const {
-    across(place, col + 4 * t, 8, p);
+    across<FIRST>(place, col + 4 * t, 8, p);
   }
   // Right operand: the 32 rows from `place` on, the 16 columns from `col` on.
   template <int M>
   __device__ __forceinline__ void right(int place, int col, delta_bf16x8 (&p)[M]) const {
-    across(place, col, 4, p);
+    across<0>(place, col, 4, p);
   }
   // What a lane has of a result in rows place + 4 q + r, columns col + i: four rows of it.
   __device__ __forceinline__ delta_f32x4 of_result(int place, int col) const {
@@ -237,20 +244,18 @@ struct DeltaTile {
   // The hardware's transposed read: of 16 lanes, lane 4 r + c gives the address of four neighbours in row r, and lane i gets number i % 4 of lane 4 r + i / 4's for r = 0..3.
   __device__ __forceinline__ delta_s16x4 four(int n, int place, int col, int step) const {
     const int lane = threadIdx.x & 63, i = lane & 15;
-    const char* at = bytes[n] + (place + (lane >> 4) * 4 + (i >> 2)) * PITCH + (col + step * (i & 3)) * 2;
+    const char* at = bytes[n] + place * (COLS * 2) + offset((lane >> 4) * 4 + (i >> 2), col + step * (i & 3));
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) delta_s16x4*)at);
   }
-  template <int M>
+  template <int FIRST, int M>
   __device__ __forceinline__ void across(int place, int col, int step, delta_bf16x8 (&p)[M]) const {
 #pragma unroll
     for (int n = 0; n < M; ++n) {
-      const delta_s16x4 a = four(n, place, col, step), b = four(n, place + 16, col, step);
+      const delta_s16x4 a = four(FIRST + n, place, col, step), b = four(FIRST + n, place + 16, col, step);
       p[n] = __builtin_bit_cast(delta_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 };
-// Pitches that spread 16 rows over all banks: an odd number of 16 bytes; 3 more than a multiple of 128 elements: the transposed reads' four rows and four places too.
-constexpr int delta_pitch(int width) { return width * 2 + (width == 32 ? 16 : 48); }
 
 // Eight neighbours of a row, of which it has `left`, and 0 behind them.
 __device__ __forceinline__ int delta_left(int col, int width) { return width - col < 0 ? 0 : (width - col < 8 ? width - col : 8); }
@@ -269,6 +274,34 @@ __device__ __forceinline__ delta_bf16x8 delta_load8(const __bf16* at, int left) 
   delta_bf16x8 x;
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = j < left ? at[j] : (__bf16)0.f;
+  return x;
+}
+// The same without a condition of a lane, so that no load is waited for early: the last eight of a row are read in place of what goes beyond its end (of a narrow row its elements one by
+// one, the last one for what there is not), and moved to where they belong later, by delta_placed.
+__device__ __forceinline__ int delta_read_col(int col, int width) { return width >= 8 ? (col < width - 8 ? col : width - 8) : 0; }
+template <bool NARROW = true, typename T>
+__device__ __forceinline__ auto delta_load8_any(const T* at, int col, int width) {  // at: column delta_read_col; NARROW: whether there can be fewer than eight
+  auto x = delta_load8(at, !NARROW || width >= 8 ? 8 : 0);
+  if (NARROW && width < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = at[col + j < width ? col + j : width - 1];
+  }
+  return x;
+}
+template <bool NARROW = true, typename E>
+__device__ __forceinline__ E delta_placed(E x, int col, int width, bool in) {
+  const int shift = width >= 8 ? col - delta_read_col(col, width) : 0;
+#pragma unroll
+  for (int s = 4; s; s /= 2)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = shift & s ? (j + s < 8 ? x[j + s] : 0) : x[j];
+  if (NARROW && width < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = col + j < width ? x[j] : 0;
+  }
+  in = in && shift < 8;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = in ? x[j] : 0;
   return x;
 }
 __device__ __forceinline__ void delta_parts(delta_bf16x8 x, delta_bf16x8 (&p)[1]) { p[0] = x; }
@@ -298,17 +331,23 @@ struct DeltaWhere {
   }
   __device__ __forceinline__ long long row(int i) const { return first + i * step; }
 };
-// The frames of a chunk in a tensor: where the first one's `width` elements of a head are, and how far apart frames are, in elements.
-template <typename T>
+// The frames of a chunk in a tensor.  Frame i's row of a head, from element `col` on, is at(i) + lane(0, col), or at(0) + lane(i, col) for i up to REACH: at() is made of scalars, lane()
+// is an offset of 32 bits (frames are at most kDeltaFrameBytes long) that is the same for all chunks.
+constexpr long long kDeltaFrameBytes = 1 << 26;
+template <typename T, int REACH>
 struct DeltaFrames {
-  T* base;
+  char* base;
   long long pitch;
-  __device__ __forceinline__ DeltaFrames(T* tensor, const DeltaWhere& at, long long ld, long long head) : base(tensor + at.first * ld + head), pitch(at.step * ld) {
+  unsigned apart;
+  bool turned;
+  __device__ __forceinline__ DeltaFrames(const DeltaArgs& a, T* tensor, const DeltaWhere& at, long long ld, long long head)
+      : base((char*)(tensor + (at.first * ld + head))), pitch(at.step * ld * (long long)sizeof(T)), apart((unsigned)(a.B * ld * (long long)sizeof(T))), turned(a.reverse) {
     asm("" : "+s"(pitch));  // (its multiples are computed where they are used: kept from chunk to chunk they do not fit into the scalar registers)
+    if (turned) base += REACH * pitch;
   }
+  __device__ __forceinline__ char* at(int i) const { return base + i * pitch; }
+  __device__ __forceinline__ unsigned lane(int i, int col) const { return (unsigned)(turned ? REACH - i : i) * apart + (unsigned)col * (unsigned)sizeof(T); }
 };
-// Elements i * pitch of a result's lane: rows 8 q + i of 32, and its column.
-__device__ __forceinline__ long long delta_lane(long long pitch, int col) { return (threadIdx.x >> 4 & 3) * 8 * pitch + col; }
 
 // T, P, L and the powers of a chunk, one workgroup of C / 16 wavefronts each, which have 16 rows of L and P each.  The inverse: diagonal blocks of 16 row by row, a column per
 // lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.
@@ -328,7 +367,18 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
   }
   if (at.count == 0) return;
   float* record = a.records + ((long long)bh * a.chunks + chunk) * delta_record(C);
-  float *rT = record, *rP = rT + BLOCKS * 1024, *rL = rP + BLOCKS * 1024, *rc = rL + BLOCKS * 1024;
+  float *rL = record + delta_image(C), *rc = rL + BLOCKS * 1024;
+  typedef DeltaTile<6, BLOCKS * 32, 32> Image;
+  // Number (i, j) of T (which = 0) or P (1), in three parts.
+  auto put_image = [&](int which, int block, int i, int j, float x) {
+    char* to = (char*)record + which * 3 * (int)sizeof(Image().bytes[0]) + Image::offset(delta_place(block * 32 + i), j);
+#pragma unroll
+    for (int n = 0; n < 3; ++n, to += sizeof(Image().bytes[0])) {
+      const __bf16 part = (__bf16)x;
+      *(__bf16*)to = part;
+      x -= (float)part;
+    }
+  };
   if (wave == 0) {
     const bool in = lane < at.count;
     const long long f = at.row(in ? lane : 0) * a.f.heads + at.h;
@@ -349,9 +399,8 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
   }
   // 16 rows of K and Q against all up to them
   delta_bf16x8 kf[DK / 32][NI], qf[DK / 32][NI];
-  auto fetch = [&](const void* base, long long ld, int row, delta_bf16x8(&p)[DK / 32][NI]) {
-    const DeltaFrames<const AT> frames((const AT*)base, at, ld, at.kh * a.f.dk);
-    const AT* r = frames.base + (row < at.count ? row : 0) * frames.pitch + q4 * 8;
+  auto fetch = [&](const void* tensor, long long ld, int row, delta_bf16x8(&p)[DK / 32][NI]) {
+    const AT* r = (const AT*)tensor + (at.row(row < at.count ? row : 0) * ld + at.kh * a.f.dk + q4 * 8);
 #pragma unroll
     for (int b = 0; b < DK / 32; ++b) delta_parts(delta_load8(r + b * 32, row < at.count ? delta_left(b * 32 + q4 * 8, a.f.dk) : 0), p[b]);
   };
@@ -378,7 +427,7 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
       A[i * ROW + j] = beta_of[i] * l;
       X[i * ROW + j] = 0.f;
       if (nt / 2 <= wave / 2) {
-        rP[block * 1024 + (i & 31) * 32 + (j & 31)] = p;
+        put_image(1, block, i & 31, j & 31, p);
         rL[block * 1024 + (i & 31) * 32 + (j & 31)] = l;
       }
     }
@@ -418,210 +467,221 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
   }
   for (int e = threadIdx.x; e < BLOCKS * 1024; e += C * 4) {
     const int block = e >> 10, i = (e >> 5 & 31) + (block > 0) * 32, j = (e & 31) + (block > 1) * 32;
-    rT[e] = X[i * ROW + j];
+    put_image(0, block, e >> 5 & 31, e & 31, X[i * ROW + j]);
   }
 }
 
-// What the kernels that go through a head's chunks load of one into LDS, by way of registers, so that the next chunk's are on their way while one is worked on.
+// What the kernels that go through a head's chunks load of one into LDS, by way of registers: the one behind the next is on its way while one is worked on and the next lies in LDS.
+//
+// Rows past the end are read as the last one and put as 0.
 template <typename AT, int DK, int THREADS, int NP>
 struct DeltaStage {
   static constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, BLOCKS = delta_blocks(C);
-  static constexpr int kRows = (C * DK / 8 + THREADS - 1) / THREADS, kBlocks = (BLOCKS * 128 + THREADS - 1) / THREADS;
+  static constexpr int kApart = THREADS * 8 / DK;  // rows from one of a thread's to the next
+  static constexpr int kRows = (C + kApart - 1) / kApart, kImage = ((3 + NP) * BLOCKS * 128 + THREADS - 1) / THREADS, kPowers = (3 * C + THREADS - 1) / THREADS;
   typedef decltype(delta_load8((const AT*)nullptr, 0)) Eight8;
   struct Tiles {
-    DeltaTile<NI, C, delta_pitch(DK)> K, Q;
-    DeltaTile<3, BLOCKS * 32, delta_pitch(32)> T;
-    DeltaTile<NP, BLOCKS * 32, delta_pitch(32)> P;
+    DeltaTile<NI, C, DK> K, Q;
+    DeltaTile<3 + NP, BLOCKS * 32, 32> TP;  // T, then P
     alignas(16) float powers[3][C];  // c, gamma, beta
   };
-  static constexpr int kApart = THREADS * 8 / DK, kPowers = (3 * C + THREADS - 1) / THREADS;  // rows from one of a thread's to the next
-  static_assert(THREADS % (DK / 8) == 0, "a thread's rows have the same columns");
   Eight8 k[kRows], q[kRows];
-  delta_f32x8 t[kBlocks], p[kBlocks];
+  seq_u32x4 image[kImage];
   float power[kPowers];
   int count;
-  // Nothing here depends on a condition of a lane, so that nothing waits: rows past the end are read as the last one and put as 0; the last eight columns of a row are read, and put,
-  // where the row has them, some of them twice.  (Heads of up to 32 may have fewer than eight: column by column.)
-  static __device__ __forceinline__ Eight8 eight(const AT* row, int dk) {
-    if constexpr (DK > 32) {
-      return delta_load8(row, 8);
-    } else {
-      const int col = column(dk);
-      Eight8 x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = row[col + j < dk ? j : dk - 1 - col];
-      return x;
-    }
-  }
-  static __device__ __forceinline__ int column(int dk) {
-    const int col = threadIdx.x % (DK / 8) * 8;
-    return DK > 32 && col > dk - 8 ? dk - 8 : col;
-  }
-  __device__ __forceinline__ void load(const DeltaChunkArgs& a, const DeltaWhere& at, const float* record) {
-    count = at.count;
-    const DeltaFrames<const AT> kf((const AT*)a.f.k, at, a.f.ldk, at.kh * a.f.dk), qf((const AT*)a.f.q, at, a.f.ldq, at.kh * a.f.dk);
-    const int row = row_of(0), col = column(a.f.dk);
-    if (count == C) {
-      const long long k_lane = row * kf.pitch + col, q_lane = row * qf.pitch + col;
-#pragma unroll
-      for (int n = 0; n < kRows; ++n) {
-        k[n] = eight(kf.base + n * kApart % C * kf.pitch + k_lane, a.f.dk);
-        q[n] = eight(qf.base + n * kApart % C * qf.pitch + q_lane, a.f.dk);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < kRows; ++n) {
-        const int of = row_of(n) < count ? row_of(n) : count - 1;
-        k[n] = eight(kf.base + (of * kf.pitch + col), a.f.dk);
-        q[n] = eight(qf.base + (of * qf.pitch + col), a.f.dk);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      t[n] = delta_load8(record + item_of(n) * 8, 8);
-      p[n] = delta_load8(record + BLOCKS * 1024 + item_of(n) * 8, 8);
-    }
-#pragma unroll
-    for (int n = 0; n < kPowers; ++n) power[n] = record[3 * BLOCKS * 1024 + power_of(n)];
-  }
-  static __device__ __forceinline__ int row_of(int n) { return (threadIdx.x / (DK / 8) + n * kApart) % C; }  // (where threads are more than there is, some do the same)
-  static __device__ __forceinline__ int item_of(int n) {
+  // (where threads are more than there is, some do the same)
+  static __device__ __forceinline__ int row_of(int n) { return (int)(threadIdx.x / (DK / 8) + n * kApart) % C; }
+  static __device__ __forceinline__ int image_of(int n) {
+    constexpr int all = (3 + NP) * BLOCKS * 128;
     const int item = n * THREADS + threadIdx.x;
-    return BLOCKS * 128 % THREADS == 0 || item < BLOCKS * 128 ? item : BLOCKS * 128 - 1;
+    return all % THREADS == 0 || item < all ? item : all - 1;
   }
   static __device__ __forceinline__ int power_of(int n) {
     const int item = n * THREADS + threadIdx.x;
     return 3 * C % THREADS == 0 || item < 3 * C ? item : 3 * C - 1;
   }
+  static __device__ __forceinline__ int place_col() { return threadIdx.x % (DK / 8) * 8; }
+  __device__ __forceinline__ void load(const DeltaChunkArgs& a, const DeltaWhere& at, const float* record) {
+    count = at.count;
+    const DeltaFrames<const AT, C - 1> kf(a.f, (const AT*)a.f.k, at, a.f.ldk, at.kh * a.f.dk), qf(a.f, (const AT*)a.f.q, at, a.f.ldq, at.kh * a.f.dk);
+    const int col = delta_read_col(place_col(), a.f.dk);
+#pragma unroll
+    for (int n = 0; n < kRows; ++n) {
+      const int of = row_of(n) < count ? row_of(n) : count - 1;
+      k[n] = delta_load8_any<(DK <= 32)>((const AT*)(kf.at(0) + kf.lane(of, col)), place_col(), a.f.dk);
+      q[n] = delta_load8_any<(DK <= 32)>((const AT*)(qf.at(0) + qf.lane(of, col)), place_col(), a.f.dk);
+    }
+#pragma unroll
+    for (int n = 0; n < kImage; ++n) image[n] = *(const seq_u32x4*)((const char*)record + (unsigned)image_of(n) * 16u);
+#pragma unroll
+    for (int n = 0; n < kPowers; ++n) power[n] = *(const float*)((const char*)(record + delta_image(C) + BLOCKS * 1024) + (unsigned)power_of(n) * 4u);
+  }
   __device__ __forceinline__ void store(Tiles& to, int dk) const {
-    const int col = column(dk);
     auto rows = [&](auto whole) {
 #pragma unroll
       for (int n = 0; n < kRows; ++n) {
-        Eight8 x = k[n], y = q[n];
-        if constexpr (DK == 32 || !decltype(whole)::value) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const bool in = row_of(n) < count && (DK > 32 || col + j < dk);
-            x[j] = in ? x[j] : 0, y[j] = in ? y[j] : 0;
-          }
-        }
         delta_bf16x8 parts[NI];
-        delta_parts(x, parts);
-        to.K.put(delta_place(row_of(n)), col, parts);
-        delta_parts(y, parts);
-        to.Q.put(delta_place(row_of(n)), col, parts);
+        const bool in = decltype(whole)::value || row_of(n) < count;
+        delta_parts(decltype(whole)::value ? k[n] : delta_placed<(DK <= 32)>(k[n], place_col(), dk, in), parts);
+        to.K.put(delta_place(row_of(n)), place_col(), parts);
+        delta_parts(decltype(whole)::value ? q[n] : delta_placed<(DK <= 32)>(q[n], place_col(), dk, in), parts);
+        to.Q.put(delta_place(row_of(n)), place_col(), parts);
       }
     };
-    if (count == C)
+    if (count == C && dk == DK)
       rows(std::true_type());
     else
       rows(std::false_type());
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n) {
-      const int row = item_of(n) >> 2, c8 = (item_of(n) & 3) * 8;
-      delta_bf16x8 three[3], some[NP];
-      delta_parts(t[n], three);
-      to.T.put(delta_place(row), c8, three);
-      delta_parts(p[n], some);
-      to.P.put(delta_place(row), c8, some);
-    }
+    for (int n = 0; n < kImage; ++n) *(seq_u32x4*)(&to.TP.bytes[0][0] + image_of(n) * 16) = image[n];
 #pragma unroll
     for (int n = 0; n < kPowers; ++n) (&to.powers[0][0])[power_of(n)] = power[n];
-  }
-  // Columns that no row has: 0 from the start.
-  static __device__ __forceinline__ void clear(Tiles& to, int dk) {
-    if (DK > 32 && dk < DK) {
-      for (int item = threadIdx.x; item < NI * C * DK; item += THREADS) {
-        const int n = item / (C * DK), row = item / DK % C, col = item % DK;
-        if (col >= dk) *(__bf16*)(to.K.bytes[n] + row * delta_pitch(DK) + col * 2) = *(__bf16*)(to.Q.bytes[n] + row * delta_pitch(DK) + col * 2) = (__bf16)0.f;
-      }
-    }
   }
 };
 // Four rows' numbers of tile m.
 __device__ __forceinline__ delta_f32x4 delta_rows(const float* of, int m) { return *(const delta_f32x4*)(of + (m >> 1) * 32 + ((threadIdx.x >> 4) & 3) * 8 + (m & 1) * 4); }
 
-// Sixteen columns of a head's state per wavefront, in its registers, W wavefronts per workgroup, which share K, Q, T and P in LDS.
-template <typename AT, int DK, int W, bool KEEP>
-__global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
-  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32;
-  typedef DeltaStage<AT, DK, 64 * W, OUT> Stage;
-  __shared__ typename Stage::Tiles lds;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q4 = lane >> 4, i16 = lane & 15;
-  const int strips = (a.f.dv + 16 * W - 1) / (16 * W), strip = blockIdx.x % strips, bh = blockIdx.x / strips;
-  const int col = (strip * W + wave) * 16 + i16;
-  const bool has = col < a.f.dv;
-  DeltaWhere at(a.f, bh, 0, C);
-  const int chunks = (int)((at.n + C - 1) / C);
-  const float* record = a.records + (long long)bh * a.chunks * delta_record(C);
-  const long long matrix = (long long)a.f.dk * a.f.dv;
-  delta_f32x4 S[2 * KB];
-  auto first_of = [](int tile) { return (tile >> 1) * 32 + (tile & 1) * 4; };
-  auto row_of = [&](int tile, int r) { return first_of(tile) + q4 * 8 + r; };
+// An element on its way, in a register of its own (two of 16 bits in one would be waited for to be joined).
+template <typename AT>
+struct DeltaElement;
+template <>
+struct DeltaElement<float> {
+  float x;
+  __device__ __forceinline__ void load(const void* from) { x = *(const float*)from; }
+  __device__ __forceinline__ float get() const { return x; }
+};
+template <>
+struct DeltaElement<__bf16> {
+  unsigned x;
+  __device__ __forceinline__ void load(const void* from) { x = *(const unsigned short*)from; }
+  __device__ __forceinline__ float get() const { return __builtin_bit_cast(float, x << 16); }
+};
+
+// Sixteen columns of a head per wavefront, which go through its chunks one after the other, W wavefronts per workgroup, which share what DeltaStage brings: what the forward pass and the
+// gradient have alike.  A lane has, of tile m, rows 32 (m / 2) + 8 q + 4 (m % 2) + r.
+template <typename AT, int DK, int W>
+struct DeltaStrip {
+  static constexpr int C = DeltaChunk<AT>::kFrames, M = C / 16, NB = C / 32, KB = DK / 32;
+  const DeltaChunkArgs& a;
+  int q4, col;
+  bool has;
+  int strip, bh;
+  unsigned lane_state;
+  long long pitch_state;  // (bytes)
+  __device__ __forceinline__ DeltaStrip(const DeltaChunkArgs& args) : a(args) {
+    const int lane = threadIdx.x & 63, strips = (a.f.dv + 16 * W - 1) / (16 * W);
+    q4 = lane >> 4;
+    strip = blockIdx.x % strips, bh = blockIdx.x / strips;
+    col = (strip * W + (int)(threadIdx.x >> 6)) * 16 + (lane & 15);
+    has = col < a.f.dv;
+    lane_state = (unsigned)(q4 * 8 * a.f.dv + col) * 4u;
+    pitch_state = a.f.dv * 4ll;
+  }
+  static __device__ __forceinline__ constexpr int first_of(int m) { return (m >> 1) * 32 + (m & 1) * 4; }
+  __device__ __forceinline__ int row_of(int m, int r) const { return first_of(m) + q4 * 8 + r; }
+  __device__ __forceinline__ long long matrix() const { return (long long)a.f.dk * a.f.dv; }
+  __device__ __forceinline__ long long number(int chunk) const { return (long long)bh * a.chunks + chunk; }
+  // A state, or C rows of float32 of the width dv.
+  template <int TILES>
+  __device__ __forceinline__ void get(const float* from, int rows, delta_f32x4 (&x)[TILES]) const {
 #pragma unroll
-  for (int k = 0; k < 2 * KB; ++k)
+    for (int k = 0; k < TILES; ++k)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) S[k][r] = a.f.s0 && has && row_of(k, r) < a.f.dk ? a.f.s0[bh * matrix + (long long)row_of(k, r) * a.f.dv + col] : 0.f;
-  const long long lane_state = delta_lane(a.f.dv, col);
-  const bool all_rows = a.f.dk == DK;
-  long long pitch_state = a.f.dv;
-  auto put_state = [&](float* to) {
+      for (int r = 0; r < 4; ++r) x[k][r] = from && has && row_of(k, r) < rows ? *(const float*)((const char*)from + (first_of(k) + r) * pitch_state + lane_state) : 0.f;
+  }
+  template <int TILES>
+  __device__ __forceinline__ void put(float* to, int rows, const delta_f32x4 (&x)[TILES]) const {
+    long long pitch = pitch_state;
+    asm("" : "+s"(pitch));  // (as of DeltaFrames)
     if (!has) return;
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      float* row = to + b * 32 * pitch_state;
+    for (int b = 0; b < TILES / 2; ++b) {
+      char* row = (char*)to + b * 32 * pitch;
 #pragma unroll
-      for (int j = 0; j < 8; ++j, row += pitch_state)
-        if (all_rows || b * 32 + q4 * 8 + j < a.f.dk) row[lane_state] = S[2 * b + (j >> 2)][j & 3];
+      for (int j = 0; j < 8; ++j, row += pitch)
+        if (rows == TILES * 16 || b * 32 + q4 * 8 + j < rows) *(float*)(row + lane_state) = x[2 * b + (j >> 2)][j & 3];
     }
-  };
-  Stage stage;
-  Stage::clear(lds, a.f.dk);
-  AT v[M][4];
-  auto load = [&]() {
-    stage.load(a, at, record);
-    const DeltaFrames<const AT> frames((const AT*)a.f.v, at, a.f.ldv, (long long)at.h * a.f.dv);
-    const int of = has ? col : a.f.dv - 1;  // (what is no column is computed as the last one, and what is no row is read as the last one and taken as 0)
-    if (at.count == C) {
-      const long long lane_in = delta_lane(frames.pitch, of);
+  }
+  // C frames of a tensor [T,B,heads,dv].  What is no column is computed as the last one, and what is no row is read as the last one and taken as 0.
+  __device__ __forceinline__ void load(const void* tensor, long long ld, const DeltaWhere& at, DeltaElement<AT> (&x)[M][4]) const {
+    const DeltaFrames<const AT, C - 1> frames(a.f, (const AT*)tensor, at, ld, (long long)at.h * a.f.dv);
+    // (one way for whole chunks and others: where ways meet, 16 bits would be waited for to be widened)
+    const unsigned step = frames.turned ? 0u - frames.apart : frames.apart;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const AT* from = frames.base + b * 32 * frames.pitch;
+    for (int b = 0; b < NB; ++b) {
+      const int last = at.count - 1, first = b * 32 + q4 * 8;
+      unsigned lane = frames.lane(first < last ? first : last, has ? col : a.f.dv - 1);
 #pragma unroll
-        for (int j = 0; j < 8; ++j, from += frames.pitch) v[2 * b + (j >> 2)][j & 3] = from[lane_in];
+      for (int j = 0; j < 8; ++j) {
+        x[2 * b + (j >> 2)][j & 3].load(frames.at(0) + lane);
+        lane += first + j < last ? step : 0u;
       }
-    } else {
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[m][r] = frames.base[(row_of(m, r) < at.count ? row_of(m, r) : at.count - 1) * frames.pitch + of];
     }
-  };
-  if (chunks) load();
-  for (int chunk = 0; chunk < chunks; ++chunk) {
-    const DeltaWhere here = at;
-    asm("" : "+s"(pitch_state));
-    delta_f32x4 R[M], O[M];
-    __syncthreads();
-    stage.store(lds, a.f.dk);
+  }
+  __device__ __forceinline__ void take(const DeltaElement<AT> (&x)[M][4], int count, delta_f32x4 (&to)[M]) const {
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        R[m][r] = load_f32(&v[m][r]);
-        if (here.count < C) R[m][r] = row_of(m, r) < here.count ? R[m][r] : 0.f;
+        to[m][r] = x[m][r].get();
+        if (count < C) to[m][r] = row_of(m, r) < count ? to[m][r] : 0.f;
       }
-    __syncthreads();
-    if (chunk + 1 < chunks) {
-      at.to(a.f, chunk + 1, C);
-      record += delta_record(C);
-      load();
-    }
-    if (KEEP) put_state(a.states + ((long long)bh * a.chunks + chunk) * matrix);
-    delta_f32x4 KS[M];
+  }
+  __device__ __forceinline__ void store(void* tensor, const DeltaWhere& at, const delta_f32x4 (&x)[M]) const {
+    const DeltaFrames<AT, 24> frames(a.f, (AT*)tensor, at, (long long)a.f.heads * a.f.dv, (long long)at.h * a.f.dv);
+    if (!has) return;
+    const unsigned lane = frames.lane(q4 * 8, col);
 #pragma unroll
-    for (int m = 0; m < M; ++m) KS[m] = O[m] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < NB; ++b) {
+      char* to = frames.at(b * 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j, to += frames.pitch)
+        if (at.count == C || b * 32 + q4 * 8 + j < at.count) store_f32((AT*)(to + lane), x[2 * b + (j >> 2)][j & 3]);
+    }
+  }
+};
+template <int N>
+__device__ __forceinline__ void delta_zero(delta_f32x4 (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
+}
+
+template <typename AT, int DK, int W, bool KEEP>
+__global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
+  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32;
+  typedef DeltaStage<AT, DK, 64 * W, OUT> Stage;
+  __shared__ typename Stage::Tiles tiles[2];
+  DeltaStrip<AT, DK, W> strip(a);
+  DeltaWhere at(a.f, strip.bh, 0, C);
+  const int chunks = (int)((at.n + C - 1) / C);
+  const float* records = a.records + strip.number(0) * delta_record(C);
+  delta_f32x4 S[2 * KB];
+  strip.get(a.f.s0 ? a.f.s0 + strip.bh * strip.matrix() : nullptr, a.f.dk, S);
+  Stage stage;
+  DeltaElement<AT> v[M][4];
+  auto load = [&](int chunk) {  // (the last one again where there is no next: what is loaded on a condition is waited for)
+    at.to(a.f, chunk < chunks ? chunk : chunks - 1, C);
+    stage.load(a, at, records + (long long)at.chunk * delta_record(C));
+  };
+  if (chunks) {
+    stage.load(a, at, records);
+    strip.load(a.f.v, a.f.ldv, at, v);
+    stage.store(tiles[0], a.f.dk);
+    load(1);
+    __syncthreads();
+  }
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    const typename Stage::Tiles& lds = tiles[chunk & 1];
+    DeltaWhere here = at;
+    here.to(a.f, chunk, C);
+    delta_f32x4 R[M], O[M], KS[M], U[M];
+    strip.take(v, here.count, R);
+    strip.load(a.f.v, a.f.ldv, at, v);
+    stage.store(tiles[chunk + 1 & 1], a.f.dk);
+    load(chunk + 2);
+    if (KEEP) strip.put(a.states + strip.number(chunk) * strip.matrix(), a.f.dk, S);
+    delta_zero(KS);
+    delta_zero(O);
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
       delta_bf16x8 s[3], left[NI];
@@ -640,44 +700,31 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
       R[m] = delta_rows(lds.powers[2], m) * (R[m] - c * KS[m]);
       O[m] *= c;
     }
-    delta_f32x4 U[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) U[m] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
+    delta_zero(U);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       delta_bf16x8 right[3], left[3];
       delta_parts(R[2 * b], R[2 * b + 1], right);
 #pragma unroll
       for (int m = 2 * b; m < M; ++m) {
-        lds.T.left((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
+        lds.TP.left((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
         U[m] = delta_mma<3>(left, right, U[m]);
       }
     }
+    if (KEEP) strip.put(a.writes + strip.number(chunk) * C * a.f.dv, C, U);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       delta_bf16x8 right[OUT], left[OUT];
       delta_parts(U[2 * b], U[2 * b + 1], right);
 #pragma unroll
       for (int m = 2 * b; m < M; ++m) {
-        lds.P.left((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
+        lds.TP.template left<3>((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
         O[m] = delta_mma<OUT>(left, right, O[m]);
       }
     }
-    if (has) {
-      const DeltaFrames<AT> frames((AT*)a.f.y, here, (long long)a.f.heads * a.f.dv, (long long)here.h * a.f.dv);
-      float* writes = a.writes + ((long long)bh * a.chunks + chunk) * C * a.f.dv;
-      const long long lane_out = delta_lane(frames.pitch, col);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        AT* to = frames.base + b * 32 * frames.pitch;
-        float* u = writes + b * 32 * pitch_state;
-#pragma unroll
-        for (int j = 0; j < 8; ++j, to += frames.pitch, u += pitch_state) {
-          if (here.count == C || b * 32 + q4 * 8 + j < here.count) store_f32(to + lane_out, a.f.scale * O[2 * b + (j >> 2)][j & 3]);
-          if (KEEP) u[lane_state] = U[2 * b + (j >> 2)][j & 3];
-        }
-      }
-    }
+    for (int m = 0; m < M; ++m) O[m] *= a.f.scale;
+    strip.store(a.f.y, here, O);
     const float end = lds.powers[0][C - 1];
 #pragma unroll
     for (int k = 0; k < 2 * KB; ++k) S[k] *= end;
@@ -691,8 +738,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         S[k] = delta_mma<3>(left, right, S[k]);
       }
     }
+    __syncthreads();
   }
-  put_state(a.f.sN + bh * matrix);
+  strip.put(a.f.sN + strip.bh * strip.matrix(), a.f.dk, S);
 }
 
 // ---- the gradient -----------------------------------------------------------------------------------------------------
@@ -712,76 +760,38 @@ template <typename AT, int DK, int W>
 __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, KB = DK / 32;
   typedef DeltaStage<AT, DK, 64 * W, 3> Stage;
-  __shared__ typename Stage::Tiles lds;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q4 = lane >> 4, i16 = lane & 15;
-  const int strips = (a.f.dv + 16 * W - 1) / (16 * W), strip = blockIdx.x % strips, bh = blockIdx.x / strips;
-  const int col = (strip * W + wave) * 16 + i16;
-  const bool has = col < a.f.dv;
-  DeltaWhere at(a.f, bh, 0, C);
+  __shared__ typename Stage::Tiles tiles[2];
+  DeltaStrip<AT, DK, W> strip(a);
+  DeltaWhere at(a.f, strip.bh, 0, C);
   const int chunks = (int)((at.n + C - 1) / C);
-  const long long matrix = (long long)a.f.dk * a.f.dv;
+  const float* records = a.records + strip.number(0) * delta_record(C);
   delta_f32x4 D[2 * KB];
-  auto first_of = [](int tile) { return (tile >> 1) * 32 + (tile & 1) * 4; };
-  auto row_of = [&](int tile, int r) { return first_of(tile) + q4 * 8 + r; };
-#pragma unroll
-  for (int k = 0; k < 2 * KB; ++k)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) D[k][r] = a.dsN && has && row_of(k, r) < a.f.dk ? a.dsN[bh * matrix + (long long)row_of(k, r) * a.f.dv + col] : 0.f;
-  const long long lane_state = delta_lane(a.f.dv, col);
-  const bool all_rows = a.f.dk == DK;
-  long long pitch_state = a.f.dv;
-  auto put_state = [&](float* to) {
-    if (!has) return;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      float* row = to + b * 32 * pitch_state;
-#pragma unroll
-      for (int j = 0; j < 8; ++j, row += pitch_state)
-        if (all_rows || b * 32 + q4 * 8 + j < a.f.dk) row[lane_state] = D[2 * b + (j >> 2)][j & 3];
-    }
-  };
+  strip.get(a.dsN ? a.dsN + strip.bh * strip.matrix() : nullptr, a.f.dk, D);
   Stage stage;
-  Stage::clear(lds, a.f.dk);
-  AT y[M][4];
+  DeltaElement<AT> y[M][4];
   auto load = [&](int chunk) {
-    at.to(a.f, chunk, C);
-    stage.load(a, at, a.records + ((long long)bh * a.chunks + chunk) * delta_record(C));
-    const DeltaFrames<const AT> frames((const AT*)a.dy, at, a.lddy, (long long)at.h * a.f.dv);
-    const int of = has ? col : a.f.dv - 1;  // (what is no column is computed as the last one, and what is no row is read as the last one and taken as 0)
-    if (at.count == C) {
-      const long long lane_in = delta_lane(frames.pitch, of);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const AT* from = frames.base + b * 32 * frames.pitch;
-#pragma unroll
-        for (int j = 0; j < 8; ++j, from += frames.pitch) y[2 * b + (j >> 2)][j & 3] = from[lane_in];
-      }
-    } else {
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[m][r] = frames.base[(row_of(m, r) < at.count ? row_of(m, r) : at.count - 1) * frames.pitch + of];
-    }
+    at.to(a.f, chunk > 0 ? chunk : 0, C);
+    stage.load(a, at, records + (long long)at.chunk * delta_record(C));
   };
-  if (chunks) load(chunks - 1);
+  if (chunks) {
+    load(chunks - 1);
+    strip.load(a.dy, a.lddy, at, y);
+    stage.store(tiles[chunks - 1 & 1], a.f.dk);
+    load(chunks - 2);
+    __syncthreads();
+  }
   for (int chunk = chunks - 1; chunk >= 0; --chunk) {
-    const DeltaWhere here = at;
-    asm("" : "+s"(pitch_state));
+    const typename Stage::Tiles& lds = tiles[chunk & 1];
+    DeltaWhere here = at;
+    here.to(a.f, chunk, C);
     delta_f32x4 E[M], R[M], KD[M];
-    __syncthreads();
-    stage.store(lds, a.f.dk);
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        E[m][r] = load_f32(&y[m][r]);
-        if (here.count < C) E[m][r] = row_of(m, r) < here.count ? E[m][r] : 0.f;
-      }
-    __syncthreads();
-    if (chunk) load(chunk - 1);
-    put_state(a.dstates + ((long long)bh * a.chunks + chunk) * matrix);
-#pragma unroll
-    for (int m = 0; m < M; ++m) KD[m] = R[m] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
+    strip.take(y, here.count, E);
+    strip.load(a.dy, a.lddy, at, y);
+    stage.store(tiles[chunk + 1 & 1], a.f.dk);
+    load(chunk - 2);
+    strip.put(a.dstates + strip.number(chunk) * strip.matrix(), a.f.dk, D);
+    delta_zero(KD);
+    delta_zero(R);
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
       delta_bf16x8 d[3], left[NI];
@@ -799,45 +809,28 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
       delta_parts(E[2 * b], E[2 * b + 1], right);
 #pragma unroll
       for (int m = 0; m < 2 * b + 2; ++m) {
-        lds.P.transposed((b + m / 2) * 32, 0, m & 1, left);
+        lds.TP.template transposed<3>((b + m / 2) * 32, 0, m & 1, left);
         R[m] = delta_mma<3>(left, right, R[m]);
       }
     }
     delta_f32x4 dU[M];
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      dU[m] = a.f.scale * R[m] + delta_rows(lds.powers[1], m) * KD[m];
-      R[m] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+    for (int m = 0; m < M; ++m) dU[m] = a.f.scale * R[m] + delta_rows(lds.powers[1], m) * KD[m];
+    delta_zero(R);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       delta_bf16x8 right[3], left[3];
       delta_parts(dU[2 * b], dU[2 * b + 1], right);
 #pragma unroll
       for (int m = 0; m < 2 * b + 2; ++m) {
-        lds.T.transposed((b + m / 2) * 32, 0, m & 1, left);
+        lds.TP.transposed((b + m / 2) * 32, 0, m & 1, left);
         R[m] = delta_mma<3>(left, right, R[m]);
       }
     }
-    if (has) {
-      const DeltaFrames<AT> frames((AT*)a.dv, here, (long long)a.f.heads * a.f.dv, (long long)here.h * a.f.dv);
-      float* writes = a.dwrites + ((long long)bh * a.chunks + chunk) * C * a.f.dv;
-      const long long lane_out = delta_lane(frames.pitch, col);
+    strip.put(a.dwrites + strip.number(chunk) * C * a.f.dv, C, R);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        AT* to = frames.base + b * 32 * frames.pitch;
-        float* u = writes + b * 32 * pitch_state;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const delta_f32x4 dv = delta_rows(lds.powers[2], 2 * b + t) * R[2 * b + t];
-#pragma unroll
-          for (int r = 0; r < 4; ++r, to += frames.pitch, u += pitch_state) {
-            if (here.count == C || b * 32 + q4 * 8 + t * 4 + r < here.count) store_f32(to + lane_out, dv[r]);
-            u[lane_state] = R[2 * b + t][r];
-          }
-        }
-      }
-    }
+    for (int m = 0; m < M; ++m) R[m] *= delta_rows(lds.powers[2], m);
+    strip.store(a.dv, here, R);
     const float end = lds.powers[0][C - 1];
 #pragma unroll
     for (int k = 0; k < 2 * KB; ++k) D[k] *= end;
@@ -854,7 +847,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
         D[k] = delta_mma<3>(left, right, D[k]);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) x[t] = -(delta_rows(lds.powers[0], 2 * b + t) * delta_rows(lds.powers[2], 2 * b + t)) * R[2 * b + t];
+      for (int t = 0; t < 2; ++t) x[t] = -delta_rows(lds.powers[0], 2 * b + t) * R[2 * b + t];
       delta_parts(x[0], x[1], right);
 #pragma unroll
       for (int k = 0; k < 2 * KB; ++k) {
@@ -862,8 +855,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
         D[k] = delta_mma<3>(left, right, D[k]);
       }
     }
+    __syncthreads();
   }
-  put_state(a.ds0 + bh * matrix);
+  strip.put(a.ds0 + strip.bh * strip.matrix(), a.f.dk, D);
 }
 
 // The sum over 16 neighbouring lanes, in all of them.
@@ -876,27 +870,29 @@ __device__ __forceinline__ float delta_sum16(float v) {
   return v;
 }
 
-// One chunk of one head per workgroup, DK / 16 wavefronts with 16 columns of dQ and dK each.  The values' columns pass by 32 at a time.
+// One chunk of one head per workgroup, DK / 16 wavefronts with 16 columns of dQ and dK each.  The values' columns pass by 32 at a time, the next ones on their way meanwhile.
 template <typename AT, int DK>
 __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;
-  constexpr int kTiles = BLOCKS * 4, kEach = (kTiles + W - 1) / W, kItems = C * 4, kOwn = (kItems + THREADS - 1) / THREADS, ROW = C + 1;
+  constexpr int kTiles = BLOCKS * 4, kEach = (kTiles + W - 1) / W;                                        // of C x C, for each wavefront
+  constexpr int kItems = C * 4, kTasks = (2 * kItems + THREADS - 1) / THREADS;                            // eights of 32 columns: of R and V, then of U and dY
+  constexpr int kApart = THREADS * 8 / DK;
+  typedef decltype(delta_load8((const AT*)nullptr, 0)) Eight8;
   struct Passing {  // of the values' columns
-    DeltaTile<3, C, delta_pitch(32)> U, R;
-    DeltaTile<NI, C, delta_pitch(32)> Y;
+    DeltaTile<3, C, 32> R, U;
+    DeltaTile<NI, C, 32> Y;
   };
   struct Square {
-    float N[C * ROW], XL[C * ROW];
-    DeltaTile<OUT, BLOCKS * 32, delta_pitch(32)> F, H;
+    DeltaTile<OUT, BLOCKS * 32, 32> F, H;
   };
-  __shared__ DeltaTile<NI, C, delta_pitch(DK)> K, Q;
+  __shared__ DeltaTile<NI, C, DK> K, Q;
   __shared__ union Shared {
     Passing pass;
     Square square;
   } lds;
   __shared__ alignas(16) float powers[5][C];  // c, gamma, beta, G in two parts
-  __shared__ float dots[3][W][C], rv[C], sums[2][C], xl[C], ds_of[W];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q4 = lane >> 4, i16 = lane & 15;
+  __shared__ float dots[3][W][C], rv[C], sums[3][M][C], ds_of[W];  // sums of 16 columns of N and of X o L, of 16 rows of N
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, i16 = lane & 15;
   const int chunk = blockIdx.x % a.chunks, bh = blockIdx.x / a.chunks;
   const DeltaWhere at(a.f, bh, chunk, C);
   AT *dq = (AT*)a.dq, *dk = (AT*)a.dk;
@@ -917,56 +913,84 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     if (lane == 0) a.dg[head] = a.dbeta[head] = 0.f;
   }
   if (at.count == 0) return;
-  const float* record = a.records + ((long long)bh * a.chunks + chunk) * delta_record(C);
   const long long number = (long long)bh * a.chunks + chunk, matrix = (long long)a.f.dk * a.f.dv;
-  const DeltaFrames<const AT> kf((const AT*)a.f.k, at, a.f.ldk, at.kh * a.f.dk), qf((const AT*)a.f.q, at, a.f.ldq, at.kh * a.f.dk);
-  const DeltaFrames<const AT> vf((const AT*)a.f.v, at, a.f.ldv, (long long)at.h * a.f.dv), yf((const AT*)a.dy, at, a.lddy, (long long)at.h * a.f.dv);
-  for (int item = threadIdx.x; item < C * DK / 8; item += THREADS) {
-    const int row = item / (DK / 8), c8 = item % (DK / 8) * 8, left = row < at.count ? delta_left(c8, a.f.dk) : 0;
-    delta_bf16x8 parts[NI];
-    delta_parts(delta_load8(kf.base + (row * kf.pitch + c8), left), parts);
-    K.put(delta_place(row), c8, parts);
-    delta_parts(delta_load8(qf.base + (row * qf.pitch + c8), left), parts);
-    Q.put(delta_place(row), c8, parts);
-  }
-  for (int i = threadIdx.x; i < 5 * C; i += THREADS) powers[i / C][i % C] = record[3 * BLOCKS * 1024 + i];
-
-  const delta_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  delta_f32x4 YS[M], UD[M], RS[M], X[kEach], Z[kEach];
+  const float *record = a.records + number * delta_record(C), *rL = record + delta_image(C);
+  const int width = a.f.dv;
+  const int my_row = wave * 16 + i16, state_row = my_row < a.f.dk ? my_row : a.f.dk - 1;  // of S and D
+  // What passes by, from column c0 on.
+  delta_f32x8 s, d, f[kTasks];
+  Eight8 x[kTasks];
+  auto load = [&](int c0) {
+    const unsigned state = (unsigned)(state_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
+    s = delta_load8_any((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
+    d = delta_load8_any((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
 #pragma unroll
-  for (int m = 0; m < M; ++m) YS[m] = UD[m] = RS[m] = zero;
-#pragma unroll
-  for (int n = 0; n < kEach; ++n) X[n] = Z[n] = zero;
-  const float *U = a.writes + number * C * a.f.dv, *R = a.dwrites + number * C * a.f.dv, *S = a.states + number * matrix, *D = a.dstates + number * matrix;
-  const int my_row = wave * 16 + i16;  // of S and D
-  float ds = 0.f, own_rv[kOwn] = {};
-  for (int c0 = 0; c0 < a.f.dv; c0 += 32) {
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < kOwn; ++n) {
-      const int item = n * THREADS + threadIdx.x, row = item >> 2, c8 = (item & 3) * 8;
-      if (kItems % THREADS == 0 || item < kItems) {
-        const int left = delta_left(c0 + c8, a.f.dv), in = row < at.count ? left : 0;
-        const delta_f32x8 rr = delta_load8(R + ((long long)row * a.f.dv + c0 + c8), left);
-        delta_bf16x8 parts[3], some[NI];
-        delta_parts(rr, parts);
-        lds.pass.R.put(delta_place(row), c8, parts);
-        delta_parts(delta_load8(U + ((long long)row * a.f.dv + c0 + c8), left), parts);
-        lds.pass.U.put(delta_place(row), c8, parts);
-        delta_parts(delta_load8(yf.base + (row * yf.pitch + c0 + c8), in), some);
-        lds.pass.Y.put(delta_place(row), c8, some);
-        const delta_f32x8 v = delta_wide(delta_load8(vf.base + (row * vf.pitch + c0 + c8), in));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(rr[j], v[j], own_rv[n]);
+    for (int n = 0; n < kTasks; ++n) {
+      const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, col = c0 + (item & 3) * 8;
+      if (first < 2 * kItems) {
+        f[n] = delta_load8_any((which ? a.writes : a.dwrites) + number * C * width + (row * width + delta_read_col(col, width)), col, width);
+        const AT* tensor = (const AT*)(which ? a.dy : a.f.v);
+        const long long ld = which ? a.lddy : a.f.ldv;
+        x[n] = delta_load8_any(tensor + (at.row(row < at.count ? row : at.count - 1) * ld + (long long)at.h * width + delta_read_col(col, width)), col, width);
       }
     }
-    const int left = my_row < a.f.dk ? delta_left(c0 + q4 * 8, a.f.dv) : 0;
-    const delta_f32x8 s = delta_load8(S + ((long long)my_row * a.f.dv + c0 + q4 * 8), left), d = delta_load8(D + ((long long)my_row * a.f.dv + c0 + q4 * 8), left);
+  };
+  load(0);
+  {
+    const int col = threadIdx.x % (DK / 8) * 8;
+    for (int row = threadIdx.x / (DK / 8); row < C; row += kApart) {
+      const long long r = at.row(row < at.count ? row : at.count - 1);
+      delta_bf16x8 parts[NI];
+      delta_parts(delta_placed(delta_load8_any((const AT*)a.f.k + (r * a.f.ldk + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
+      K.put(delta_place(row), col, parts);
+      delta_parts(delta_placed(delta_load8_any((const AT*)a.f.q + (r * a.f.ldq + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
+      Q.put(delta_place(row), col, parts);
+    }
+  }
+  for (int i = threadIdx.x; i < 5 * C; i += THREADS) powers[i / C][i % C] = rL[BLOCKS * 1024 + i];
+
+  delta_f32x4 YS[M], UD[M], RS[M], X[kEach], Z[kEach];
+  delta_zero(YS);
+  delta_zero(UD);
+  delta_zero(RS);
+  delta_zero(X);
+  delta_zero(Z);
+  float ds = 0.f, own_rv[kTasks] = {};
+  auto tile_m = [](int tile) { return (tile >> 2 > 0) * 2 + (tile >> 1 & 1); };
+  auto tile_o = [](int tile) { return (tile >> 2 > 1) * 2 + (tile & 1); };
+  for (int c0 = 0; c0 < width; c0 += 32) {
+    const bool whole = c0 + 32 <= width && at.count == C && a.f.dk == DK;
+    if (!whole) {
+      s = delta_placed(s, c0 + q4 * 8, width, my_row < a.f.dk);
+      d = delta_placed(d, c0 + q4 * 8, width, my_row < a.f.dk);
+    }
+#pragma unroll
+    for (int n = 0; n < kTasks; ++n) {
+      const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, c8 = (item & 3) * 8;
+      if (first < 2 * kItems) {
+        if (!whole) {
+          f[n] = delta_placed(f[n], c0 + c8, width, true);
+          x[n] = delta_placed(x[n], c0 + c8, width, row < at.count);
+        }
+        delta_bf16x8 parts[3], some[NI];
+        delta_parts(f[n], parts);
+        (which ? lds.pass.U : lds.pass.R).put(delta_place(row), c8, parts);
+        if (which) {
+          delta_parts(x[n], some);
+          lds.pass.Y.put(delta_place(row), c8, some);
+        } else {
+          const delta_f32x8 v = delta_wide(x[n]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(f[n][j], v[j], own_rv[n]);
+        }
+      }
+    }
     delta_bf16x8 sp[3], dp[3];
 #pragma unroll
     for (int j = 0; j < 8; ++j) ds = __builtin_fmaf(s[j], d[j], ds);
     delta_parts(s, sp);
     delta_parts(d, dp);
+    if (c0 + 32 < width) load(c0 + 32);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m) {
@@ -980,53 +1004,61 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     }
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
-      const int tile = n * W + wave, block = tile >> 2;
+      const int tile = n * W + wave;
       if (kTiles % W == 0 || tile < kTiles) {
-        const int m = (block > 0) * 2 + (tile >> 1 & 1), o = (block > 1) * 2 + (tile & 1);
         delta_bf16x8 left[3], some[NI], right[3];
-        lds.pass.U.left(o * 16, 0, right);
-        lds.pass.R.left(m * 16, 0, left);
+        lds.pass.U.left(tile_o(tile) * 16, 0, right);
+        lds.pass.R.left(tile_m(tile) * 16, 0, left);
         X[n] = delta_mma<3>(left, right, X[n]);
-        lds.pass.Y.left(m * 16, 0, some);
+        lds.pass.Y.left(tile_m(tile) * 16, 0, some);
         Z[n] = delta_mma<3>(some, right, Z[n]);
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
 #pragma unroll
-  for (int n = 0; n < kOwn; ++n) {
-    const int item = n * THREADS + threadIdx.x;
-    float v = own_rv[n];
-    v += __shfl_xor(v, 1);
-    v += __shfl_xor(v, 2);
-    if (item < kItems && (item & 3) == 0) rv[item >> 2] = v;
+  for (int n = 0; n < kTasks; ++n) {
+    const int first = n * THREADS + wave * 64, item = first + lane;
+    if (first < kItems) {
+      float v = own_rv[n];
+      v += __shfl_xor(v, 1);
+      v += __shfl_xor(v, 2);
+      if ((item & 3) == 0) rv[item >> 2] = v;
+    }
   }
-  for (int e = threadIdx.x; e < C * ROW; e += THREADS) lds.square.N[e] = lds.square.XL[e] = 0.f;
-  __syncthreads();
 #pragma unroll
   for (int n = 0; n < kEach; ++n) {
     const int tile = n * W + wave, block = tile >> 2;
     if (kTiles % W == 0 || tile < kTiles) {
-      const int m = (block > 0) * 2 + (tile >> 1 & 1), o = (block > 1) * 2 + (tile & 1);
+      const int m = tile_m(tile), o = tile_o(tile);
       const int j = (o >> 1) * 32 + (i16 >> 2) * 8 + (o & 1) * 4 + (i16 & 3);
+      float column = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4 + r, in_block = block * 1024 + (i & 31) * 32 + (j & 31);
+        const int i = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4 + r, place = block * 32 + (m & 1) * 16 + q4 * 4 + r;
+        const char* image = (const char*)record + 3 * BLOCKS * 2048 + DeltaTile<3, BLOCKS * 32, 32>::offset(place, j & 31);
+        float p = 0.f;
+#pragma unroll
+        for (int k = 2; k >= 0; --k) p += (float)*(const __bf16*)(image + k * BLOCKS * 2048);
+        const float l = rL[block * 1024 + (i & 31) * 32 + (j & 31)];
         const float x = i > j ? X[n][r] : 0.f, z = i >= j ? a.f.scale * Z[n][r] : 0.f;
         const float e = i >= j ? expf((powers[3][i] - powers[3][j]) + (powers[4][i] - powers[4][j])) : 0.f, beta = powers[2][i];
-        const float p = record[BLOCKS * 1024 + in_block], l = record[2 * BLOCKS * 1024 + in_block];
-        lds.square.N[i * ROW + j] = z * p - x * (beta * l);
-        lds.square.XL[i * ROW + j] = x * l;
-        const int place = block * 32 + delta_place(i & 31);
+        const float both = z * p - x * (beta * l), row = delta_sum16(both), with_l = delta_sum16(x * l);
+        column += both;
+        if (i16 == 0) sums[0][o][i] = row, sums[1][o][i] = with_l;
         float f = z * e, h = -(x * beta * e);
+        const int to = DeltaTile<OUT, BLOCKS * 32, 32>::offset(place, j & 31);
 #pragma unroll
         for (int k = 0; k < OUT; ++k) {
           const __bf16 fp = (__bf16)f, hp = (__bf16)h;
-          *(__bf16*)(lds.square.F.bytes[k] + place * delta_pitch(32) + (j & 31) * 2) = fp;
-          *(__bf16*)(lds.square.H.bytes[k] + place * delta_pitch(32) + (j & 31) * 2) = hp;
+          *(__bf16*)(lds.square.F.bytes[k] + to) = fp;
+          *(__bf16*)(lds.square.H.bytes[k] + to) = hp;
           f -= (float)fp, h -= (float)hp;
         }
       }
+      column += __shfl_xor(column, 16);
+      column += __shfl_xor(column, 32);
+      if (q4 == 0) sums[2][m][j] = column;
     }
   }
   ds = delta_sum16(ds);
@@ -1048,20 +1080,6 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     UD[m] = gamma * UD[m] - beta * c * RS[m];
   }
   __syncthreads();
-  // sums of rows and columns, eight threads each
-  for (int item = threadIdx.x; item < C * 8; item += THREADS) {
-    const int i = item >> 3, part = item & 7;
-    float row = 0.f, column = 0.f, with_l = 0.f;
-#pragma unroll
-    for (int o = 0; o < C / 8; ++o) {
-      const int j = part + 8 * o;
-      row += lds.square.N[i * ROW + j], column += lds.square.N[j * ROW + i], with_l += lds.square.XL[i * ROW + j];
-    }
-    float d = row - column;
-#pragma unroll
-    for (int step = 1; step < 8; step *= 2) d += __shfl_xor(d, step), with_l += __shfl_xor(with_l, step);
-    if (part == 0) sums[0][i] = d, xl[i] = with_l;
-  }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     delta_bf16x8 k_right[NI], q_right[NI], left[OUT];
@@ -1100,15 +1118,19 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
         }
       }
     }
-  __syncthreads();
   if (wave == 0) {
-    const int i = lane < C ? lane : 0;
-    float x = 0.f, y = 0.f, z = 0.f, all = 0.f;
+    const int i = lane < C ? lane : 0, block = i >> 5;
+    float x = 0.f, y = 0.f, z = 0.f, all = 0.f, row = 0.f, with_l = 0.f, column = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) x += dots[0][w][i], y += dots[1][w][i], z += dots[2][w][i], all += ds_of[w];
+#pragma unroll
+    for (int o = 0; o < M; ++o) {
+      row += o < 2 * block + 2 ? sums[0][o][i] : 0.f, with_l += o < 2 * block + 2 ? sums[1][o][i] : 0.f;
+      column += o >= 2 * block ? sums[2][o][i] : 0.f;
+    }
     const float c = powers[0][i], gamma = powers[1][i], beta = powers[2][i];
     float end = lane < C ? gamma * z : 0.f;
-    float d = lane < C ? a.f.scale * c * x - beta * c * y - gamma * z + sums[0][i] : 0.f;
+    float d = lane < C ? a.f.scale * c * x - beta * c * y - gamma * z + (row - column) : 0.f;
     end = delta_sum16(end);
     end += __shfl_xor(end, 16);
     end += __shfl_xor(end, 32);
@@ -1121,7 +1143,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     if (lane < at.count) {
       const long long to = at.row(lane) * a.f.heads + at.h;
       a.dg[to] = d + end;
-      a.dbeta[to] = rv[lane] - c * y - xl[lane];
+      a.dbeta[to] = rv[lane] - c * y - with_l;
     }
   }
 }

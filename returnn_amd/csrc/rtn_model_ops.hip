@@ -50,11 +50,21 @@ void with_delta(const DeltaSizes& z, F f) {
       f(type, Count<128>());
   });
 }
-constexpr int kDeltaWaves = 4;
-int64_t delta_strips(const DeltaSizes& z) { return (z.dv + 16 * kDeltaWaves - 1) / (16 * kDeltaWaves); }
-bool delta_fits(const DeltaSizes& z) {
+// Wavefronts of a workgroup that goes through a head's chunks.
+int delta_waves(const DeltaSizes& z) { return z.dv > 64 && (int64_t)z.B * z.heads * ((z.dv + 127) / 128) >= 128 ? 8 : 4; }
+int64_t delta_strips(const DeltaSizes& z) { return (z.dv + 16 * delta_waves(z) - 1) / (16 * delta_waves(z)); }
+template <typename F>
+void with_waves(const DeltaSizes& z, F f) {
+  if (delta_waves(z) == 8)
+    f(Count<8>());
+  else
+    f(Count<4>());
+}
+// Whether launches and offsets are within what 32 bits count; widest: elements of a frame of the widest tensor, with its pitch.
+bool delta_fits(const DeltaSizes& z, int64_t widest) {
   const int64_t most = max_blocks(512) / std::max<int64_t>(1, (int64_t)z.B * z.heads);
-  return delta_chunks(z) <= most && delta_strips(z) <= most && (!delta_shared(z) || delta_shared(z) / 256 < (size_t)max_blocks(256));
+  return delta_chunks(z) <= most && delta_strips(z) <= most && (!delta_shared(z) || delta_shared(z) / 256 < (size_t)max_blocks(256)) &&
+         std::max(widest, (int64_t)z.heads * z.dv) <= kDeltaFrameBytes / size_of(z.dtype) / z.B;
 }
 int delta_check(const char* what, const DeltaSizes& z, int32_t direction) {
   if (z.T < 0 || z.B < 0 || z.key_heads < 0 || z.heads < 0 || z.T > kMaxFrames || z.dk < 1 || z.dk > kMaxKeyDim || z.dv < 1 || z.dv > kMaxValueDim)
@@ -120,7 +130,7 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     });
     return launched(what);
   }
-  if (!delta_fits(z)) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
+  if (!delta_fits(z, std::max({ldq, ldk, ldv}))) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
   const size_t need = rtn_delta_rule_fwd_workspace_bytes(T, B, key_heads, heads, dk, dv, dtype, saved != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
@@ -133,10 +143,13 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     constexpr int DK = decltype(width)::value;
     const dim3 heads_grid((unsigned)(B * heads * delta_strips(z)));
     if (T) hipLaunchKernelGGL((k_delta_chunks<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DeltaChunk<AT>::kFrames * 4), 0, stream, c);
-    if (saved)
-      hipLaunchKernelGGL((k_delta_forward<AT, DK, kDeltaWaves, true>), heads_grid, dim3(64 * kDeltaWaves), 0, stream, c);
-    else
-      hipLaunchKernelGGL((k_delta_forward<AT, DK, kDeltaWaves, false>), heads_grid, dim3(64 * kDeltaWaves), 0, stream, c);
+    with_waves(z, [&](auto waves) {
+      constexpr int W = decltype(waves)::value;
+      if (saved)
+        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, true>), heads_grid, dim3(64 * W), 0, stream, c);
+      else
+        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, false>), heads_grid, dim3(64 * W), 0, stream, c);
+    });
   });
   return launched(what);
 }
@@ -160,7 +173,7 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(dy, e) || !aligned(dq, e) || !aligned(dk_out, e) || !aligned(dv_out, e) || !aligned(g, 4) || !aligned(beta, 4) ||
       !aligned(dsN, 4) || !aligned(dg, 4) || !aligned(dbeta, 4) || !aligned(ds0, 4) || !aligned(lens, 8) || !aligned(saved, 16))
     return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
-  if (!delta_fits(z)) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
+  if (!delta_fits(z, std::max({ldq, ldk, ldv, lddy}))) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d heads=%d dv=%d are too many for one call", what, (long long)T, B, heads, dv);
   const size_t need = rtn_delta_rule_bwd_workspace_bytes(T, B, key_heads, heads, dk, dv, dtype);
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
@@ -176,7 +189,10 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     typedef decltype(type) AT;
     constexpr int DK = decltype(width)::value;
     const hipStream_t stream = (hipStream_t)hip_stream;
-    hipLaunchKernelGGL((k_delta_backward<AT, DK, kDeltaWaves>), dim3((unsigned)(B * heads * delta_strips(z))), dim3(64 * kDeltaWaves), 0, stream, c);
+    with_waves(z, [&](auto waves) {
+      constexpr int W = decltype(waves)::value;
+      hipLaunchKernelGGL((k_delta_backward<AT, DK, W>), dim3((unsigned)(B * heads * delta_strips(z))), dim3(64 * W), 0, stream, c);
+    });
     if (T) hipLaunchKernelGGL((k_delta_gradients<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DK * 4), 0, stream, c);
     if (delta_shared(z)) {
       const int64_t items = T * B * key_heads * (int64_t)dk;

@@ -152,7 +152,7 @@ struct DeltaChunkArgs {
   DeltaArgs f;
   int chunks;      // of T frames
   float* records;  // [B,heads,chunks][record]
-  float* states;   // [B,heads,chunks][dk][dv] before each chunk, or NULL
+  float* states;   // [B,heads,chunks][DK][dv] before each chunk (DK: dk as in LDS), or NULL
   float* writes;   // [B,heads,chunks][C][dv]: U, or NULL
   const void* dy;
   long long lddy;
@@ -196,6 +196,22 @@ __device__ __forceinline__ delta_f32x4 delta_mma(const delta_bf16x8 (&a)[NA], co
       if (i < NA && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
   return c;
 }
+
+// The same for several tiles with one right operand, tile after tile, so that no product waits for the one before it.
+template <int ORDER, int TILES, int NA, int NB>
+__device__ __forceinline__ void delta_mma(const delta_bf16x8 (&a)[TILES][NA], const delta_bf16x8 (&b)[NB], delta_f32x4* c) {
+#pragma unroll
+  for (int s = ORDER - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i <= s; ++i)
+      if (i < NA && s - i < NB) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) c[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][i], b[s - i], c[t], 0, 0, 0);
+      }
+}
+// Between what is asked for and the products that do not need it yet: left to itself the compiler reads every operand just before its product, and each of these waits for LDS
+// (T=4000, one sequence of 8 heads of 128 x 128 in bf16: 331 us).
+__device__ __forceinline__ void delta_ahead() { __builtin_amdgcn_sched_barrier(0); }
 
 // A matrix in LDS as N planes of R rows of COLS columns, without gaps.  Groups of eight columns change places by the row, so that 16 neighbouring rows of a column lie in different banks, and
 // so do four rows of four neighbouring groups.
@@ -580,6 +596,7 @@ struct DeltaStrip {
   static __device__ __forceinline__ constexpr int first_of(int m) { return (m >> 1) * 32 + (m & 1) * 4; }
   __device__ __forceinline__ int row_of(int m, int r) const { return first_of(m) + q4 * 8 + r; }
   __device__ __forceinline__ long long matrix() const { return (long long)a.f.dk * a.f.dv; }
+  __device__ __forceinline__ long long kept() const { return (long long)DK * a.f.dv; }
   __device__ __forceinline__ long long number(int chunk) const { return (long long)bh * a.chunks + chunk; }
   // A state, or C rows of float32 of the width dv.
   template <int TILES>
@@ -648,7 +665,7 @@ __device__ __forceinline__ void delta_zero(delta_f32x4 (&x)[N]) {
 
 template <typename AT, int DK, int W, bool KEEP>
 __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
-  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32;
+  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32, BLOCKS = delta_blocks(C);
   typedef DeltaStage<AT, DK, 64 * W, OUT> Stage;
   __shared__ typename Stage::Tiles tiles[2];
   DeltaStrip<AT, DK, W> strip(a);
@@ -679,65 +696,96 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
     strip.load(a.f.v, a.f.ldv, at, v);
     stage.store(tiles[chunk + 1 & 1], a.f.dk);
     load(chunk + 2);
-    if (KEEP) strip.put(a.states + strip.number(chunk) * strip.matrix(), a.f.dk, S);
+    if (KEEP) strip.put(a.states + strip.number(chunk) * strip.kept(), DK, S);
     delta_zero(KS);
     delta_zero(O);
+    delta_zero(U);
+    {
+      delta_bf16x8 k[2][M][NI], q[2][M][NI], p[2][3];
+      auto ask = [&](int b) {
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      delta_bf16x8 s[3], left[NI];
-      delta_parts(S[2 * b], S[2 * b + 1], s);
+        for (int m = 0; m < M; ++m) {
+          lds.K.left(m * 16, b * 32, k[b & 1][m]);
+          lds.Q.left(m * 16, b * 32, q[b & 1][m]);
+        }
+      };
+      ask(0);
+      delta_parts(S[0], S[1], p[0]);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        lds.K.left(m * 16, b * 32, left);
-        KS[m] = delta_mma<3>(left, s, KS[m]);
-        lds.Q.left(m * 16, b * 32, left);
-        O[m] = delta_mma<OUT>(left, s, O[m]);
+      for (int b = 0; b < KB; ++b) {
+        if (b + 1 < KB) ask(b + 1);
+        delta_ahead();
+        if (b + 1 < KB) delta_parts(S[2 * b + 2], S[2 * b + 3], p[b + 1 & 1]);
+        delta_mma<3>(k[b & 1], p[b & 1], KS);
+        delta_mma<OUT>(q[b & 1], p[b & 1], O);
       }
     }
+    {
+      // T and P: blocks (0,0), (1,0), (1,1), of two tiles of 16 rows each
+      delta_bf16x8 t[BLOCKS][2][3], p[BLOCKS][2][OUT], right[3], some[OUT];
+      auto ask_t = [&](int n) {
+        lds.TP.left(n * 32, 0, t[n][0]);
+        lds.TP.left(n * 32 + 16, 0, t[n][1]);
+      };
+      auto ask_p = [&](int n) {
+        lds.TP.template left<3>(n * 32, 0, p[n][0]);
+        lds.TP.template left<3>(n * 32 + 16, 0, p[n][1]);
+      };
+      ask_t(0);
+      if constexpr (NB == 2) ask_t(1);
+      delta_ahead();
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const delta_f32x4 c = delta_rows(lds.powers[0], m);
-      R[m] = delta_rows(lds.powers[2], m) * (R[m] - c * KS[m]);
-      O[m] *= c;
-    }
-    delta_zero(U);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      delta_bf16x8 right[3], left[3];
-      delta_parts(R[2 * b], R[2 * b + 1], right);
-#pragma unroll
-      for (int m = 2 * b; m < M; ++m) {
-        lds.TP.left((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
-        U[m] = delta_mma<3>(left, right, U[m]);
+      for (int m = 0; m < M; ++m) {
+        const delta_f32x4 c = delta_rows(lds.powers[0], m);
+        R[m] = delta_rows(lds.powers[2], m) * (R[m] - c * KS[m]);
+        O[m] *= c;
+      }
+      delta_parts(R[0], R[1], right);
+      delta_mma<3>(t[0], right, U);
+      ask_p(0);
+      if constexpr (NB == 2) {
+        ask_t(2);
+        delta_ahead();
+        delta_mma<3>(t[1], right, U + 2);
+        delta_parts(R[2], R[3], right);
+        delta_parts(U[0], U[1], some);
+        delta_mma<3>(t[2], right, U + 2);
+        ask_p(1);
+        ask_p(2);
+        delta_ahead();
+        delta_mma<OUT>(p[0], some, O);
+        delta_mma<OUT>(p[1], some, O + 2);
+        delta_parts(U[2], U[3], some);
+        delta_mma<OUT>(p[2], some, O + 2);
+      } else {
+        delta_parts(U[0], U[1], some);
+        delta_mma<OUT>(p[0], some, O);
       }
     }
     if (KEEP) strip.put(a.writes + strip.number(chunk) * C * a.f.dv, C, U);
+    {
+      delta_bf16x8 k[2][KB][NI], right[NB][3];
+      // (half of the tiles at a time)
+      auto ask = [&](int n) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      delta_bf16x8 right[OUT], left[OUT];
-      delta_parts(U[2 * b], U[2 * b + 1], right);
+        for (int i = 0; i < KB; ++i) lds.K.transposed(n / 2 * 32, (n % 2 * KB + i) / 2 * 32, (n % 2 * KB + i) % 2, k[n & 1][i]);
+      };
+      ask(0);
+      const float end = lds.powers[0][C - 1];
 #pragma unroll
-      for (int m = 2 * b; m < M; ++m) {
-        lds.TP.template left<3>((m / 2 + b) * 32 + (m & 1) * 16, 0, left);
-        O[m] = delta_mma<OUT>(left, right, O[m]);
+      for (int k = 0; k < 2 * KB; ++k) S[k] *= end;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) delta_parts(delta_rows(lds.powers[1], 2 * b) * U[2 * b], delta_rows(lds.powers[1], 2 * b + 1) * U[2 * b + 1], right[b]);
+#pragma unroll
+      for (int n = 0; n < 2 * NB; ++n) {
+        if (n + 1 < 2 * NB) ask(n + 1);
+        delta_ahead();
+        delta_mma<3>(k[n & 1], right[n / 2], S + n % 2 * KB);
       }
     }
 #pragma unroll
     for (int m = 0; m < M; ++m) O[m] *= a.f.scale;
     strip.store(a.f.y, here, O);
-    const float end = lds.powers[0][C - 1];
-#pragma unroll
-    for (int k = 0; k < 2 * KB; ++k) S[k] *= end;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      delta_bf16x8 right[3], left[NI];
-      delta_parts(delta_rows(lds.powers[1], 2 * b) * U[2 * b], delta_rows(lds.powers[1], 2 * b + 1) * U[2 * b + 1], right);
-#pragma unroll
-      for (int k = 0; k < 2 * KB; ++k) {
-        lds.K.transposed(b * 32, (k >> 1) * 32, k & 1, left);
-        S[k] = delta_mma<3>(left, right, S[k]);
-      }
-    }
     __syncthreads();
   }
   strip.put(a.f.sN + strip.bh * strip.matrix(), a.f.dk, S);
@@ -789,7 +837,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
     strip.load(a.dy, a.lddy, at, y);
     stage.store(tiles[chunk + 1 & 1], a.f.dk);
     load(chunk - 2);
-    strip.put(a.dstates + strip.number(chunk) * strip.matrix(), a.f.dk, D);
+    strip.put(a.dstates + strip.number(chunk) * strip.kept(), DK, D);
     delta_zero(KD);
     delta_zero(R);
 #pragma unroll
@@ -913,15 +961,15 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     if (lane == 0) a.dg[head] = a.dbeta[head] = 0.f;
   }
   if (at.count == 0) return;
-  const long long number = (long long)bh * a.chunks + chunk, matrix = (long long)a.f.dk * a.f.dv;
+  const long long number = (long long)bh * a.chunks + chunk, matrix = (long long)DK * a.f.dv;
   const float *record = a.records + number * delta_record(C), *rL = record + delta_image(C);
   const int width = a.f.dv;
-  const int my_row = wave * 16 + i16, state_row = my_row < a.f.dk ? my_row : a.f.dk - 1;  // of S and D
+  const int my_row = wave * 16 + i16;  // of S and D
   // What passes by, from column c0 on.
   delta_f32x8 s, d, f[kTasks];
   Eight8 x[kTasks];
   auto load = [&](int c0) {
-    const unsigned state = (unsigned)(state_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
+    const unsigned state = (unsigned)(my_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
     s = delta_load8_any((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
     d = delta_load8_any((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
 #pragma unroll
@@ -959,10 +1007,10 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   auto tile_m = [](int tile) { return (tile >> 2 > 0) * 2 + (tile >> 1 & 1); };
   auto tile_o = [](int tile) { return (tile >> 2 > 1) * 2 + (tile & 1); };
   for (int c0 = 0; c0 < width; c0 += 32) {
-    const bool whole = c0 + 32 <= width && at.count == C && a.f.dk == DK;
+    const bool whole = c0 + 32 <= width && at.count == C;
     if (!whole) {
-      s = delta_placed(s, c0 + q4 * 8, width, my_row < a.f.dk);
-      d = delta_placed(d, c0 + q4 * 8, width, my_row < a.f.dk);
+      s = delta_placed(s, c0 + q4 * 8, width, true);
+      d = delta_placed(d, c0 + q4 * 8, width, true);
     }
 #pragma unroll
     for (int n = 0; n < kTasks; ++n) {

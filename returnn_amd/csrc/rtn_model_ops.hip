@@ -32,7 +32,8 @@ int64_t delta_chunks(const DeltaSizes& z) { return (z.T + delta_frames(z) - 1) /
 size_t delta_all_chunks(const DeltaSizes& z) { return (size_t)z.B * (size_t)z.heads * (size_t)delta_chunks(z); }
 // Numbers of float32 in the sections of what the gradient wants to know, and of its workspace.
 size_t delta_records(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)delta_record(delta_frames(z)); }
-size_t delta_states(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)z.dk * (size_t)z.dv; }
+int delta_key_width(const DeltaSizes& z) { return z.dk <= 32 ? 32 : (z.dk <= 64 ? 64 : 128); }
+size_t delta_states(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)delta_key_width(z) * (size_t)z.dv; }
 size_t delta_writes(const DeltaSizes& z) { return delta_all_chunks(z) * (size_t)delta_frames(z) * (size_t)z.dv; }
 size_t delta_shared(const DeltaSizes& z) { return z.heads == z.key_heads ? 0 : (size_t)z.T * (size_t)z.B * (size_t)z.heads * (size_t)z.dk; }
 

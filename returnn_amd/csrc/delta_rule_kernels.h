@@ -161,6 +161,10 @@ struct DeltaChunkArgs {
   void *dq, *dk, *dv;
   float *dq_each, *dk_each;  // [T,B,heads,dk], where heads share queries and keys
   float *dg, *dbeta, *ds0;
+  int segments, per;  // of a sequence's chunks, and chunks of each
+  float* borders;     // [B,heads,segments - 1][DK][dv]: the state between two segments, or its error
+  // [B,heads,segments - 1][3][DK][DK]: what a segment makes of the state before it, in three parts, as a left operand; and transposed
+  __bf16 *through, *through_t;
 };
 
 __device__ __forceinline__ int delta_place(int row) { return (row & ~31) | ((row >> 2 & 1) << 4) | ((row >> 3 & 3) << 2) | (row & 3); }
@@ -490,14 +494,15 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
 // What the kernels that go through a head's chunks load of one into LDS, by way of registers: the one behind the next is on its way while one is worked on and the next lies in LDS.
 //
 // Rows past the end are read as the last one and put as 0.
-template <typename AT, int DK, int THREADS, int NP>
+template <typename AT, int DK, int THREADS, int NP, bool WITH_Q = true>
 struct DeltaStage {
   static constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, BLOCKS = delta_blocks(C);
   static constexpr int kApart = THREADS * 8 / DK;  // rows from one of a thread's to the next
   static constexpr int kRows = (C + kApart - 1) / kApart, kImage = ((3 + NP) * BLOCKS * 128 + THREADS - 1) / THREADS, kPowers = (3 * C + THREADS - 1) / THREADS;
   typedef decltype(delta_load8((const AT*)nullptr, 0)) Eight8;
   struct Tiles {
-    DeltaTile<NI, C, DK> K, Q;
+    DeltaTile<NI, C, DK> K;
+    DeltaTile<NI, WITH_Q ? C : 1, DK> Q;
     DeltaTile<3 + NP, BLOCKS * 32, 32> TP;  // T, then P
     alignas(16) float powers[3][C];  // c, gamma, beta
   };
@@ -525,7 +530,7 @@ struct DeltaStage {
     for (int n = 0; n < kRows; ++n) {
       const int of = row_of(n) < count ? row_of(n) : count - 1;
       k[n] = delta_load8_any<(DK <= 32)>((const AT*)(kf.at(0) + kf.lane(of, col)), place_col(), a.f.dk);
-      q[n] = delta_load8_any<(DK <= 32)>((const AT*)(qf.at(0) + qf.lane(of, col)), place_col(), a.f.dk);
+      if constexpr (WITH_Q) q[n] = delta_load8_any<(DK <= 32)>((const AT*)(qf.at(0) + qf.lane(of, col)), place_col(), a.f.dk);
     }
 #pragma unroll
     for (int n = 0; n < kImage; ++n) image[n] = *(const seq_u32x4*)((const char*)record + (unsigned)image_of(n) * 16u);
@@ -540,8 +545,10 @@ struct DeltaStage {
         const bool in = decltype(whole)::value || row_of(n) < count;
         delta_parts(decltype(whole)::value ? k[n] : delta_placed<(DK <= 32)>(k[n], place_col(), dk, in), parts);
         to.K.put(delta_place(row_of(n)), place_col(), parts);
-        delta_parts(decltype(whole)::value ? q[n] : delta_placed<(DK <= 32)>(q[n], place_col(), dk, in), parts);
-        to.Q.put(delta_place(row_of(n)), place_col(), parts);
+        if constexpr (WITH_Q) {
+          delta_parts(decltype(whole)::value ? q[n] : delta_placed<(DK <= 32)>(q[n], place_col(), dk, in), parts);
+          to.Q.put(delta_place(row_of(n)), place_col(), parts);
+        }
       }
     };
     if (count == C && dk == DK)
@@ -584,15 +591,19 @@ struct DeltaStrip {
   int strip, bh;
   unsigned lane_state;
   long long pitch_state;  // (bytes)
-  __device__ __forceinline__ DeltaStrip(const DeltaChunkArgs& args) : a(args) {
-    const int lane = threadIdx.x & 63, strips = (a.f.dv + 16 * W - 1) / (16 * W);
+  int segment;
+  // `columns` of all strips; segments from `first` on, as many as there are launched
+  __device__ __forceinline__ DeltaStrip(const DeltaChunkArgs& args, int columns, int first, int segments) : a(args) {
+    const int lane = threadIdx.x & 63, strips = (columns + 16 * W - 1) / (16 * W);
     q4 = lane >> 4;
-    strip = blockIdx.x % strips, bh = blockIdx.x / strips;
+    const int rest = blockIdx.x / strips;
+    strip = blockIdx.x % strips, segment = first + rest % segments, bh = rest / segments;
     col = (strip * W + (int)(threadIdx.x >> 6)) * 16 + (lane & 15);
     has = col < a.f.dv;
     lane_state = (unsigned)(q4 * 8 * a.f.dv + col) * 4u;
     pitch_state = a.f.dv * 4ll;
   }
+  __device__ __forceinline__ float* border(int n) const { return a.borders + ((long long)bh * (a.segments - 1) + n) * kept(); }
   static __device__ __forceinline__ constexpr int first_of(int m) { return (m >> 1) * 32 + (m & 1) * 4; }
   __device__ __forceinline__ int row_of(int m, int r) const { return first_of(m) + q4 * 8 + r; }
   __device__ __forceinline__ long long matrix() const { return (long long)a.f.dk * a.f.dv; }
@@ -663,31 +674,46 @@ __device__ __forceinline__ void delta_zero(delta_f32x4 (&x)[N]) {
   for (int n = 0; n < N; ++n) x[n] = (delta_f32x4){0.f, 0.f, 0.f, 0.f};
 }
 
-template <typename AT, int DK, int W, bool KEEP>
+// Where sequences and heads are few, their chunks are dealt to segments that work side by side.  A segment makes B + A S of a state S: a first pass (KIND kDeltaThrough) finds B, the state behind
+// it from none before it, and A, its columns from those of the unit matrix without values; k_delta_join goes from segment to segment; then all segments begin with their state.
+enum { kDeltaPlain, kDeltaKeep, kDeltaThrough };
+template <typename AT, int DK, int W, int KIND>
 __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
+  constexpr bool KEEP = KIND == kDeltaKeep, THROUGH = KIND == kDeltaThrough;
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32, BLOCKS = delta_blocks(C);
-  typedef DeltaStage<AT, DK, 64 * W, OUT> Stage;
+  typedef DeltaStage<AT, DK, 64 * W, THROUGH ? 0 : OUT, !THROUGH> Stage;
   __shared__ typename Stage::Tiles tiles[2];
-  DeltaStrip<AT, DK, W> strip(a);
+  const int values = (a.f.dv + 15) / 16 * 16;
+  DeltaStrip<AT, DK, W> strip(a, THROUGH ? values + DK : a.f.dv, 0, THROUGH ? a.segments - 1 : a.segments);
+  const bool unit = THROUGH && strip.col >= values;  // (the same in all lanes)
+  if (THROUGH && strip.segment == 0 && strip.strip * W * 16 >= values) return;
   DeltaWhere at(a.f, strip.bh, 0, C);
-  const int chunks = (int)((at.n + C - 1) / C);
+  const int all_chunks = (int)((at.n + C - 1) / C), chunk0 = strip.segment * a.per, chunks = all_chunks < chunk0 + a.per ? all_chunks : chunk0 + a.per;
   const float* records = a.records + strip.number(0) * delta_record(C);
   delta_f32x4 S[2 * KB];
-  strip.get(a.f.s0 ? a.f.s0 + strip.bh * strip.matrix() : nullptr, a.f.dk, S);
+  if (THROUGH && strip.segment) {
+#pragma unroll
+    for (int k = 0; k < 2 * KB; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[k][r] = strip.row_of(k, r) == strip.col - values ? 1.f : 0.f;
+  } else {
+    const bool border = strip.segment > 0;
+    strip.get(border ? strip.border(strip.segment - 1) : (a.f.s0 ? a.f.s0 + strip.bh * strip.matrix() : nullptr), border ? DK : a.f.dk, S);
+  }
   Stage stage;
   DeltaElement<AT> v[M][4];
   auto load = [&](int chunk) {  // (the last one again where there is no next: what is loaded on a condition is waited for)
     at.to(a.f, chunk < chunks ? chunk : chunks - 1, C);
     stage.load(a, at, records + (long long)at.chunk * delta_record(C));
   };
-  if (chunks) {
-    stage.load(a, at, records);
+  if (chunk0 < chunks) {
+    load(chunk0);
     strip.load(a.f.v, a.f.ldv, at, v);
-    stage.store(tiles[0], a.f.dk);
-    load(1);
+    stage.store(tiles[chunk0 & 1], a.f.dk);
+    load(chunk0 + 1);
     __syncthreads();
   }
-  for (int chunk = 0; chunk < chunks; ++chunk) {
+  for (int chunk = chunk0; chunk < chunks; ++chunk) {
     const typename Stage::Tiles& lds = tiles[chunk & 1];
     DeltaWhere here = at;
     here.to(a.f, chunk, C);
@@ -696,6 +722,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
     strip.load(a.f.v, a.f.ldv, at, v);
     stage.store(tiles[chunk + 1 & 1], a.f.dk);
     load(chunk + 2);
+    if (unit) delta_zero(R);
     if (KEEP) strip.put(a.states + strip.number(chunk) * strip.kept(), DK, S);
     delta_zero(KS);
     delta_zero(O);
@@ -706,7 +733,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
 #pragma unroll
         for (int m = 0; m < M; ++m) {
           lds.K.left(m * 16, b * 32, k[b & 1][m]);
-          lds.Q.left(m * 16, b * 32, q[b & 1][m]);
+          if constexpr (!THROUGH) lds.Q.left(m * 16, b * 32, q[b & 1][m]);
         }
       };
       ask(0);
@@ -717,7 +744,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         delta_ahead();
         if (b + 1 < KB) delta_parts(S[2 * b + 2], S[2 * b + 3], p[b + 1 & 1]);
         delta_mma<3>(k[b & 1], p[b & 1], KS);
-        delta_mma<OUT>(q[b & 1], p[b & 1], O);
+        if constexpr (!THROUGH) delta_mma<OUT>(q[b & 1], p[b & 1], O);
       }
     }
     {
@@ -728,8 +755,10 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         lds.TP.left(n * 32 + 16, 0, t[n][1]);
       };
       auto ask_p = [&](int n) {
-        lds.TP.template left<3>(n * 32, 0, p[n][0]);
-        lds.TP.template left<3>(n * 32 + 16, 0, p[n][1]);
+        if constexpr (!THROUGH) {
+          lds.TP.template left<3>(n * 32, 0, p[n][0]);
+          lds.TP.template left<3>(n * 32 + 16, 0, p[n][1]);
+        }
       };
       ask_t(0);
       if constexpr (NB == 2) ask_t(1);
@@ -753,11 +782,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         ask_p(1);
         ask_p(2);
         delta_ahead();
-        delta_mma<OUT>(p[0], some, O);
-        delta_mma<OUT>(p[1], some, O + 2);
-        delta_parts(U[2], U[3], some);
-        delta_mma<OUT>(p[2], some, O + 2);
-      } else {
+        if constexpr (!THROUGH) {
+          delta_mma<OUT>(p[0], some, O);
+          delta_mma<OUT>(p[1], some, O + 2);
+          delta_parts(U[2], U[3], some);
+          delta_mma<OUT>(p[2], some, O + 2);
+        }
+      } else if constexpr (!THROUGH) {
         delta_parts(U[0], U[1], some);
         delta_mma<OUT>(p[0], some, O);
       }
@@ -783,12 +814,65 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         delta_mma<3>(k[n & 1], right[n / 2], S + n % 2 * KB);
       }
     }
+    if constexpr (!THROUGH) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) O[m] *= a.f.scale;
-    strip.store(a.f.y, here, O);
+      for (int m = 0; m < M; ++m) O[m] *= a.f.scale;
+      strip.store(a.f.y, here, O);
+    }
     __syncthreads();
   }
-  strip.put(a.f.sN + strip.bh * strip.matrix(), a.f.dk, S);
+  if constexpr (THROUGH) {
+    if (!unit) {
+      strip.put(strip.border(strip.segment), DK, S);
+    } else if (strip.col < values + DK) {
+      const long long first = ((long long)strip.bh * (a.segments - 1) + strip.segment) * 3 * DK * DK;
+      const int of = strip.col - values;
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        delta_bf16x8 p[3];
+        delta_parts(S[2 * b], S[2 * b + 1], p);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          if (a.through_t) *(delta_bf16x8*)(a.through_t + first + (n * DK + of) * DK + b * 32 + strip.q4 * 8) = p[n];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a.through[first + (n * DK + b * 32 + strip.q4 * 8 + j) * DK + of] = p[n][j];
+        }
+      }
+    }
+  } else if (strip.segment == (all_chunks ? (all_chunks - 1) / a.per : 0)) {
+    strip.put(a.f.sN + strip.bh * strip.matrix(), a.f.dk, S);
+  }
+}
+
+// States at the segments' borders, one after the other: border n is what segment n (n + 1 for the error of a state, whose segments are gone through from the last one) makes of none, and what it makes
+// of the border before it is added.  Sixteen columns per wavefront.
+template <typename AT, int DK, bool BACK>
+__global__ __launch_bounds__(64) void k_delta_join(DeltaChunkArgs a) {
+  constexpr int KB = DK / 32;
+  DeltaStrip<AT, DK, 1> strip(a, a.f.dv, 0, 1);
+  const int row16 = ((threadIdx.x & 15) >> 2) * 8 + (threadIdx.x & 3), borders = a.segments - 1;
+  delta_f32x4 S[2 * KB], next[2 * KB];
+  strip.get(strip.border(BACK ? borders - 1 : 0), DK, S);
+  for (int n = 1; n < borders; ++n) {
+    const int border = BACK ? borders - 1 - n : n, segment = BACK ? border + 1 : border;
+    const __bf16* A = (BACK ? a.through_t : a.through) + ((long long)strip.bh * borders + segment) * 3 * DK * DK;
+    strip.get(strip.border(border), DK, next);
+    delta_bf16x8 p[KB][3];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) delta_parts(S[2 * b], S[2 * b + 1], p[b]);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      delta_bf16x8 left[2 * KB][3];
+#pragma unroll
+      for (int k = 0; k < 2 * KB; ++k)
+#pragma unroll
+        for (int m = 0; m < 3; ++m) left[k][m] = *(const delta_bf16x8*)(A + (m * DK + strip.first_of(k) + row16) * DK + b * 32 + strip.q4 * 8);
+      delta_mma<3>(left, p[b], next);
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * KB; ++k) S[k] = next[k];
+    strip.put(strip.border(border), DK, S);
+  }
 }
 
 // ---- the gradient -----------------------------------------------------------------------------------------------------
@@ -804,31 +888,37 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
 //   of the chunk's last frame also sum_j gamma_j k_j.(D U_j) + c_C <D, S>;  dg is its sum over all later frames of the chunk.
 //
 // k_delta_backward goes through the chunks of a head from its last one, as k_delta_forward, and leaves R and D; k_delta_gradients does the rest, all chunks side by side.
-template <typename AT, int DK, int W>
+// (THROUGH: as of the forward pass, but of the segments behind the first one, and with what their transitions left.)
+template <typename AT, int DK, int W, bool THROUGH>
 __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, KB = DK / 32;
   typedef DeltaStage<AT, DK, 64 * W, 3> Stage;
   __shared__ typename Stage::Tiles tiles[2];
-  DeltaStrip<AT, DK, W> strip(a);
+  DeltaStrip<AT, DK, W> strip(a, a.f.dv, THROUGH, THROUGH ? a.segments - 1 : a.segments);
   DeltaWhere at(a.f, strip.bh, 0, C);
-  const int chunks = (int)((at.n + C - 1) / C);
+  const int all_chunks = (int)((at.n + C - 1) / C), chunk0 = strip.segment * a.per, chunks = all_chunks < chunk0 + a.per ? all_chunks : chunk0 + a.per;
   const float* records = a.records + strip.number(0) * delta_record(C);
   delta_f32x4 D[2 * KB];
-  strip.get(a.dsN ? a.dsN + strip.bh * strip.matrix() : nullptr, a.f.dk, D);
+  if (strip.segment == a.segments - 1)
+    strip.get(a.dsN ? a.dsN + strip.bh * strip.matrix() : nullptr, a.f.dk, D);
+  else if (THROUGH)
+    delta_zero(D);
+  else
+    strip.get(strip.border(strip.segment), DK, D);
   Stage stage;
   DeltaElement<AT> y[M][4];
   auto load = [&](int chunk) {
-    at.to(a.f, chunk > 0 ? chunk : 0, C);
+    at.to(a.f, chunk > chunk0 ? chunk : chunk0, C);
     stage.load(a, at, records + (long long)at.chunk * delta_record(C));
   };
-  if (chunks) {
+  if (chunk0 < chunks) {
     load(chunks - 1);
     strip.load(a.dy, a.lddy, at, y);
     stage.store(tiles[chunks - 1 & 1], a.f.dk);
     load(chunks - 2);
     __syncthreads();
   }
-  for (int chunk = chunks - 1; chunk >= 0; --chunk) {
+  for (int chunk = chunks - 1; chunk >= chunk0; --chunk) {
     const typename Stage::Tiles& lds = tiles[chunk & 1];
     DeltaWhere here = at;
     here.to(a.f, chunk, C);
@@ -837,7 +927,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
     strip.load(a.dy, a.lddy, at, y);
     stage.store(tiles[chunk + 1 & 1], a.f.dk);
     load(chunk - 2);
-    strip.put(a.dstates + strip.number(chunk) * strip.kept(), DK, D);
+    if (!THROUGH) strip.put(a.dstates + strip.number(chunk) * strip.kept(), DK, D);
     delta_zero(KD);
     delta_zero(R);
 #pragma unroll
@@ -875,10 +965,10 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
         R[m] = delta_mma<3>(left, right, R[m]);
       }
     }
-    strip.put(a.dwrites + strip.number(chunk) * C * a.f.dv, C, R);
+    if (!THROUGH) strip.put(a.dwrites + strip.number(chunk) * C * a.f.dv, C, R);
 #pragma unroll
     for (int m = 0; m < M; ++m) R[m] *= delta_rows(lds.powers[2], m);
-    strip.store(a.dv, here, R);
+    if (!THROUGH) strip.store(a.dv, here, R);
     const float end = lds.powers[0][C - 1];
 #pragma unroll
     for (int k = 0; k < 2 * KB; ++k) D[k] *= end;
@@ -905,7 +995,10 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
     }
     __syncthreads();
   }
-  strip.put(a.ds0 + strip.bh * strip.matrix(), a.f.dk, D);
+  if (THROUGH)
+    strip.put(strip.border(strip.segment - 1), DK, D);
+  else if (strip.segment == 0)
+    strip.put(a.ds0 + strip.bh * strip.matrix(), a.f.dk, D);
 }
 
 // The sum over 16 neighbouring lanes, in all of them.

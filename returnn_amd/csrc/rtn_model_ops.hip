@@ -61,6 +61,25 @@ void with_waves(const DeltaSizes& z, F f) {
   else
     f(Count<4>());
 }
+// Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.6, and both
+// passes run in rounds of as many workgroups as there are compute units.
+int64_t delta_segments(const DeltaSizes& z) {
+  const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * delta_waves(z);
+  const int64_t strips = delta_strips(z), strips_through = ((z.dv + 15) / 16 * 16 + delta_key_width(z) + width - 1) / width;
+  auto rounds = [&](int64_t blocks) { return (double)((blocks + 255) / 256); };
+  double least = rounds(lines * strips) * chunks;
+  int64_t best = 1;
+  for (int64_t some : {3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
+    if (some > chunks / 2 || lines * strips * some > 1024) break;
+    const int64_t per = (chunks + some - 1) / some, n = (chunks + per - 1) / per;
+    const double t = per * (rounds(lines * strips * n) + 0.8 * rounds(lines * strips_through * (n - 1))) + 0.6 * n + 4;
+    if (t < least) least = t, best = n;
+  }
+  return best;
+}
+size_t delta_borders(const DeltaSizes& z) { return (size_t)(delta_segments(z) - 1) * z.B * z.heads * delta_key_width(z) * z.dv; }
+size_t delta_through(const DeltaSizes& z) { return (size_t)(delta_segments(z) - 1) * z.B * z.heads * 3 * delta_key_width(z) * delta_key_width(z) / 2; }
+
 // Whether launches and offsets are within what 32 bits count; widest: elements of a frame of the widest tensor, with its pitch.
 bool delta_fits(const DeltaSizes& z, int64_t widest) {
   const int64_t most = max_blocks(512) / std::max<int64_t>(1, (int64_t)z.B * z.heads);
@@ -93,15 +112,16 @@ const char* rtn_model_ops_last_error(void) { return g_last_error.c_str(); }
 
 size_t rtn_delta_rule_fwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype, int32_t keep) {
   const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
-  return !valid(z) || keep || T <= kStepFrames ? 0 : delta_records(z) * 4;
+  if (!valid(z) || nothing(z) || (!keep && T <= kStepFrames)) return 0;
+  return ((keep ? 0 : delta_records(z)) + delta_borders(z) + delta_through(z)) * 4;
 }
 size_t rtn_delta_rule_saved_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype) {
   const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
-  return valid(z) ? (delta_records(z) + delta_states(z) + delta_writes(z)) * 4 : 0;
+  return valid(z) && !nothing(z) ? (delta_records(z) + delta_through(z) + delta_states(z) + delta_writes(z)) * 4 : 0;
 }
 size_t rtn_delta_rule_bwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype) {
   const DeltaSizes z{T, B, key_heads, heads, dk, dv, dtype};
-  return valid(z) ? (delta_states(z) + delta_writes(z) + 2 * delta_shared(z)) * 4 : 0;
+  return valid(z) && !nothing(z) ? (delta_borders(z) + delta_states(z) + delta_writes(z) + 2 * delta_shared(z)) * 4 : 0;
 }
 
 int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* g, const float* beta, const float* s0,
@@ -137,19 +157,31 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
   DeltaChunkArgs c{};
   c.f = a, c.chunks = (int)delta_chunks(z);
-  c.records = (float*)(saved ? saved : workspace);
-  if (saved) c.states = c.records + delta_records(z), c.writes = c.states + delta_states(z);
+  c.segments = (int)delta_segments(z), c.per = (int)((c.chunks + c.segments - 1) / c.segments);
+  float* free = (float*)workspace;
+  c.through = (__bf16*)free, free += delta_through(z);
+  c.borders = free, free += delta_borders(z);
+  c.records = (float*)(saved ? saved : free);
+  if (saved) {
+    c.through_t = (__bf16*)(c.records + delta_records(z));
+    c.states = c.records + delta_records(z) + delta_through(z), c.writes = c.states + delta_states(z);
+  }
   with_delta(z, [&](auto type, auto width) {
     typedef decltype(type) AT;
     constexpr int DK = decltype(width)::value;
-    const dim3 heads_grid((unsigned)(B * heads * delta_strips(z)));
+    const dim3 heads_grid((unsigned)(B * heads * c.segments * delta_strips(z)));
     if (T) hipLaunchKernelGGL((k_delta_chunks<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DeltaChunk<AT>::kFrames * 4), 0, stream, c);
     with_waves(z, [&](auto waves) {
       constexpr int W = decltype(waves)::value;
+      if (c.segments > 1) {
+        const int64_t strips = ((dv + 15) / 16 * 16 + DK + 16 * W - 1) / (16 * W);
+        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaThrough>), dim3((unsigned)(B * heads * (c.segments - 1) * strips)), dim3(64 * W), 0, stream, c);
+        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, false>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(64), 0, stream, c);
+      }
       if (saved)
-        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, true>), heads_grid, dim3(64 * W), 0, stream, c);
+        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaKeep>), heads_grid, dim3(64 * W), 0, stream, c);
       else
-        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, false>), heads_grid, dim3(64 * W), 0, stream, c);
+        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaPlain>), heads_grid, dim3(64 * W), 0, stream, c);
     });
   });
   return launched(what);
@@ -181,9 +213,12 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   DeltaChunkArgs c{};
   c.f = DeltaArgs{q, k, v, ldq, ldk, ldv, g, beta, nullptr, lens, nullptr, nullptr, T, B, key_heads, heads, dk, dv, scale, direction < 0};
   c.chunks = (int)delta_chunks(z);
-  c.records = (float*)saved, c.states = c.records + delta_records(z), c.writes = c.states + delta_states(z);
+  c.segments = (int)delta_segments(z), c.per = (int)((c.chunks + c.segments - 1) / c.segments);
+  c.records = (float*)saved, c.through_t = (__bf16*)(c.records + delta_records(z));
+  c.states = c.records + delta_records(z) + delta_through(z), c.writes = c.states + delta_states(z);
   c.dy = dy, c.lddy = lddy, c.dsN = dsN;
-  c.dstates = (float*)workspace, c.dwrites = c.dstates + delta_states(z);
+  c.borders = (float*)workspace;
+  c.dstates = c.borders + delta_borders(z), c.dwrites = c.dstates + delta_states(z);
   if (delta_shared(z)) c.dq_each = c.dwrites + delta_writes(z), c.dk_each = c.dq_each + delta_shared(z);
   c.dq = dq, c.dk = dk_out, c.dv = dv_out, c.dg = dg, c.dbeta = dbeta, c.ds0 = ds0;
   with_delta(z, [&](auto type, auto width) {
@@ -192,7 +227,11 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     const hipStream_t stream = (hipStream_t)hip_stream;
     with_waves(z, [&](auto waves) {
       constexpr int W = decltype(waves)::value;
-      hipLaunchKernelGGL((k_delta_backward<AT, DK, W>), dim3((unsigned)(B * heads * delta_strips(z))), dim3(64 * W), 0, stream, c);
+      if (c.segments > 1) {
+        hipLaunchKernelGGL((k_delta_backward<AT, DK, W, true>), dim3((unsigned)(B * heads * (c.segments - 1) * delta_strips(z))), dim3(64 * W), 0, stream, c);
+        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, true>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(64), 0, stream, c);
+      }
+      hipLaunchKernelGGL((k_delta_backward<AT, DK, W, false>), dim3((unsigned)(B * heads * c.segments * delta_strips(z))), dim3(64 * W), 0, stream, c);
     });
     if (T) hipLaunchKernelGGL((k_delta_gradients<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DK * 4), 0, stream, c);
     if (delta_shared(z)) {

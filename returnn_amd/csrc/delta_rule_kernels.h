@@ -845,33 +845,53 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
 }
 
 // States at the segments' borders, one after the other: border n is what segment n (n + 1 for the error of a state, whose segments are gone through from the last one) makes of none, and what it makes
-// of the border before it is added.  Sixteen columns per wavefront.
+// of the border before it is added.  Sixteen columns per workgroup, 16 rows of them per wavefront; the state goes around through LDS, in parts and as the right operand that all need.
 template <typename AT, int DK, bool BACK>
-__global__ __launch_bounds__(64) void k_delta_join(DeltaChunkArgs a) {
+__global__ __launch_bounds__(DK * 4) void k_delta_join(DeltaChunkArgs a) {
   constexpr int KB = DK / 32;
-  DeltaStrip<AT, DK, 1> strip(a, a.f.dv, 0, 1);
-  const int row16 = ((threadIdx.x & 15) >> 2) * 8 + (threadIdx.x & 3), borders = a.segments - 1;
-  delta_f32x4 S[2 * KB], next[2 * KB];
-  strip.get(strip.border(BACK ? borders - 1 : 0), DK, S);
-  for (int n = 1; n < borders; ++n) {
-    const int border = BACK ? borders - 1 - n : n, segment = BACK ? border + 1 : border;
-    const __bf16* A = (BACK ? a.through_t : a.through) + ((long long)strip.bh * borders + segment) * 3 * DK * DK;
-    strip.get(strip.border(border), DK, next);
-    delta_bf16x8 p[KB][3];
+  __shared__ alignas(16) char state[2][KB][3][64][16];
+  const int lane = threadIdx.x & 63, k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, i16 = lane & 15, borders = a.segments - 1;
+  const int strips = (a.f.dv + 15) / 16, bh = blockIdx.x / strips, col = blockIdx.x % strips * 16 + i16, first = (k >> 1) * 32 + (k & 1) * 4;
+  const bool has = col < a.f.dv;
+  const long long row = (long long)(first + q4 * 8) * a.f.dv + col;
+  auto border_of = [&](int n) { return BACK ? borders - 1 - n : n; };
+  auto border = [&](int n) { return a.borders + ((long long)bh * borders + border_of(n)) * DK * a.f.dv + row; };
+  auto get = [&](int n, delta_f32x4& x) {
 #pragma unroll
-    for (int b = 0; b < KB; ++b) delta_parts(S[2 * b], S[2 * b + 1], p[b]);
+    for (int r = 0; r < 4; ++r) x[r] = has ? border(n)[r * a.f.dv] : 0.f;
+  };
+  delta_bf16x8 A[KB][3];
+  auto ask = [&](int n) {
+    const __bf16* from = (BACK ? a.through_t : a.through) + ((long long)bh * borders + border_of(n) + BACK) * 3 * DK * DK;
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int m = 0; m < 3; ++m) A[b][m] = *(const delta_bf16x8*)(from + (m * DK + first + (i16 >> 2) * 8 + (i16 & 3)) * DK + b * 32 + q4 * 8);
+  };
+  delta_f32x4 S, next;
+  get(0, S);
+  get(1, next);
+  ask(1);
+  for (int n = 1;; ++n) {
+    const delta_f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    delta_bf16x8 p[3];
+    delta_parts(S, none, p);
+#pragma unroll
+    for (int m = 0; m < 3; ++m) *(unsigned long long*)(state[n & 1][k >> 1][m][lane] + (k & 1) * 8) = __builtin_bit_cast(seq_u32x4, p[m])[0] | (unsigned long long)__builtin_bit_cast(seq_u32x4, p[m])[1] << 32;
+    __syncthreads();
+    S = next;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      delta_bf16x8 left[2 * KB][3];
 #pragma unroll
-      for (int k = 0; k < 2 * KB; ++k)
-#pragma unroll
-        for (int m = 0; m < 3; ++m) left[k][m] = *(const delta_bf16x8*)(A + (m * DK + strip.first_of(k) + row16) * DK + b * 32 + strip.q4 * 8);
-      delta_mma<3>(left, p[b], next);
+      for (int m = 0; m < 3; ++m) p[m] = *(const delta_bf16x8*)state[n & 1][b][m][lane];
+      S = delta_mma<3>(A[b], p, S);
     }
+    if (has)
 #pragma unroll
-    for (int k = 0; k < 2 * KB; ++k) S[k] = next[k];
-    strip.put(strip.border(border), DK, S);
+      for (int r = 0; r < 4; ++r) border(n)[r * a.f.dv] = S[r];
+    if (n + 1 == borders) break;
+    get(n + 1, next);
+    ask(n + 1);
   }
 }
 
@@ -1012,7 +1032,8 @@ __device__ __forceinline__ float delta_sum16(float v) {
 }
 
 // One chunk of one head per workgroup, DK / 16 wavefronts with 16 columns of dQ and dK each.  The values' columns pass by 32 at a time, the next ones on their way meanwhile.
-template <typename AT, int DK>
+// NARROW: values of fewer than eight columns.
+template <typename AT, int DK, bool NARROW>
 __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;
   constexpr int kTiles = BLOCKS * 4, kEach = (kTiles + W - 1) / W;                                        // of C x C, for each wavefront
@@ -1059,32 +1080,35 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   const int width = a.f.dv;
   const int my_row = wave * 16 + i16;  // of S and D
   // What passes by, from column c0 on.
-  delta_f32x8 s, d, f[kTasks];
-  Eight8 x[kTasks];
-  auto load = [&](int c0) {
+  struct Passed {
+    delta_f32x8 s, d, f[kTasks];
+    Eight8 x[kTasks];
+  } passed[2];
+  auto load = [&](Passed& p, int c0) {
     const unsigned state = (unsigned)(my_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
-    s = delta_load8_any((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
-    d = delta_load8_any((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
+    p.s = delta_load8_any<NARROW>((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
+    p.d = delta_load8_any<NARROW>((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
 #pragma unroll
     for (int n = 0; n < kTasks; ++n) {
       const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, col = c0 + (item & 3) * 8;
       if (first < 2 * kItems) {
-        f[n] = delta_load8_any((which ? a.writes : a.dwrites) + number * C * width + (row * width + delta_read_col(col, width)), col, width);
+        p.f[n] = delta_load8_any<NARROW>((which ? a.writes : a.dwrites) + number * C * width + (row * width + delta_read_col(col, width)), col, width);
         const AT* tensor = (const AT*)(which ? a.dy : a.f.v);
         const long long ld = which ? a.lddy : a.f.ldv;
-        x[n] = delta_load8_any(tensor + (at.row(row < at.count ? row : at.count - 1) * ld + (long long)at.h * width + delta_read_col(col, width)), col, width);
+        p.x[n] = delta_load8_any<NARROW>(tensor + (at.row(row < at.count ? row : at.count - 1) * ld + (long long)at.h * width + delta_read_col(col, width)), col, width);
       }
     }
   };
-  load(0);
+  load(passed[0], 0);
+  load(passed[1], 32 < width ? 32 : 0);
   {
     const int col = threadIdx.x % (DK / 8) * 8;
     for (int row = threadIdx.x / (DK / 8); row < C; row += kApart) {
       const long long r = at.row(row < at.count ? row : at.count - 1);
       delta_bf16x8 parts[NI];
-      delta_parts(delta_placed(delta_load8_any((const AT*)a.f.k + (r * a.f.ldk + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
+      delta_parts(delta_placed<(DK <= 32)>(delta_load8_any<(DK <= 32)>((const AT*)a.f.k + (r * a.f.ldk + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
       K.put(delta_place(row), col, parts);
-      delta_parts(delta_placed(delta_load8_any((const AT*)a.f.q + (r * a.f.ldq + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
+      delta_parts(delta_placed<(DK <= 32)>(delta_load8_any<(DK <= 32)>((const AT*)a.f.q + (r * a.f.ldq + at.kh * a.f.dk + delta_read_col(col, a.f.dk)), col, a.f.dk), col, a.f.dk, row < at.count), parts);
       Q.put(delta_place(row), col, parts);
     }
   }
@@ -1099,30 +1123,31 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   float ds = 0.f, own_rv[kTasks] = {};
   auto tile_m = [](int tile) { return (tile >> 2 > 0) * 2 + (tile >> 1 & 1); };
   auto tile_o = [](int tile) { return (tile >> 2 > 1) * 2 + (tile & 1); };
-  for (int c0 = 0; c0 < width; c0 += 32) {
+  auto pass = [&](Passed& now, int c0) {
+    delta_f32x8 s = now.s, d = now.d;
     const bool whole = c0 + 32 <= width && at.count == C;
     if (!whole) {
-      s = delta_placed(s, c0 + q4 * 8, width, true);
-      d = delta_placed(d, c0 + q4 * 8, width, true);
+      s = delta_placed<NARROW>(s, c0 + q4 * 8, width, true);
+      d = delta_placed<NARROW>(d, c0 + q4 * 8, width, true);
     }
 #pragma unroll
     for (int n = 0; n < kTasks; ++n) {
       const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, c8 = (item & 3) * 8;
       if (first < 2 * kItems) {
         if (!whole) {
-          f[n] = delta_placed(f[n], c0 + c8, width, true);
-          x[n] = delta_placed(x[n], c0 + c8, width, row < at.count);
+          now.f[n] = delta_placed<NARROW>(now.f[n], c0 + c8, width, true);
+          now.x[n] = delta_placed<NARROW>(now.x[n], c0 + c8, width, row < at.count);
         }
         delta_bf16x8 parts[3], some[NI];
-        delta_parts(f[n], parts);
+        delta_parts(now.f[n], parts);
         (which ? lds.pass.U : lds.pass.R).put(delta_place(row), c8, parts);
         if (which) {
-          delta_parts(x[n], some);
+          delta_parts(now.x[n], some);
           lds.pass.Y.put(delta_place(row), c8, some);
         } else {
-          const delta_f32x8 v = delta_wide(x[n]);
+          const delta_f32x8 v = delta_wide(now.x[n]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(f[n][j], v[j], own_rv[n]);
+          for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(now.f[n][j], v[j], own_rv[n]);
         }
       }
     }
@@ -1131,7 +1156,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     for (int j = 0; j < 8; ++j) ds = __builtin_fmaf(s[j], d[j], ds);
     delta_parts(s, sp);
     delta_parts(d, dp);
-    if (c0 + 32 < width) load(c0 + 32);
+    load(now, c0 + 64 < width ? c0 + 64 : c0);  // (what is loaded on a condition is waited for)
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m) {
@@ -1156,6 +1181,10 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
       }
     }
     __syncthreads();
+  };
+  for (int c0 = 0; c0 < width; c0 += 64) {
+    pass(passed[0], c0);
+    if (c0 + 32 < width) pass(passed[1], c0 + 32);
   }
 #pragma unroll
   for (int n = 0; n < kTasks; ++n) {

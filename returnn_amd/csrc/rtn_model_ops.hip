@@ -61,7 +61,7 @@ void with_waves(const DeltaSizes& z, F f) {
   else
     f(Count<4>());
 }
-// Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.6, and both
+// Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.3, and both
 // passes run in rounds of as many workgroups as there are compute units.
 int64_t delta_segments(const DeltaSizes& z) {
   const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * delta_waves(z);
@@ -72,7 +72,7 @@ int64_t delta_segments(const DeltaSizes& z) {
   for (int64_t some : {3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
     if (some > chunks / 2 || lines * strips * some > 1024) break;
     const int64_t per = (chunks + some - 1) / some, n = (chunks + per - 1) / per;
-    const double t = per * (rounds(lines * strips * n) + 0.8 * rounds(lines * strips_through * (n - 1))) + 0.6 * n + 4;
+    const double t = per * (rounds(lines * strips * n) + 0.8 * rounds(lines * strips_through * (n - 1))) + 0.3 * n + 3;
     if (t < least) least = t, best = n;
   }
   return best;
@@ -176,7 +176,7 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
       if (c.segments > 1) {
         const int64_t strips = ((dv + 15) / 16 * 16 + DK + 16 * W - 1) / (16 * W);
         hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaThrough>), dim3((unsigned)(B * heads * (c.segments - 1) * strips)), dim3(64 * W), 0, stream, c);
-        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, false>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(64), 0, stream, c);
+        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, false>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
       }
       if (saved)
         hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaKeep>), heads_grid, dim3(64 * W), 0, stream, c);
@@ -229,11 +229,14 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
       constexpr int W = decltype(waves)::value;
       if (c.segments > 1) {
         hipLaunchKernelGGL((k_delta_backward<AT, DK, W, true>), dim3((unsigned)(B * heads * (c.segments - 1) * delta_strips(z))), dim3(64 * W), 0, stream, c);
-        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, true>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(64), 0, stream, c);
+        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, true>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
       }
       hipLaunchKernelGGL((k_delta_backward<AT, DK, W, false>), dim3((unsigned)(B * heads * c.segments * delta_strips(z))), dim3(64 * W), 0, stream, c);
     });
-    if (T) hipLaunchKernelGGL((k_delta_gradients<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DK * 4), 0, stream, c);
+    if (T)
+      with_bool(dv < 8, [&](auto narrow) {
+        hipLaunchKernelGGL((k_delta_gradients<AT, DK, decltype(narrow)::value>), dim3((unsigned)delta_all_chunks(z)), dim3(DK * 4), 0, stream, c);
+      });
     if (delta_shared(z)) {
       const int64_t items = T * B * key_heads * (int64_t)dk;
       hipLaunchKernelGGL(k_delta_shared<AT>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, c);

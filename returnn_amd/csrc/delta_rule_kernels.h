@@ -388,15 +388,16 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
   if (at.count == 0) return;
   float* record = a.records + ((long long)bh * a.chunks + chunk) * delta_record(C);
   float *rL = record + delta_image(C), *rc = rL + BLOCKS * 1024;
-  typedef DeltaTile<6, BLOCKS * 32, 32> Image;
-  // Number (i, j) of T (which = 0) or P (1), in three parts.
-  auto put_image = [&](int which, int block, int i, int j, float x) {
-    char* to = (char*)record + which * 3 * (int)sizeof(Image().bytes[0]) + Image::offset(delta_place(block * 32 + i), j);
+  // T (which = 0) or P (1) out of LDS, in three parts, by threads `from` to `to`, eight numbers each.
+  auto put_image = [&](int which, const float* of, int from, int to) {
+    typedef DeltaTile<6, BLOCKS * 32, 32> Image;
+    for (int item = (int)threadIdx.x - from; item >= 0 && item < BLOCKS * 128; item += to - from) {
+      const int block = item >> 7, row = item >> 2 & 31, col = (item & 3) * 8;
+      const float* x = of + (row + (block > 0) * 32) * ROW + col + (block > 1) * 32;
+      delta_bf16x8 parts[3];
+      delta_parts(*(const delta_f32x4*)x, *(const delta_f32x4*)(x + 4), parts);
 #pragma unroll
-    for (int n = 0; n < 3; ++n, to += sizeof(Image().bytes[0])) {
-      const __bf16 part = (__bf16)x;
-      *(__bf16*)to = part;
-      x -= (float)part;
+      for (int n = 0; n < 3; ++n) *(delta_bf16x8*)((char*)record + (which * 3 + n) * (int)sizeof(Image().bytes[0]) + Image::offset(delta_place(block * 32 + row), col)) = parts[n];
     }
   };
   if (wave == 0) {
@@ -446,13 +447,14 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
       const float l = i > j ? kk[r] * e : 0.f, p = i >= j ? qk[r] * e : 0.f;
       A[i * ROW + j] = beta_of[i] * l;
       X[i * ROW + j] = 0.f;
+      Y[i * ROW + j] = p;
       if (nt / 2 <= wave / 2) {
-        put_image(1, block, i & 31, j & 31, p);
         rL[block * 1024 + (i & 31) * 32 + (j & 31)] = l;
       }
     }
   }
   __syncthreads();
+  if (wave) put_image(1, Y, 64, C * 4);
   if (wave == 0 && q4 < W) {
     const float* D = A + (q4 * 16) * ROW + q4 * 16;
     float x[16];
@@ -485,10 +487,7 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
     product(X, Y, X, mt, nt, 2, 4, -1.f);
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < BLOCKS * 1024; e += C * 4) {
-    const int block = e >> 10, i = (e >> 5 & 31) + (block > 0) * 32, j = (e & 31) + (block > 1) * 32;
-    put_image(0, block, e >> 5 & 31, e & 31, X[i * ROW + j]);
-  }
+  put_image(0, X, 0, C * 4);
 }
 
 // What the kernels that go through a head's chunks load of one into LDS, by way of registers: the one behind the next is on its way while one is worked on and the next lies in LDS.

@@ -52,25 +52,53 @@ __device__ __forceinline__ unsigned token_key(const EmbeddingArgs& a, long long 
   return t < 0 || t >= a.V ? (unsigned)a.V : (unsigned)t;  // (rows without a token come last)
 }
 
-// Where a row comes: after all of lower tokens and the earlier ones of the same, counted.  64 rows per workgroup, each of its 16 wavefronts counts among a 16th of all.
+// Zeros for all of the table, by the workgroups behind the `first` of a launch, while these sort: rows that tokens have are written again, at most as many as there are tokens.
+constexpr long long kFilled = 1 << 16;  // bytes for each of them
+struct EmbeddingFill {
+  long long bytes, from;  // of the table, and how many workgroups of earlier launches have been at it
+};
+__device__ __forceinline__ void embedding_fill(const EmbeddingArgs& a, unsigned first, EmbeddingFill fill) {
+  const long long bytes = fill.bytes;
+  char* to = (char*)a.out;
+  // (whole words of 16 bytes; what is before and behind them, byte by byte)
+  const long long head = ((16 - (long long)((unsigned long long)to & 15)) & 15) < bytes ? (16 - (long long)((unsigned long long)to & 15)) & 15 : bytes, words = (bytes - head) / 16;
+  const long long start = (fill.from + (blockIdx.x - first)) * (kFilled / 16);
+  const seq_u32x4 none = {0, 0, 0, 0};
+  for (int i = threadIdx.x; i < kFilled / 16; i += 1024)
+    if (start + i < words) __builtin_nontemporal_store(none, (seq_u32x4*)(to + head) + start + i);
+  if (start == 0 && threadIdx.x < 32) {
+    const long long tail = head + words * 16 + threadIdx.x - 16;
+    if (threadIdx.x < 16 ? (long long)threadIdx.x < head : tail < bytes) to[threadIdx.x < 16 ? (long long)threadIdx.x : tail] = 0;
+  }
+}
+
+// Where a row comes: after all of lower tokens and the earlier ones of the same, counted.  16 rows per workgroup, each against a 64th of all by 64 threads.
 constexpr int kCountedRows = 8192;
-__global__ __launch_bounds__(1024) void k_embedding_order(EmbeddingArgs a) {
+__global__ __launch_bounds__(1024) void k_embedding_order(EmbeddingArgs a, unsigned sorting, EmbeddingFill fill) {
   __shared__ alignas(16) unsigned keys[kCountedRows];
-  __shared__ unsigned before_of[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = (int)a.rows, r = blockIdx.x * 64 + lane;
-  const int padded = (rows + 63) / 64 * 64, part = padded / 16;  // (a multiple of 4)
+  __shared__ unsigned before_of[16][16];
+  if (blockIdx.x >= sorting) return embedding_fill(a, sorting, fill);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = (int)a.rows, r = blockIdx.x * 16 + (lane & 15);
+  const int padded = (rows + 255) / 256 * 256, part = padded / 64, first = (int)(threadIdx.x >> 4) * part;  // (a multiple of 4)
   for (int i = threadIdx.x; i < padded; i += 1024) keys[i] = i < rows ? token_key(a, i) : 0xFFFFFFFFu;
   __syncthreads();
   const unsigned mine = r < rows ? keys[r] : 0;
   unsigned before = 0;
-  for (int i = wave * part; i < (wave + 1) * part; i += 4) {
-    const seq_u32x4 k = *(const seq_u32x4*)(keys + i);
+  if (first + part <= (int)blockIdx.x * 16 || first >= (int)blockIdx.x * 16 + 16) {  // (all of the part on one side of the workgroup's rows)
+    const unsigned below = mine + (first < (int)blockIdx.x * 16);
+    for (int i = first; i < first + part; i += 4) {
+      const seq_u32x4 k = *(const seq_u32x4*)(keys + i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) before += k[j] < mine + (i + j < r);
+      for (int j = 0; j < 4; ++j) before += k[j] < below;
+    }
+  } else {
+    for (int i = first; i < first + part; ++i) before += keys[i] < mine + (i < r);
   }
-  before_of[wave][lane] = before;
+  before += __shfl_xor(before, 16);
+  before += __shfl_xor(before, 32);
+  if (lane < 16) before_of[wave][lane] = before;
   __syncthreads();
-  if (wave == 0 && r < rows) {
+  if (threadIdx.x < 16 && r < rows) {
     before = 0;
 #pragma unroll
     for (int w = 0; w < 16; ++w) before += before_of[w][lane];
@@ -79,9 +107,9 @@ __global__ __launch_bounds__(1024) void k_embedding_order(EmbeddingArgs a) {
   }
 }
 
-// More rows: one pass for 8 bits of the token after the other, from the lowest on; each pass counts digits in blocks of rows, then every block moves its rows behind
+// More rows: one pass for 9 bits of the token after the other, from the lowest on; each pass counts digits in blocks of rows, then every block moves its rows behind
 // those of lower digits and those of earlier blocks.  Within a block a wavefront has 64 neighbouring rows at a time; lanes of one digit find each other by ballots.
-constexpr int kDigits = 256, kSortedRows = 4096;  // rows of a block: 16 wavefronts with four times 64
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortedRows = 4096;  // rows of a block: 16 wavefronts with four times 64
 struct SortArgs {
   EmbeddingArgs e;
   const unsigned *order, *token_of;  // of the pass before, or NULL: rows as they come
@@ -89,8 +117,9 @@ struct SortArgs {
   int blocks, shift;
 };
 __device__ __forceinline__ unsigned sort_key(const SortArgs& a, long long i) { return a.token_of ? a.token_of[i] : token_key(a.e, i); }
-__global__ __launch_bounds__(1024) void k_embedding_digits(SortArgs a) {
+__global__ __launch_bounds__(1024) void k_embedding_digits(SortArgs a, EmbeddingFill fill) {
   __shared__ unsigned count[kDigits];
+  if (blockIdx.x >= (unsigned)a.blocks) return embedding_fill(a.e, a.blocks, fill);
   if (threadIdx.x < kDigits) count[threadIdx.x] = 0;
   __syncthreads();
   for (int n = 0; n < kSortedRows / 1024; ++n) {
@@ -100,15 +129,16 @@ __global__ __launch_bounds__(1024) void k_embedding_digits(SortArgs a) {
   __syncthreads();
   if (threadIdx.x < kDigits) a.counts[(long long)blockIdx.x * kDigits + threadIdx.x] = count[threadIdx.x];
 }
-__global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a) {
-  __shared__ unsigned at_of[16][kDigits], all_of[4][kDigits], earlier_of[4][kDigits];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digit = threadIdx.x & (kDigits - 1), quarter = threadIdx.x / kDigits;
+__global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a, EmbeddingFill fill) {
+  __shared__ unsigned at_of[16][kDigits], all_of[2][kDigits], earlier_of[2][kDigits];
+  if (blockIdx.x >= (unsigned)a.blocks) return embedding_fill(a.e, a.blocks, fill);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digit = threadIdx.x & (kDigits - 1), half = threadIdx.x / kDigits;
   unsigned all = 0, earlier = 0;
-  for (int b = quarter; b < a.blocks; b += 4) {
+  for (int b = half; b < a.blocks; b += 2) {
     const unsigned n = a.counts[(long long)b * kDigits + digit];
     all += n, earlier += b < (int)blockIdx.x ? n : 0;
   }
-  all_of[quarter][digit] = all, earlier_of[quarter][digit] = earlier;
+  all_of[half][digit] = all, earlier_of[half][digit] = earlier;
   for (int w = threadIdx.x; w < 16 * kDigits; w += 1024) (&at_of[0][0])[w] = 0;
   __syncthreads();
   unsigned key[kSortedRows / 1024], row[kSortedRows / 1024], rank[kSortedRows / 1024];
@@ -121,7 +151,7 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a) {
     const unsigned d = key[n] >> a.shift & (kDigits - 1);
     unsigned long long same = __ballot(in);
 #pragma unroll
-    for (int bit = 0; bit < 8; ++bit) {
+    for (int bit = 0; bit < kDigitBits; ++bit) {
       const unsigned long long ones = __ballot(d >> bit & 1);
       same &= d >> bit & 1 ? ones : ~ones;
     }
@@ -134,12 +164,12 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a) {
     }
   }
   __syncthreads();
-  if (threadIdx.x < 64) {  // where the digits begin: four digits a lane
-    unsigned of[4], sum = 0;
+  if (threadIdx.x < 64) {  // where the digits begin: eight digits a lane
+    unsigned of[8], sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       of[j] = sum;
-      sum += all_of[0][lane * 4 + j] + all_of[1][lane * 4 + j] + all_of[2][lane * 4 + j] + all_of[3][lane * 4 + j];
+      sum += all_of[0][lane * 8 + j] + all_of[1][lane * 8 + j];
     }
     unsigned up = sum;
 #pragma unroll
@@ -148,11 +178,11 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a) {
       if (lane >= step) up += o;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) all_of[0][lane * 4 + j] = up - sum + of[j];
+    for (int j = 0; j < 8; ++j) all_of[0][lane * 8 + j] = up - sum + of[j];
   }
   __syncthreads();
   if (threadIdx.x < kDigits) {  // and the wavefronts' rows of them
-    unsigned at = all_of[0][digit] + earlier_of[0][digit] + earlier_of[1][digit] + earlier_of[2][digit] + earlier_of[3][digit];
+    unsigned at = all_of[0][digit] + earlier_of[0][digit] + earlier_of[1][digit];
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
       const unsigned n = at_of[w][digit];
@@ -170,24 +200,26 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a) {
     }
 }
 
-// Sums: a wavefront takes kRun rows in the order of their tokens and 512 columns.  A run of one token inside of them is a row of the table; of a run that goes on the sum so far is
-// kept, of one that has begun before the sum of what is here.  The other wavefronts write the rows of the table that no token has.
-constexpr int kRun = 32, kBare = 64;  // rows of a wavefront
+// Sums: up to 64 lanes, of 8 columns each, take `run` rows in the order of their tokens.  A run of one token inside of them is a row of the table; of a run that goes on the sum so far
+// is kept, of one that has begun before the sum of what is here.
 struct EmbeddingSumArgs {
   EmbeddingArgs e;
   float *begun, *rest;  // [pieces][D]
   int pieces, strips;
-  long long sums;  // wavefronts of them
+  int lanes;  // of a piece and strip: a power of two
+  int run;
 };
 template <typename AT>
 __device__ __forceinline__ void embedding_put(AT* to, int left, const float (&v)[8], float scale) {
   if (left >= 8) {
     float w[8];
+#pragma unroll
     for (int k = 0; k < 8; ++k) w[k] = v[k] * scale;
     Eight<AT> q;
     q.set(w);
     q.store_streamed(to);
   } else {
+#pragma unroll
     for (int k = 0; k < 8; ++k)
       if (k < left) store_f32(to + k, v[k] * scale);
   }
@@ -195,42 +227,25 @@ __device__ __forceinline__ void embedding_put(AT* to, int left, const float (&v)
 template <typename AT>
 __global__ __launch_bounds__(256) void k_embedding_sums(EmbeddingSumArgs s) {
   const EmbeddingArgs& a = s.e;
-  const int lane = threadIdx.x & 63;
-  const long long item = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned V = (unsigned)a.V;
-  if (item >= s.sums) {
-    const long long v0 = (item - s.sums) * kBare, v = v0 + lane;
-    if (v0 >= a.V) return;
-    unsigned lo = 0, hi = (unsigned)a.rows;
-    while (lo < hi) {  // (as many turns in all lanes, or one fewer)
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (a.token_of[mid] < (unsigned)v)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    unsigned long long bare = __ballot(v < a.V && !(lo < a.rows && a.token_of[lo] == (unsigned)v));
-    const float none[8] = {};
-    for (; bare; bare &= bare - 1) {
-      AT* to = (AT*)a.out + (v0 + __builtin_ctzll(bare)) * a.D;
-      for (long long e = lane * 8; e < a.D; e += 512) embedding_put(to + e, (int)(a.D - e < 8 ? a.D - e : 8), none, 0.f);
-    }
-    return;
-  }
+  const long long item = (blockIdx.x * 256ll + threadIdx.x) / s.lanes;
   const int piece = (int)(item / s.strips), strip = (int)(item - (long long)piece * s.strips);
-  const long long col = strip * 512ll + lane * 8, first = (long long)piece * kRun;
-  const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8)), rows = (int)(a.rows - first < kRun ? a.rows - first : kRun);
+  if (piece >= s.pieces) return;
+  const unsigned V = (unsigned)a.V;
+  const long long col = ((long long)strip * s.lanes + threadIdx.x % s.lanes) * 8, first = (long long)piece * s.run;
+  const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8)), rows = (int)(a.rows - first < s.run ? a.rows - first : s.run);
+  if (left == 0) return;
   const unsigned before = first ? a.token_of[first - 1] : 0xFFFFFFFFu, after = first + rows < a.rows ? a.token_of[first + rows] : 0xFFFFFFFFu;
   float sum[8] = {};
   unsigned token = a.token_of[first];
   bool begun_here = token != before;
   auto flush = [&](bool ends_here) {
-    if (token >= V || left == 0) return;
+    if (token >= V) return;
     if (begun_here && ends_here) {
       embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
     } else {
       // (a run that fills this piece and goes on is part of the run that began earlier)
       float* to = (begun_here ? s.begun : s.rest) + piece * a.D + col;
+#pragma unroll
       for (int k = 0; k < 8; ++k)
         if (k < left) to[k] = sum[k];
     }
@@ -238,70 +253,90 @@ __global__ __launch_bounds__(256) void k_embedding_sums(EmbeddingSumArgs s) {
   constexpr int AHEAD = 8;
   for (int p0 = 0; p0 < rows; p0 += AHEAD) {
     Eight<AT> q[AHEAD];
-    unsigned key[AHEAD];
-    float part[AHEAD][8];
+    unsigned key[AHEAD], row[AHEAD];
+    float part[8];
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) {
       const long long at = first + (p0 + p < rows ? p0 + p : rows - 1);
-      key[p] = a.token_of[at];
-      const AT* from = (const AT*)a.in + a.order[at] * a.ld + col;
-      const bool wanted = p0 + p < rows && key[p] < V;
+      key[p] = p0 + p < rows ? a.token_of[at] : V;
+      row[p] = a.order[at];
+    }
+#pragma unroll
+    for (int p = 0; p < AHEAD; ++p) {
+      const AT* from = (const AT*)a.in + row[p] * a.ld + col;
+      const bool wanted = key[p] < V;
       if (wanted && left == 8) {
         q[p].load(from);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) part[p][k] = wanted && k < left ? load_f32(from + k) : 0.f;
-        q[p].set(part[p]);
+        for (int k = 0; k < 8; ++k) part[k] = wanted && k < left ? load_f32(from + k) : 0.f;
+        q[p].set(part);
       }
     }
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) {
-      if (p0 + p >= rows) break;
-      if (key[p] != token) {
-        flush(true);
-        token = key[p], begun_here = true;
+      if (p0 + p < rows) {
+        if (key[p] != token) {
+          flush(true);
+          token = key[p], begun_here = true;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+          for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+        }
+        q[p].get(part);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += part[k];
       }
-      q[p].get(part[p]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += part[p][k];
     }
   }
   flush(token != after);
 }
 
-// Rows of the table whose run goes over several pieces.
+// Rows of the table whose run goes over several pieces: a wavefront for each piece and 512 columns; most pieces have none that begins in them and goes on.
 template <typename AT>
 __global__ __launch_bounds__(256) void k_embedding_join(EmbeddingSumArgs s) {
   const EmbeddingArgs& a = s.e;
   const int lane = threadIdx.x & 63;
   const long long item = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= s.sums) return;
   const int piece = (int)(item / s.strips), strip = (int)(item - (long long)piece * s.strips);
-  const long long col = strip * 512ll + lane * 8, first = (long long)piece * kRun, next = first + kRun;
+  const long long first = (long long)piece * s.run, next = first + s.run;
   if (next >= a.rows) return;
   const unsigned token = a.token_of[next];
-  // (the run has to go on behind this piece, and to begin in it)
   if (token >= (unsigned)a.V || a.token_of[next - 1] != token || (first && a.token_of[first - 1] == token)) return;
-  long long lo = next, hi = a.rows;
-  while (lo < hi) {
-    const long long mid = lo + (hi - lo) / 2;
-    if (a.token_of[mid] == token)
-      lo = mid + 1;
-    else
-      hi = mid;
+  int count = 0;  // pieces behind this one that begin with the token
+  for (;;) {
+    const long long at = next + (long long)(count + lane) * s.run;
+    const unsigned long long other = ~__ballot(at < a.rows && a.token_of[at < a.rows ? at : next] == token);
+    if (other) {
+      count += __builtin_ctzll(other);
+      break;
+    }
+    count += 64;
   }
-  const int last = (int)((lo - 1) / kRun), left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8));
-  if (left == 0) return;
+  const long long col = strip * 512ll + lane * 8;
+  const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8));
   float sum[8];
+  if (left == 8) {
+    Eight<float> q;
+    q.load(s.begun + piece * a.D + col);
+    q.get(sum);
+#pragma unroll 8
+    for (int p = piece + 1; p <= piece + count; ++p) {
+      float part[8];
+      Eight<float> q;
+      q.load(s.rest + p * a.D + col);
+      q.get(part);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) sum[k] = k < left ? s.begun[piece * a.D + col + k] : 0.f;
-#pragma unroll 4
-  for (int p = piece + 1; p <= last; ++p)
+      for (int k = 0; k < 8; ++k) sum[k] += part[k];
+    }
+  } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum[k] += k < left ? s.rest[p * a.D + col + k] : 0.f;
-  embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
+    for (int k = 0; k < 8; ++k) {
+      if (k >= left) break;
+      sum[k] = s.begun[piece * a.D + col + k];
+      for (int p = piece + 1; p <= piece + count; ++p) sum[k] += s.rest[p * a.D + col + k];
+    }
+  }
+  if (left) embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
 }
 
 }  // namespace rtn

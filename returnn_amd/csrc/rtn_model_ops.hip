@@ -274,14 +274,17 @@ int rtn_embedding_fwd(const int64_t* tokens, const void* table, int64_t ld, void
 // Workspace of the gradient: the sorted rows and their tokens, twice and counts of digits where there is more than one pass of sorting; the sums of runs over several pieces.
 struct EmbeddingPlan {
   int64_t pieces, strips, blocks;
-  int passes;
+  int passes, lanes, run;
   size_t rows, counts, parts;  // of 4 bytes
   EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
-    pieces = (n + kRun - 1) / kRun, strips = (D + 511) / 512;
+    strips = (D + 511) / 512;
+    run = n * strips >= 16384 ? 64 : 16;  // (rows of a piece: four wavefronts for every compute unit, and no more of them than that takes)
+    pieces = (n + run - 1) / run;
+    for (lanes = 1; lanes < 64 && lanes * 8 < D;) lanes *= 2;
     passes = 0, blocks = 0;
     if (n > kCountedRows) {
       blocks = (n + kSortedRows - 1) / kSortedRows;
-      for (int64_t v = V; v; v >>= 8) ++passes;  // (V itself stands for no token)
+      for (int64_t v = V; v; v >>= kDigitBits) ++passes;  // (V itself stands for no token)
     }
     rows = (size_t)(n + 3) / 4 * 4;
     counts = (size_t)blocks * kDigits;
@@ -303,9 +306,10 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
   if (!V || !D) return RTN_OK;
   if (!Dtable || (rows && (!tokens || !dy))) return fail(RTN_ERR_ARG, "%s: null pointer", what);
   const EmbeddingPlan p(rows, V, D);
-  const int64_t bare = (V + kBare - 1) / kBare, sums = p.pieces * p.strips;
-  if (p.strips > 4 * max_blocks(256) / (p.pieces + bare + 1) || (rows && D > INT64_MAX / 32 / rows))
+  const int e = size_of(dtype);
+  if (D > INT64_MAX / 16 / V || D > INT64_MAX / 16 / (rows + 1) || D * V * e / kFilled >= max_blocks(1024) / 2 || p.strips > max_blocks(256) / 2 / (p.pieces + 1))
     return fail(RTN_ERR_SHAPE, "%s: %lld rows of a table [%lld,%lld] are too many for one call", what, (long long)rows, (long long)V, (long long)D);
+  const int64_t bytes = D * V * e, filling = (bytes + kFilled - 1) / kFilled;
   const size_t need = rows ? p.bytes() : 0;
   if (need && (!workspace || workspace_bytes < need)) return fail(RTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
   if (!aligned(workspace, 16)) return fail(RTN_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
@@ -314,24 +318,31 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
   EmbeddingArgs a{tokens, dy, ld, Dtable, rows, V, D, scale, nullptr, nullptr};
   if (p.passes) {
     SortArgs s{a, nullptr, nullptr, counts, (int)p.blocks, 0};
-    for (int pass = 0; pass < p.passes; ++pass, s.shift += 8) {
+    // (each launch fills its share of the table)
+    auto launch = [&](void (*kernel)(SortArgs, EmbeddingFill), int part) {
+      const int64_t from = filling * part / (2 * p.passes), to = filling * (part + 1) / (2 * p.passes);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(p.blocks + to - from)), dim3(1024), 0, stream, s, EmbeddingFill{bytes, from});
+    };
+    for (int pass = 0; pass < p.passes; ++pass, s.shift += kDigitBits) {
       s.e.order = now, s.e.token_of = now + p.rows;
-      hipLaunchKernelGGL(k_embedding_digits, dim3((unsigned)p.blocks), dim3(1024), 0, stream, s);
-      hipLaunchKernelGGL(k_embedding_move, dim3((unsigned)p.blocks), dim3(1024), 0, stream, s);
+      launch(k_embedding_digits, 2 * pass);
+      launch(k_embedding_move, 2 * pass + 1);
       s.order = s.e.order, s.token_of = s.e.token_of;
       std::swap(now, other);
     }
     a.order = s.e.order, a.token_of = s.e.token_of;
   } else {
     a.order = now, a.token_of = now + p.rows;
-    if (rows) hipLaunchKernelGGL(k_embedding_order, dim3((unsigned)((rows + 63) / 64)), dim3(1024), 0, stream, a);
+    const unsigned sorting = (unsigned)((rows + 15) / 16);
+    hipLaunchKernelGGL(k_embedding_order, dim3(sorting + (unsigned)filling), dim3(1024), 0, stream, a, sorting, EmbeddingFill{bytes, 0});
   }
-  EmbeddingSumArgs s{a, (float*)(counts + p.counts), (float*)(counts + p.counts) + p.parts, (int)p.pieces, (int)p.strips, sums};
-  with_type(dtype, [&](auto type) {
-    typedef decltype(type) AT;
-    hipLaunchKernelGGL(k_embedding_sums<AT>, dim3((unsigned)((sums + bare + 3) / 4)), dim3(256), 0, stream, s);
-    if (rows > kRun) hipLaunchKernelGGL(k_embedding_join<AT>, dim3((unsigned)((sums + 3) / 4)), dim3(256), 0, stream, s);
-  });
+  const EmbeddingSumArgs s{a, (float*)(counts + p.counts), (float*)(counts + p.counts) + p.parts, (int)p.pieces, (int)p.strips, p.lanes, p.run};
+  if (rows)
+    with_type(dtype, [&](auto type) {
+      typedef decltype(type) AT;
+      hipLaunchKernelGGL(k_embedding_sums<AT>, dim3((unsigned)((p.pieces * p.strips * p.lanes + 255) / 256)), dim3(256), 0, stream, s);
+      if (p.pieces > 1) hipLaunchKernelGGL(k_embedding_join<AT>, dim3((unsigned)((p.pieces * p.strips + 3) / 4)), dim3(256), 0, stream, s);
+    });
   return launched(what);
 }
 

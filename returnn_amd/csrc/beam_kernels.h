@@ -208,6 +208,16 @@ __global__ __launch_bounds__(64 * W) void k_beam_pieces(BeamArgs a) {
   const float total = a.totals[row];
   const bool ended = a.ended && a.ended[row];
   const AT* scores = (const AT*)a.scores + row * a.ld;
+  unsigned long long* to = a.to + (long long)blockIdx.x * a.beam;
+  if (ended && total < __builtin_inff()) {  // (nothing to look for: the end, unless that is at minus infinity as well, and the lowest tokens)
+    const int end = (int)a.end_token, first = end >= v0 && end < v1 && total > -__builtin_inff();
+    if ((int)threadIdx.x < a.beam) {
+      int v = v0 + (int)threadIdx.x - first;
+      if (first && v >= end) ++v;
+      to[threadIdx.x] = first && threadIdx.x == 0 ? alternative(total, (unsigned)(k * a.V + end)) : (v < v1 ? alternative(-__builtin_inff(), (unsigned)(k * a.V + v)) : 0);
+    }
+    return;
+  }
   unsigned high[E];
   auto own = [&](int j) { return v0 + (j * 64 * W + (int)threadIdx.x) * 8; };
   if (!ended) {
@@ -234,7 +244,6 @@ __global__ __launch_bounds__(64 * W) void k_beam_pieces(BeamArgs a) {
       high[e] = v < v1 ? order_of(total + (v == a.end_token ? 0.f : -__builtin_inff())) : 0;
     }
   }
-  unsigned long long* to = a.to + (long long)blockIdx.x * a.beam;
   const int n = beam_best<W, E>(
       scratch, high, [&](int e) { return ~(unsigned)(k * a.V + own(e / 8) + e % 8); }, a.beam, true, [&](int rank, unsigned long long q) { to[rank] = q; });
   for (int rank = n + threadIdx.x; rank < a.beam; rank += 64 * W) to[rank] = 0;

@@ -330,11 +330,11 @@ __global__ __launch_bounds__(256) void k_embedding_join(EmbeddingSumArgs s) {
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k >= left) break;
-      sum[k] = s.begun[piece * a.D + col + k];
-      for (int p = piece + 1; p <= piece + count; ++p) sum[k] += s.rest[p * a.D + col + k];
-    }
+    for (int k = 0; k < 8; ++k) sum[k] = k < left ? s.begun[piece * a.D + col + k] : 0.f;
+#pragma unroll 4
+    for (int p = piece + 1; p <= piece + count; ++p)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += k < left ? s.rest[p * a.D + col + k] : 0.f;
   }
   if (left) embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
 }

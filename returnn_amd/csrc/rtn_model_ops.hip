@@ -278,7 +278,7 @@ struct EmbeddingPlan {
   size_t rows, counts, parts;  // of 4 bytes
   EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
     strips = (D + 511) / 512;
-    run = n * strips >= 16384 ? 64 : 16;  // (rows of a piece: four wavefronts for every compute unit, and no more of them than that takes)
+    run = n * strips >= 16384 ? 64 : 8;  // (rows of a piece: four wavefronts for every compute unit, and no more of them than that takes)
     pieces = (n + run - 1) / run;
     for (lanes = 1; lanes < 64 && lanes * 8 < D;) lanes *= 2;
     passes = 0, blocks = 0;
@@ -357,7 +357,7 @@ struct BeamPlan {
       return;
     }
     splits = (V + kBeamLong - 1) / kBeamLong;
-    if (const int64_t small = (V + kBeamShort - 1) / kBeamShort; (int64_t)B * K * small <= 512) splits = small;
+    if (const int64_t small = (V + kBeamShort - 1) / kBeamShort; K * small * beam <= kBeamJoined || (int64_t)B * K * small <= 512) splits = small;
     segment = ((V + splits - 1) / splits + 7) / 8 * 8;
     lists = K * splits;
   }
@@ -410,7 +410,10 @@ int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const u
       a.lists = (int)lists, a.next = (int)next;
       unsigned long long* const other = (unsigned long long*)workspace + (a.to == workspace ? (size_t)B * (size_t)p.lists * (size_t)beam : 0);
       a.from = a.to, a.to = other;
-      hipLaunchKernelGGL((k_beam_join<16, kBeamJoined / 1024>), dim3((unsigned)(B * next)), dim3(1024), 0, stream, a);
+      if (lists * beam <= 1024)
+        hipLaunchKernelGGL((k_beam_join<4, 4>), dim3((unsigned)B), dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_beam_join<16, kBeamJoined / 1024>), dim3((unsigned)(B * next)), dim3(1024), 0, stream, a);
       if (next == 1) break;
       lists = next;
     }
@@ -433,6 +436,7 @@ int rtn_reorder_rows(int32_t count, const void* const* in, void* const* out, con
     if ((row_bytes[n] + kReorderPiece - 1) / kReorderPiece > max_blocks(256) / rows / kReordered)
       return fail(RTN_ERR_SHAPE, "%s: %lld rows of %lld bytes are too many for one call", what, (long long)rows, (long long)row_bytes[n]);
   }
+  bool any = false;
   for (int first = 0; first < count; first += kReordered) {
     ReorderArgs a{{}, {}, {}, sources, B, K, beam, 1};
     const int some = std::min(count - first, kReordered);
@@ -443,10 +447,10 @@ int rtn_reorder_rows(int32_t count, const void* const* in, void* const* out, con
     }
     const int64_t pieces = (most + kReorderPiece - 1) / kReorderPiece;
     if (!pieces) continue;
-    a.pieces = (int)pieces;
+    a.pieces = (int)pieces, any = true;
     hipLaunchKernelGGL(k_reorder_rows, dim3((unsigned)(rows * pieces), some), dim3(256), 0, (hipStream_t)hip_stream, a);
   }
-  return launched(what);
+  return any ? launched(what) : RTN_OK;
 }
 
 }  // extern "C"

@@ -1,9 +1,10 @@
 """
 A recurrent language model of this package's operators: the path on which they run together.
 
-Embedding, a stack of recurrent layers (:class:`returnn_amd.recurrence.GatedRecurrence`, or :class:`returnn_amd.lstm.LSTM`) with
-dropout between them, added to what went in, and a projection to the vocabulary, whose logits go through
-:func:`returnn_amd.scoring.token_log_probs`: the loss in training, scores of given texts, and the alternatives of every hypothesis in search.
+Embedding (:class:`returnn_amd.embedding.Embedding`), a stack of recurrent layers (:class:`returnn_amd.recurrence.GatedRecurrence`,
+:class:`returnn_amd.delta_rule.DeltaRecurrence` or :class:`returnn_amd.lstm.LSTM`) with dropout between them, added to what went in, and a projection to
+the vocabulary, whose logits go through :func:`returnn_amd.scoring.token_log_probs`: the loss in training, scores of given texts, and the alternatives of
+every hypothesis in search, of which :func:`returnn_amd.beam_search.beam_select` takes the best.
 
 ``python -m returnn_amd.language_model`` trains a small one on a made-up text on the GPU and completes it.
 """
@@ -15,7 +16,10 @@ from typing import List, NamedTuple, Optional, Tuple, Union
 
 import torch
 
+from .beam_search import beam_select, reorder_states
+from .delta_rule import DeltaRecurrence
 from .dropout import Dropout
+from .embedding import Embedding
 from .lstm import LSTM, LstmState
 from .recurrence import GatedRecurrence
 from .scoring import TokenScores, token_log_probs
@@ -34,7 +38,7 @@ class RecurrentLanguageModel(torch.nn.Module):
     """
     :param num_tokens: size of the vocabulary
     :param dim: width of the embedding and of every layer
-    :param layer: "gated" (parallel in time) or "lstm"
+    :param layer: "gated" (parallel in time), "delta" (likewise, with matrices as state) or "lstm"
     :param drop_prob: of the embedding and of every layer's output
     :param same_over_time: one dropout mask for all frames of a sequence
     """
@@ -44,12 +48,13 @@ class RecurrentLanguageModel(torch.nn.Module):
         device=None, dtype=None,
     ):  # fmt: skip
         super().__init__()
-        if layer not in ("gated", "lstm"):
-            raise ValueError("RecurrentLanguageModel: layer must be 'gated' or 'lstm', got %r" % (layer,))
+        kinds = {"gated": GatedRecurrence, "delta": DeltaRecurrence, "lstm": LSTM}
+        if layer not in kinds:
+            raise ValueError("RecurrentLanguageModel: layer must be 'gated', 'delta' or 'lstm', got %r" % (layer,))
         self.num_tokens, self.dim = int(num_tokens), int(dim)
         kw = dict(device=device, dtype=dtype)
-        self.embedding = torch.nn.Embedding(self.num_tokens, self.dim, **kw)
-        self.layers = torch.nn.ModuleList((GatedRecurrence if layer == "gated" else LSTM)(self.dim, self.dim, **kw) for _ in range(int(num_layers)))
+        self.embedding = Embedding(self.num_tokens, self.dim, **kw)
+        self.layers = torch.nn.ModuleList(kinds[layer](self.dim, self.dim, **kw) for _ in range(int(num_layers)))
         # (a seed of its own for each, so that no two masks of a step are alike)
         self.dropouts = torch.nn.ModuleList(Dropout(drop_prob, seed=seed * 1009 + k, same_over_time=same_over_time) for k in range(int(num_layers) + 1))
         self.output = torch.nn.Linear(self.dim, self.num_tokens, **kw)
@@ -138,12 +143,13 @@ class RecurrentLanguageModel(torch.nn.Module):
         tokens = torch.empty((1, 0), dtype=torch.int64, device=start.device)
         for _ in range(int(length)):
             s, state = self.scores(last, state=state, top_k=k)
-            joint = (total[:, None] + s.top_log_probs).flatten()
-            total, at = joint.topk(min(int(beam), joint.numel()))
-            source = torch.div(at, k, rounding_mode="floor")
-            last = s.top_ids.flatten()[at]
-            tokens = torch.cat((tokens[source], last[:, None]), dim=1)
-            state = [LstmState(h=v.h[source], c=v.c[source]) if isinstance(v, LstmState) else v[source] for v in state]
+            total, source, at = beam_select(s.top_log_probs, total, min(int(beam), s.top_ids.numel()))
+            last = s.top_ids[source, at]
+            flat = [t for v in state for t in (v if isinstance(v, LstmState) else (v,))]
+            tokens, *flat = reorder_states([tokens] + flat, source)
+            tokens = torch.cat((tokens, last[:, None]), dim=1)
+            flat = iter(flat)
+            state = [LstmState(*(next(flat) for _ in v)) if isinstance(v, LstmState) else next(flat) for v in state]
         return Hypotheses(tokens, total)
 
 
@@ -152,7 +158,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     import argparse
 
     ap = argparse.ArgumentParser(prog="python -m returnn_amd.language_model", description=main.__doc__)
-    ap.add_argument("--layer", choices=["gated", "lstm"], default="gated")
+    ap.add_argument("--layer", choices=["gated", "delta", "lstm"], default="gated")
     ap.add_argument("--steps", type=int, default=150)
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():

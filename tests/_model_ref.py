@@ -74,7 +74,7 @@ def embed(tokens, weight, scale=1.0):
 def embed_grad(tokens, dy, V, scale=1.0):
     """:return: dW [V,D], sums of absolute values [V,D], how many there are of each token"""
     flat, dy = numpy.asarray(tokens).reshape(-1), numpy.asarray(dy, numpy.float64)
-    dy = dy.reshape(flat.size, -1)
+    dy = dy.reshape(flat.size, dy.shape[-1])
     inside = (flat >= 0) & (flat < V)
     out, most = numpy.zeros((2, V, dy.shape[1]))
     numpy.add.at(out, flat[inside], scale * dy[inside])

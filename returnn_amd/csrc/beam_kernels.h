@@ -254,13 +254,15 @@ template <int W, int E>
 __global__ __launch_bounds__(64 * W) void k_beam_join(BeamArgs a) {
   __shared__ BeamScratch<W> scratch;
   const int b = blockIdx.x / (unsigned)a.next, part = (int)(blockIdx.x - (unsigned)b * a.next), per = kBeamJoined / a.beam;
-  const int count = (a.lists - part * per < per ? a.lists - part * per : per) * a.beam;
+  const int lists = a.lists - part * per < per ? a.lists - part * per : per;
   const unsigned long long* from = a.from + ((long long)b * a.lists + part * per) * a.beam;
+  // The first of all lists, then the second of all: so the groups of beam_best have their shares of the best.  (List by list the first ones of 64 lists of 64 were in 4 of the 256 groups, their bound
+  // let hundreds through, and the choice was made digit by digit: one search of 64 hypotheses with 32000 scores, 64 of them: 77 us, so 29.)
   unsigned high[E], low[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int at = e * 64 * W + threadIdx.x;
-    const unsigned long long q = at < count ? from[at] : 0;
+    const int at = e * 64 * W + threadIdx.x, rank = (unsigned)at / (unsigned)lists, list = at - rank * lists;
+    const unsigned long long q = rank < a.beam ? from[list * a.beam + rank] : 0;
     high[e] = (unsigned)(q >> 32), low[e] = (unsigned)q;
   }
   unsigned long long* to = a.to + ((long long)b * a.next + part) * a.beam;

@@ -51,19 +51,38 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
       for (int c = 0; c < 4; ++c) S[i][c] = in && col + c < a.dv ? a.s0[at + c] : 0.f;
     }
   }
-  for (long long p = 0; p < n; ++p) {
-    const long long t = a.reverse ? n - 1 - p : p, frame = t * a.B + b;
-    float k[R], q[R], v[4];
+  // A frame's numbers, asked for a frame ahead.  (What is not there is read at the end of what is, and taken as 0: what is loaded on a condition of a lane is waited for at once.)
+  struct Frame {
+    AT k[R], q[R], v[4];
+    float g, beta;
+    long long at;
+  } next;
+  auto load = [&](long long p) {
+    const long long frame = (a.reverse ? n - 1 - p : p) * a.B + b;
     const AT *kp = (const AT*)a.k + frame * a.ldk + kh * a.dk, *qp = (const AT*)a.q + frame * a.ldq + kh * a.dk, *vp = (const AT*)a.v + frame * a.ldv + h * a.dv;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const bool in = row + i < a.dk;
-      k[i] = in ? load_f32(kp + row + i) : 0.f;
-      q[i] = in ? load_f32(qp + row + i) : 0.f;
+      const int e = row + i < a.dk ? row + i : a.dk - 1;
+      next.k[i] = kp[e], next.q[i] = qp[e];
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = col + c < a.dv ? load_f32(vp + col + c) : 0.f;
-    const float decay = expf(a.g[frame * a.heads + h]), beta = a.beta[frame * a.heads + h];
+    for (int c = 0; c < 4; ++c) next.v[c] = vp[col + c < a.dv ? col + c : a.dv - 1];
+    next.g = a.g[frame * a.heads + h], next.beta = a.beta[frame * a.heads + h], next.at = frame;
+  };
+  if (n) load(0);
+  for (long long p = 0; p < n; ++p) {
+    float k[R], q[R], v[4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool in = row + i < a.dk;
+      k[i] = in ? (float)next.k[i] : 0.f;
+      q[i] = in ? (float)next.q[i] : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = (float)next.v[c];
+    const float decay = expf(next.g), beta = next.beta;
+    const long long frame = next.at;
+    load(p + 1 < n ? p + 1 : p);
     float sum[9] = {};
 #pragma unroll
     for (int i = 0; i < R; ++i) {

@@ -26,6 +26,8 @@ bool nothing(const DeltaSizes& z) { return z.B == 0 || z.heads == 0; }
 bool valid(const DeltaSizes& z) {
   return z.T >= 0 && z.T <= kMaxFrames && z.B >= 0 && z.key_heads >= 0 && z.heads >= 0 && z.dk >= 1 && z.dk <= kMaxKeyDim && z.dv >= 1 && z.dv <= kMaxValueDim && known(z.dtype);
 }
+// Calls of at most these frames that no gradient follows go frame by frame.  (12 sequences of 8 heads of 128 x 128 in bf16, frame by frame and in chunks: 1 frame 7.1 and 33 us, 16 frames 26.7 and
+// 31.5, 24 frames 37 and 32; of one sequence 25 and 28.5, 35 and 29; of 64 54 and 66, 76 and 69.)
 constexpr int kStepFrames = 16;
 int delta_frames(const DeltaSizes& z) { return z.dtype == RTN_DTYPE_BF16 ? DeltaChunk<__bf16>::kFrames : DeltaChunk<float>::kFrames; }
 int64_t delta_chunks(const DeltaSizes& z) { return (z.T + delta_frames(z) - 1) / delta_frames(z); }
@@ -51,8 +53,12 @@ void with_delta(const DeltaSizes& z, F f) {
       f(type, Count<128>());
   });
 }
-// Wavefronts of a workgroup that goes through a head's chunks.
-int delta_waves(const DeltaSizes& z) { return z.dv > 64 && (int64_t)z.B * z.heads * ((z.dv + 127) / 128) >= 128 ? 8 : 4; }
+// Wavefronts of a workgroup that goes through a head's chunks, with 16 columns of the state each.  Four take three quarters of the time that eight take, for half the columns: T=1000, heads of
+// 128 x 128 in bf16, four and eight: 128 heads (one round of workgroups, one) 140 and 185 us, with the gradient 609 and 680; 256 heads (two, one) 294 and 282, 1177 and 1036.
+int delta_waves(const DeltaSizes& z) {
+  const int64_t lines = (int64_t)z.B * z.heads, four = (lines * ((z.dv + 63) / 64) + 255) / 256, eight = (lines * ((z.dv + 127) / 128) + 255) / 256;  // rounds of the device
+  return 4 * eight < 3 * four ? 8 : 4;
+}
 int64_t delta_strips(const DeltaSizes& z) { return (z.dv + 16 * delta_waves(z) - 1) / (16 * delta_waves(z)); }
 template <typename F>
 void with_waves(const DeltaSizes& z, F f) {
@@ -62,7 +68,8 @@ void with_waves(const DeltaSizes& z, F f) {
     f(Count<4>());
 }
 // Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.3, and both
-// passes run in rounds of as many workgroups as there are compute units.
+// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 323 us, 4 164, 8 116, what is chosen (11) 122, 32 177;
+// T=8192, two of 8 heads of 64 x 128: 554, 256, 177, 191, 212; T=1000, 16 of 8 of 128 x 128: one 140, 4 290.
 int64_t delta_segments(const DeltaSizes& z) {
   const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * delta_waves(z);
   const int64_t strips = delta_strips(z), strips_through = ((z.dv + 15) / 16 * 16 + delta_key_width(z) + width - 1) / width;
@@ -278,7 +285,9 @@ struct EmbeddingPlan {
   size_t rows, counts, parts;  // of 4 bytes
   EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
     strips = (D + 511) / 512;
-    run = n * strips >= 16384 ? 64 : 8;  // (rows of a piece: four wavefronts for every compute unit, and no more of them than that takes)
+    // Rows of a piece: few, so that there are wavefronts enough, until the pieces' own starts and ends cost more (rows of 512 bf16, forward and gradient, 8, 16 and 32 rows: of 8192 rows 31.8, 33.0 and
+    // 37.6 us, of 32768 58.0, 56.2 and 58.7, of 131072 151, 134 and 128).
+    run = n * strips < 16384 ? 8 : (n * strips < 65536 ? 16 : 32);
     pieces = (n + run - 1) / run;
     for (lanes = 1; lanes < 64 && lanes * 8 < D;) lanes *= 2;
     passes = 0, blocks = 0;
@@ -347,8 +356,9 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
 }
 
 // ---- beam search ----------------------------------------------------------------------------------------------------
-// Pieces: all continuations of a search at once where they are few; else pieces of hypotheses, as long as a workgroup can hold, or shorter where there would be too few
-// of them to fill the device; and as many rounds of joining their choices as it takes.
+// Pieces: all continuations of a search at once where they are few (64 searches of 8 hypotheses with 1000 scores, 8 of them: 7.9 us, in pieces 10.7).  Else pieces of hypotheses: short ones, several of
+// which are on a compute unit at once, where one round joins their choices (256 searches of 12 with 32000 scores in bf16, 12 of them: 69 us, in long pieces 85); long ones, as long as a workgroup can hold,
+// where there are too many of these (one search of 64 with 32000 scores, 64 of them: 20 us, in short pieces 29).
 struct BeamPlan {
   int64_t splits, segment, lists;  // lists: of choices, per search, behind the first round
   BeamPlan(int32_t B, int32_t K, int64_t V, int32_t beam) {
@@ -357,7 +367,7 @@ struct BeamPlan {
       return;
     }
     splits = (V + kBeamLong - 1) / kBeamLong;
-    if (const int64_t small = (V + kBeamShort - 1) / kBeamShort; K * small * beam <= kBeamJoined || (int64_t)B * K * small <= 512) splits = small;
+    if (const int64_t small = (V + kBeamShort - 1) / kBeamShort; K * small * beam <= kBeamJoined) splits = small;
     segment = ((V + splits - 1) / splits + 7) / 8 * 8;
     lists = K * splits;
   }

@@ -188,6 +188,13 @@ struct DeltaChunkArgs {
 
 __device__ __forceinline__ int delta_place(int row) { return (row & ~31) | ((row >> 2 & 1) << 4) | ((row >> 3 & 3) << 2) | (row & 3); }
 
+// Where an element of a DK x DK matrix lies that is kept as left operands: tile by tile of 16 places and 32 columns, lane by lane, so that a wavefront's read of one is 1 KB.
+template <int DK>
+__device__ __forceinline__ int delta_left_at(int row, int col) {
+  const int place = delta_place(row);
+  return (((place >> 4) * (DK / 32) + (col >> 5)) * 64 + (col >> 3 & 3) * 16 + (place & 15)) * 8 + (col & 7);
+}
+
 // Eight numbers as N parts, by pairs (element by element the compiler rounds each of them twice).
 template <int N>
 __device__ __forceinline__ void delta_parts(delta_f32x8 x, delta_bf16x8 (&p)[N]) {
@@ -387,6 +394,18 @@ struct DeltaFrames {
   __device__ __forceinline__ char* at(int i) const { return base + i * pitch; }
   __device__ __forceinline__ unsigned lane(int i, int col) const { return (unsigned)(turned ? REACH - i : i) * apart + (unsigned)col * (unsigned)sizeof(T); }
 };
+
+// Which line and which of its strips a workgroup has.  Neighbouring workgroups go to the eight XCDs in turn; strips of a line, which read the same, are eight apart, on one XCD with its L2.
+__device__ __forceinline__ void delta_spread(int strips, int* line, int* strip) {
+  const int all = gridDim.x / strips, even = all & ~7, block = blockIdx.x;
+  if (block < even * strips) {
+    const int eight = block >> 3;
+    *strip = eight % strips, *line = eight / strips * 8 + (block & 7);
+  } else {
+    const int rest = block - even * strips;
+    *line = even + rest / strips, *strip = rest % strips;
+  }
+}
 
 // T, P, L and the powers of a chunk, one workgroup of C / 16 wavefronts each, which have 16 rows of L and P each.  The inverse: diagonal blocks of 16 row by row, a column per
 // lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.
@@ -614,8 +633,9 @@ struct DeltaStrip {
   __device__ __forceinline__ DeltaStrip(const DeltaChunkArgs& args, int columns, int first, int segments) : a(args) {
     const int lane = threadIdx.x & 63, strips = (columns + 16 * W - 1) / (16 * W);
     q4 = lane >> 4;
-    const int rest = blockIdx.x / strips;
-    strip = blockIdx.x % strips, segment = first + rest % segments, bh = rest / segments;
+    int rest;
+    delta_spread(strips, &rest, &strip);
+    segment = first + rest % segments, bh = rest / segments;
     col = (strip * W + (int)(threadIdx.x >> 6)) * 16 + (lane & 15);
     has = col < a.f.dv;
     lane_state = (unsigned)(q4 * 8 * a.f.dv + col) * 4u;
@@ -851,9 +871,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         delta_parts(S[2 * b], S[2 * b + 1], p);
 #pragma unroll
         for (int n = 0; n < 3; ++n) {
-          if (a.through_t) *(delta_bf16x8*)(a.through_t + first + (n * DK + of) * DK + b * 32 + strip.q4 * 8) = p[n];
+          if (a.through_t) *(delta_bf16x8*)(a.through_t + first + n * DK * DK + delta_left_at<DK>(of, b * 32 + strip.q4 * 8)) = p[n];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a.through[first + (n * DK + b * 32 + strip.q4 * 8 + j) * DK + of] = p[n][j];
+          for (int j = 0; j < 8; ++j) a.through[first + n * DK * DK + delta_left_at<DK>(b * 32 + strip.q4 * 8 + j, of)] = p[n][j];
         }
       }
     }
@@ -864,52 +884,67 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
 
 // States at the segments' borders, one after the other: border n is what segment n (n + 1 for the error of a state, whose segments are gone through from the last one) makes of none, and what it makes
 // of the border before it is added.  Sixteen columns per workgroup, 16 rows of them per wavefront; the state goes around through LDS, in parts and as the right operand that all need.
+// Bound by what one compute unit gets from memory: 98 KB a border of 128 x 128.  With these read row by row, 64 bytes of each, and asked for a border ahead a border took 2.2 us; in the order of operands,
+// 1 KB at a time, three borders ahead, 1.2.
 template <typename AT, int DK, bool BACK>
 __global__ __launch_bounds__(DK * 4) void k_delta_join(DeltaChunkArgs a) {
   constexpr int KB = DK / 32;
   __shared__ alignas(16) char state[2][KB][3][64][16];
   const int lane = threadIdx.x & 63, k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, i16 = lane & 15, borders = a.segments - 1;
-  const int strips = (a.f.dv + 15) / 16, bh = blockIdx.x / strips, col = blockIdx.x % strips * 16 + i16, first = (k >> 1) * 32 + (k & 1) * 4;
+  int bh, strip;
+  delta_spread((a.f.dv + 15) / 16, &bh, &strip);
+  const int col = strip * 16 + i16, first = (k >> 1) * 32 + (k & 1) * 4;
   const bool has = col < a.f.dv;
-  const long long row = (long long)(first + q4 * 8) * a.f.dv + col;
+  const long long row = (long long)(first + q4 * 8) * a.f.dv + (has ? col : a.f.dv - 1);
   auto border_of = [&](int n) { return BACK ? borders - 1 - n : n; };
   auto border = [&](int n) { return a.borders + ((long long)bh * borders + border_of(n)) * DK * a.f.dv + row; };
+  struct Ahead {  // of a border
+    delta_f32x4 own;
+    delta_bf16x8 A[KB][3];
+  } ahead[3];
   auto get = [&](int n, delta_f32x4& x) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = has ? border(n)[r * a.f.dv] : 0.f;
+    for (int r = 0; r < 4; ++r) x[r] = border(n)[r * a.f.dv];
   };
-  delta_bf16x8 A[KB][3];
-  auto ask = [&](int n) {
+  auto ask = [&](int n, Ahead& of) {
+    n = n < borders ? n : borders - 1;
+    get(n, of.own);
     const __bf16* from = (BACK ? a.through_t : a.through) + ((long long)bh * borders + border_of(n) + BACK) * 3 * DK * DK;
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int m = 0; m < 3; ++m) A[b][m] = *(const delta_bf16x8*)(from + (m * DK + first + (i16 >> 2) * 8 + (i16 & 3)) * DK + b * 32 + q4 * 8);
+      for (int m = 0; m < 3; ++m) of.A[b][m] = *(const delta_bf16x8*)(from + m * DK * DK + ((k * KB + b) * 64 + lane) * 8);
   };
-  delta_f32x4 S, next;
+  delta_f32x4 S;
   get(0, S);
-  get(1, next);
-  ask(1);
-  for (int n = 1;; ++n) {
+#pragma unroll
+  for (int j = 0; j < 3; ++j) ask(1 + j, ahead[j]);
+  auto step = [&](int n, Ahead& now) {
     const delta_f32x4 none = {0.f, 0.f, 0.f, 0.f};
     delta_bf16x8 p[3];
     delta_parts(S, none, p);
 #pragma unroll
     for (int m = 0; m < 3; ++m) *(unsigned long long*)(state[n & 1][k >> 1][m][lane] + (k & 1) * 8) = __builtin_bit_cast(seq_u32x4, p[m])[0] | (unsigned long long)__builtin_bit_cast(seq_u32x4, p[m])[1] << 32;
     __syncthreads();
-    S = next;
+    S = now.own;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
 #pragma unroll
       for (int m = 0; m < 3; ++m) p[m] = *(const delta_bf16x8*)state[n & 1][b][m][lane];
-      S = delta_mma<3>(A[b], p, S);
+      S = delta_mma<3>(now.A[b], p, S);
     }
     if (has)
 #pragma unroll
       for (int r = 0; r < 4; ++r) border(n)[r * a.f.dv] = S[r];
-    if (n + 1 == borders) break;
-    get(n + 1, next);
-    ask(n + 1);
+    ask(n + 3, now);
+  };
+  for (int n = 1;; n += 3) {
+    step(n, ahead[0]);
+    if (n + 1 >= borders) break;
+    step(n + 1, ahead[1]);
+    if (n + 2 >= borders) break;
+    step(n + 2, ahead[2]);
+    if (n + 3 >= borders) break;
   }
 }
 

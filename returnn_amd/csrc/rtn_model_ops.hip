@@ -68,8 +68,8 @@ void with_waves(const DeltaSizes& z, F f) {
     f(Count<4>());
 }
 // Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.3, and both
-// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 323 us, 4 164, 8 116, what is chosen (11) 122, 32 177;
-// T=8192, two of 8 heads of 64 x 128: 554, 256, 177, 191, 212; T=1000, 16 of 8 of 128 x 128: one 140, 4 290.
+// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 331 us, 4 161, 8 107, 16 96, what is chosen (13) 99, 32 129;
+// T=8192, two of 8 heads of 64 x 128: 541, 254, 170, 176, 183, 191; T=1000, 16 of 8 of 128 x 128: one 140, 4 266.
 int64_t delta_segments(const DeltaSizes& z) {
   const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * delta_waves(z);
   const int64_t strips = delta_strips(z), strips_through = ((z.dv + 15) / 16 * 16 + delta_key_width(z) + width - 1) / width;

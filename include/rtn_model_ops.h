@@ -33,7 +33,8 @@ const char* rtn_model_ops_last_error(void);
  *   S_t = a_t S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),   y_t = scale S_t^T q_t
  *
  * q, k   [T,B,key_heads,dk], v [T,B,heads,dv]; row (t,b) starts at element (t*B+b)*ld (0: contiguous).  heads is a multiple of key_heads,
- *        heads / key_heads neighbouring heads share queries and keys.  1 <= dk <= 128, 1 <= dv <= 65536, T up to 2^30.
+ *        heads / key_heads neighbouring heads share queries and keys.  1 <= dk <= 128, 1 <= dv <= 65536, T up to 2^30.  Beyond 16 frames, and with a
+ *        gradient, a frame of all sequences (B*ld elements) is at most 64 MiB (RTN_ERR_SHAPE).
  * g, beta [T,B,heads] float32; g is at most 0 (log of the decay; minus infinity forgets everything before)
  * s0     [B,heads,dk,dv] float32 state before the first frame; NULL: zeros
  * lens   [B] frames per sequence (clamped to 0..T); NULL: T each.  Frames past them are not read: y is 0 there and the state stays.

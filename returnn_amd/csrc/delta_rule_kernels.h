@@ -27,7 +27,8 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float delta_f32x4;
 typedef delta_f32x4 __attribute__((aligned(4))) delta_f32x4_any;
 
 // Frame by frame: 64 columns of a head's state per workgroup, each thread 4 columns of R of the 16 R rows in registers.  What a state gives to a key and to a query is one
-// pass over it: S_t^T q = a S_{t-1}^T q + (k.q) u.
+// pass over it: S_t^T q = a S_{t-1}^T q + (k.q) u.  A single frame is bound by a launch and the state's way in and out (12 sequences of 8 heads of 128 x 128: 7 us for 12.6 MB; 64: 14.3, 4.7 TB/s);
+// further ones by the sums' way through shuffles and LDS, 1.3 us each (2.2 where a frame's numbers were asked for when they were needed).
 template <typename AT, int R>
 __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
   __shared__ float parts[2][4][16][9];
@@ -239,8 +240,7 @@ __device__ __forceinline__ void delta_mma(const delta_bf16x8 (&a)[TILES][NA], co
         for (int t = 0; t < TILES; ++t) c[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t][i], b[s - i], c[t], 0, 0, 0);
       }
 }
-// Between what is asked for and the products that do not need it yet: left to itself the compiler reads every operand just before its product, and each of these waits for LDS
-// (T=4000, one sequence of 8 heads of 128 x 128 in bf16: 331 us).
+// Between what is asked for and the products that do not need it yet: left to itself the compiler reads every operand just before its product, and each of these waits for LDS.
 __device__ __forceinline__ void delta_ahead() { __builtin_amdgcn_sched_barrier(0); }
 
 // A matrix in LDS as N planes of R rows of COLS columns, without gaps.  Groups of eight columns change places by the row, so that 16 neighbouring rows of a column lie in different banks, and
@@ -408,7 +408,8 @@ __device__ __forceinline__ void delta_spread(int strips, int* line, int* strip) 
 }
 
 // T, P, L and the powers of a chunk, one workgroup of C / 16 wavefronts each, which have 16 rows of L and P each.  The inverse: diagonal blocks of 16 row by row, a column per
-// lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.
+// lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.  Bound by latency, of rows of K and of 16 steps of a column each, three workgroups on a compute unit: T=1000,
+// 32 ragged sequences of 8 heads, keys of 128 in bf16: 91 us, 3.1 TB/s, of which the records are the larger part.  (Rows read without a condition, a tile ahead, cost more in selections than they save: 121.)
 template <typename AT, int DK>
 __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, W = C / 16, BLOCKS = delta_blocks(C), ROW = C + 4;
@@ -714,6 +715,11 @@ __device__ __forceinline__ void delta_zero(delta_f32x4 (&x)[N]) {
 
 // Where sequences and heads are few, their chunks are dealt to segments that work side by side.  A segment makes B + A S of a state S: a first pass (KIND kDeltaThrough) finds B, the state behind
 // it from none before it, and A, its columns from those of the unit matrix without values; k_delta_join goes from segment to segment; then all segments begin with their state.
+//
+// A chunk needs the one before it, so a workgroup's time is its chain of products, of LDS reads between them and of barriers: 11 us a chunk of 64 frames, keys and values of 128 in bf16, with eight wavefronts
+// (matrix instructions 15 %, others 25 %, waiting 43 %).  Hence 16 columns of the state per wavefront, in registers from the first chunk to the last, with U and Y going from product to product without leaving them, and
+// everything of the next chunk asked for a chunk ahead.  T=1000, 32 ragged sequences of 8 heads, and all that the gradient wants kept: 214-220 us, 343 MB read, 382 written.  T=4000, one sequence: 30 us for each of
+// the two passes.  (Loads on a condition of a lane, each of which the compiler waits for where paths meet again: 300 us for what now takes 200.)
 enum { kDeltaPlain, kDeltaKeep, kDeltaThrough };
 template <typename AT, int DK, int W, int KIND>
 __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
@@ -961,7 +967,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_join(DeltaChunkArgs a) {
 //   of the chunk's last frame also sum_j gamma_j k_j.(D U_j) + c_C <D, S>;  dg is its sum over all later frames of the chunk.
 //
 // k_delta_backward goes through the chunks of a head from its last one, as k_delta_forward, and leaves R and D; k_delta_gradients does the rest, all chunks side by side.
-// (THROUGH: as of the forward pass, but of the segments behind the first one, and with what their transitions left.)
+// (THROUGH: as of the forward pass, but of the segments behind the first one, and with what their transitions left.)  Bound as that is: 193-204 us for the same 32 sequences.
 template <typename AT, int DK, int W, bool THROUGH>
 __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, KB = DK / 32;
@@ -1086,6 +1092,10 @@ __device__ __forceinline__ float delta_sum16(float v) {
 
 // One chunk of one head per workgroup, DK / 16 wavefronts with 16 columns of dQ and dK each.  The values' columns pass by 32 at a time, the next ones on their way meanwhile.
 // NARROW: values of fewer than eight columns.
+// Of 64 500 clocks of a chunk (keys and values of 128 in bf16) 15 300 go until the first
+// columns, Q and K are there, 26 100 into the columns, 11 300 into N, F and H, 3500 into the rows' sums, 2700 into the last products and 5700 into results.  The accumulators take a compute unit's registers, one
+// workgroup each, which does nothing while it waits.  T=1000, 32 ragged sequences of 8 heads: 465-482 us, 946 MB read, 150 written.  Slower: 16 wavefronts of half the columns' work (509 us).  Workgroups that stay for chunk after chunk and
+// ask for the next one's columns took 446 there, but 35 us where the short ones of T=333, 55 sequences and heads of 50 x 71 float32 take 29.
 template <typename AT, int DK, bool NARROW>
 __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;

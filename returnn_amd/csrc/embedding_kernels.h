@@ -19,7 +19,7 @@ struct EmbeddingArgs {
   unsigned *order, *token_of;  // [rows]: rows in the order of their tokens, and these tokens
 };
 
-// Eight elements of a row per thread; those of a row's end one by one.
+// Eight elements of a row per thread; those of a row's end one by one.  Bound by memory: the largest measured call moves 99 MB in 18-20 us, 5.2 TB/s; few rows by a launch (2.2 us).
 template <typename AT>
 __global__ __launch_bounds__(256) void k_embedding(EmbeddingArgs a) {
   const long long groups = (a.D + 7) / 8, item = blockIdx.x * 256ll + threadIdx.x;
@@ -72,7 +72,8 @@ __device__ __forceinline__ void embedding_fill(const EmbeddingArgs& a, unsigned 
   }
 }
 
-// Where a row comes: after all of lower tokens and the earlier ones of the same, counted.  16 rows per workgroup, each against a 64th of all by 64 threads.
+// Where a row comes: after all of lower tokens and the earlier ones of the same, counted.  16 rows per workgroup, each against a 64th of all by 64 threads.  One launch in place of four for two digits:
+// 1000, 4096 and 8192 rows of 512 bf16, forward and gradient, 16, 20 and 32 us, with digits 25, 32 and 37.  Bound by its comparisons, beside which the table's zeros are written.
 constexpr int kCountedRows = 8192;
 __global__ __launch_bounds__(1024) void k_embedding_order(EmbeddingArgs a, unsigned sorting, EmbeddingFill fill) {
   __shared__ alignas(16) unsigned keys[kCountedRows];
@@ -202,6 +203,8 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a, EmbeddingFi
 
 // Sums: up to 64 lanes, of 8 columns each, take `run` rows in the order of their tokens.  A run of one token inside of them is a row of the table; of a run that goes on the sum so far
 // is kept, of one that has begun before the sum of what is here.
+// Pieces, not tokens, share out the work, so that one token of many rows costs no more than others; eight rows are on their way at a time, and no atomics are needed, whose order would change sums.  Bound by memory: the
+// largest measured call moves 75 MB in 16-18 us; few rows by latency (6 us).
 struct EmbeddingSumArgs {
   EmbeddingArgs e;
   float *begun, *rest;  // [pieces][D]

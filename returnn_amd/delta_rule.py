@@ -34,7 +34,7 @@ def gated_delta_rule(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """
     :param query: [T,B,key_heads,dk], time-major, or [B,key_heads,dk] for a single step; float32 or bfloat16, on the GPU; 1 <= dk <= 128; frames may have a pitch
-        (e.g. a slice of a wider projection).  (In a region of ``torch.autocast`` float16 is taken as float32.)
+        (e.g. a slice of a wider projection), of all sequences together up to 64 MiB.  (In a region of ``torch.autocast`` float16 is taken as float32.)
     :param key: like ``query``, of length 1 at most: of longer ones (with ``beta`` near 1) the state grows without bounds
     :param value: [T,B,heads,dv] or [B,heads,dv] of the same type; ``heads`` is a multiple of ``key_heads``, neighbouring heads share queries and keys
     :param log_decay: [T,B,heads] or [B,heads], at most 0, taken as float32; minus infinity forgets all that was before

@@ -41,6 +41,7 @@ const char* rtn_model_ops_last_error(void);
  *        direction -1: from each sequence's last frame to its first.
  * y      [T,B,heads,dv] in the type of q, k and v; sN [B,heads,dk,dv] float32, the state behind the last frame visited
  * saved  what the gradient wants to know (rtn_delta_rule_saved_bytes), or NULL
+ * A number that is not finite in a frame that there is spoils the outputs of its head from its chunk of 64 frames (float32: 32) on, not from its own frame on.
  */
 size_t rtn_delta_rule_fwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype, int32_t keep);
 size_t rtn_delta_rule_saved_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype);

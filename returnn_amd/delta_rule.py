@@ -45,7 +45,8 @@ def gated_delta_rule(
         the state as it is.
     :param direction: +1, or -1 to go from each sequence's last frame to its first
     :return: output like ``value``, state [B,heads,dk,dv] after the last frame visited, float32.
-        Both differentiable (once) with respect to all inputs but the lengths.
+        Both differentiable (once) with respect to all inputs but the lengths.  A number that is not finite spoils the outputs of its head from the 64 frames (float32: 32)
+        that are computed with it on, not from its own frame on.
     """
     return native().gated_delta_rule(query, key, value, log_decay, beta, scale, state, seq_lens, direction)
 

@@ -188,3 +188,6 @@ def test_module_and_refusals():
     with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
         embed(tokens, torch.autograd.forward_ad.make_dual(w, w))
     assert embed(tokens[0], w).shape == (6,) and embed(tokens[:0], w).shape == (0, 6)
+    leaf = w.clone().requires_grad_()
+    embed(tokens[0], leaf, scale=2.0).sum().backward()  # (one token by itself)
+    assert leaf.grad[3].eq(2.0).all() and int(leaf.grad.count_nonzero()) == 6

@@ -10,6 +10,8 @@ import torch
 from _gpu_util import announce
 from returnn_amd import language_model
 from returnn_amd.beam_search import beam_select, reorder_states
+from returnn_amd.delta_rule import gated_delta_rule
+from returnn_amd.embedding import embed
 from returnn_amd.language_model import RecurrentLanguageModel
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +174,59 @@ def test_the_program_runs(capsys):
     announce("model path program")
     assert language_model.main(["--layer", "delta", "--steps", "3"]) == 0
     assert "nats per token" in capsys.readouterr().out
+
+
+def test_views_that_are_to_be_negated():
+    """The imaginary part of a conjugated tensor is a view whose numbers lie in memory with the other sign."""
+    announce("model path negated views")
+    gen = torch.Generator(device=DEV).manual_seed(7)
+
+    def negated(*shape):
+        v = torch.view_as_complex(torch.randn(shape + (2,), device=DEV, generator=gen)).conj().imag
+        assert v.is_neg()
+        return v, v.resolve_neg().contiguous()
+
+    for T in (5, 40):
+        (q, q1), (v, v1) = negated(T, 2, 1, 8), negated(T, 2, 1, 8)
+        k = torch.nn.functional.normalize(torch.randn((T, 2, 1, 8), device=DEV, generator=gen), dim=-1)
+        g, b = -torch.rand((T, 2, 1), device=DEV, generator=gen), torch.rand((T, 2, 1), device=DEV, generator=gen)
+        assert all(torch.equal(x, y) for x, y in zip(gated_delta_rule(q, k, v, g, b), gated_delta_rule(q1, k, v1, g, b)))
+    (w, w1), tokens = negated(9, 6), torch.tensor([2, 8, -1], device=DEV)
+    assert torch.equal(embed(tokens, w), embed(tokens, w1))
+    (scores, scores1), (totals, totals1) = negated(2, 3, 50), negated(2, 3)
+    a, b = beam_select(scores, totals, 4), beam_select(scores1, totals1, 4)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    state = torch.view_as_complex(torch.randn((2, 3, 5, 2), device=DEV, generator=gen)).conj()
+    for s in (state, state.imag, scores):
+        (r,) = reorder_states([s], a.sources)
+        assert torch.equal(r, s[torch.arange(2, device=DEV)[:, None], a.sources])
+
+
+def test_calls_side_by_side():
+    """Two streams with the same calls on other numbers, each with workspaces of its own."""
+    announce("model path two streams")
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    jobs = []
+    for _ in range(2):
+        q, k, v = (torch.nn.functional.normalize(torch.randn((700, 2, 2, 32), device=DEV, generator=gen), dim=-1) for _ in "qkv")
+        g, b = -torch.rand((700, 2, 2), device=DEV, generator=gen), torch.rand((700, 2, 2), device=DEV, generator=gen)
+        jobs.append((q, k, v, g, b, torch.randint(0, 900, (10000,), device=DEV, generator=gen), torch.randn((900, 33), device=DEV, generator=gen),
+                     torch.randn((10000, 33), device=DEV, generator=gen), torch.randn((3, 40, 9000), device=DEV, generator=gen), torch.randn((3, 40), device=DEV, generator=gen)))  # fmt: skip
+
+    def run(q, k, v, g, b, tokens, w, dy, scores, totals):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, g, b, w)]
+        y, s = gated_delta_rule(*leaves[:5])
+        x = embed(tokens, leaves[5])
+        step = beam_select(scores, totals, 64)
+        return (y, s, x) + torch.autograd.grad((y, s, x), leaves, (v, s.detach(), dy)) + tuple(step) + tuple(reorder_states([totals], step.sources))
+
+    want = [run(*j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for stream, j in zip(streams, jobs):
+            with torch.cuda.stream(stream):
+                got.append(run(*j))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, r in zip(want, got) for a, b in zip(w, r))

@@ -1116,7 +1116,9 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     Square square;
   } lds;
   __shared__ alignas(16) float powers[5][C];  // c, gamma, beta, G in two parts
-  __shared__ float dots[3][W][C], rv[C], sums[3][M][C], ds_of[W];  // sums of 16 columns of N and of X o L, of 16 rows of N
+  __shared__ alignas(16) float dots[3][W][C];
+  __shared__ float rv[C], ds_of[W];
+  __shared__ alignas(16) float sums[3][M][C];  // sums of 16 columns of N and of X o L, of 16 rows of N
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, i16 = lane & 15;
   const int chunk = blockIdx.x % a.chunks, bh = blockIdx.x / a.chunks;
   const DeltaWhere at(a.f, bh, chunk, C);
@@ -1249,6 +1251,21 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     pass(passed[0], c0);
     if (c0 + 32 < width) pass(passed[1], c0 + 32);
   }
+  // P and L, all of a lane's at once, before the rows' sums
+  unsigned short of_P[kEach][4][3];
+  float of_L[kEach][4];
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int tile = kTiles % W == 0 || n * W + wave < kTiles ? n * W + wave : 0, block = tile >> 2, m = tile_m(tile), o = tile_o(tile);
+    const int j = (i16 >> 2) * 8 + (o & 1) * 4 + (i16 & 3);  // (row and column of the block)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const char* image = (const char*)record + 3 * BLOCKS * 2048 + DeltaTile<3, BLOCKS * 32, 32>::offset(block * 32 + (m & 1) * 16 + q4 * 4 + r, j);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) of_P[n][r][k] = *(const unsigned short*)(image + k * BLOCKS * 2048);
+      of_L[n][r] = rL[block * 1024 + (q4 * 8 + (m & 1) * 4 + r) * 32 + j];
+    }
+  }
 #pragma unroll
   for (int n = 0; n < kTasks; ++n) {
     const int first = n * THREADS + wave * 64, item = first + lane;
@@ -1259,6 +1276,19 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
       if ((item & 3) == 0) rv[item >> 2] = v;
     }
   }
+  // dots of rows, and factors
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const delta_f32x4 qv = Q.of_result(m * 16, wave * 16), kv = K.of_result(m * 16, wave * 16);
+    const int first = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4;
+    delta_f32x4 x = qv * YS[m], y = kv * RS[m], z = kv * UD[m];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = delta_sum16(x[r]), y[r] = delta_sum16(y[r]), z[r] = delta_sum16(z[r]);
+    if (i16 == 0) *(delta_f32x4*)&dots[0][wave][first] = x, *(delta_f32x4*)&dots[1][wave][first] = y, *(delta_f32x4*)&dots[2][wave][first] = z;
+    const delta_f32x4 c = delta_rows(powers[0], m), gamma = delta_rows(powers[1], m), beta = delta_rows(powers[2], m);
+    YS[m] *= a.f.scale * c;
+    UD[m] = gamma * UD[m] - beta * c * RS[m];
+  }
 #pragma unroll
   for (int n = 0; n < kEach; ++n) {
     const int tile = n * W + wave, block = tile >> 2;
@@ -1266,19 +1296,19 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
       const int m = tile_m(tile), o = tile_o(tile);
       const int j = (o >> 1) * 32 + (i16 >> 2) * 8 + (o & 1) * 4 + (i16 & 3);
       float column = 0.f;
+      delta_f32x4 row, with_l;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4 + r, place = block * 32 + (m & 1) * 16 + q4 * 4 + r;
-        const char* image = (const char*)record + 3 * BLOCKS * 2048 + DeltaTile<3, BLOCKS * 32, 32>::offset(place, j & 31);
         float p = 0.f;
 #pragma unroll
-        for (int k = 2; k >= 0; --k) p += (float)*(const __bf16*)(image + k * BLOCKS * 2048);
-        const float l = rL[block * 1024 + (i & 31) * 32 + (j & 31)];
-        const float x = i > j ? X[n][r] : 0.f, z = i >= j ? a.f.scale * Z[n][r] : 0.f;
-        const float e = i >= j ? expf((powers[3][i] - powers[3][j]) + (powers[4][i] - powers[4][j])) : 0.f, beta = powers[2][i];
-        const float both = z * p - x * (beta * l), row = delta_sum16(both), with_l = delta_sum16(x * l);
+        for (int k = 2; k >= 0; --k) p += __builtin_bit_cast(float, (unsigned)of_P[n][r][k] << 16);
+        const float l = of_L[n][r], beta = powers[2][i];
+        const float power = expf(i >= j ? (powers[3][i] - powers[3][j]) + (powers[4][i] - powers[4][j]) : 0.f);  // (not on a condition, which would be a way of its own for each)
+        const float x = i > j ? X[n][r] : 0.f, z = i >= j ? a.f.scale * Z[n][r] : 0.f, e = i >= j ? power : 0.f;
+        const float both = z * p - x * (beta * l);
         column += both;
-        if (i16 == 0) sums[0][o][i] = row, sums[1][o][i] = with_l;
+        row[r] = delta_sum16(both), with_l[r] = delta_sum16(x * l);
         float f = z * e, h = -(x * beta * e);
         const int to = DeltaTile<OUT, BLOCKS * 32, 32>::offset(place, j & 31);
 #pragma unroll
@@ -1289,6 +1319,8 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
           f -= (float)fp, h -= (float)hp;
         }
       }
+      const int first = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4;
+      if (i16 == 0) *(delta_f32x4*)&sums[0][o][first] = row, *(delta_f32x4*)&sums[1][o][first] = with_l;
       column += __shfl_xor(column, 16);
       column += __shfl_xor(column, 32);
       if (q4 == 0) sums[2][m][j] = column;
@@ -1298,20 +1330,6 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   ds += __shfl_xor(ds, 16);
   ds += __shfl_xor(ds, 32);
   if (lane == 0) ds_of[wave] = ds;
-  // dots of rows, and factors
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    const delta_f32x4 qv = Q.of_result(m * 16, wave * 16), kv = K.of_result(m * 16, wave * 16);
-    const int first = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float x = delta_sum16(qv[r] * YS[m][r]), y = delta_sum16(kv[r] * RS[m][r]), z = delta_sum16(kv[r] * UD[m][r]);
-      if (i16 == 0) dots[0][wave][first + r] = x, dots[1][wave][first + r] = y, dots[2][wave][first + r] = z;
-    }
-    const delta_f32x4 c = delta_rows(powers[0], m), gamma = delta_rows(powers[1], m), beta = delta_rows(powers[2], m);
-    YS[m] *= a.f.scale * c;
-    UD[m] = gamma * UD[m] - beta * c * RS[m];
-  }
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < NB; ++b) {

@@ -1148,7 +1148,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   struct Passed {
     delta_f32x8 s, d, f[kTasks];
     Eight8 x[kTasks];
-  } passed[2];
+  } passed[1];
   auto load = [&](Passed& p, int c0) {
     const unsigned state = (unsigned)(my_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
     p.s = delta_load8_any<NARROW>((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
@@ -1165,7 +1165,6 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     }
   };
   load(passed[0], 0);
-  load(passed[1], 32 < width ? 32 : 0);
   {
     const int col = threadIdx.x % (DK / 8) * 8;
     for (int row = threadIdx.x / (DK / 8); row < C; row += kApart) {
@@ -1221,36 +1220,36 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     for (int j = 0; j < 8; ++j) ds = __builtin_fmaf(s[j], d[j], ds);
     delta_parts(s, sp);
     delta_parts(d, dp);
-    load(now, c0 + 64 < width ? c0 + 64 : c0);  // (what is loaded on a condition is waited for)
+    load(now, c0 + 32 < width ? c0 + 32 : c0);  // (what is loaded on a condition is waited for)
     __syncthreads();
+    // (the operands of a step are read during the one before it)
+    delta_bf16x8 of_Y[2][NI], of_U[2][3], of_R[2][3];
+    auto fetch = [&](int step) {
+      const int tile = (step - M) * W + wave, at = step & 1, some = kTiles % W == 0 || tile < kTiles ? tile : 0;
+      const int m = step < M ? step : tile_m(some), o = step < M ? step : tile_o(some);
+      lds.pass.Y.left(m * 16, 0, of_Y[at]);
+      lds.pass.U.left(o * 16, 0, of_U[at]);
+      lds.pass.R.left(m * 16, 0, of_R[at]);
+    };
+    fetch(0);
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      delta_bf16x8 left[3], some[NI];
-      lds.pass.Y.left(m * 16, 0, some);
-      YS[m] = delta_mma<3>(some, sp, YS[m]);
-      lds.pass.U.left(m * 16, 0, left);
-      UD[m] = delta_mma<3>(left, dp, UD[m]);
-      lds.pass.R.left(m * 16, 0, left);
-      RS[m] = delta_mma<3>(left, sp, RS[m]);
-    }
-#pragma unroll
-    for (int n = 0; n < kEach; ++n) {
-      const int tile = n * W + wave;
-      if (kTiles % W == 0 || tile < kTiles) {
-        delta_bf16x8 left[3], some[NI], right[3];
-        lds.pass.U.left(tile_o(tile) * 16, 0, right);
-        lds.pass.R.left(tile_m(tile) * 16, 0, left);
-        X[n] = delta_mma<3>(left, right, X[n]);
-        lds.pass.Y.left(tile_m(tile) * 16, 0, some);
-        Z[n] = delta_mma<3>(some, right, Z[n]);
+    for (int step = 0; step < M + kEach; ++step) {
+      const int at = step & 1;
+      if (step + 1 < M + kEach) fetch(step + 1);
+      delta_ahead();
+      if (step < M) {
+        YS[step % M] = delta_mma<3>(of_Y[at], sp, YS[step % M]);
+        UD[step % M] = delta_mma<3>(of_U[at], dp, UD[step % M]);
+        RS[step % M] = delta_mma<3>(of_R[at], sp, RS[step % M]);
+      } else if (kTiles % W == 0 || (step - M) * W + wave < kTiles) {
+        const int n = (step + kEach - M) % kEach;
+        X[n] = delta_mma<3>(of_R[at], of_U[at], X[n]);
+        Z[n] = delta_mma<3>(of_Y[at], of_U[at], Z[n]);
       }
     }
     __syncthreads();
   };
-  for (int c0 = 0; c0 < width; c0 += 64) {
-    pass(passed[0], c0);
-    if (c0 + 32 < width) pass(passed[1], c0 + 32);
-  }
+  for (int c0 = 0; c0 < width; c0 += 32) pass(passed[0], c0);
   // P and L, all of a lane's at once, before the rows' sums
   unsigned short of_P[kEach][4][3];
   float of_L[kEach][4];

@@ -1112,7 +1112,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   };
   __shared__ DeltaTile<NI, C, DK> K, Q;
   __shared__ union Shared {
-    Passing pass;
+    Passing pass[2];
     Square square;
   } lds;
   __shared__ alignas(16) float powers[5][C];  // c, gamma, beta, G in two parts
@@ -1144,27 +1144,30 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   const float *record = a.records + number * delta_record(C), *rL = record + delta_image(C);
   const int width = a.f.dv;
   const int my_row = wave * 16 + i16;  // of S and D
-  // What passes by, from column c0 on.
-  struct Passed {
-    delta_f32x8 s, d, f[kTasks];
-    Eight8 x[kTasks];
-  } passed[1];
-  auto load = [&](Passed& p, int c0) {
+  // What passes by, from column c0 on, asked for a pass ahead.
+  delta_f32x8 s, d, f[kTasks];
+  Eight8 x[kTasks];
+  auto load_states = [&](int c0) {
+    c0 = c0 < width ? c0 : 0;  // (what is loaded on a condition is waited for)
     const unsigned state = (unsigned)(my_row * width + delta_read_col(c0 + q4 * 8, width)) * 4u;
-    p.s = delta_load8_any<NARROW>((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
-    p.d = delta_load8_any<NARROW>((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
+    s = delta_load8_any<NARROW>((const float*)((const char*)(a.states + number * matrix) + state), c0 + q4 * 8, width);
+    d = delta_load8_any<NARROW>((const float*)((const char*)(a.dstates + number * matrix) + state), c0 + q4 * 8, width);
+  };
+  auto load_frames = [&](int c0) {
+    c0 = c0 < width ? c0 : 0;
 #pragma unroll
     for (int n = 0; n < kTasks; ++n) {
       const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, col = c0 + (item & 3) * 8;
       if (first < 2 * kItems) {
-        p.f[n] = delta_load8_any<NARROW>((which ? a.writes : a.dwrites) + number * C * width + (row * width + delta_read_col(col, width)), col, width);
+        f[n] = delta_load8_any<NARROW>((which ? a.writes : a.dwrites) + number * C * width + (row * width + delta_read_col(col, width)), col, width);
         const AT* tensor = (const AT*)(which ? a.dy : a.f.v);
         const long long ld = which ? a.lddy : a.f.ldv;
-        p.x[n] = delta_load8_any<NARROW>(tensor + (at.row(row < at.count ? row : at.count - 1) * ld + (long long)at.h * width + delta_read_col(col, width)), col, width);
+        x[n] = delta_load8_any<NARROW>(tensor + (at.row(row < at.count ? row : at.count - 1) * ld + (long long)at.h * width + delta_read_col(col, width)), col, width);
       }
     }
   };
-  load(passed[0], 0);
+  load_frames(0);
+  load_states(0);
   {
     const int col = threadIdx.x % (DK / 8) * 8;
     for (int row = threadIdx.x / (DK / 8); row < C; row += kApart) {
@@ -1187,49 +1190,52 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   float ds = 0.f, own_rv[kTasks] = {};
   auto tile_m = [](int tile) { return (tile >> 2 > 0) * 2 + (tile >> 1 & 1); };
   auto tile_o = [](int tile) { return (tile >> 2 > 1) * 2 + (tile & 1); };
-  auto pass = [&](Passed& now, int c0) {
-    delta_f32x8 s = now.s, d = now.d;
+  auto put_frames = [&](int c0, Passing& to) {
     const bool whole = c0 + 32 <= width && at.count == C;
-    if (!whole) {
-      s = delta_placed<NARROW>(s, c0 + q4 * 8, width, true);
-      d = delta_placed<NARROW>(d, c0 + q4 * 8, width, true);
-    }
 #pragma unroll
     for (int n = 0; n < kTasks; ++n) {
       const int first = n * THREADS + wave * 64, which = first >= kItems, item = first + lane - which * kItems, row = item >> 2, c8 = (item & 3) * 8;
       if (first < 2 * kItems) {
         if (!whole) {
-          now.f[n] = delta_placed<NARROW>(now.f[n], c0 + c8, width, true);
-          now.x[n] = delta_placed<NARROW>(now.x[n], c0 + c8, width, row < at.count);
+          f[n] = delta_placed<NARROW>(f[n], c0 + c8, width, true);
+          x[n] = delta_placed<NARROW>(x[n], c0 + c8, width, row < at.count);
         }
         delta_bf16x8 parts[3], some[NI];
-        delta_parts(now.f[n], parts);
-        (which ? lds.pass.U : lds.pass.R).put(delta_place(row), c8, parts);
+        delta_parts(f[n], parts);
+        (which ? to.U : to.R).put(delta_place(row), c8, parts);
         if (which) {
-          delta_parts(now.x[n], some);
-          lds.pass.Y.put(delta_place(row), c8, some);
+          delta_parts(x[n], some);
+          to.Y.put(delta_place(row), c8, some);
         } else {
-          const delta_f32x8 v = delta_wide(now.x[n]);
+          const delta_f32x8 v = delta_wide(x[n]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(now.f[n][j], v[j], own_rv[n]);
+          for (int j = 0; j < 8; ++j) own_rv[n] = __builtin_fmaf(f[n][j], v[j], own_rv[n]);
         }
       }
     }
-    delta_bf16x8 sp[3], dp[3];
+    load_frames(c0 + 32);
+  };
+  delta_bf16x8 sp[3], dp[3];
+  auto take_states = [&](int c0) {
+    if (c0 + 32 > width) {
+      s = delta_placed<NARROW>(s, c0 + q4 * 8, width, true);
+      d = delta_placed<NARROW>(d, c0 + q4 * 8, width, true);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) ds = __builtin_fmaf(s[j], d[j], ds);
     delta_parts(s, sp);
     delta_parts(d, dp);
-    load(now, c0 + 32 < width ? c0 + 32 : c0);  // (what is loaded on a condition is waited for)
-    __syncthreads();
+    load_states(c0 + 32);
+  };
+  auto products = [&](const Passing& of) {
     // (the operands of a step are read during the one before it)
     delta_bf16x8 of_Y[2][NI], of_U[2][3], of_R[2][3];
     auto fetch = [&](int step) {
       const int tile = (step - M) * W + wave, at = step & 1, some = kTiles % W == 0 || tile < kTiles ? tile : 0;
       const int m = step < M ? step : tile_m(some), o = step < M ? step : tile_o(some);
-      lds.pass.Y.left(m * 16, 0, of_Y[at]);
-      lds.pass.U.left(o * 16, 0, of_U[at]);
-      lds.pass.R.left(m * 16, 0, of_R[at]);
+      of.Y.left(m * 16, 0, of_Y[at]);
+      of.U.left(o * 16, 0, of_U[at]);
+      of.R.left(m * 16, 0, of_R[at]);
     };
     fetch(0);
 #pragma unroll
@@ -1247,9 +1253,19 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
         Z[n] = delta_mma<3>(of_Y[at], of_U[at], Z[n]);
       }
     }
-    __syncthreads();
   };
-  for (int c0 = 0; c0 < width; c0 += 32) pass(passed[0], c0);
+  put_frames(0, lds.pass[0]);
+  take_states(0);
+  __syncthreads();
+  int now = 0;
+  for (int c0 = 32; c0 < width; c0 += 32, now ^= 1) {
+    put_frames(c0, lds.pass[now ^ 1]);
+    products(lds.pass[now]);
+    take_states(c0);
+    __syncthreads();
+  }
+  products(lds.pass[now]);
+  __syncthreads();
   // P and L, all of a lane's at once, before the rows' sums
   unsigned short of_P[kEach][4][3];
   float of_L[kEach][4];

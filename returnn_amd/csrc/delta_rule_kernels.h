@@ -1092,10 +1092,11 @@ __device__ __forceinline__ float delta_sum16(float v) {
 
 // One chunk of one head per workgroup, DK / 16 wavefronts with 16 columns of dQ and dK each.  The values' columns pass by 32 at a time, the next ones on their way meanwhile.
 // NARROW: values of fewer than eight columns.
-// Of 64 500 clocks of a chunk (keys and values of 128 in bf16) 15 300 go until the first
-// columns, Q and K are there, 26 100 into the columns, 11 300 into N, F and H, 3500 into the rows' sums, 2700 into the last products and 5700 into results.  The accumulators take a compute unit's registers, one
-// workgroup each, which does nothing while it waits.  T=1000, 32 ragged sequences of 8 heads: 465-482 us, 946 MB read, 150 written.  Slower: 16 wavefronts of half the columns' work (509 us).  Workgroups that stay for chunk after chunk and
-// ask for the next one's columns took 446 there, but 35 us where the short ones of T=333, 55 sequences and heads of 50 x 71 float32 take 29.
+// Columns go into one half of LDS while products are made of the other, the operands of a product are read during the one before it, and what is chosen by an element is computed without ways of its own.  Of 48 800 clocks
+// of a chunk (keys and values of 128 in bf16) 14 000 go until the first columns, Q and K are there, 19 300 into the columns, 8500 into the rows' sums, N, F and H, 3000 into the last products and 4000 into results.  The
+// accumulators take a compute unit's registers, one workgroup each, which does nothing else while it waits.  T=1000, 32 ragged sequences of 8 heads: 381-410 us, 946 MB read, 150 written (482 with one half, each operand read
+// when it was wanted, and a way of its own for each element of P).  Slower: 16 wavefronts of half the columns' work, 509 for 480; the frames' and states' numbers kept in the order in which they are read, which costs the
+// kernels that write them 25 us and does not help this one; a compute unit's next chunk's columns asked for during its last products, 446 for 480, but 35 for 29 where chunks are few.
 template <typename AT, int DK, bool NARROW>
 __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;
@@ -1369,21 +1370,31 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     }
   }
   const int col = wave * 16 + i16;
+  if (each) {
+    if (col < a.f.dk)
 #pragma unroll
-  for (int m = 0; m < M; ++m)
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4 + r;
-      if (i < at.count && col < a.f.dk) {
-        const long long to = (at.row(i) * a.f.heads + at.h) * a.f.dk + col;
-        if (each) {
-          a.dq_each[to] = YS[m][r], a.dk_each[to] = UD[m][r];
-        } else {
-          store_f32(dq + to, YS[m][r]);
-          store_f32(dk + to, UD[m][r]);
+        for (int r = 0; r < 4; ++r) {
+          const int i = (m >> 1) * 32 + q4 * 8 + (m & 1) * 4 + r;
+          const long long to = (at.row(i) * a.f.heads + at.h) * a.f.dk + col;
+          if (at.count == C || i < at.count) a.dq_each[to] = YS[m][r], a.dk_each[to] = UD[m][r];
         }
-      }
-    }
+  } else {
+    const DeltaFrames<AT, 24> to_q(a.f, dq, at, (long long)a.f.heads * a.f.dk, (long long)at.h * a.f.dk), to_k(a.f, dk, at, (long long)a.f.heads * a.f.dk, (long long)at.h * a.f.dk);
+    const unsigned to = to_q.lane(q4 * 8, col);
+    if (col < a.f.dk)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = (m >> 1) * 32 + (m & 1) * 4 + r;
+          if (at.count == C || i + q4 * 8 < at.count) {
+            store_f32((AT*)(to_q.at(i) + to), YS[m][r]);
+            store_f32((AT*)(to_k.at(i) + to), UD[m][r]);
+          }
+        }
+  }
   if (wave == 0) {
     const int i = lane < C ? lane : 0, block = i >> 5;
     float x = 0.f, y = 0.f, z = 0.f, all = 0.f, row = 0.f, with_l = 0.f, column = 0.f;

@@ -353,3 +353,27 @@ def test_layer(dtype):
     if dtype == torch.float32:
         with torch.autocast("cuda", dtype=torch.bfloat16):
             assert m(x)[0].dtype == torch.bfloat16
+
+
+def test_offsets_beyond_32_bits():
+    """States of more than 2^32 bytes kept for the gradient: a long call against its two halves, the state handed on."""
+    announce("delta rule, long")
+    T, half, B, H, d = 70000, 35008, 8, 8, 128
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    q, k = (torch.nn.functional.normalize(torch.randn((T, B, H, d), device=DEV, generator=gen, dtype=torch.bfloat16), dim=-1) for _ in "qk")
+    v, dy = (torch.randn((T, B, H, d), device=DEV, generator=gen, dtype=torch.bfloat16) for _ in "ve")
+    g, b = -torch.rand((T, B, H), device=DEV, generator=gen) * 0.1, torch.rand((T, B, H), device=DEV, generator=gen)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, b)]
+    y, s = gated_delta_rule(*leaves)
+    whole = torch.autograd.grad(y, leaves, dy)
+    state, parts = None, []
+    for part in (slice(0, half), slice(half, T)):
+        y1, state = gated_delta_rule(*(t[part] for t in leaves), state=state)
+        parts.append(y1)
+    chained = torch.autograd.grad(parts, leaves, [dy[:half], dy[half:]])
+    assert (s - state).detach().norm() <= 1e-5 * s.detach().norm()
+    # (two roundings to bfloat16 of numbers that agree to 1e-5)
+    for a, c in [(y.detach(), torch.cat(parts).detach())] + list(zip(whole, chained)):
+        for at in (slice(0, 2000), slice(half - 1000, half + 1000), slice(T - 2000, T)):
+            x, z = a[at].float(), c[at].float()
+            assert torch.isfinite(x).all() and (x - z).norm() <= (2.0**-7 if a.dtype == torch.bfloat16 else 1e-4) * x.norm()

@@ -27,7 +27,8 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float delta_f32x4;
 typedef delta_f32x4 __attribute__((aligned(4))) delta_f32x4_any;
 
 // Frame by frame: 64 columns of a head's state per workgroup, each thread 4 columns of R of the 16 R rows in registers.  What a state gives to a key and to a query is one
-// pass over it: S_t^T q = a S_{t-1}^T q + (k.q) u.  A single frame is bound by a launch and the state's way in and out (12 sequences of 8 heads of 128 x 128: 7 us for 12.6 MB; 64: 14.3, 4.7 TB/s);
+// pass over it: S_t^T q = a S_{t-1}^T q + (k.q) u.  A single frame is bound by a launch and the state's way in and out (12 sequences of 8 heads of 128 x 128: 5.9 us for 12.6 MB; 64: 11.7, 5.7 TB/s; 7.1 and
+// 14.3 where a row was loaded on a lane's condition);
 // further ones by the sums' way through shuffles and LDS, 1.3 us each (2.2 where a frame's numbers were asked for when they were needed).
 template <typename AT, int R>
 __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
@@ -38,20 +39,6 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
   const long long n = frames_of(a.lens, b, a.T);
   const long long matrix = ((long long)b * a.heads + h) * a.dk * a.dv;
   const bool whole = col + 4 <= a.dv;
-  float S[R][4];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const long long at = matrix + (long long)(row + i) * a.dv + col;
-    const bool in = a.s0 && row + i < a.dk;
-    if (in && whole) {
-      const delta_f32x4 w = *(const delta_f32x4_any*)(a.s0 + at);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) S[i][c] = w[c];
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) S[i][c] = in && col + c < a.dv ? a.s0[at + c] : 0.f;
-    }
-  }
   // A frame's numbers, asked for a frame ahead.  (What is not there is read at the end of what is, and taken as 0: what is loaded on a condition of a lane is waited for at once.)
   struct Frame {
     AT k[R], q[R], v[4];
@@ -71,6 +58,21 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
     next.g = a.g[frame * a.heads + h], next.beta = a.beta[frame * a.heads + h], next.at = frame;
   };
   if (n) load(0);
+  float S[R][4] = {};
+  if (a.s0 && a.dv % 4 == 0) {
+    delta_f32x4 w[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) w[i] = *(const delta_f32x4_any*)(a.s0 + (matrix + (long long)(row + i < a.dk ? row + i : a.dk - 1) * a.dv + (whole ? col : 0)));
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) S[i][c] = row + i < a.dk ? w[i][c] : 0.f;
+  } else if (a.s0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) S[i][c] = row + i < a.dk && col + c < a.dv ? a.s0[matrix + (long long)(row + i) * a.dv + col + c] : 0.f;
+  }
   for (long long p = 0; p < n; ++p) {
     float k[R], q[R], v[4];
 #pragma unroll

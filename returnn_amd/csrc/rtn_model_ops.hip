@@ -26,8 +26,8 @@ bool nothing(const DeltaSizes& z) { return z.B == 0 || z.heads == 0; }
 bool valid(const DeltaSizes& z) {
   return z.T >= 0 && z.T <= kMaxFrames && z.B >= 0 && z.key_heads >= 0 && z.heads >= 0 && z.dk >= 1 && z.dk <= kMaxKeyDim && z.dv >= 1 && z.dv <= kMaxValueDim && known(z.dtype);
 }
-// Calls of at most these frames that no gradient follows go frame by frame.  (12 sequences of 8 heads of 128 x 128 in bf16, frame by frame and in chunks: 1 frame 7.1 and 33 us, 16 frames 26.7 and
-// 31.5, 24 frames 37 and 32; of one sequence 25 and 28.5, 35 and 29; of 64 54 and 66, 76 and 69.)
+// Calls of at most these frames that no gradient follows go frame by frame.  (12 sequences of 8 heads of 128 x 128 in bf16, frame by frame and in chunks: 1 frame 5.9 and 33 us, 16 frames 24.8 and
+// 31.5, 24 frames 35 and 31; 16 frames of one sequence 23.7 and 28.5, of 64 51 and 66.)
 constexpr int kStepFrames = 16;
 int delta_frames(const DeltaSizes& z) { return z.dtype == RTN_DTYPE_BF16 ? DeltaChunk<__bf16>::kFrames : DeltaChunk<float>::kFrames; }
 int64_t delta_chunks(const DeltaSizes& z) { return (z.T + delta_frames(z) - 1) / delta_frames(z); }

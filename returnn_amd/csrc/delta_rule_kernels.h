@@ -145,7 +145,8 @@ __global__ __launch_bounds__(256) void k_delta_steps(DeltaArgs a) {
 // k_delta_chunks leaves T, P, L and the powers of every chunk, all chunks side by side; k_delta_forward goes through the chunks of a head.
 //
 // Matrix instructions take bfloat16 and add in float32.  A float32 number goes in as up to three bfloat16 whose sum it is (8 bits of it each), a product of two of them as
-// those products of parts that count: with all whose order is below 3, 2^-24 of it is lost.
+// those products of parts that count: with all whose order is below 3, 2^-24 of it is lost.  So too where the result is rounded to bfloat16 in the end: what it is the sum of (S and U, of which a write may take
+// away what the state holds) can be a thousand times as large, and with two parts 2^-17 of that would be lost.
 //
 // Where a matrix of 32 rows comes out of 16 x 16 tiles and goes into the next product as its right operand, nothing is moved: lane (quarter q, i) has column i
 // and, of tile t, rows 4 q + r; the operand wants rows 8 q + 0..7 of it.  So tile t is made of rows 8 q + 4 t + r, which its left operand's lane i = 4 q + r reads.  Left operands lie in LDS
@@ -158,11 +159,11 @@ template <typename AT>
 struct DeltaChunk;
 template <>
 struct DeltaChunk<__bf16> {
-  static constexpr int kFrames = 64, kInput = 1, kOut = 2;  // frames; parts of an input, and order up to which products count that end in a result of the input's type
+  static constexpr int kFrames = 64, kInput = 1;  // frames; parts of an input
 };
 template <>
 struct DeltaChunk<float> {
-  static constexpr int kFrames = 32, kInput = 3, kOut = 3;  // (K and Q in three parts: 32 frames are what fits into LDS)
+  static constexpr int kFrames = 32, kInput = 3;  // (K and Q in three parts: 32 frames are what fits into LDS)
 };
 constexpr int delta_blocks(int frames) { return frames == 64 ? 3 : 1; }  // of 32 x 32, of a lower triangular matrix
 // What is kept of a chunk, in numbers of float32: T and P in three parts each, as they lie in LDS (DeltaTile, blocks (0,0), (1,0), (1,1)); L, block by block, row-major; c, gamma, beta,
@@ -220,10 +221,10 @@ __device__ __forceinline__ void delta_parts(delta_f32x4 a, delta_f32x4 b, delta_
   delta_parts(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7), p);
 }
 // c + a b, the smallest products first.
-template <int ORDER, int NA, int NB>
+template <int NA, int NB>
 __device__ __forceinline__ delta_f32x4 delta_mma(const delta_bf16x8 (&a)[NA], const delta_bf16x8 (&b)[NB], delta_f32x4 c) {
 #pragma unroll
-  for (int s = ORDER - 1; s >= 0; --s)
+  for (int s = 2; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i <= s; ++i)
       if (i < NA && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
@@ -231,10 +232,10 @@ __device__ __forceinline__ delta_f32x4 delta_mma(const delta_bf16x8 (&a)[NA], co
 }
 
 // The same for several tiles with one right operand, tile after tile, so that no product waits for the one before it.
-template <int ORDER, int TILES, int NA, int NB>
+template <int TILES, int NA, int NB>
 __device__ __forceinline__ void delta_mma(const delta_bf16x8 (&a)[TILES][NA], const delta_bf16x8 (&b)[NB], delta_f32x4* c) {
 #pragma unroll
-  for (int s = ORDER - 1; s >= 0; --s)
+  for (int s = 2; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i <= s; ++i)
       if (i < NA && s - i < NB) {
@@ -476,8 +477,8 @@ __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(De
       fetch(a.f.k, a.f.ldk, nt * 16 + i16, other);
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
-        kk = delta_mma<3>(kf[b], other[b], kk);
-        qk = delta_mma<3>(qf[b], other[b], qk);
+        kk = delta_mma(kf[b], other[b], kk);
+        qk = delta_mma(qf[b], other[b], qk);
       }
     }
     const int j = nt * 16 + i16, block = wave / 2 + nt / 2;
@@ -726,8 +727,8 @@ enum { kDeltaPlain, kDeltaKeep, kDeltaThrough };
 template <typename AT, int DK, int W, int KIND>
 __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
   constexpr bool KEEP = KIND == kDeltaKeep, THROUGH = KIND == kDeltaThrough;
-  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, KB = DK / 32, BLOCKS = delta_blocks(C);
-  typedef DeltaStage<AT, DK, 64 * W, THROUGH ? 0 : OUT, !THROUGH> Stage;
+  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, KB = DK / 32, BLOCKS = delta_blocks(C);
+  typedef DeltaStage<AT, DK, 64 * W, THROUGH ? 0 : 3, !THROUGH> Stage;
   __shared__ typename Stage::Tiles tiles[2];
   const int values = (a.f.dv + 15) / 16 * 16;
   DeltaStrip<AT, DK, W> strip(a, THROUGH ? values + DK : a.f.dv, 0, THROUGH ? a.segments - 1 : a.segments);
@@ -789,13 +790,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         if (b + 1 < KB) ask(b + 1);
         delta_ahead();
         if (b + 1 < KB) delta_parts(S[2 * b + 2], S[2 * b + 3], p[b + 1 & 1]);
-        delta_mma<3>(k[b & 1], p[b & 1], KS);
-        if constexpr (!THROUGH) delta_mma<OUT>(q[b & 1], p[b & 1], O);
+        delta_mma(k[b & 1], p[b & 1], KS);
+        if constexpr (!THROUGH) delta_mma(q[b & 1], p[b & 1], O);
       }
     }
     {
       // T and P: blocks (0,0), (1,0), (1,1), of two tiles of 16 rows each
-      delta_bf16x8 t[BLOCKS][2][3], p[BLOCKS][2][OUT], right[3], some[OUT];
+      delta_bf16x8 t[BLOCKS][2][3], p[BLOCKS][2][3], right[3], some[3];
       auto ask_t = [&](int n) {
         lds.TP.left(n * 32, 0, t[n][0]);
         lds.TP.left(n * 32 + 16, 0, t[n][1]);
@@ -816,27 +817,27 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
         O[m] *= c;
       }
       delta_parts(R[0], R[1], right);
-      delta_mma<3>(t[0], right, U);
+      delta_mma(t[0], right, U);
       ask_p(0);
       if constexpr (NB == 2) {
         ask_t(2);
         delta_ahead();
-        delta_mma<3>(t[1], right, U + 2);
+        delta_mma(t[1], right, U + 2);
         delta_parts(R[2], R[3], right);
         delta_parts(U[0], U[1], some);
-        delta_mma<3>(t[2], right, U + 2);
+        delta_mma(t[2], right, U + 2);
         ask_p(1);
         ask_p(2);
         delta_ahead();
         if constexpr (!THROUGH) {
-          delta_mma<OUT>(p[0], some, O);
-          delta_mma<OUT>(p[1], some, O + 2);
+          delta_mma(p[0], some, O);
+          delta_mma(p[1], some, O + 2);
           delta_parts(U[2], U[3], some);
-          delta_mma<OUT>(p[2], some, O + 2);
+          delta_mma(p[2], some, O + 2);
         }
       } else if constexpr (!THROUGH) {
         delta_parts(U[0], U[1], some);
-        delta_mma<OUT>(p[0], some, O);
+        delta_mma(p[0], some, O);
       }
     }
     if (KEEP) strip.put(a.writes + strip.number(chunk) * C * a.f.dv, C, U);
@@ -857,7 +858,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
       for (int n = 0; n < 2 * NB; ++n) {
         if (n + 1 < 2 * NB) ask(n + 1);
         delta_ahead();
-        delta_mma<3>(k[n & 1], right[n / 2], S + n % 2 * KB);
+        delta_mma(k[n & 1], right[n / 2], S + n % 2 * KB);
       }
     }
     if constexpr (!THROUGH) {
@@ -939,7 +940,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_join(DeltaChunkArgs a) {
     for (int b = 0; b < KB; ++b) {
 #pragma unroll
       for (int m = 0; m < 3; ++m) p[m] = *(const delta_bf16x8*)state[n & 1][b][m][lane];
-      S = delta_mma<3>(now.A[b], p, S);
+      S = delta_mma(now.A[b], p, S);
     }
     if (has)
 #pragma unroll
@@ -1018,7 +1019,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         lds.K.left(m * 16, b * 32, left);
-        KD[m] = delta_mma<3>(left, d, KD[m]);
+        KD[m] = delta_mma(left, d, KD[m]);
       }
     }
     // dU: rows of block m / 2 from all blocks behind it
@@ -1029,7 +1030,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
 #pragma unroll
       for (int m = 0; m < 2 * b + 2; ++m) {
         lds.TP.template transposed<3>((b + m / 2) * 32, 0, m & 1, left);
-        R[m] = delta_mma<3>(left, right, R[m]);
+        R[m] = delta_mma(left, right, R[m]);
       }
     }
     delta_f32x4 dU[M];
@@ -1043,7 +1044,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
 #pragma unroll
       for (int m = 0; m < 2 * b + 2; ++m) {
         lds.TP.transposed((b + m / 2) * 32, 0, m & 1, left);
-        R[m] = delta_mma<3>(left, right, R[m]);
+        R[m] = delta_mma(left, right, R[m]);
       }
     }
     if (!THROUGH) strip.put(a.dwrites + strip.number(chunk) * C * a.f.dv, C, R);
@@ -1063,7 +1064,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
 #pragma unroll
       for (int k = 0; k < 2 * KB; ++k) {
         lds.Q.transposed(b * 32, (k >> 1) * 32, k & 1, left);
-        D[k] = delta_mma<3>(left, right, D[k]);
+        D[k] = delta_mma(left, right, D[k]);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) x[t] = -delta_rows(lds.powers[0], 2 * b + t) * R[2 * b + t];
@@ -1071,7 +1072,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
 #pragma unroll
       for (int k = 0; k < 2 * KB; ++k) {
         lds.K.transposed(b * 32, (k >> 1) * 32, k & 1, left);
-        D[k] = delta_mma<3>(left, right, D[k]);
+        D[k] = delta_mma(left, right, D[k]);
       }
     }
     __syncthreads();
@@ -1101,7 +1102,7 @@ __device__ __forceinline__ float delta_sum16(float v) {
 // kernels that write them 25 us and does not help this one; a compute unit's next chunk's columns asked for during its last products, 446 for 480, but 35 for 29 where chunks are few.
 template <typename AT, int DK, bool NARROW>
 __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
-  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, OUT = DeltaChunk<AT>::kOut, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;
+  constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, BLOCKS = delta_blocks(C), W = DK / 16, THREADS = 64 * W;
   constexpr int kTiles = BLOCKS * 4, kEach = (kTiles + W - 1) / W;                                        // of C x C, for each wavefront
   constexpr int kItems = C * 4, kTasks = (2 * kItems + THREADS - 1) / THREADS;                            // eights of 32 columns: of R and V, then of U and dY
   constexpr int kApart = THREADS * 8 / DK;
@@ -1111,7 +1112,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
     DeltaTile<NI, C, 32> Y;
   };
   struct Square {
-    DeltaTile<OUT, BLOCKS * 32, 32> F, H;
+    DeltaTile<3, BLOCKS * 32, 32> F, H;
   };
   __shared__ DeltaTile<NI, C, DK> K, Q;
   __shared__ union Shared {
@@ -1247,13 +1248,13 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
       if (step + 1 < M + kEach) fetch(step + 1);
       delta_ahead();
       if (step < M) {
-        YS[step % M] = delta_mma<3>(of_Y[at], sp, YS[step % M]);
-        UD[step % M] = delta_mma<3>(of_U[at], dp, UD[step % M]);
-        RS[step % M] = delta_mma<3>(of_R[at], sp, RS[step % M]);
+        YS[step % M] = delta_mma(of_Y[at], sp, YS[step % M]);
+        UD[step % M] = delta_mma(of_U[at], dp, UD[step % M]);
+        RS[step % M] = delta_mma(of_R[at], sp, RS[step % M]);
       } else if (kTiles % W == 0 || (step - M) * W + wave < kTiles) {
         const int n = (step + kEach - M) % kEach;
-        X[n] = delta_mma<3>(of_R[at], of_U[at], X[n]);
-        Z[n] = delta_mma<3>(of_Y[at], of_U[at], Z[n]);
+        X[n] = delta_mma(of_R[at], of_U[at], X[n]);
+        Z[n] = delta_mma(of_Y[at], of_U[at], Z[n]);
       }
     }
   };
@@ -1328,9 +1329,9 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
         column += both;
         row[r] = delta_sum16(both), with_l[r] = delta_sum16(x * l);
         float f = z * e, h = -(x * beta * e);
-        const int to = DeltaTile<OUT, BLOCKS * 32, 32>::offset(place, j & 31);
+        const int to = DeltaTile<3, BLOCKS * 32, 32>::offset(place, j & 31);
 #pragma unroll
-        for (int k = 0; k < OUT; ++k) {
+        for (int k = 0; k < 3; ++k) {
           const __bf16 fp = (__bf16)f, hp = (__bf16)h;
           *(__bf16*)(lds.square.F.bytes[k] + to) = fp;
           *(__bf16*)(lds.square.H.bytes[k] + to) = hp;
@@ -1351,7 +1352,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    delta_bf16x8 k_right[NI], q_right[NI], left[OUT];
+    delta_bf16x8 k_right[NI], q_right[NI], left[3];
     K.right(b * 32, wave * 16, k_right);
     Q.right(b * 32, wave * 16, q_right);
 #pragma unroll
@@ -1359,15 +1360,15 @@ __global__ __launch_bounds__(DK * 4) void k_delta_gradients(DeltaChunkArgs a) {
       if (m / 2 >= b) {
         const int place = (m / 2 + b) * 32 + (m & 1) * 16;
         lds.square.F.left(place, 0, left);
-        YS[m] = delta_mma<OUT>(left, k_right, YS[m]);
+        YS[m] = delta_mma(left, k_right, YS[m]);
         lds.square.H.left(place, 0, left);
-        UD[m] = delta_mma<OUT>(left, k_right, UD[m]);
+        UD[m] = delta_mma(left, k_right, UD[m]);
       }
       if (m / 2 <= b) {
         lds.square.F.transposed((b + m / 2) * 32, 0, m & 1, left);
-        UD[m] = delta_mma<OUT>(left, q_right, UD[m]);
+        UD[m] = delta_mma(left, q_right, UD[m]);
         lds.square.H.transposed((b + m / 2) * 32, 0, m & 1, left);
-        UD[m] = delta_mma<OUT>(left, k_right, UD[m]);
+        UD[m] = delta_mma(left, k_right, UD[m]);
       }
     }
   }

@@ -147,6 +147,48 @@ def test_decays_and_strengths_at_their_ends(dtype):
     assert not got[7].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("B,H,dv", [(2, 2, 1), (1, 3, 40), (13, 10, 128)])
+@pytest.mark.parametrize("T", [16, 128])
+def test_large_states_that_cancel(T, B, H, dv, dtype):
+    """
+    A state a thousand times the values, of which a frame's write takes away just what its query asks for: key and query t are the unit vector t, so that y_t = scale (S_t + (v_t - S_t)).
+
+    A chunk takes y_t from row t of the state before it, S (at most as large as s0 or v), and from u_t = v_t - S: together at most 2 |s0| + 3 |v|, no other number enters, and each is exact in three parts.
+    So y is off by a few roundings to float32 of these, of which 10 of 2^-23 are allowed (products, their sums part by part, scale), and its own rounding.  A third part left out would be up to 2^-17.
+    dq_t likewise, with an error dy_t of one column: element i from row i of S and from u_i where a frame i has written it.
+    """
+    announce("delta cancelling", T, B, H, dv, dtype)
+    x, dy, ds = inputs(T, B, H, H, 128, dv, dtype, seed=21)
+    unit = torch.eye(128, device=DEV, dtype=dtype)[:T, None, None, :].expand(T, B, H, 128)
+    x[0], x[1], x[5] = unit.clone(), unit.clone(), 1000 * x[5]
+    x[3].zero_()
+    x[4].fill_(1.0)
+    dy = dy * torch.eye(dv, device=DEV, dtype=dtype)[torch.arange(T) % dv][:, None, None, :]
+    leaves = [t.clone().requires_grad_() for t in x]
+    y, s = gated_delta_rule(*leaves[:5], state=leaves[5])
+    (dq,) = torch.autograd.grad(y, leaves[0], dy)
+    with torch.no_grad():
+        z, r = gated_delta_rule(*x[:5], state=x[5])
+    a = [numbers(t) for t in x]
+    scale, e = 128**-0.5, abs(numbers(dy))
+    want, state, _ = ref.delta(*a)
+    want_q = ref.delta_grad(*a[:5], numbers(dy), numpy.zeros_like(a[5]), a[5])[0]
+    half = torch.finfo(dtype).eps / 2
+    parts = 2 * abs(a[5])
+    parts[:, :, :T] += 3 * abs(a[2]).transpose(1, 2, 0, 3)
+    for t in range(T):
+        tol = half * abs(want[t]) + 10 * 2.0**-23 * scale * parts[:, :, t]
+        for got in (y, z):
+            off = abs(numbers(got[t]) - want[t])
+            assert (off <= tol).all(), ("y", t, (off / tol).max())
+        tol = half * abs(want_q[t]) + 10 * 2.0**-23 * scale * numpy.einsum("bhij,bhj->bhi", parts, e[t]) + 1e-30
+        off = abs(numbers(dq[t]) - want_q[t])
+        assert (off <= tol).all(), ("dq", t, (off / tol).max())
+    for got in (s, r):
+        assert (abs(numbers(got) - state) <= 8 * 2.0**-24 * abs(a[5]).max()).all()
+
+
 def test_equal_keys():
     """The same key at every frame, written at full strength without decay: each value replaces the one before it; the inverse's entries are 1 and -1."""
     announce("delta equal keys")

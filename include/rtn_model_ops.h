@@ -53,7 +53,7 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
  * Its gradient.  dy [T,B,heads,dv] (rows lddy elements apart, 0: contiguous), not read past a sequence's length; dsN [B,heads,dk,dv] float32 or NULL (zero).
  * dq, dk_out [T,B,key_heads,dk], dv_out [T,B,heads,dv] contiguous, in the type of q, k and v; dg, dbeta [T,B,heads], ds0 [B,heads,dk,dv] float32; all but ds0 are 0 past a
  * sequence's length.  `saved` is what the forward call with the same q, k, v, g, beta, s0, lens and direction left.  Heads that share queries and keys are
- * added in their order.
+ * added in their order; without any (heads = 0) the gradients of queries and keys are 0.
  */
 size_t rtn_delta_rule_bwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype);
 int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const float* g, const float* beta, const int64_t* lens,

@@ -108,7 +108,7 @@ std::tuple<Tensor, Tensor> gated_delta_rule(const Tensor& query, const Tensor& k
   const int64_t B = v.size(-3), H = v.size(-2), Hk = q.size(-2), dk = q.size(-1), dv = v.size(-1);
   TORCH_CHECK(Hk ? H % Hk == 0 : H == 0, what, ": ", H, " heads of values cannot share ", Hk, " heads of queries and keys evenly");
   TORCH_CHECK(dk >= 1 && dk <= 128 && dv >= 1 && dv <= 65536, what, ": keys of 1 to 128 and values of 1 to 65536 elements needed, got ", dk, " and ", dv);
-  TORCH_CHECK(B <= INT_MAX && H <= INT_MAX, what, ": values ", v.sizes(), " are too large");
+  TORCH_CHECK(B <= INT_MAX && H <= INT_MAX && Hk <= INT_MAX, what, ": queries ", q.sizes(), " and values ", v.sizes(), " are too large");
   TORCH_CHECK(direction == 1 || direction == -1, what, ": direction must be +1 or -1");
   auto of_heads = [&](const Tensor& t, const char* name) {
     TORCH_CHECK(t.sizes() == v.sizes().slice(0, v.dim() - 1), what, ": ", name, " ", t.sizes(), ", expected ", v.sizes().slice(0, v.dim() - 1));

@@ -207,7 +207,18 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
   if (rc == RTN_OK) rc = pitch_check(what, "v", &ldv, (int64_t)heads * dv);
   if (rc == RTN_OK) rc = pitch_check(what, "dy", &lddy, (int64_t)heads * dv);
   if (rc != RTN_OK) return rc;
-  if (nothing(z)) return RTN_OK;
+  if (nothing(z)) {  // (keys may be there without values: sums over no heads)
+    if (!T || !B || !key_heads) return RTN_OK;
+    if (!dq || !dk_out) return fail(RTN_ERR_ARG, "%s: null pointer", what);
+    if (!aligned(dq, size_of(dtype)) || !aligned(dk_out, size_of(dtype))) return fail(RTN_ERR_ARG, "%s: misaligned pointer", what);
+    if (T > max_blocks(256) * 256 / dk / B / key_heads) return fail(RTN_ERR_SHAPE, "%s: T=%lld B=%d key_heads=%d are too many for one call", what, (long long)T, B, key_heads);
+    DeltaChunkArgs c{};
+    c.f.T = T, c.f.B = B, c.f.key_heads = key_heads, c.f.dk = dk, c.dq = dq, c.dk = dk_out;
+    with_type(dtype, [&](auto type) {
+      hipLaunchKernelGGL(k_delta_shared<decltype(type)>, dim3((unsigned)((T * B * key_heads * (int64_t)dk + 255) / 256)), dim3(256), 0, (hipStream_t)hip_stream, c);
+    });
+    return launched(what);
+  }
   if ((T && (!q || !k || !v || !g || !beta || !dy || !saved || !dq || !dk_out || !dv_out || !dg || !dbeta)) || !ds0) return fail(RTN_ERR_ARG, "%s: null pointer", what);
   const int e = size_of(dtype);
   if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(dy, e) || !aligned(dq, e) || !aligned(dk_out, e) || !aligned(dv_out, e) || !aligned(g, 4) || !aligned(beta, 4) ||

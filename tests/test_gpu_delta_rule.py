@@ -343,6 +343,21 @@ def test_empty():
         assert y.shape == (6, B, H, 5) and s.shape == (B, H, 4, 5)
 
 
+def test_no_heads_of_values():
+    """Queries and keys of heads that have no values: their gradient is zero."""
+    announce("delta no values")
+    for dtype in (torch.float32, torch.bfloat16):
+        for T in (1, 6, 70):
+            q, k = (torch.ones((T, 2, 3, 24), device=DEV, dtype=dtype, requires_grad=True) for _ in "qk")
+            v, g = torch.zeros((T, 2, 0, 5), device=DEV, dtype=dtype), torch.zeros((T, 2, 0), device=DEV)
+            y, s = gated_delta_rule(q, k, v, g, g)
+            assert y.shape == (T, 2, 0, 5) and s.shape == (2, 0, 24, 5)
+            used = [torch.full_like(q, float("nan")) for _ in range(4)]
+            del used  # (what memory holds that is given out next)
+            for d in torch.autograd.grad(y.sum() + s.sum(), [q, k]):
+                assert torch.equal(d, torch.zeros_like(q))
+
+
 def test_refusals():
     announce("delta refusals")
     x, _, _ = inputs(5, 2, 2, 4, 8, 6, torch.float32)

@@ -105,6 +105,21 @@ def test_delta_gradient_refusals(cabi, change, code):
 @pytest.mark.parametrize(
     "change,code",
     [
+        (dict(), ARG), (dict(dq=P), ARG), (dict(dq=P, dk_=P + 1), ARG), (dict(dq=P, dk_=P, T=1 << 30, B=1 << 30), SHAPE), (dict(dq=P, dk_=P, Hk=(1 << 31) - 1), SHAPE),
+        (dict(T=0), OK), (dict(B=0), OK), (dict(Hk=0), OK),
+    ],
+)  # fmt: skip
+def test_delta_gradient_refusals_without_values(cabi, change, code):
+    """Queries and keys without a head of values: their gradients are asked for all the same, and nothing else."""
+    a = dict(q=P, ldq=0, k=P, ldk=0, v=None, ldv=0, g=None, beta=None, lens=None, saved=None, dy=None, ldy=0, ds=None, dq=None, dk_=None, dv_=None, dg=None, db=None, ds0=None, T=100, B=3, Hk=2, H=0,
+             dk=8, dv=10, dtype=BF16, scale=1.0, direction=1, ws=None, bytes=0)  # fmt: skip
+    a.update(change)
+    assert cabi.rtn_delta_rule_bwd(*a.values(), None) == code
+
+
+@pytest.mark.parametrize(
+    "change,code",
+    [
         (dict(rows=-1), SHAPE), (dict(rows=1 << 31), SHAPE), (dict(V=-1), SHAPE), (dict(V=1 << 31), SHAPE), (dict(D=-1), SHAPE), (dict(ld=4), SHAPE), (dict(dtype=9), ARG),
         (dict(tokens=None), ARG), (dict(table=None), ARG), (dict(y=None), ARG), (dict(tokens=P + 4), ARG), (dict(table=P + 1), ARG), (dict(y=P + 1), ARG),
         (dict(rows=(1 << 31) - 1, D=1 << 20), SHAPE), (dict(rows=0), OK), (dict(D=0), OK),

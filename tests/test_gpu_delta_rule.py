@@ -343,6 +343,41 @@ def test_empty():
         assert y.shape == (6, B, H, 5) and s.shape == (B, H, 4, 5)
 
 
+def bf16_bound(got, want, terms):
+    """As `tolerances`, but with all numbers in three parts: what ends in bfloat16 is off by its own rounding and as float32 results are."""
+    for name, g, w in zip(NAMES, got, want):
+        most = abs(w).max(initial=0.0)
+        tol = (2.0**-8 * abs(w) if name in ("y", "dq", "dk", "dv") else 0.0) + terms * 2.0**-23 * most + 1e-30
+        off = abs(g - w)
+        assert (off <= tol).all(), (name, off.max(), (off / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("Hk,dk,dv,direction", [(3, 20, 128, 1), (1, 40, 71, -1), (3, 128, 128, -1), (1, 128, 100, 1)])
+def test_many_heads(Hk, dk, dv, direction, dtype):
+    """129 heads of more than 64 columns: eight wavefronts a workgroup, of several widths, ragged, with shared queries and keys."""
+    announce("delta many heads", Hk, dk, dv, direction, dtype)
+    T, B, H = 70, 43, 3
+    x, dy, ds = inputs(T, B, Hk, H, dk, dv, dtype, seed=dk + dv)
+    lens = [T - n % 9 * 7 for n in range(B)]
+    lens[3:5] = 0, 1
+    got = check(x, dy, ds, lens=lens, direction=direction)
+    a = [numbers(t) for t in x]
+    want = list(ref.delta(*a, lens, direction)[:2]) + list(ref.delta_grad(*a[:5], numbers(dy), numbers(ds), a[5], lens, direction))
+    if dtype == torch.bfloat16:
+        bf16_bound(got, want, max(dk, dv) + 4 * 64)
+    y, s = gated_delta_rule(*x[:5], state=x[5], seq_lens=torch.tensor(lens), direction=direction)  # (no gradient follows)
+    assert numpy.array_equal(numbers(y), got[0]) and numpy.array_equal(numbers(s), got[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_shared_heads_in_segments(dtype):
+    announce("delta shared heads in segments", dtype)
+    x, dy, ds = inputs(1100, 2, 2, 6, 40, 24, dtype, seed=8, decay=0.05)
+    for direction in (1, -1):
+        check(x, dy, ds, lens=[1100, 700], direction=direction)
+
+
 def test_no_heads_of_values():
     """Queries and keys of heads that have no values: their gradient is zero."""
     announce("delta no values")

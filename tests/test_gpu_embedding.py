@@ -56,6 +56,16 @@ def test_rows(rows, dtype):
     check(torch.where(torch.rand((rows,), generator=gen) < 0.2, -1, tokens), 700, 24, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,D", [(70000, 24), (33000, 600), (20000, 600), (66000, 3)])
+def test_many_rows(rows, D, dtype):
+    """Pieces of 16 and 32 rows."""
+    announce("embedding many rows", rows, D, dtype)
+    gen = torch.Generator().manual_seed(rows)
+    tokens = torch.randint(-1, 900, (rows,), generator=gen)
+    check(torch.where(torch.rand((rows,), generator=gen) < 0.05, 333, tokens), 890, D, dtype)
+
+
 @pytest.mark.parametrize("V", [1, 2, 255, 256, 511, 512, 513, 70000, 262143, 262144])
 @pytest.mark.parametrize("rows", [300, 9000])
 def test_vocabularies(V, rows):

@@ -67,11 +67,14 @@ void with_waves(const DeltaSizes& z, F f) {
   else
     f(Count<4>());
 }
+constexpr int kSegmentWaves = 4;
 // Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.3, and both
-// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 331 us, 4 161, 8 107, 16 96, what is chosen (13) 99, 32 129;
-// T=8192, two of 8 heads of 64 x 128: 541, 254, 170, 176, 183, 191; T=1000, 16 of 8 of 128 x 128: one 140, 4 266.
+// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 331 us, 4 161, 8 107, 16 (chosen) 96, 32 129;
+// T=8192, two of 8 heads of 64 x 128: 541, 254, 170, 176, 183, 191; T=1000, 16 of 8 of 128 x 128: one 140, 4 266.  One segment or at least three; where eight wavefronts are taken half of the compute units
+// have work, and the estimate never finds segments worth their second pass.
 int64_t delta_segments(const DeltaSizes& z) {
-  const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * delta_waves(z);
+  if (delta_waves(z) != kSegmentWaves) return 1;
+  const int64_t chunks = delta_chunks(z), lines = (int64_t)z.B * z.heads, width = 16 * kSegmentWaves;
   const int64_t strips = delta_strips(z), strips_through = ((z.dv + 15) / 16 * 16 + delta_key_width(z) + width - 1) / width;
   auto rounds = [&](int64_t blocks) { return (double)((blocks + 255) / 256); };
   double least = rounds(lines * strips) * chunks;
@@ -178,13 +181,13 @@ int rtn_delta_rule_fwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     constexpr int DK = decltype(width)::value;
     const dim3 heads_grid((unsigned)(B * heads * c.segments * delta_strips(z)));
     if (T) hipLaunchKernelGGL((k_delta_chunks<AT, DK>), dim3((unsigned)delta_all_chunks(z)), dim3(DeltaChunk<AT>::kFrames * 4), 0, stream, c);
+    if (c.segments > 1) {
+      const int64_t strips = ((dv + 15) / 16 * 16 + DK + 16 * kSegmentWaves - 1) / (16 * kSegmentWaves);
+      hipLaunchKernelGGL((k_delta_forward<AT, DK, kSegmentWaves, kDeltaThrough>), dim3((unsigned)(B * heads * (c.segments - 1) * strips)), dim3(64 * kSegmentWaves), 0, stream, c);
+      hipLaunchKernelGGL((k_delta_join<AT, DK, false>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
+    }
     with_waves(z, [&](auto waves) {
       constexpr int W = decltype(waves)::value;
-      if (c.segments > 1) {
-        const int64_t strips = ((dv + 15) / 16 * 16 + DK + 16 * W - 1) / (16 * W);
-        hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaThrough>), dim3((unsigned)(B * heads * (c.segments - 1) * strips)), dim3(64 * W), 0, stream, c);
-        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, false>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
-      }
       if (saved)
         hipLaunchKernelGGL((k_delta_forward<AT, DK, W, kDeltaKeep>), heads_grid, dim3(64 * W), 0, stream, c);
       else
@@ -243,12 +246,12 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
     typedef decltype(type) AT;
     constexpr int DK = decltype(width)::value;
     const hipStream_t stream = (hipStream_t)hip_stream;
+    if (c.segments > 1) {
+      hipLaunchKernelGGL((k_delta_backward<AT, DK, kSegmentWaves, true>), dim3((unsigned)(B * heads * (c.segments - 1) * delta_strips(z))), dim3(64 * kSegmentWaves), 0, stream, c);
+      hipLaunchKernelGGL((k_delta_join<AT, DK, true>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
+    }
     with_waves(z, [&](auto waves) {
       constexpr int W = decltype(waves)::value;
-      if (c.segments > 1) {
-        hipLaunchKernelGGL((k_delta_backward<AT, DK, W, true>), dim3((unsigned)(B * heads * (c.segments - 1) * delta_strips(z))), dim3(64 * W), 0, stream, c);
-        if (c.segments > 2) hipLaunchKernelGGL((k_delta_join<AT, DK, true>), dim3((unsigned)(B * heads * ((dv + 15) / 16))), dim3(DK * 4), 0, stream, c);
-      }
       hipLaunchKernelGGL((k_delta_backward<AT, DK, W, false>), dim3((unsigned)(B * heads * c.segments * delta_strips(z))), dim3(64 * W), 0, stream, c);
     });
     if (T)

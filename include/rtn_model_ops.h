@@ -70,7 +70,8 @@ int rtn_delta_rule_bwd(const void* q, int64_t ldq, const void* k, int64_t ldk, c
 int rtn_embedding_fwd(const int64_t* tokens, const void* table, int64_t ld, void* y, int64_t rows, int64_t V, int64_t D, int32_t dtype, float scale, void* hip_stream);
 
 /*
- * Its gradient: Dtable[v] = scale * the sum of dy[r] over the rows of token v, added in float32 in the order of r.
+ * Its gradient: Dtable[v] = scale * the sum of dy[r] over the rows of token v, in float32: these rows are added in the order of r in blocks of 8, 16 or 32 (by rows and D), and
+ * the blocks' sums in order.  So the rows of other tokens have no part in how they are added.
  * dy [rows,D] (rows ld elements apart, 0: D), not read where there is no token of the table; Dtable [V,D] contiguous.
  */
 size_t rtn_embedding_bwd_workspace_bytes(int64_t rows, int64_t V, int64_t D, int32_t dtype);

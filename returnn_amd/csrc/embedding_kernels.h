@@ -1,6 +1,6 @@
 // gfx950 kernels of an embedding table: rows of tokens, scaled, and the table's gradient.
 //
-//   y_r = scale W[token_r],   dW[v] = scale sum_{r: token_r = v} dy_r, added in the order of r
+//   y_r = scale W[token_r],   dW[v] = scale sum_{r: token_r = v} dy_r, added in the order of r by blocks of them
 #pragma once
 
 #include "sequence_common.h"
@@ -201,10 +201,11 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a, EmbeddingFi
     }
 }
 
-// Sums: up to 64 lanes, of 8 columns each, take `run` rows in the order of their tokens.  A run of one token inside of them is a row of the table; of a run that goes on the sum so far
-// is kept, of one that has begun before the sum of what is here.
-// Pieces, not tokens, share out the work, so that one token of many rows costs no more than others; eight rows are on their way at a time, and no atomics are needed, whose order would change sums.  Bound by memory: the
-// largest measured call moves 75 MB in 16-18 us; few rows by latency (6 us).
+// Sums: the rows of a token, in order, are cut into blocks of `run` from the token's first row on, so that how they are added does not depend on the rows of other tokens.  Up to 64 lanes, of 8 columns
+// each, take the blocks that begin in `run` places of the sorted rows: one that goes on from an earlier place at most, then tokens' first ones, of which the last may have more behind it.  The sum of all rows of a token
+// is a row of the table; those of a block with others before or behind it are kept, and joined in order.
+// Eight rows are on their way at a time, and no atomics are needed, whose order would change sums.  Bound by memory: the largest measured call moves 75 MB in 16-18 us; few rows by latency (6 us,
+// 10 where runs go over several pieces: where they begin is looked for first).
 struct EmbeddingSumArgs {
   EmbeddingArgs e;
   float *begun, *rest;  // [pieces][D]
@@ -227,47 +228,116 @@ __device__ __forceinline__ void embedding_put(AT* to, int left, const float (&v)
       if (k < left) store_f32(to + k, v[k] * scale);
   }
 }
+// Where the run of the token at `first - 1` begins, which is the token at `first` too.  A wavefront looks at 64 places at a time: the nearest ones and every 65th behind them at once, then ever wider apart
+// while all are the token's, then between two of them.  (Of a run of up to 64 rows one round of loads, of up to 4224 two, of up to 278848 four.)
+__device__ __forceinline__ long long embedding_run_begin(const EmbeddingArgs& a, long long first, unsigned token) {
+  const int lane = threadIdx.x & 63;
+  // (how many of the places at - step, at - 2 step, .. are the token's, of 64 that are above `above`)
+  auto place_of = [&](long long at, long long step) { return at - step * (lane + 1); };
+  auto key_of = [&](long long place, long long above) { return a.token_of[place > above ? place : first]; };
+  auto count = [&](long long place, long long above, unsigned key) {
+    const unsigned long long other = ~__ballot(place > above && key == token);
+    return other ? __builtin_ctzll(other) : 64;
+  };
+  long long in = first - 1, out = -1, step = 65;  // the lowest place known to be the token's, and the highest known not to be
+  const long long near = place_of(in, 1), far = place_of(in - 64, step);
+  const unsigned near_key = key_of(near, -1), far_key = key_of(far, -1);
+  int n = count(near, -1, near_key);
+  if (n < 64) return in - n;
+  in -= 64;
+  auto look = [&]() { return count(place_of(in, step), out, key_of(place_of(in, step), out)); };
+  for (n = count(far, -1, far_key);; n = look()) {
+    in -= step * n;
+    if (n < 64) break;
+    step *= 65;
+  }
+  out = in - step < -1 ? -1 : in - step;
+  while (in - out > 1) {
+    step = (in - out - 1) / 65 + 1;
+    n = look();
+    in -= step * n;
+    if (n < 64 && in - step > out) out = in - step;
+  }
+  return in;
+}
 template <typename AT>
 __global__ __launch_bounds__(256) void k_embedding_sums(EmbeddingSumArgs s) {
   const EmbeddingArgs& a = s.e;
   const long long item = (blockIdx.x * 256ll + threadIdx.x) / s.lanes;
   const int piece = (int)(item / s.strips), strip = (int)(item - (long long)piece * s.strips);
-  if (piece >= s.pieces) return;
-  const unsigned V = (unsigned)a.V;
-  const long long col = ((long long)strip * s.lanes + threadIdx.x % s.lanes) * 8, first = (long long)piece * s.run;
-  const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8)), rows = (int)(a.rows - first < s.run ? a.rows - first : s.run);
-  if (left == 0) return;
-  const unsigned before = first ? a.token_of[first - 1] : 0xFFFFFFFFu, after = first + rows < a.rows ? a.token_of[first + rows] : 0xFFFFFFFFu;
+  const unsigned V = (unsigned)a.V, kEnd = 0xFFFFFFFFu;  // (no token)
+  const long long col = ((long long)strip * s.lanes + threadIdx.x % s.lanes) * 8, first = (long long)piece * s.run, end = first + s.run;
+  const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8));
+  auto key_at = [&](long long place) {
+    const unsigned key = a.token_of[place < a.rows ? place : a.rows - 1];
+    return place < a.rows ? key : kEnd;
+  };
+  unsigned token = key_at(first);
+  const unsigned before = first ? key_at(first - 1) : kEnd;
+  long long place = first, begin = first;  // of the row, and of its block
+  bool whole = true;                       // whether the block is its token's first one
+  // (a wavefront's pieces, if it has several, are neighbours: one search for all that begin inside of the same run)
+  const bool inside = token < V && before == token;
+  long long run_begin = first;
+  for (unsigned long long wanted = __ballot(inside); wanted;) {
+    const int lane = __builtin_ctzll(wanted);
+    const unsigned of = (unsigned)__builtin_amdgcn_readlane((int)token, lane);
+    const long long found = embedding_run_begin(a, (long long)__builtin_amdgcn_readlane(piece, lane) * s.run, of);
+    const bool mine = inside && token == of;
+    if (mine) run_begin = found;
+    wanted &= ~__ballot(mine);
+  }
+  // The first block that begins in the piece: of that run, or where it ends before that.
+  const int done = (int)(first - run_begin) & (s.run - 1);
+  const long long next = done ? end - done : first;
+  const bool ends_here = inside && key_at(next) != token;
+  if (inside && !ends_here) place = begin = next, whole = false;
+  for (unsigned long long wanted = __ballot(ends_here); wanted;) {
+    const int lane = __builtin_ctzll(wanted), at = __builtin_amdgcn_readlane(piece, lane);
+    const unsigned of = (unsigned)__builtin_amdgcn_readlane((int)token, lane), key = key_at((long long)at * s.run + (threadIdx.x & 63));
+    const int rows = __builtin_ctzll(__ballot(key != of));  // (of the run in the piece, which has fewer than 64 places)
+    const bool mine = piece == at;
+    if (mine) place = begin = first + rows;
+    if (mine) token = (unsigned)__builtin_amdgcn_readlane((int)key, rows);
+    wanted &= ~__ballot(mine);
+  }
+  if (token >= V || left == 0) return;  // (rows without a token are the last ones)
   float sum[8] = {};
-  unsigned token = a.token_of[first];
-  bool begun_here = token != before;
-  auto flush = [&](bool ends_here) {
-    if (token >= V) return;
-    if (begun_here && ends_here) {
-      embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
+  unsigned owner = token;  // (whose sum this is)
+  auto flush = [&](bool ends) {
+    if (whole && ends) {
+      embedding_put((AT*)a.out + owner * a.D + col, left, sum, a.scale);
     } else {
-      // (a run that fills this piece and goes on is part of the run that began earlier)
-      float* to = (begun_here ? s.begun : s.rest) + piece * a.D + col;
+      float* to = (whole ? s.begun : s.rest) + piece * a.D + col;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (k < left) to[k] = sum[k];
     }
   };
   constexpr int AHEAD = 8;
-  for (int p0 = 0; p0 < rows; p0 += AHEAD) {
+  bool ends = false;
+  for (bool done = false; !done; place += AHEAD) {
     Eight<AT> q[AHEAD];
-    unsigned key[AHEAD], row[AHEAD];
+    unsigned key[AHEAD + 1], row[AHEAD], taken = 0, begins = 0;
     float part[8];
 #pragma unroll
-    for (int p = 0; p < AHEAD; ++p) {
-      const long long at = first + (p0 + p < rows ? p0 + p : rows - 1);
-      key[p] = p0 + p < rows ? a.token_of[at] : V;
-      row[p] = a.order[at];
+    for (int p = 0; p <= AHEAD; ++p) {
+      key[p] = key_at(place + p);
+      if (p < AHEAD) row[p] = a.order[place + p < a.rows ? place + p : a.rows - 1];
+    }
+#pragma unroll
+    for (int p = 0; p <= AHEAD; ++p) {
+      const bool other = key[p] != token, over = other ? place + p >= end || key[p] >= V : place + p - begin == s.run;
+      if (!done && over) done = true, ends = other;
+      if (p < AHEAD && !done) {
+        if (other) token = key[p], begin = place + p, begins |= 1u << p;
+        taken |= 1u << p;
+      }
     }
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) {
       const AT* from = (const AT*)a.in + row[p] * a.ld + col;
-      const bool wanted = key[p] < V;
+      const bool wanted = taken >> p & 1;
       if (wanted && left == 8) {
         q[p].load(from);
       } else {
@@ -278,33 +348,39 @@ __global__ __launch_bounds__(256) void k_embedding_sums(EmbeddingSumArgs s) {
     }
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) {
-      if (p0 + p < rows) {
-        if (key[p] != token) {
-          flush(true);
-          token = key[p], begun_here = true;
+      if (begins >> p & 1) {
+        flush(true);
+        owner = key[p], whole = true;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sum[k] = 0.f;
-        }
+        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+      }
+      if (taken >> p & 1) {
         q[p].get(part);
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] += part[k];
       }
     }
   }
-  flush(token != after);
+  flush(ends);
 }
 
-// Rows of the table whose run goes over several pieces: a wavefront for each piece and 512 columns; most pieces have none that begins in them and goes on.
+// Rows of the table that are the sum of several blocks: a wavefront for each piece and 512 columns, which adds the blocks of the run that begins in the piece and is longer than one, if there is one; most pieces have none.
+// The blocks of one token are added one after the other, 16 on their way at a time: a token of very many rows takes longer than the others together (131072 rows of 512 bf16, forward and gradient: 122 us
+// with no token frequent, 240 with half of the rows one token, 323 with all).
 template <typename AT>
 __global__ __launch_bounds__(256) void k_embedding_join(EmbeddingSumArgs s) {
   const EmbeddingArgs& a = s.e;
   const int lane = threadIdx.x & 63;
   const long long item = blockIdx.x * 4ll + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int piece = (int)(item / s.strips), strip = (int)(item - (long long)piece * s.strips);
-  const long long first = (long long)piece * s.run, next = first + s.run;
-  if (next >= a.rows) return;
-  const unsigned token = a.token_of[next];
-  if (token >= (unsigned)a.V || a.token_of[next - 1] != token || (first && a.token_of[first - 1] == token)) return;
+  const long long first = (long long)piece * s.run;
+  if (first + s.run >= a.rows) return;
+  // (a lane for each of the piece's places, and for as many behind them: of a run that begins at the piece's place n the next block begins n lanes behind the last one's)
+  const unsigned key = a.token_of[first + lane < a.rows ? first + lane : a.rows - 1], token = (unsigned)__builtin_amdgcn_readlane((int)key, s.run - 1);
+  const int at = __builtin_ctzll(__ballot(key == token));
+  if (token >= (unsigned)a.V || (at == 0 && first && a.token_of[first - 1] == token)) return;
+  const long long next = first + at + s.run;
+  if (next >= a.rows || (unsigned)__builtin_amdgcn_readlane((int)key, at + s.run) != token) return;
   int count = 0;  // pieces behind this one that begin with the token
   for (;;) {
     const long long at = next + (long long)(count + lane) * s.run;
@@ -317,29 +393,43 @@ __global__ __launch_bounds__(256) void k_embedding_join(EmbeddingSumArgs s) {
   }
   const long long col = strip * 512ll + lane * 8;
   const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8));
-  float sum[8];
-  if (left == 8) {
-    Eight<float> q;
-    q.load(s.begun + piece * a.D + col);
-    q.get(sum);
-#pragma unroll 8
-    for (int p = piece + 1; p <= piece + count; ++p) {
-      float part[8];
-      Eight<float> q;
-      q.load(s.rest + p * a.D + col);
-      q.get(part);
+  float sum[8], part[8];
+  const float* from = s.begun + piece * a.D + col;
+  // (all of them asked for before the first is added: left to itself the compiler may ask for each only then)
+  constexpr int AHEAD = 16;
+  auto add = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    auto get = [&](const float* at, Eight<float>& q) {
+      if (WHOLE) {
+        q.load(at);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += part[k];
+        for (int k = 0; k < 8; ++k) part[k] = at[k < left ? k : 0];
+        q.set(part);
+      }
+    };
+    Eight<float> q[AHEAD];
+    get(from, q[0]);
+    q[0].get(sum);
+    from = s.rest + (piece + 1) * a.D + col;
+    for (int p0 = 0; p0 < count; p0 += AHEAD) {
+#pragma unroll
+      for (int p = 0; p < AHEAD; ++p) get(from + (p0 + p < count ? p0 + p : p0) * a.D, q[p]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int p = 0; p < AHEAD; ++p) {
+        q[p].get(part);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = p0 + p < count ? sum[k] + part[k] : sum[k];
+      }
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum[k] = k < left ? s.begun[piece * a.D + col + k] : 0.f;
-#pragma unroll 4
-    for (int p = piece + 1; p <= piece + count; ++p)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += k < left ? s.rest[p * a.D + col + k] : 0.f;
-  }
-  if (left) embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
+  };
+  if (left == 0) return;
+  if (a.D - strip * 512ll >= 512 || a.D % 8 == 0)
+    add(std::true_type());
+  else
+    add(std::false_type());
+  embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
 }
 
 }  // namespace rtn

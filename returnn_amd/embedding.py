@@ -1,6 +1,6 @@
 """
 An embedding table: scaled rows of tokens, and the table's gradient, in which the errors of one token are added in the order of
-their frames, so that repeated calls agree bit for bit.
+their frames, by blocks of 8 to 32 of them, so that repeated calls agree bit for bit, whatever the other tokens are.
 """
 
 from __future__ import annotations

@@ -103,6 +103,23 @@ def test_order_does_not_change():
         assert all(torch.equal(runs[0], r) for r in runs[1:])
 
 
+@pytest.mark.parametrize("rows,D", [(3000, 200), (3000, 8), (3000, 40), (8192, 512), (20000, 200), (20000, 1500), (70000, 16)])
+def test_other_tokens_do_not_change_a_sum(rows, D):
+    """The rows of one token stay, those of others become other tokens: the token's sum is the same bit for bit."""
+    announce("embedding other tokens", rows, D)
+    gen = torch.Generator(device=DEV).manual_seed(rows + D)
+    tokens = torch.randint(0, 50, (rows,), device=DEV, generator=gen)
+    tokens[torch.rand((rows,), device=DEV, generator=gen) < 0.2] = 20
+    dy = torch.randn((rows, D), device=DEV, generator=gen)
+    w = torch.zeros((60, D), device=DEV, requires_grad=True)
+    keep = (tokens == 20) | (tokens == 31)
+    want = torch.autograd.grad(embed(tokens, w), w, dy)[0]
+    for low, high in ((0, 20), (40, 60), (32, 60), (0, 5)):
+        others = torch.randint(low, high, (rows,), device=DEV, generator=gen)
+        got = torch.autograd.grad(embed(torch.where(keep, tokens, others), w), w, dy)[0]
+        assert torch.equal(got[20], want[20]) and torch.equal(got[31], want[31])
+
+
 def test_padding_is_not_read():
     announce("embedding padding")
     tokens = torch.tensor([[0, -1, 2], [-7, 1, 5]], device=DEV)

@@ -41,7 +41,8 @@ const char* rtn_model_ops_last_error(void);
  *        direction -1: from each sequence's last frame to its first.
  * y      [T,B,heads,dv] in the type of q, k and v; sN [B,heads,dk,dv] float32, the state behind the last frame visited
  * saved  what the gradient wants to know (rtn_delta_rule_saved_bytes), or NULL
- * A number that is not finite in a frame that there is spoils the outputs of its head from its chunk of 64 frames (float32: 32) on, not from its own frame on.
+ * A number that is not finite (or of float32 and above 3.38e38, the largest of bfloat16) in a frame that there is spoils the outputs of its head from its chunk of 64 frames (float32: 32) on,
+ *        not from its own frame on.  (Up to 16 frames without `saved` go frame by frame, where it does so from its own on.)
  */
 size_t rtn_delta_rule_fwd_workspace_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype, int32_t keep);
 size_t rtn_delta_rule_saved_bytes(int64_t T, int32_t B, int32_t key_heads, int32_t heads, int32_t dk, int32_t dv, int32_t dtype);
@@ -87,7 +88,8 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
  * ended  [B,K] (0 or not), or NULL: the scores of a hypothesis that has ended are taken as 0 for v = end_token and -inf for all others, and not
  *        read.  end_token in 0..V-1 where `ended` is not NULL.
  * out_totals, sources, tokens [B,beam]: joint, k and v of the `beam` largest of a search in descending order, among equal ones the lowest k first and
- *        among those the lowest v; a NaN before everything.  1 <= beam <= min(64, K V), V up to 2^26, K V below 2^31.
+ *        among those the lowest v; a NaN before everything.  1 <= beam <= min(64, K V), V up to 2^26, K V below 2^31, and B K pieces of a hypothesis'
+ *        scores (of 8192 at least) below 2^22 (else RTN_ERR_SHAPE).
  */
 size_t rtn_beam_select_workspace_bytes(int32_t B, int32_t K, int64_t V, int32_t dtype, int32_t beam);
 int rtn_beam_select(const void* scores, int64_t ld, const float* totals, const uint8_t* ended, int64_t end_token, float* out_totals, int64_t* sources, int64_t* tokens,

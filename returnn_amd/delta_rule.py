@@ -35,7 +35,8 @@ def gated_delta_rule(
     """
     :param query: [T,B,key_heads,dk], time-major, or [B,key_heads,dk] for a single step; float32 or bfloat16, on the GPU; 1 <= dk <= 128; frames may have a pitch
         (e.g. a slice of a wider projection), of all sequences together up to 64 MiB.  (In a region of ``torch.autocast`` float16 is taken as float32.)
-    :param key: like ``query``, of length 1 at most: of longer ones (with ``beta`` near 1) the state grows without bounds
+    :param key: like ``query``.  A step multiplies what the state holds along the key by ``exp(log_decay) (1 - beta |key|^2)``: with ``beta |key|^2`` above 2 it grows without bounds unless
+        it decays.  (With ``beta`` near 2 keys have to be a little shorter than 1: rounded to bfloat16, keys of length 1 can be longer by 2^-8.)
     :param value: [T,B,heads,dv] or [B,heads,dv] of the same type; ``heads`` is a multiple of ``key_heads``, neighbouring heads share queries and keys
     :param log_decay: [T,B,heads] or [B,heads], at most 0, taken as float32; minus infinity forgets all that was before
     :param beta: like ``log_decay``; how much of what is missing is written, 0 to 1 (up to 2 for states that may change their sign)
@@ -45,8 +46,8 @@ def gated_delta_rule(
         the state as it is.
     :param direction: +1, or -1 to go from each sequence's last frame to its first
     :return: output like ``value``, state [B,heads,dk,dv] after the last frame visited, float32.
-        Both differentiable (once) with respect to all inputs but the lengths.  A number that is not finite spoils the outputs of its head from the 64 frames (float32: 32)
-        that are computed with it on, not from its own frame on.
+        Both differentiable (once) with respect to all inputs but the lengths.  A number that is not finite (or, of a float32 state or value, above 3.38e38, the largest of bfloat16)
+        spoils the outputs of its head from the 64 frames (float32: 32) that are computed with it on, not from its own frame on; in a call of up to 16 frames without a gradient, from its own.
     """
     return native().gated_delta_rule(query, key, value, log_decay, beta, scale, state, seq_lens, direction)
 

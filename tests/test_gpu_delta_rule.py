@@ -352,6 +352,20 @@ def bf16_bound(got, want, terms):
         assert (off <= tol).all(), (name, off.max(), (off / tol).max())
 
 
+@pytest.mark.parametrize("T,B,Hk,H,dk,dv,direction,lens", [
+    (17, 2, 1, 2, 24, 20, 1, None), (100, 6, 2, 4, 17, 19, -1, [100, 0, 1, 51, 105, -3]), (200, 2, 2, 2, 128, 130, 1, None), (70, 2, 2, 2, 65, 3, -1, None),
+    (900, 2, 2, 2, 128, 16, 1, [900, 310]), (2200, 2, 1, 1, 64, 130, -1, [1, 2200]),
+])  # fmt: skip
+def test_bfloat16_is_rounded_once(T, B, Hk, H, dk, dv, direction, lens):
+    """Short, ragged, wide and narrow calls and such in segments against the bound that has no place for a part left out."""
+    announce("delta rounded once", T, B, Hk, H, dk, dv, direction)
+    x, dy, ds = inputs(T, B, Hk, H, dk, dv, torch.bfloat16, seed=T + dv, decay=0.05 if T > 200 else 1.0)
+    got = check(x, dy, ds, lens=lens, direction=direction)
+    a = [numbers(t) for t in x]
+    want = list(ref.delta(*a, lens, direction)[:2]) + list(ref.delta_grad(*a[:5], numbers(dy), numbers(ds), a[5], lens, direction))
+    bf16_bound(got, want, max(dk, dv) + 4 * 64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("Hk,dk,dv,direction", [(3, 20, 128, 1), (1, 40, 71, -1), (3, 128, 128, -1), (1, 128, 100, 1)])
 def test_many_heads(Hk, dk, dv, direction, dtype):

@@ -208,7 +208,8 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a, EmbeddingFi
 // 10 where runs go over several pieces: where they begin is looked for first).
 struct EmbeddingSumArgs {
   EmbeddingArgs e;
-  float *begun, *rest;  // [pieces][D]
+  float *begun, *rest;  // [pieces][pitch]
+  long long pitch;      // D and what it lacks to a multiple of 8
   int pieces, strips;
   int lanes;  // of a piece and strip: a power of two
   int run;
@@ -308,10 +309,9 @@ __global__ __launch_bounds__(256) void k_embedding_sums(EmbeddingSumArgs s) {
     if (whole && ends) {
       embedding_put((AT*)a.out + owner * a.D + col, left, sum, a.scale);
     } else {
-      float* to = (whole ? s.begun : s.rest) + piece * a.D + col;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < left) to[k] = sum[k];
+      Eight<float> q;
+      q.set(sum);
+      q.store((whole ? s.begun : s.rest) + piece * s.pitch + col);
     }
   };
   constexpr int AHEAD = 8;
@@ -393,42 +393,25 @@ __global__ __launch_bounds__(256) void k_embedding_join(EmbeddingSumArgs s) {
   }
   const long long col = strip * 512ll + lane * 8;
   const int left = (int)(a.D - col < 0 ? 0 : (a.D - col < 8 ? a.D - col : 8));
-  float sum[8], part[8];
-  const float* from = s.begun + piece * a.D + col;
+  if (left == 0) return;
   // (all of them asked for before the first is added: left to itself the compiler may ask for each only then)
   constexpr int AHEAD = 16;
-  auto add = [&](auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    auto get = [&](const float* at, Eight<float>& q) {
-      if (WHOLE) {
-        q.load(at);
-      } else {
+  Eight<float> q[AHEAD];
+  float sum[8], part[8];
+  q[0].load(s.begun + piece * s.pitch + col);
+  q[0].get(sum);
+  const float* from = s.rest + (piece + 1) * s.pitch + col;
+  for (int p0 = 0; p0 < count; p0 += AHEAD) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) part[k] = at[k < left ? k : 0];
-        q.set(part);
-      }
-    };
-    Eight<float> q[AHEAD];
-    get(from, q[0]);
-    q[0].get(sum);
-    from = s.rest + (piece + 1) * a.D + col;
-    for (int p0 = 0; p0 < count; p0 += AHEAD) {
+    for (int p = 0; p < AHEAD; ++p) q[p].load(from + (p0 + p < count ? p0 + p : p0) * s.pitch);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int p = 0; p < AHEAD; ++p) get(from + (p0 + p < count ? p0 + p : p0) * a.D, q[p]);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int p = 0; p < AHEAD; ++p) {
+      q[p].get(part);
 #pragma unroll
-      for (int p = 0; p < AHEAD; ++p) {
-        q[p].get(part);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] = p0 + p < count ? sum[k] + part[k] : sum[k];
-      }
+      for (int k = 0; k < 8; ++k) sum[k] = p0 + p < count ? sum[k] + part[k] : sum[k];
     }
-  };
-  if (left == 0) return;
-  if (a.D - strip * 512ll >= 512 || a.D % 8 == 0)
-    add(std::true_type());
-  else
-    add(std::false_type());
+  }
   embedding_put((AT*)a.out + token * a.D + col, left, sum, a.scale);
 }
 

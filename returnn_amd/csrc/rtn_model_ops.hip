@@ -294,7 +294,7 @@ int rtn_embedding_fwd(const int64_t* tokens, const void* table, int64_t ld, void
 
 // Workspace of the gradient: the sorted rows and their tokens, twice and counts of digits where there is more than one pass of sorting; the sums of runs over several pieces.
 struct EmbeddingPlan {
-  int64_t pieces, strips, blocks;
+  int64_t pieces, strips, blocks, pitch;  // pitch: of sums
   int passes, lanes, run;
   size_t rows, counts, parts;  // of 4 bytes
   EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
@@ -311,7 +311,8 @@ struct EmbeddingPlan {
     }
     rows = (size_t)(n + 3) / 4 * 4;
     counts = (size_t)blocks * kDigits;
-    parts = (size_t)pieces * (size_t)D;
+    pitch = (D + 7) / 8 * 8;
+    parts = (size_t)pieces * (size_t)pitch;
   }
   size_t bytes() const { return (rows * (passes > 1 ? 4 : 2) + counts + 2 * parts) * 4; }
 };
@@ -359,7 +360,7 @@ int rtn_embedding_bwd(const int64_t* tokens, const void* dy, int64_t ld, void* D
     const unsigned sorting = (unsigned)((rows + 15) / 16);
     hipLaunchKernelGGL(k_embedding_order, dim3(sorting + (unsigned)filling), dim3(1024), 0, stream, a, sorting, EmbeddingFill{bytes, 0});
   }
-  const EmbeddingSumArgs s{a, (float*)(counts + p.counts), (float*)(counts + p.counts) + p.parts, (int)p.pieces, (int)p.strips, p.lanes, p.run};
+  const EmbeddingSumArgs s{a, (float*)(counts + p.counts), (float*)(counts + p.counts) + p.parts, p.pitch, (int)p.pieces, (int)p.strips, p.lanes, p.run};
   if (rows)
     with_type(dtype, [&](auto type) {
       typedef decltype(type) AT;

@@ -412,7 +412,7 @@ __device__ __forceinline__ void delta_spread(int strips, int* line, int* strip) 
 
 // T, P, L and the powers of a chunk, one workgroup of C / 16 wavefronts each, which have 16 rows of L and P each.  The inverse: diagonal blocks of 16 row by row, a column per
 // lane; then T_21 = - T_22 A_21 T_11 for blocks of 16 and of 32, in float32 matrix instructions.  Bound by latency, of rows of K and of 16 steps of a column each, three workgroups on a compute unit: T=1000,
-// 32 ragged sequences of 8 heads, keys of 128 in bf16: 91 us, 3.1 TB/s, of which the records are the larger part.  (Rows read without a condition, a tile ahead, cost more in selections than they save: 121.)
+// 32 ragged sequences of 8 heads, keys of 128 in bf16: 88-92 us, 3.1 TB/s, of which the records are the larger part.  (Rows read without a condition, a tile ahead, cost more in selections than they save: 121.)
 template <typename AT, int DK>
 __global__ __launch_bounds__(DeltaChunk<AT>::kFrames * 4) void k_delta_chunks(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, W = C / 16, BLOCKS = delta_blocks(C), ROW = C + 4;
@@ -719,10 +719,11 @@ __device__ __forceinline__ void delta_zero(delta_f32x4 (&x)[N]) {
 // Where sequences and heads are few, their chunks are dealt to segments that work side by side.  A segment makes B + A S of a state S: a first pass (KIND kDeltaThrough) finds B, the state behind
 // it from none before it, and A, its columns from those of the unit matrix without values; k_delta_join goes from segment to segment; then all segments begin with their state.
 //
-// A chunk needs the one before it, so a workgroup's time is its chain of products, of LDS reads between them and of barriers: 11 us a chunk of 64 frames, keys and values of 128 in bf16, with eight wavefronts
-// (matrix instructions 15 %, others 25 %, waiting 43 %).  Hence 16 columns of the state per wavefront, in registers from the first chunk to the last, with U and Y going from product to product without leaving them, and
-// everything of the next chunk asked for a chunk ahead.  T=1000, 32 ragged sequences of 8 heads, and all that the gradient wants kept: 214-220 us, 343 MB read, 382 written.  T=4000, one sequence: 30 us for each of
-// the two passes.  (Loads on a condition of a lane, each of which the compiler waits for where paths meet again: 300 us for what now takes 200.)
+// A chunk needs the one before it, so a workgroup's time is its chain of products, of LDS reads between them and of barriers: 14 us a chunk of 64 frames, keys and values of 128 in bf16, with eight wavefronts
+// (matrix instructions 18 %, others 26 %, waiting 50 %).  Hence 16 columns of the state per wavefront, in registers from the first chunk to the last, with U and Y going from product to product without leaving them, and
+// everything of the next chunk asked for a chunk ahead.  T=1000, 32 ragged sequences of 8 heads, and all that the gradient wants kept: 225-234 us, 384 MB read, 383 written.  T=4000, one sequence: 30 us for each of
+// the two passes.  (Loads on a condition of a lane, each of which the compiler waits for where paths meet again: 300 us for what then took 200.  Outputs
+// from three parts of states and writes cost 4 %: one more plane of P, and 15 to 18 registers that go through memory with eight wavefronts and keys of more than 64.)
 enum { kDeltaPlain, kDeltaKeep, kDeltaThrough };
 template <typename AT, int DK, int W, int KIND>
 __global__ __launch_bounds__(64 * W) void k_delta_forward(DeltaChunkArgs a) {
@@ -970,7 +971,7 @@ __global__ __launch_bounds__(DK * 4) void k_delta_join(DeltaChunkArgs a) {
 //   of the chunk's last frame also sum_j gamma_j k_j.(D U_j) + c_C <D, S>;  dg is its sum over all later frames of the chunk.
 //
 // k_delta_backward goes through the chunks of a head from its last one, as k_delta_forward, and leaves R and D; k_delta_gradients does the rest, all chunks side by side.
-// (THROUGH: as of the forward pass, but of the segments behind the first one, and with what their transitions left.)  Bound as that is: 193-204 us for the same 32 sequences.
+// (THROUGH: as of the forward pass, but of the segments behind the first one, and with what their transitions left.)  Bound as that is: 200-214 us for the same 32 sequences.
 template <typename AT, int DK, int W, bool THROUGH>
 __global__ __launch_bounds__(64 * W) void k_delta_backward(DeltaChunkArgs a) {
   constexpr int C = DeltaChunk<AT>::kFrames, NI = DeltaChunk<AT>::kInput, M = C / 16, NB = C / 32, KB = DK / 32;
@@ -1097,7 +1098,7 @@ __device__ __forceinline__ float delta_sum16(float v) {
 // NARROW: values of fewer than eight columns.
 // Columns go into one half of LDS while products are made of the other, the operands of a product are read during the one before it, and what is chosen by an element is computed without ways of its own.  Of 48 800 clocks
 // of a chunk (keys and values of 128 in bf16) 14 000 go until the first columns, Q and K are there, 19 300 into the columns, 8500 into the rows' sums, N, F and H, 3000 into the last products and 4000 into results.  The
-// accumulators take a compute unit's registers, one workgroup each, which does nothing else while it waits.  T=1000, 32 ragged sequences of 8 heads: 381-410 us, 946 MB read, 150 written (482 with one half, each operand read
+// accumulators take a compute unit's registers, one workgroup each, which does nothing else while it waits.  T=1000, 32 ragged sequences of 8 heads: 376-398 us, 1070 MB read, 150 written (482 with one half, each operand read
 // when it was wanted, and a way of its own for each element of P).  Slower: 16 wavefronts of half the columns' work, 509 for 480; the frames' and states' numbers kept in the order in which they are read, which costs the
 // kernels that write them 25 us and does not help this one; a compute unit's next chunk's columns asked for during its last products, 446 for 480, but 35 for 29 where chunks are few.
 template <typename AT, int DK, bool NARROW>

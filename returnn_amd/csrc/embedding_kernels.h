@@ -73,7 +73,7 @@ __device__ __forceinline__ void embedding_fill(const EmbeddingArgs& a, unsigned 
 }
 
 // Where a row comes: after all of lower tokens and the earlier ones of the same, counted.  16 rows per workgroup, each against a 64th of all by 64 threads.  One launch in place of four for two digits:
-// 1000, 4096 and 8192 rows of 512 bf16, forward and gradient, 16, 20 and 32 us, with digits 25, 32 and 37.  Bound by its comparisons, beside which the table's zeros are written.
+// 1000, 4096 and 8192 rows of 512 bf16, forward and gradient, 20, 25 and 37 us, with digits 29, 37 and 43.  Bound by its comparisons, beside which the table's zeros are written.
 constexpr int kCountedRows = 8192;
 __global__ __launch_bounds__(1024) void k_embedding_order(EmbeddingArgs a, unsigned sorting, EmbeddingFill fill) {
   __shared__ alignas(16) unsigned keys[kCountedRows];
@@ -204,8 +204,8 @@ __global__ __launch_bounds__(1024) void k_embedding_move(SortArgs a, EmbeddingFi
 // Sums: the rows of a token, in order, are cut into blocks of `run` from the token's first row on, so that how they are added does not depend on the rows of other tokens.  Up to 64 lanes, of 8 columns
 // each, take the blocks that begin in `run` places of the sorted rows: one that goes on from an earlier place at most, then tokens' first ones, of which the last may have more behind it.  The sum of all rows of a token
 // is a row of the table; those of a block with others before or behind it are kept, and joined in order.
-// Eight rows are on their way at a time, and no atomics are needed, whose order would change sums.  Bound by memory: the largest measured call moves 75 MB in 16-18 us; few rows by latency (6 us,
-// 10 where runs go over several pieces: where they begin is looked for first).
+// Eight rows are on their way at a time, and no atomics are needed, whose order would change sums.  Bound by memory: the largest measured call moves 73 MB in 19-20 us; few rows by latency (6 us,
+// 9-10 where runs go over several pieces: where they begin is looked for first).
 struct EmbeddingSumArgs {
   EmbeddingArgs e;
   float *begun, *rest;  // [pieces][pitch]

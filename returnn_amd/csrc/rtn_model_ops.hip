@@ -26,8 +26,8 @@ bool nothing(const DeltaSizes& z) { return z.B == 0 || z.heads == 0; }
 bool valid(const DeltaSizes& z) {
   return z.T >= 0 && z.T <= kMaxFrames && z.B >= 0 && z.key_heads >= 0 && z.heads >= 0 && z.dk >= 1 && z.dk <= kMaxKeyDim && z.dv >= 1 && z.dv <= kMaxValueDim && known(z.dtype);
 }
-// Calls of at most these frames that no gradient follows go frame by frame.  (12 sequences of 8 heads of 128 x 128 in bf16, frame by frame and in chunks: 1 frame 5.9 and 33 us, 16 frames 24.8 and
-// 31.5, 24 frames 35 and 31; 16 frames of one sequence 23.7 and 28.5, of 64 51 and 66.)
+// Calls of at most these frames that no gradient follows go frame by frame.  (12 sequences of 8 heads of 128 x 128 in bf16, frame by frame and in chunks: 1 frame 5.9 and 33 us, 16 frames 25.1 and
+// 30.7, 24 frames 35 and 31.5; 16 frames of one sequence 23.7 and 29.3, of 64 52 and 54.)
 constexpr int kStepFrames = 16;
 int delta_frames(const DeltaSizes& z) { return z.dtype == RTN_DTYPE_BF16 ? DeltaChunk<__bf16>::kFrames : DeltaChunk<float>::kFrames; }
 int64_t delta_chunks(const DeltaSizes& z) { return (z.T + delta_frames(z) - 1) / delta_frames(z); }
@@ -54,7 +54,7 @@ void with_delta(const DeltaSizes& z, F f) {
   });
 }
 // Wavefronts of a workgroup that goes through a head's chunks, with 16 columns of the state each.  Four take three quarters of the time that eight take, for half the columns: T=1000, heads of
-// 128 x 128 in bf16, four and eight: 128 heads (one round of workgroups, one) 140 and 185 us, with the gradient 609 and 680; 256 heads (two, one) 294 and 282, 1177 and 1036.
+// 128 x 128 in bf16, four and eight: 128 heads (one round of workgroups, one) 147 and 191 us, with the gradient 553 and 640; 256 heads (two, one) 313 and 284, 1071 and 946.
 int delta_waves(const DeltaSizes& z) {
   const int64_t lines = (int64_t)z.B * z.heads, four = (lines * ((z.dv + 63) / 64) + 255) / 256, eight = (lines * ((z.dv + 127) / 128) + 255) / 256;  // rounds of the device
   return 4 * eight < 3 * four ? 8 : 4;
@@ -69,8 +69,8 @@ void with_waves(const DeltaSizes& z, F f) {
 }
 constexpr int kSegmentWaves = 4;
 // Segments of the chunks, where sequences and heads are few: as many as a time estimate is least for, in which a chunk takes 1 (and 0.8 more in the first pass), a border 0.3, and both
-// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 331 us, 4 161, 8 107, 16 (chosen) 96, 32 129;
-// T=8192, two of 8 heads of 64 x 128: 541, 254, 170, 176, 183, 191; T=1000, 16 of 8 of 128 x 128: one 140, 4 266.  One segment or at least three; where eight wavefronts are taken half of the compute units
+// passes run in rounds of as many workgroups as there are compute units.  T=4000, one sequence of 8 heads of 128 x 128 in bf16: one segment 354 us, 4 166, 8 110, 16 (chosen) 96-100;
+// T=8192, two of 8 heads of 64 x 128: 584, 265, 175, 181-185 (chosen), 32 196; T=1000, 16 of 8 of 128 x 128: one (chosen) 146, 4 274.  One segment or at least three; where eight wavefronts are taken half of the compute units
 // have work, and the estimate never finds segments worth their second pass.
 int64_t delta_segments(const DeltaSizes& z) {
   if (delta_waves(z) != kSegmentWaves) return 1;
@@ -299,8 +299,8 @@ struct EmbeddingPlan {
   size_t rows, counts, parts;  // of 4 bytes
   EmbeddingPlan(int64_t n, int64_t V, int64_t D) {
     strips = (D + 511) / 512;
-    // Rows of a piece: few, so that there are wavefronts enough, until the pieces' own starts and ends cost more (rows of 512 bf16, forward and gradient, 8, 16 and 32 rows: of 8192 rows 31.8, 33.0 and
-    // 37.6 us, of 32768 58.0, 56.2 and 58.7, of 131072 151, 134 and 128).
+    // Rows of a piece: few, so that there are wavefronts enough, until the pieces' own starts and ends cost more (rows of 512 bf16, tokens as frequent as in a text, forward and gradient, 8, 16 and 32 rows:
+    // of 8192 rows 36.5, 38.4 and 44.3 us, of 32768 65.2, 62.0 and 66.4, of 131072 159, 138 and 127).
     run = n * strips < 16384 ? 8 : (n * strips < 65536 ? 16 : 32);
     pieces = (n + run - 1) / run;
     for (lanes = 1; lanes < 64 && lanes * 8 < D;) lanes *= 2;
